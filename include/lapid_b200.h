@@ -390,6 +390,77 @@ LAPID_B200_API lapid_b200_status lapid_b200_silu_mul_act(lapid_b200_device *dev,
                                                          lapid_b200_buffer *out, uint64_t rows, uint64_t cols,
                                                          lapid_b200_buffer *qact, int32_t layout);
 
+/* ---- the paged key/value cache and the attention over it -------------------------------------- */
+/* What lies between the q / k / v projections of a layer and its output projection when many requests are served
+ * together (lapid-nn's Attention and KvCache hold one request each). The cache of a layer is two buffers,
+ * k and v, each [pages][kv_heads][page_size][head_dim] in the cache's type; a request's keys lie in the pages that its
+ * row of the block table names. Three calls, queued on the device's stream and not waited for:
+ *   lapid_b200_paged_plan       once a step: block table, slots and positions from the requests' lengths, on the device, and how
+ *                               the step's attention is cut over the SMs (in `plan`, read by every layer's attention)
+ *   lapid_b200_paged_append     once a layer: rotary embedding, rounding, k and v to their slots, q in the cache's type
+ *   lapid_b200_paged_attention  once a layer: softmax(scale q k^T) v of the new tokens over cached and new keys
+ * None of them allocates or waits, so a step can be captured in a graph; lengths are read on the device, so a captured
+ * step serves whatever lengths fit the bounds below. What a kernel finds wrong on the device is reported by the next call that
+ * waits (execute, device_synchronize): "shape_mismatch" (a length is negative, or outside max_new, max_blocks or tokens: such a request
+ * takes no part), "out_of_memory" (the list of free pages ran out), "index_out_of_range" (a page, slot or position outside
+ * its range; it is not read or written), "invalid_launch" (the plan was made for another description).
+ *
+ * lapid_b200_paged describes a step; zero-fill it first. */
+#define LAPID_B200_MASK_FULL 0   /* a new token sees all keys, cached and new */
+#define LAPID_B200_MASK_CAUSAL 1 /* ... up to its own; with window > 0 the last `window` of these */
+#define LAPID_B200_MASK_CROSS 2  /* ... the cached ones only: nothing is appended (slots are -1) */
+typedef struct lapid_b200_paged {
+    int32_t dtype;       /* of the cache, q and out: F16 or BF16 */
+    uint32_t q_heads;    /* a multiple of kv_heads: query head h reads key/value head h / (q_heads / kv_heads) */
+    uint32_t kv_heads;
+    uint32_t head_dim;   /* a multiple of 8, 16..128 */
+    uint32_t page_size;  /* tokens in a page: 16, 32, 64 or 128 */
+    int32_t mask;        /* LAPID_B200_MASK_* */
+    uint64_t pages;      /* of the cache; pages * page_size < 2^31 */
+    uint64_t requests;   /* rows of the block table */
+    uint64_t tokens;     /* rows of q, k, v and out: the sum of the new lengths, or more (rows behind the sum are left alone) */
+    uint64_t max_blocks; /* columns of the block table */
+    uint64_t max_new;    /* no request has more new tokens */
+    uint64_t window;     /* CAUSAL: 0, or how many keys a token sees */
+    float scale;         /* of the scores; 0: 1 / sqrt(head_dim) */
+} lapid_b200_paged;
+/* Bytes of the plan buffer of such a step (16-byte aligned; its contents need no clearing). Host only; needs no device. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_plan_bytes(const lapid_b200_paged *desc, uint64_t *bytes);
+/* new_lens, cached_lens: i32 [requests], tokens to append and tokens already there. The pages that a request's new tokens
+ * need beyond ceil(cached / page_size) are taken from free_pages (i32 [n_free], in order, requests in order; NULL with
+ * n_free 0 when none are needed) and entered in its row of block_table (i32 [requests, max_blocks]; entries of cached tokens are
+ * read, others left alone). Out: slots and positions i32 [tokens] (page * page_size + place, and the token's index in its request;
+ * -1 behind the last token), kv_lens i32 [requests] (what the next step passes as cached_lens), used i32 [1]
+ * (how many free pages the step takes, also when there are fewer), plan. Running it again on the same inputs gives the same result. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_plan(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *new_lens,
+                                                       const lapid_b200_buffer *cached_lens, const lapid_b200_buffer *free_pages, uint64_t n_free,
+                                                       lapid_b200_buffer *block_table, lapid_b200_buffer *slots, lapid_b200_buffer *positions,
+                                                       lapid_b200_buffer *kv_lens, lapid_b200_buffer *used, lapid_b200_buffer *plan);
+/* q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim] of type src_dtype (F32, F16 or BF16), each through its view
+ * (offset; batch_stride from head to head, row_stride from token to token, in elements; NULL: contiguous), so that they may be parts
+ * of one fused projection's rows. rope (NULL: none): f32 [rope_rows, rot], row p the cosines of position p's rot / 2 angles, then their
+ * sines; the first rot (a multiple of 8) elements of each q and k head are turned in pairs (i, i + rot / 2), or with
+ * neighbours = 1 (2 i, 2 i + 1), in f32. Results are rounded once to the cache's type: k and v to their slots, q to q_out
+ * [tokens, q_heads, head_dim] contiguous (q and q_out NULL: only k and v). Rows with position -1 are skipped, with slot -1 not stored. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_append(lapid_b200_device *dev, const lapid_b200_paged *desc, int32_t src_dtype,
+                                                         const lapid_b200_buffer *q, const lapid_b200_matview *q_view, const lapid_b200_buffer *k,
+                                                         const lapid_b200_matview *k_view, const lapid_b200_buffer *v, const lapid_b200_matview *v_view,
+                                                         const lapid_b200_buffer *rope, uint64_t rope_rows, uint32_t rot, int32_t neighbours,
+                                                         const lapid_b200_buffer *slots, const lapid_b200_buffer *positions, lapid_b200_buffer *k_cache,
+                                                         lapid_b200_buffer *v_cache, lapid_b200_buffer *q_out);
+/* out[t, h, :] = softmax over the keys j that the mask leaves token t of (scale q[t, h] . k[j]) times v[j]; a row without keys is 0. q and out
+ * [tokens, q_heads, head_dim] through views as above (NULL: contiguous) in the cache's type: what an output projection takes as
+ * a_dtype F16 / BF16. lse (or NULL): f32 [tokens, q_heads], the logarithm of the softmax's sum (-inf: no keys), with which
+ * results over parts of the keys can be joined. Scores, sums and accumulators are f32; the softmax's weights are rounded to
+ * the cache's type for their product with v. What lies in pages behind a request's keys, or in front of its window, may be anything; a value
+ * of v that is not finite, though, also reaches rows of the same few tokens that do not see it (0 times infinity). `plan` also holds this call's intermediate results: attention calls with the same
+ * plan must not overlap on the GPU (calls on one stream never do). */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan,
+                                                            const lapid_b200_buffer *q, const lapid_b200_matview *q_view,
+                                                            const lapid_b200_buffer *k_cache, const lapid_b200_buffer *v_cache,
+                                                            const lapid_b200_buffer *block_table, lapid_b200_buffer *out,
+                                                            const lapid_b200_matview *out_view, lapid_b200_buffer *lse);
+
 /* ---- decode without allocation ------------------------------------------------------------ */
 /* This entry point has no counterpart in the reference. It exists for hosts that may not allocate
  * device memory when they need a matvec (an engine that gave all device memory to its own arena at

@@ -9,6 +9,8 @@ like the reference's own:
   -- crates/lapid-compiler/src/ir.rs:226-282, :483-488
 * :mod:`lapid_b200.quant` -- ``lapid_quant::{Format, layout, quantize, dequantize,
   from_ggml_blocks}`` (crates/lapid-quant/src/lib.rs:27-160)
+* :mod:`lapid_b200.paged` -- a paged key/value cache and the attention over it (lapid-nn's ``Attention`` and ``KvCache``
+  for many requests at once)
 * :mod:`lapid_b200.gguf` -- the GGUF tensor table and its "keep the blocks" import
   (crates/lapid-convert/src/gguf.rs:1-12, :177-215)
 
@@ -20,3 +22,5 @@ from .backend import (Backend, Buffer, DType, Epilogue, Launch, MatMulDims, MatM
                       gather_launch, matmul_id_launch, matmul_launch)
 from . import quant  # noqa: F401
 from . import gguf  # noqa: F401
+from . import paged  # noqa: F401
+from .paged import Mask, PagedSpec  # noqa: F401

@@ -47,6 +47,13 @@ class IoC(C.Structure):
     _fields_ = [("buffer", C.c_uint32), ("launch", C.c_uint32), ("offset", C.c_uint64), ("host", C.c_void_p), ("bytes", C.c_uint64)]
 
 
+class PagedC(C.Structure):
+    """lapid_b200_paged: a step over a paged key/value cache."""
+    _fields_ = [("dtype", C.c_int32), ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("page_size", C.c_uint32),
+                ("mask", C.c_int32), ("pages", C.c_uint64), ("requests", C.c_uint64), ("tokens", C.c_uint64), ("max_blocks", C.c_uint64),
+                ("max_new", C.c_uint64), ("window", C.c_uint64), ("scale", C.c_float)]
+
+
 class ProfileEntryC(C.Structure):
     _fields_ = [("kind", C.c_char * 24), ("launches", C.c_uint64), ("ms", C.c_double)]
 
@@ -103,6 +110,11 @@ SYMBOLS = {
     "lapid_b200_rms_norm_act": (C.c_int32, [P, P, P, P, P, P, C.c_uint64, C.c_uint64, C.c_float, P, C.c_int32]),
     "lapid_b200_tp_rms_norm_act": (C.c_int32, [P, P, P, P, P, C.c_uint64, C.c_uint64, C.c_float, P, C.c_int32]),
     "lapid_b200_silu_mul_act": (C.c_int32, [P, P, P, P, C.c_uint64, C.c_uint64, P, C.c_int32]),
+    "lapid_b200_paged_plan_bytes": (C.c_int32, [C.POINTER(PagedC), C.POINTER(C.c_uint64)]),
+    "lapid_b200_paged_plan": (C.c_int32, [P, C.POINTER(PagedC), P, P, P, C.c_uint64, P, P, P, P, P, P]),
+    "lapid_b200_paged_append": (C.c_int32, [P, C.POINTER(PagedC), C.c_int32, P, C.POINTER(MatViewC), P, C.POINTER(MatViewC), P, C.POINTER(MatViewC),
+                                           P, C.c_uint64, C.c_uint32, C.c_int32, P, P, P, P, P]),
+    "lapid_b200_paged_attention": (C.c_int32, [P, C.POINTER(PagedC), P, P, C.POINTER(MatViewC), P, P, P, P, C.POINTER(MatViewC), P]),
     "lapid_b200_gemv_q4k_static": (C.c_int32, [C.c_int32, P, P, P, C.c_uint64, P, C.c_uint32, C.c_uint32, C.c_uint32]),
     "lapid_b200_gemv_q4k_static_status": (C.c_int32, [C.c_int32, C.POINTER(C.c_int32)]),
 }

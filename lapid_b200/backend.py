@@ -431,6 +431,60 @@ class Backend:
         check(_lib.lib().lapid_b200_act_layout(self._h, C.byref(c), C.byref(lay), C.byref(nbytes)))
         return int(lay.value), int(nbytes.value)
 
+    # ---- the paged key/value cache (queued on the device's stream, not waited for); see lapid_b200.paged
+    def _paged_call(self, fn, spec, args, buffers):
+        c = spec.to_c()
+        ref, h = C.byref(c), self._h
+
+        def run():
+            check(fn(h, ref, *args))
+        run.keep = (c, args, buffers)
+        return run
+
+    @staticmethod
+    def _view(v: Optional[MatView]):
+        return C.byref(_lib.MatViewC(v.offset, v.batch_stride, v.row_stride)) if v is not None else None
+
+    def packed_paged_plan(self, spec, new_lens: Buffer, cached_lens: Buffer, block_table: Buffer, slots: Buffer, positions: Buffer, kv_lens: Buffer,
+                          used: Buffer, plan: Buffer, *, free_pages: Optional[Buffer] = None, n_free: int = 0):
+        """``paged_plan`` as a zero-argument callable for hot loops (no Python-side conversion per call), like ``packed``."""
+        bufs = (new_lens, cached_lens, free_pages, block_table, slots, positions, kv_lens, used, plan)
+        h = [b._h if b is not None else None for b in bufs]
+        return self._paged_call(_lib.lib().lapid_b200_paged_plan, spec, (h[0], h[1], h[2], n_free, *h[3:]), bufs)
+
+    def paged_plan(self, *args, **kw) -> None:
+        """Block table entries, slots and positions of a step's new tokens, from its lengths on the device, and the cut of its
+        attention over the SMs into ``plan`` (``lapid_b200_paged_plan``). Arguments: ``packed_paged_plan``."""
+        self.packed_paged_plan(*args, **kw)()
+
+    def packed_paged_append(self, spec, src_dtype: DType, q: Optional[Buffer], k: Buffer, v: Buffer, slots: Buffer, positions: Buffer, k_cache: Buffer,
+                            v_cache: Buffer, q_out: Optional[Buffer], *, rope: Optional[Buffer] = None, rope_rows: int = 0, rot: int = 0,
+                            neighbours: bool = False, q_view: Optional[MatView] = None, k_view: Optional[MatView] = None,
+                            v_view: Optional[MatView] = None):
+        """``paged_append`` as a zero-argument callable."""
+        bufs = (q, k, v, rope, slots, positions, k_cache, v_cache, q_out)
+        h = [b._h if b is not None else None for b in bufs]
+        return self._paged_call(_lib.lib().lapid_b200_paged_append, spec,
+                                (int(src_dtype), h[0], self._view(q_view), h[1], self._view(k_view), h[2], self._view(v_view), h[3], rope_rows, rot,
+                                 int(bool(neighbours)), *h[4:]), bufs)
+
+    def paged_append(self, *args, **kw) -> None:
+        """Rotary embedding of q and k, rounding to the cache's type, k and v to their slots, q to ``q_out``
+        (``lapid_b200_paged_append``). A view is a ``MatView``: ``batch_stride`` from head to head, ``row_stride`` from token to token."""
+        self.packed_paged_append(*args, **kw)()
+
+    def packed_paged_attention(self, spec, plan: Buffer, q: Buffer, k_cache: Buffer, v_cache: Buffer, block_table: Buffer, out: Buffer, *,
+                               lse: Optional[Buffer] = None, q_view: Optional[MatView] = None, out_view: Optional[MatView] = None):
+        """``paged_attention`` as a zero-argument callable."""
+        bufs = (plan, q, k_cache, v_cache, block_table, out, lse)
+        h = [b._h if b is not None else None for b in bufs]
+        return self._paged_call(_lib.lib().lapid_b200_paged_attention, spec,
+                                (h[0], h[1], self._view(q_view), h[2], h[3], h[4], h[5], self._view(out_view), h[6]), bufs)
+
+    def paged_attention(self, *args, **kw) -> None:
+        """Attention of the new tokens of every request over its pages (``lapid_b200_paged_attention``)."""
+        self.packed_paged_attention(*args, **kw)()
+
     def take_launch_count(self) -> int:
         return int(_lib.lib().lapid_b200_take_launch_count(self._h))
 

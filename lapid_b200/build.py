@@ -39,6 +39,8 @@ SOURCES = {
     "noalloc.cu": [],
     "glue.cu": [],
     "moe.cu": [],
+    "paged.cu": [],
+    "paged_attn.cu": [],
     "tp_allreduce.cu": [],
     "backend.cc": ["-x", "cu"],
 }

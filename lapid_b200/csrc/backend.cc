@@ -1127,10 +1127,17 @@ void check_status_word(lapid_b200_device *dev) {
     // a launch that gave up may have left partial sums in the decode workspace
     cudaMemsetAsync(dev->stream_ws.pairs, 0, dev->stream_ws.total_bytes, dev->stream);
     cudaStreamSynchronize(dev->stream);
-    if (st == 128) fail("index_out_of_range", "an index of a gather or an expert id of a matmul_id is out of range; the rows it selects were not computed");
-    // (which kernel sets which bit: 1 decode, 2 to 32 the waits of the tensor-core prefill, 64 tensor-parallel exchange, 128 a bad index, 256 exact-f32 GEMM)
+    constexpr int BAD_INDEX = 128, PAGED_INDEX = 512, PAGED_PAGES = 1024, PAGED_LENGTHS = 4096, PAGED_PLAN = 8192;
+    if ((st & ~(BAD_INDEX | PAGED_INDEX | PAGED_PAGES | PAGED_LENGTHS | PAGED_PLAN)) == 0) {  // no wait gave up
+        if (st & PAGED_PLAN) fail("invalid_launch", "paged attention: the plan buffer was not made for this description");
+        if (st & PAGED_LENGTHS) fail("shape_mismatch", "paged plan: a request's length is negative or outside max_new, max_blocks or tokens; it took no part");
+        if (st & PAGED_PAGES) fail("out_of_memory", "paged plan: the list of free pages ran out");
+        if (st & PAGED_INDEX) fail("index_out_of_range", "paged cache: a page, slot or position is out of range; what it names was not read or written");
+        fail("index_out_of_range", "an index of a gather or an expert id of a matmul_id is out of range; the rows it selects were not computed");
+    }
+    // (which kernel sets which bit: 1 decode, 2 to 32 the waits of the tensor-core prefill, 64 tensor-parallel exchange, 128 a bad index, 256 exact-f32 GEMM, 2048 paged attention)
     std::string who;
-    for (auto [bits, name] : {std::pair<int, const char *>{1, "decode"}, {2 | 4 | 8 | 16 | 32, "tensor-core prefill"}, {64, "tensor-parallel exchange"}, {256, "exact-f32 GEMM"}})
+    for (auto [bits, name] : {std::pair<int, const char *>{1, "decode"}, {2 | 4 | 8 | 16 | 32, "tensor-core prefill"}, {64, "tensor-parallel exchange"}, {256, "exact-f32 GEMM"}, {2048, "paged attention"}})
         if (st & bits) who += (who.empty() ? ": " : ", ") + std::string(name);
     fail("backend", "a device-side wait gave up (status " + std::to_string(st) + who + "); the results of this call are invalid");
 }
@@ -1567,6 +1574,74 @@ void execute_io_impl(lapid_b200_device *dev, const lapid_b200_launch *launches, 
     cuda_check(cudaStreamSynchronize(dev->io_out), "execute_io");
     check_status_word(dev);
 }
+
+// ------------------------------------------------------------------ the paged cache's descriptions
+// A step's description, checked: every product that the kernels form in 32 bits stays below 2^31 (rows of the cache, packed rows, units of work)
+lb::PagedShape paged_shape(const lapid_b200_paged *d) {
+    if (!d) fail("invalid_argument", "the paged description is NULL");
+    if (d->dtype != LAPID_B200_DTYPE_F16 && d->dtype != LAPID_B200_DTYPE_BF16)
+        fail("unsupported_dtype", "paged cache: dtype must be F16 or BF16, got " + std::to_string(d->dtype));
+    if (d->kv_heads == 0 || d->q_heads == 0 || d->q_heads % d->kv_heads != 0 || d->q_heads > 4096)
+        fail("invalid_launch", "paged cache: q_heads (at most 4096) must be a multiple of kv_heads, got " + std::to_string(d->q_heads) + " and " + std::to_string(d->kv_heads));
+    if (d->head_dim < 16 || d->head_dim > 128 || d->head_dim % 8 != 0)
+        fail("unsupported", "paged cache: head_dim must be a multiple of 8 in 16..128, got " + std::to_string(d->head_dim));
+    if (d->page_size != 16 && d->page_size != 32 && d->page_size != 64 && d->page_size != 128)
+        fail("unsupported", "paged cache: page_size must be 16, 32, 64 or 128, got " + std::to_string(d->page_size));
+    if (d->mask < LAPID_B200_MASK_FULL || d->mask > LAPID_B200_MASK_CROSS) fail("invalid_argument", "paged cache: unknown mask " + std::to_string(d->mask));
+    if (d->window && d->mask != LAPID_B200_MASK_CAUSAL) fail("invalid_argument", "paged cache: a window needs the causal mask");
+    if (d->pages == 0) fail("invalid_launch", "paged cache: no pages");
+    const uint64_t most = (1ull << 31) - 1, g = d->q_heads / d->kv_heads;
+    auto product_ok = [&](uint64_t x, uint64_t y) { return y == 0 || x <= most / y; };
+    if (!product_ok(d->pages, d->page_size) || !product_ok(d->pages * d->page_size, d->kv_heads)) fail("too_large", "paged cache: pages * kv_heads * page_size must be below 2^31");
+    if (d->requests > most || !product_ok(d->requests, d->max_blocks) || !product_ok(d->requests, d->max_new) || !product_ok(d->max_blocks, d->page_size))
+        fail("too_large", "paged cache: requests * max_blocks, requests * max_new and max_blocks * page_size must be below 2^31");
+    if (d->tokens > most || !product_ok(d->tokens, d->q_heads) || !product_ok(d->max_new, g)) fail("too_large", "paged cache: tokens * q_heads must be below 2^31");
+    // units of work: (tiles of rows) x heads x (steps of 64 keys), with the smaller tile
+    const uint64_t tiles = d->tokens * g / lb::PAGED_SMALL_ROWS + d->requests + 1, steps = d->max_blocks * d->page_size / lb::PAGED_SMALL_KEYS + 2;
+    if (!product_ok(tiles, steps) || !product_ok(tiles * steps, d->kv_heads)) fail("too_large", "paged cache: the step's (tokens x keys) is too large");
+    if (d->window > most) fail("too_large", "paged cache: window must be below 2^31");
+    const float scale = d->scale == 0.0f ? 1.0f / std::sqrt((float)d->head_dim) : d->scale;
+    if (!std::isfinite(scale)) fail("invalid_argument", "paged cache: scale is not finite");
+    lb::PagedShape s{};
+    s.bf16 = d->dtype == LAPID_B200_DTYPE_BF16;
+    s.hq = d->q_heads;
+    s.hkv = d->kv_heads;
+    s.g = (uint32_t)g;
+    s.d = d->head_dim;
+    s.page = d->page_size;
+    s.pages = (uint32_t)d->pages;
+    s.requests = (uint32_t)d->requests;
+    s.tokens = (uint32_t)d->tokens;
+    s.max_blocks = (uint32_t)d->max_blocks;
+    s.max_new = (uint32_t)d->max_new;
+    s.mask = (uint32_t)d->mask;
+    s.window = (uint32_t)d->window;
+    s.scale = scale;
+    return s;
+}
+void paged_buffer(const lapid_b200_device *dev, const lapid_b200_buffer *b, const char *what, uint64_t bytes) {
+    if (!b) fail("invalid_argument", std::string(what) + " is NULL");
+    if (b->dev != dev) fail("wrong_backend", std::string(what) + " belongs to another device");
+    if (b->bytes < bytes) fail("out_of_bounds", std::string(what) + ": needs " + std::to_string(bytes) + " bytes, buffer has " + std::to_string(b->bytes));
+    if ((uintptr_t)b->ptr & 15) fail("invalid_launch", std::string(what) + " must be 16-byte aligned");
+}
+// A view of [tokens, heads, d], checked against its buffer
+lb::PagedView paged_view(const lapid_b200_device *dev, const lapid_b200_buffer *b, const lapid_b200_matview *v, const char *what, uint64_t tokens, uint64_t heads,
+                         uint64_t d, uint64_t elem) {
+    lb::PagedView r{0, d, heads * d};
+    if (v) r = {v->offset, v->batch_stride, v->row_stride};
+    paged_buffer(dev, b, what, 0);
+    const uint64_t most = 1ull << 60;
+    if (r.off > most || (heads > 1 && r.head > most / heads) || (tokens > 1 && r.token > most / tokens)) fail("too_large", std::string(what) + ": view overflows");
+    const uint64_t end = tokens ? r.off + (tokens - 1) * r.token + (heads - 1) * r.head + d : 0;
+    if (end > b->bytes / elem) fail("out_of_bounds", std::string(what) + ": the view ends at element " + std::to_string(end) + ", the buffer at " + std::to_string(b->bytes / elem));
+    return r;
+}
+bool paged_overlap(const lapid_b200_buffer *a, const lapid_b200_buffer *b) {
+    const char *x = (const char *)a->ptr, *y = (const char *)b->ptr;
+    return x < y + b->bytes && y < x + a->bytes;
+}
+int paged_sms(const lapid_b200_device *dev) { return dev->sm_count < (int)lb::PAGED_MAX_SMS ? dev->sm_count : (int)lb::PAGED_MAX_SMS; }
 
 }  // namespace
 
@@ -2275,6 +2350,171 @@ lapid_b200_status lapid_b200_silu_mul_act(lapid_b200_device *dev, lapid_b200_buf
         cuda_check(lb::launch_silu_mul((const float *)gate->ptr, (const float *)up->ptr, (float *)out->ptr, count, (uint32_t)(qact ? cols : 0), q,
                                        dev->sm_count, dev->pdl, dev->stream), "silu_mul launch");
         if (count) dev->note_glue();
+        dev->launches++;
+    });
+}
+
+// ------------------------------------------------------------------ the paged key/value cache
+lapid_b200_status lapid_b200_paged_plan_bytes(const lapid_b200_paged *desc, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) fail("invalid_argument", "bytes is NULL");
+        *bytes = lb::paged_plan_layout(paged_shape(desc)).bytes;
+    });
+}
+
+lapid_b200_status lapid_b200_paged_plan(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *new_lens,
+                                        const lapid_b200_buffer *cached_lens, const lapid_b200_buffer *free_pages, uint64_t n_free,
+                                        lapid_b200_buffer *block_table, lapid_b200_buffer *slots, lapid_b200_buffer *positions,
+                                        lapid_b200_buffer *kv_lens, lapid_b200_buffer *used, lapid_b200_buffer *plan) {
+    return guard([&] {
+        need(dev);
+        lb::PagedPlanArgs a{};
+        a.s = paged_shape(desc);
+        a.l = lb::paged_plan_layout(a.s);
+        if (n_free >= (1ull << 31)) fail("too_large", "paged_plan: n_free must be below 2^31");
+        const uint64_t R = a.s.requests, T = a.s.tokens;
+        paged_buffer(dev, new_lens, "paged_plan: new_lens", R * 4);
+        paged_buffer(dev, cached_lens, "paged_plan: cached_lens", R * 4);
+        if (free_pages || n_free) paged_buffer(dev, free_pages, "paged_plan: free_pages", n_free * 4);
+        paged_buffer(dev, block_table, "paged_plan: block_table", R * a.s.max_blocks * 4);
+        paged_buffer(dev, slots, "paged_plan: slots", T * 4);
+        paged_buffer(dev, positions, "paged_plan: positions", T * 4);
+        paged_buffer(dev, kv_lens, "paged_plan: kv_lens", R * 4);
+        paged_buffer(dev, used, "paged_plan: used", 4);
+        paged_buffer(dev, plan, "paged_plan: plan", a.l.bytes);
+        const lapid_b200_buffer *ins[] = {new_lens, cached_lens, free_pages}, *outs[] = {block_table, slots, positions, kv_lens, used, plan};
+        for (size_t i = 0; i < 6; i++) {
+            for (const lapid_b200_buffer *b : ins)
+                if (b && paged_overlap(b, outs[i])) fail("buffer_aliasing", "paged_plan: an output aliases an input");
+            for (size_t j = 0; j < i; j++)
+                if (paged_overlap(outs[i], outs[j])) fail("buffer_aliasing", "paged_plan: two outputs alias");
+        }
+        std::lock_guard<std::mutex> lock(dev->mu);
+        dev->make_current();
+        a.new_lens = (const int32_t *)new_lens->ptr;
+        a.cached = (const int32_t *)cached_lens->ptr;
+        a.free_pages = free_pages ? (const int32_t *)free_pages->ptr : nullptr;
+        a.n_free = (uint32_t)n_free;
+        a.table = (int32_t *)block_table->ptr;
+        a.slots = (int32_t *)slots->ptr;
+        a.positions = (int32_t *)positions->ptr;
+        a.kv_lens = (int32_t *)kv_lens->ptr;
+        a.used = (int32_t *)used->ptr;
+        a.plan = (uint32_t *)plan->ptr;
+        a.status = dev->status_dev;
+        a.stamp = lb::paged_stamp(a.s);
+        const int sms = paged_sms(dev);
+        a.ctas_small = lb::paged_attn_small_ctas(sms);
+        a.ctas_large = a.s.max_new * (uint64_t)a.s.g > lb::PAGED_SMALL_LIMIT ? lb::paged_attn_large_ctas(sms) : 0;
+        cuda_check(lb::launch_paged_plan(a, sms, dev->pdl, dev->stream), "paged_plan launch");
+        dev->launches++;
+    });
+}
+
+lapid_b200_status lapid_b200_paged_append(lapid_b200_device *dev, const lapid_b200_paged *desc, int32_t src_dtype, const lapid_b200_buffer *q,
+                                          const lapid_b200_matview *q_view, const lapid_b200_buffer *k, const lapid_b200_matview *k_view,
+                                          const lapid_b200_buffer *v, const lapid_b200_matview *v_view, const lapid_b200_buffer *rope,
+                                          uint64_t rope_rows, uint32_t rot, int32_t neighbours, const lapid_b200_buffer *slots,
+                                          const lapid_b200_buffer *positions, lapid_b200_buffer *k_cache, lapid_b200_buffer *v_cache,
+                                          lapid_b200_buffer *q_out) {
+    return guard([&] {
+        need(dev);
+        lb::PagedAppendArgs a{};
+        a.s = paged_shape(desc);
+        if (!is_act_float(src_dtype)) fail("unsupported_dtype", "paged_append: src_dtype must be F32, F16 or BF16, got " + std::to_string(src_dtype));
+        if (a.s.mask == lb::PAGED_CROSS) fail("invalid_launch", "paged_append: a CROSS step appends nothing");
+        if ((q == nullptr) != (q_out == nullptr)) fail("invalid_argument", "paged_append: q and q_out come together");
+        if ((rope == nullptr) != (rot == 0)) fail("invalid_argument", "paged_append: rope and rot come together");
+        if (rot % 8 != 0 || rot > a.s.d) fail("invalid_launch", "paged_append: rot must be a multiple of 8 and at most head_dim, got " + std::to_string(rot));
+        if (neighbours != 0 && neighbours != 1) fail("invalid_argument", "paged_append: neighbours must be 0 or 1");
+        if (rope_rows >= (1ull << 31)) fail("too_large", "paged_append: rope_rows must be below 2^31");
+        const uint64_t T = a.s.tokens, eb = act_elem_size(src_dtype), cache = (uint64_t)a.s.pages * a.s.hkv * a.s.page * a.s.d * 2;
+        if (q) a.qv = paged_view(dev, q, q_view, "paged_append: q", T, a.s.hq, a.s.d, eb);
+        a.kv = paged_view(dev, k, k_view, "paged_append: k", T, a.s.hkv, a.s.d, eb);
+        a.vv = paged_view(dev, v, v_view, "paged_append: v", T, a.s.hkv, a.s.d, eb);
+        if (rope) paged_buffer(dev, rope, "paged_append: rope", rope_rows * rot * 4);
+        paged_buffer(dev, slots, "paged_append: slots", T * 4);
+        paged_buffer(dev, positions, "paged_append: positions", T * 4);
+        paged_buffer(dev, k_cache, "paged_append: k_cache", cache);
+        paged_buffer(dev, v_cache, "paged_append: v_cache", cache);
+        if (q_out) paged_buffer(dev, q_out, "paged_append: q_out", T * a.s.hq * a.s.d * 2);
+        const lapid_b200_buffer *ins[] = {q, k, v, rope, slots, positions}, *outs[] = {k_cache, v_cache, q_out};
+        for (size_t i = 0; i < 3; i++) {
+            if (!outs[i]) continue;
+            for (const lapid_b200_buffer *b : ins)
+                if (b && paged_overlap(b, outs[i])) fail("buffer_aliasing", "paged_append: an output aliases an input");
+            for (size_t j = 0; j < i; j++)
+                if (paged_overlap(outs[i], outs[j])) fail("buffer_aliasing", "paged_append: two outputs alias");
+        }
+        if (T == 0) return;
+        std::lock_guard<std::mutex> lock(dev->mu);
+        dev->make_current();
+        a.src_type = act_type_of(src_dtype);
+        a.q = q ? q->ptr : nullptr;
+        a.k = k->ptr;
+        a.v = v->ptr;
+        a.rope = rope ? (const float *)rope->ptr : nullptr;
+        a.rope_rows = (uint32_t)rope_rows;
+        a.rot = rot;
+        a.neighbours = (uint32_t)neighbours;
+        a.slots = (const int32_t *)slots->ptr;
+        a.positions = (const int32_t *)positions->ptr;
+        a.k_cache = k_cache->ptr;
+        a.v_cache = v_cache->ptr;
+        a.q_out = q_out ? q_out->ptr : nullptr;
+        a.status = dev->status_dev;
+        cuda_check(lb::launch_paged_append(a, dev->pdl, dev->stream), "paged_append launch");
+        dev->launches++;
+    });
+}
+
+lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan,
+                                             const lapid_b200_buffer *q, const lapid_b200_matview *q_view, const lapid_b200_buffer *k_cache,
+                                             const lapid_b200_buffer *v_cache, const lapid_b200_buffer *block_table, lapid_b200_buffer *out,
+                                             const lapid_b200_matview *out_view, lapid_b200_buffer *lse) {
+    return guard([&] {
+        need(dev);
+        lb::PagedAttnArgs a{};
+        a.s = paged_shape(desc);
+        a.l = lb::paged_plan_layout(a.s);
+        const uint64_t T = a.s.tokens, cache = (uint64_t)a.s.pages * a.s.hkv * a.s.page * a.s.d * 2;
+        paged_buffer(dev, plan, "paged_attention: plan", a.l.bytes);
+        a.qv = paged_view(dev, q, q_view, "paged_attention: q", T, a.s.hq, a.s.d, 2);
+        paged_buffer(dev, k_cache, "paged_attention: k_cache", cache);
+        paged_buffer(dev, v_cache, "paged_attention: v_cache", cache);
+        paged_buffer(dev, block_table, "paged_attention: block_table", (uint64_t)a.s.requests * a.s.max_blocks * 4);
+        a.ov = paged_view(dev, out, out_view, "paged_attention: out", T, a.s.hq, a.s.d, 2);
+        // each element of out is written by one row only
+        const uint64_t D = a.s.d, H = a.s.hq;
+        const bool heads_inside = a.ov.head >= D && (T <= 1 || a.ov.token >= (H - 1) * a.ov.head + D), tokens_inside = a.ov.token >= D && a.ov.head >= (T - 1) * a.ov.token + D;
+        if (T && !((H == 1 && (T <= 1 || a.ov.token >= D)) || heads_inside || tokens_inside)) fail("invalid_launch", "paged_attention: rows of out overlap");
+        if (lse) paged_buffer(dev, lse, "paged_attention: lse", T * H * 4);
+        const lapid_b200_buffer *ins[] = {q, k_cache, v_cache, block_table}, *outs[] = {plan, out, lse};
+        for (size_t i = 0; i < 3; i++) {
+            if (!outs[i]) continue;
+            for (const lapid_b200_buffer *b : ins)
+                if (paged_overlap(b, outs[i])) fail("buffer_aliasing", "paged_attention: an output aliases an input");
+            for (size_t j = 0; j < i; j++)
+                if (paged_overlap(outs[i], outs[j])) fail("buffer_aliasing", "paged_attention: two outputs alias");
+        }
+        if (T == 0 || a.s.requests == 0) return;
+        std::lock_guard<std::mutex> lock(dev->mu);
+        dev->make_current();
+        a.stamp = lb::paged_stamp(a.s);
+        a.plan = (uint32_t *)plan->ptr;
+        a.q = q->ptr;
+        a.k_cache = k_cache->ptr;
+        a.v_cache = v_cache->ptr;
+        a.table = (const int32_t *)block_table->ptr;
+        a.out = out->ptr;
+        a.lse = lse ? (float *)lse->ptr : nullptr;
+        a.status = dev->status_dev;
+        // requests of many rows first: their CTAs run longest
+        if (a.s.max_new * (uint64_t)a.s.g > lb::PAGED_SMALL_LIMIT) {
+            cuda_check(lb::launch_paged_attn_large(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
+            dev->launches++;
+        }
+        cuda_check(lb::launch_paged_attn_small(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
         dev->launches++;
     });
 }

@@ -389,6 +389,68 @@ bool rms_norm_quant_ok(uint32_t cols);  // the row's parts (CTAs of the tensor-p
 cudaError_t launch_silu_mul(const float *gate, const float *up, float *out, uint64_t n, uint32_t cols, const ActOut &q, int sm_count,
                             bool pdl, cudaStream_t stream);
 
+// ---- paged.cu, paged_attn.cu, paged_attn_tc.cu: the paged key/value cache and the attention over it
+constexpr uint32_t PAGED_FULL = 0, PAGED_CAUSAL = 1, PAGED_CROSS = 2;  // LAPID_B200_MASK_*
+constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile and step of the kernel for few rows
+constexpr uint32_t PAGED_SMALL_LIMIT = 16;                             // requests of at most so many packed rows go to it
+constexpr uint32_t PAGED_LARGE_ROWS = 256, PAGED_LARGE_KEYS = 128;     // tile and step of the tensor-memory kernel
+constexpr uint32_t PAGED_SMALL_MIN = 4, PAGED_LARGE_MIN = 2;             // fewest steps worth a CTA of its own
+constexpr uint32_t PAGED_MAX_SMS = 160;
+struct PagedShape {
+    int bf16;  // cache, q and out: bf16, else f16
+    uint32_t hq, hkv, g, d, page, pages, requests, tokens, max_blocks, max_new, mask, window;
+    float scale;
+};
+// Places in a plan buffer (32-bit words; the partial results behind them at byte offsets)
+struct PagedPlanLayout {
+    uint32_t q_start, kv_len, units_small, units_large, start_small, start_large, count_small, count_large;
+    size_t part_small, part_large, bytes;  // part_*: [CTA][2] results of cut tiles: rows x (d padded + 2) f32
+};
+PagedPlanLayout paged_plan_layout(const PagedShape &s);
+uint32_t paged_stamp(const PagedShape &s);  // what a plan was made for
+uint32_t paged_part_floats(const PagedShape &s, uint32_t rows);
+struct PagedPlanArgs {
+    PagedShape s;
+    PagedPlanLayout l;
+    const int32_t *new_lens, *cached, *free_pages;
+    uint32_t n_free, stamp, ctas_small, ctas_large;
+    int32_t *table, *slots, *positions, *kv_lens, *used;
+    uint32_t *plan;
+    int *status;
+};
+cudaError_t launch_paged_plan(const PagedPlanArgs &a, int sm_count, bool pdl, cudaStream_t stream);
+struct PagedView {
+    uint64_t off, head, token;  // elements: start, from head to head, from token to token
+};
+struct PagedAppendArgs {
+    PagedShape s;
+    int src_type;  // ACT_F32 / ACT_F16 / ACT_BF16
+    const void *q, *k, *v;
+    PagedView qv, kv, vv;
+    const float *rope;  // [rope_rows][rot]: cos, then sin
+    uint32_t rope_rows, rot, neighbours;
+    const int32_t *slots, *positions;
+    void *k_cache, *v_cache, *q_out;
+    int *status;
+};
+cudaError_t launch_paged_append(const PagedAppendArgs &a, bool pdl, cudaStream_t stream);
+struct PagedAttnArgs {
+    PagedShape s;
+    PagedPlanLayout l;
+    uint32_t stamp;
+    uint32_t *plan;
+    const void *q, *k_cache, *v_cache;
+    PagedView qv, ov;
+    const int32_t *table;
+    void *out;
+    float *lse;
+    int *status;
+};
+uint32_t paged_attn_small_ctas(int sm_count);
+uint32_t paged_attn_large_ctas(int sm_count);
+cudaError_t launch_paged_attn_small(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream);
+cudaError_t launch_paged_attn_large(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream);
+
 // ---- tp_allreduce.cu: one-shot all-reduce over peer-mapped memory
 struct TpAllReduceArgs {
     void *peer[TP_MAX_RANKS];  // every rank's symmetric buffer as mapped on this GPU; peer[rank] is this rank's own

@@ -1,0 +1,381 @@
+// The paged key/value cache: block tables and slot maps from the requests' lengths, and the append of new keys and values.
+//
+// plan    start[r] = sum of the new lengths before r, first[r] = sum of the pages taken before r; token t of r lies at position cached + t,
+//         in block pos / page of its table row, slot = table[r][block] * page + pos % page. New blocks take the pages
+//         free_pages[first[r]...] in the requests' order, so the result does not depend on timing. The plan also cuts the work of
+//         the attention launches that follow (paged.cuh): which request, head, tile and step each CTA begins with. That is
+//         done once a step, and every layer's launch reads it.
+//         What bounds it is latency: one launch, two scans over the requests, a search a token. Every CTA scans the lengths
+//         itself (1024 requests at a time) so that nothing passes between CTAs; CTA 0 cuts the work, the others fill tokens and blocks.
+// append  (x, y) -> (x cos - y sin, y cos + x sin) in f32 for the rotary pairs of q and k, one rounding to the cache's type; k and v go
+//         to their slots. Bound by memory: each element is read once and written once; a thread keeps the angles of its
+//         four pairs in registers over the heads of a token.
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "paged.cuh"
+
+namespace lb {
+
+// ------------------------------------------------------------------ layout of a plan (host)
+static uint32_t words_up(uint32_t w) { return (w + 63) & ~63u; }
+
+uint32_t paged_part_floats(const PagedShape &s, uint32_t rows) { return rows * ((s.d > 64 ? 128 : 64) + 2); }
+
+PagedPlanLayout paged_plan_layout(const PagedShape &s) {
+    PagedPlanLayout l{};
+    uint32_t w = PLAN_HEADER;
+    auto take = [&](uint32_t n) {
+        const uint32_t at = w;
+        w = words_up(w + n);
+        return at;
+    };
+    const bool large = (uint64_t)s.max_new * s.g > PAGED_SMALL_LIMIT;
+    const uint32_t cs = paged_attn_small_ctas(PAGED_MAX_SMS), cl = large ? paged_attn_large_ctas(PAGED_MAX_SMS) : 0;
+    l.q_start = take(s.requests + 1);
+    l.kv_len = take(s.requests);
+    l.units_small = take(s.requests + 1);
+    l.units_large = take(s.requests + 1);
+    l.start_small = take(4 * cs);
+    l.start_large = take(4 * cl);
+    l.count_small = take(cs);
+    l.count_large = take(cl);
+    l.part_small = (size_t)w * 4;
+    l.part_large = l.part_small + (size_t)cs * 2 * paged_part_floats(s, PAGED_SMALL_ROWS) * 4;
+    l.bytes = l.part_large + (size_t)cl * 2 * paged_part_floats(s, PAGED_LARGE_ROWS) * 4;
+    return l;
+}
+
+uint32_t paged_stamp(const PagedShape &s) {
+    uint32_t h = 2166136261u;  // (Fowler, Noll and Vo's hash over the words a plan depends on)
+    for (uint32_t v : {s.g, s.hkv, s.page, s.requests, s.tokens, s.max_blocks, s.max_new, s.mask, s.window, s.d > 64 ? 128u : 64u})
+        for (int b = 0; b < 4; b++) h = (h ^ ((v >> (8 * b)) & 0xff)) * 16777619u;
+    return h | 1u;  // never what a zeroed buffer holds
+}
+
+// ------------------------------------------------------------------ plan
+constexpr uint32_t PLAN_THREADS = 1024;
+
+struct PlanShared {
+    uint32_t warp_sum[32];
+    uint32_t start[PLAN_THREADS + 1], first[PLAN_THREADS + 1], cached[PLAN_THREADS], have[PLAN_THREADS];
+};
+
+// Sum over the threads before this one; `total`: over all
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, PlanShared &sh, uint32_t &total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+    }
+    __syncthreads();  // the sums of the scan before have been read
+    if (lane == 31) sh.warp_sum[warp] = inc;
+    __syncthreads();
+    uint32_t w = sh.warp_sum[lane], winc = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, winc, o);
+        if (lane >= o) winc += x;
+    }
+    total = __shfl_sync(0xffffffffu, winc, 31);
+    return __shfl_sync(0xffffffffu, winc - w, warp) + inc - v;
+}
+
+// The last i < n with a[i] <= x (a rises, a[0] <= x)
+template <class T> __device__ __forceinline__ uint32_t last_at_most(const T *a, uint32_t n, uint32_t x) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (a[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Steps of all tiles of a request and one key/value head; long requests are shared by the warp (every lane of a warp calls it)
+__device__ uint32_t head_steps(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t rows, uint32_t keys, bool mine) {
+    const uint32_t lane = threadIdx.x & 31, tiles = mine && n ? paged_tiles(s, n, rows) : 0;
+    uint32_t sum = 0;
+    if (tiles <= 16)
+        for (uint32_t i = 0; i < tiles; i++) sum += paged_tile(s, n, kv, i, rows, keys).steps;
+    for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 16); many; many &= many - 1) {
+        const int who = __ffs(many) - 1;
+        const uint32_t n1 = __shfl_sync(0xffffffffu, n, who), kv1 = __shfl_sync(0xffffffffu, kv, who), t1 = __shfl_sync(0xffffffffu, tiles, who);
+        uint32_t part = 0;
+        for (uint32_t i = lane; i < t1; i += 32) part += paged_tile(s, n1, kv1, i, rows, keys).steps;
+        part = __reduce_add_sync(0xffffffffu, part);
+        if ((int)lane == who) sum = part;
+    }
+    return sum;
+}
+
+// Where CTA b begins: {request, head, tile, step of the tile}; a warp for each CTA
+__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, const uint32_t *prefix, uint32_t *starts, uint32_t rows, uint32_t keys) {
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t b = threadIdx.x >> 5; b < ctas; b += PLAN_THREADS / 32) {
+        const uint32_t x = paged_span(units, ctas, b);
+        const uint32_t r = last_at_most(prefix, a.s.requests, x);
+        const uint32_t per_head = (prefix[r + 1] - prefix[r]) / a.s.hkv, off = x - prefix[r], head = off / per_head;
+        uint32_t rem = off - head * per_head;
+        const uint32_t n = a.plan[a.l.q_start + r + 1] - a.plan[a.l.q_start + r], kv = a.plan[a.l.kv_len + r], tiles = paged_tiles(a.s, n, rows);
+        uint32_t tile = 0;
+        for (uint32_t i0 = 0; i0 < tiles; i0 += 32) {
+            const uint32_t mine = i0 + lane < tiles ? paged_tile(a.s, n, kv, i0 + lane, rows, keys).steps : 0;
+            uint32_t inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const uint32_t behind = __ballot_sync(0xffffffffu, inc > rem);
+            if (behind) {
+                const int who = __ffs(behind) - 1;
+                tile = i0 + who;
+                rem -= __shfl_sync(0xffffffffu, inc - mine, who);
+                break;
+            }
+            rem -= __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) ((uint4 *)starts)[b] = make_uint4(r, head, tile, rem);
+    }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ PlanShared sh;
+    const PagedShape &s = a.s;
+    const uint32_t tid = threadIdx.x, workers = gridDim.x > 1 ? gridDim.x - 1 : 1, worker = gridDim.x > 1 ? blockIdx.x - 1 : 0;
+    const bool cuts = blockIdx.x == 0, fills = gridDim.x == 1 || blockIdx.x > 0;
+    uint32_t base = 0, taken = 0, small = 0, large = 0;  // tokens, pages and units of the chunks before
+    uint32_t bad = 0;
+    for (uint32_t r0 = 0; r0 < s.requests; r0 += PLAN_THREADS) {
+        const uint32_t r = r0 + tid, count = min(PLAN_THREADS, s.requests - r0);
+        uint32_t n = 0, c = 0, have = 0, need = 0;
+        if (r < s.requests) {
+            const int32_t n0 = a.new_lens[r], c0 = a.cached[r];
+            const int64_t blocks = ((int64_t)c0 + (s.mask == PAGED_CROSS ? 0 : n0) + s.page - 1) / s.page;
+            if (n0 < 0 || c0 < 0 || n0 > (int64_t)s.max_new || blocks > (int64_t)s.max_blocks) {
+                bad |= PAGED_STATUS_LENGTHS;  // such a request takes no part
+            } else {
+                n = (uint32_t)n0, c = (uint32_t)c0;
+                have = (c + s.page - 1) / s.page;
+                need = (uint32_t)blocks;
+            }
+        }
+        uint32_t total_n, total_p;
+        const uint32_t at_n = base + block_scan(n, sh, total_n), at_p = taken + block_scan(need - have, sh, total_p);
+        // (rows behind the last one of q: such tokens take no part)
+        const uint32_t lo = min(at_n, s.tokens), hi = min(at_n + n, s.tokens);
+        if (hi - lo != n) bad |= PAGED_STATUS_LENGTHS;
+        n = hi - lo;
+        sh.start[tid] = lo;
+        sh.first[tid] = at_p;
+        sh.cached[tid] = c;
+        sh.have[tid] = have;
+        const uint32_t end_n = min(base + total_n, s.tokens), end_p = taken + total_p;
+        if (tid == 0) sh.start[count] = end_n, sh.first[count] = end_p;  // (count < PLAN_THREADS: the thread of that place writes the same)
+        if (cuts) {
+            const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
+            const bool few = paged_is_small(s, n);
+            const uint32_t us = head_steps(s, n, kv, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, few) * s.hkv;
+            const uint32_t ul = head_steps(s, n, kv, PAGED_LARGE_ROWS, PAGED_LARGE_KEYS, !few) * s.hkv;
+            uint32_t total_s, total_l;
+            const uint32_t at_s = small + block_scan(us, sh, total_s), at_l = large + block_scan(ul, sh, total_l);
+            if (r < s.requests) {
+                a.plan[a.l.q_start + r] = lo;
+                a.plan[a.l.kv_len + r] = kv;
+                a.plan[a.l.units_small + r] = at_s;
+                a.plan[a.l.units_large + r] = at_l;
+                a.kv_lens[r] = (int32_t)kv;
+            }
+            small += total_s, large += total_l;
+        }
+        __syncthreads();
+        if (fills) {
+            for (uint32_t j = taken + worker * PLAN_THREADS + tid; j < end_p; j += workers * PLAN_THREADS) {
+                const uint32_t i = last_at_most(sh.first, count, j);
+                int32_t page = -1;
+                if (j >= a.n_free) bad |= PAGED_STATUS_PAGES;
+                else if ((page = a.free_pages[j]) < 0 || (uint32_t)page >= s.pages) page = -1, bad |= PAGED_STATUS_INDEX;
+                a.table[(size_t)(r0 + i) * s.max_blocks + sh.have[i] + (j - sh.first[i])] = page;
+            }
+            for (uint32_t t = base + worker * PLAN_THREADS + tid; t < end_n; t += workers * PLAN_THREADS) {
+                const uint32_t i = last_at_most(sh.start, count, t), pos = sh.cached[i] + (t - sh.start[i]), block = pos / s.page;
+                int32_t slot = -1;
+                if (s.mask != PAGED_CROSS) {
+                    int32_t page = -1;
+                    if (block < sh.have[i]) page = a.table[(size_t)(r0 + i) * s.max_blocks + block];
+                    else if (sh.first[i] + (block - sh.have[i]) < a.n_free) page = a.free_pages[sh.first[i] + (block - sh.have[i])];
+                    if (page >= 0 && (uint32_t)page < s.pages) slot = (int32_t)((uint32_t)page * s.page + pos % s.page);
+                    else if (block < sh.have[i]) bad |= PAGED_STATUS_INDEX;
+                }
+                a.slots[t] = slot;
+                a.positions[t] = (int32_t)pos;
+            }
+        }
+        base += total_n;
+        if (base > s.tokens) base = s.tokens;
+        taken = end_p;
+        __syncthreads();  // the tables of this chunk are read
+    }
+    if (fills)
+        for (uint32_t t = base + worker * PLAN_THREADS + tid; t < s.tokens; t += workers * PLAN_THREADS) a.slots[t] = a.positions[t] = -1;
+    if (bad && a.status) atomicOr(a.status, (int)bad);
+    if (!cuts) return;
+    const uint32_t cs = small < a.ctas_small * PAGED_SMALL_MIN ? (small + PAGED_SMALL_MIN - 1) / PAGED_SMALL_MIN : a.ctas_small;
+    const uint32_t cl = large < a.ctas_large * PAGED_LARGE_MIN ? (large + PAGED_LARGE_MIN - 1) / PAGED_LARGE_MIN : a.ctas_large;
+    if (tid == 0) {
+        a.plan[PLAN_STAMP] = a.stamp;
+        a.plan[PLAN_TOKENS] = base;
+        a.plan[PLAN_UNITS_SMALL] = small;
+        a.plan[PLAN_CTAS_SMALL] = cs;
+        a.plan[PLAN_UNITS_LARGE] = large;
+        a.plan[PLAN_CTAS_LARGE] = cl;
+        a.plan[a.l.q_start + s.requests] = base;
+        a.plan[a.l.units_small + s.requests] = small;
+        a.plan[a.l.units_large + s.requests] = large;
+        *a.used = (int32_t)taken;
+    }
+    for (uint32_t b = tid; b < a.ctas_small; b += PLAN_THREADS) a.plan[a.l.count_small + b] = 0;
+    for (uint32_t b = tid; b < a.ctas_large; b += PLAN_THREADS) a.plan[a.l.count_large + b] = 0;
+    __syncthreads();
+    if (small) cut_units(a, small, cs, a.plan + a.l.units_small, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS);
+    if (large) cut_units(a, large, cl, a.plan + a.l.units_large, a.plan + a.l.start_large, PAGED_LARGE_ROWS, PAGED_LARGE_KEYS);
+}
+
+static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim3 grid, unsigned threads, size_t smem, bool pdl, cudaStream_t stream) {
+    cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+}
+
+cudaError_t launch_paged_plan(const PagedPlanArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
+    const uint32_t want = (a.s.tokens + PLAN_THREADS - 1) / PLAN_THREADS;
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[1];
+    paged_config(cfg, attr, dim3(1 + (want < (uint32_t)sm_count - 1 ? want : (uint32_t)sm_count - 1)), PLAN_THREADS, 0, pdl, stream);
+    return cudaLaunchKernelEx(&cfg, paged_plan_kernel, a);
+}
+
+// ------------------------------------------------------------------ append
+constexpr uint32_t APPEND_THREADS = 256, APPEND_HEADS = 3;  // heads whose loads a thread has in flight
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+        return *(const uint32_t *)&r;
+    }
+    const __half2 r = __floats2half2_rn(a, b);
+    return *(const uint32_t *)&r;
+}
+// four elements from `i` on of the row at `row`
+template <int SRC, bool VEC> __device__ __forceinline__ float4 load4(const void *row, uint32_t i) {
+    if constexpr (!VEC) return make_float4(load_act(row, i, SRC), load_act(row, i + 1, SRC), load_act(row, i + 2, SRC), load_act(row, i + 3, SRC));
+    else if constexpr (SRC == ACT_F32) return *(const float4 *)((const float *)row + i);
+    else {
+        const uint2 w = *(const uint2 *)((const unsigned short *)row + i);
+        return make_float4(widen_act(w.x & 0xffff, SRC), widen_act(w.x >> 16, SRC), widen_act(w.y & 0xffff, SRC), widen_act(w.y >> 16, SRC));
+    }
+}
+
+// blockIdx.x walks the tokens, blockIdx.y takes every gridDim.y-th batch of heads. A thread owns eight elements of a head: the rotary pairs
+// (i, i + rot / 2), i = 4 c..4 c + 3 (halves), or the neighbours (2 i, 2 i + 1) of the same i, or eight elements as they are. VEC: the rows allow loads of four elements.
+template <int SRC, bool VEC> __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(PagedAppendArgs p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const PagedShape &s = p.s;
+    const uint32_t chunks = s.d / 8, lanes = APPEND_THREADS / chunks, c = threadIdx.x % chunks, hl = threadIdx.x / chunks;
+    if (hl >= lanes) return;
+    const uint32_t hq = p.q ? s.hq : 0, heads = hq + 2 * s.hkv, half = p.rot / 2;
+    const bool turned = c < p.rot / 8;
+    const bool bf16 = s.bf16;
+    for (uint32_t t = blockIdx.x; t < s.tokens; t += gridDim.x) {
+        const int32_t slot = p.slots[t], pos = p.positions[t];
+        if (pos < 0) continue;  // no token
+        const bool stored = slot >= 0 && (uint32_t)slot < s.pages * s.page;
+        if ((p.rot && (uint32_t)pos >= p.rope_rows) || (slot >= 0 && !stored)) {
+            if (threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
+            continue;
+        }
+        float4 cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (turned) {
+            cs = *(const float4 *)(p.rope + (size_t)pos * p.rot + 4 * c);
+            sn = *(const float4 *)(p.rope + (size_t)pos * p.rot + half + 4 * c);
+        }
+        const uint32_t page = (uint32_t)slot / s.page, in_page = (uint32_t)slot % s.page;
+        for (uint32_t h0 = blockIdx.y * lanes * APPEND_HEADS; h0 < heads; h0 += gridDim.y * lanes * APPEND_HEADS) {
+            float4 x[APPEND_HEADS], y[APPEND_HEADS];
+#pragma unroll
+            for (uint32_t j = 0; j < APPEND_HEADS; j++) {
+                const uint32_t h = h0 + j * lanes + hl;
+                if (h >= heads) continue;
+                const bool is_q = h < hq, is_v = h >= hq + s.hkv;
+                const PagedView &w = is_q ? p.qv : is_v ? p.vv : p.kv;
+                const uint32_t hh = is_q ? h : is_v ? h - hq - s.hkv : h - hq;
+                const void *base = is_q ? p.q : is_v ? p.v : p.k;
+                const void *row = (const char *)base + (w.off + (uint64_t)t * w.token + (uint64_t)hh * w.head) * act_elem_bytes(SRC);
+                const bool split = turned && !is_v && !p.neighbours;
+                x[j] = load4<SRC, VEC>(row, split ? 4 * c : 8 * c);
+                y[j] = load4<SRC, VEC>(row, split ? 4 * c + half : 8 * c + 4);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < APPEND_HEADS; j++) {
+                const uint32_t h = h0 + j * lanes + hl;
+                if (h >= heads) continue;
+                const bool is_q = h < hq, is_v = h >= hq + s.hkv;
+                if (!is_q && !stored) continue;
+                const uint32_t hh = is_q ? h : is_v ? h - hq - s.hkv : h - hq;
+                uint16_t *row = is_q ? (uint16_t *)p.q_out + ((size_t)t * s.hq + hh) * s.d
+                                     : (uint16_t *)(is_v ? p.v_cache : p.k_cache) + (((size_t)page * s.hkv + hh) * s.page + in_page) * s.d;
+                const float4 u = x[j], v = y[j];
+                if (turned && !is_v && !p.neighbours) {
+                    const uint2 lo = make_uint2(pack_half(fmaf(u.x, cs.x, -v.x * sn.x), fmaf(u.y, cs.y, -v.y * sn.y), bf16),
+                                                pack_half(fmaf(u.z, cs.z, -v.z * sn.z), fmaf(u.w, cs.w, -v.w * sn.w), bf16));
+                    const uint2 hi = make_uint2(pack_half(fmaf(v.x, cs.x, u.x * sn.x), fmaf(v.y, cs.y, u.y * sn.y), bf16),
+                                                pack_half(fmaf(v.z, cs.z, u.z * sn.z), fmaf(v.w, cs.w, u.w * sn.w), bf16));
+                    *(uint2 *)(row + 4 * c) = lo;
+                    *(uint2 *)(row + 4 * c + half) = hi;
+                } else if (turned && !is_v) {
+                    *(uint4 *)(row + 8 * c) = make_uint4(pack_half(fmaf(u.x, cs.x, -u.y * sn.x), fmaf(u.y, cs.x, u.x * sn.x), bf16),
+                                                         pack_half(fmaf(u.z, cs.y, -u.w * sn.y), fmaf(u.w, cs.y, u.z * sn.y), bf16),
+                                                         pack_half(fmaf(v.x, cs.z, -v.y * sn.z), fmaf(v.y, cs.z, v.x * sn.z), bf16),
+                                                         pack_half(fmaf(v.z, cs.w, -v.w * sn.w), fmaf(v.w, cs.w, v.z * sn.w), bf16));
+                } else {
+                    *(uint4 *)(row + 8 * c) = make_uint4(pack_half(u.x, u.y, bf16), pack_half(u.z, u.w, bf16), pack_half(v.x, v.y, bf16), pack_half(v.z, v.w, bf16));
+                }
+            }
+        }
+    }
+}
+
+template <int SRC> static cudaError_t append_src(const PagedAppendArgs &a, bool vec, const cudaLaunchConfig_t &cfg) {
+    return vec ? cudaLaunchKernelEx(&cfg, paged_append_kernel<SRC, true>, a) : cudaLaunchKernelEx(&cfg, paged_append_kernel<SRC, false>, a);
+}
+
+cudaError_t launch_paged_append(const PagedAppendArgs &a, bool pdl, cudaStream_t stream) {
+    const uint32_t eb = act_elem_bytes(a.src_type), per = APPEND_THREADS / (a.s.d / 8) * APPEND_HEADS, heads = (a.q ? a.s.hq : 0) + 2 * a.s.hkv;
+    bool vec = true;  // every group of four elements starts on a multiple of its size
+    auto check = [&](const void *base, const PagedView &v) {
+        if (base && (((uintptr_t)base + v.off * eb) % (4 * eb) || v.head % 4 || v.token % 4)) vec = false;
+    };
+    check(a.q, a.qv);
+    check(a.k, a.kv);
+    check(a.v, a.vv);
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[1];
+    // few tokens: a CTA for each batch of heads; many: one CTA walks a token's heads and keeps its angles
+    const uint32_t batches = (heads + per - 1) / per;
+    paged_config(cfg, attr, dim3(a.s.tokens < (1u << 20) ? a.s.tokens : 1u << 20, a.s.tokens < 512 ? batches : 1), APPEND_THREADS, 0, pdl, stream);
+    return a.src_type == ACT_F32 ? append_src<ACT_F32>(a, vec, cfg) : a.src_type == ACT_F16 ? append_src<ACT_F16>(a, vec, cfg) : append_src<ACT_BF16>(a, vec, cfg);
+}
+
+}  // namespace lb
