@@ -1,89 +1,437 @@
-// Attention of the new tokens of every request over its pages, the form that is simplest: a warp for each (token, query head) walks the keys
-// with the running maximum m, sum l and accumulator of the softmax; a lane holds four elements of the head.
+// Attention over the pages for requests of few rows: single tokens, a few speculated ones, short chunks.
+//
+//   s = scale q k^T over the keys that the mask leaves a row;  m = max s, p = exp(s - m), l = sum p, out = sum p v / l
+//
+// in one pass over the keys: m, l and the accumulator are rescaled when m grows. What bounds it is HBM: every key and value is read once
+// for the g query heads that share it (g x 2 operations a byte), so the query heads of one key/value head are the 16 rows of `mma.sync.m16n8k16`
+// -- the operands it multiplies come straight from the copied pages, and the results are where the next product wants them; the
+// tensor-memory instruction would want 128 rows and its softmax weights back in tensor memory.
+//
+// The steps (64 keys of one tile) of all requests and heads are one sequence, cut into equal spans, one a CTA (paged.cuh): requests of any
+// lengths keep every SM busy to the end. A producer warp fills a ring of steps with TMA copies of (parts of) pages, four warps take 16
+// keys of every step each, with maxima, sums and accumulators of their own, which meet at the end of a tile. A tile that a span's end
+// cuts is left in the plan buffer by each of its CTAs; the one that comes last adds the pieces up, in the order of the keys.
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "pipe.cuh"
 
 namespace lb {
 
-__device__ __forceinline__ float4 load_half4(const void *row, uint32_t i, bool bf16) {
-    const uint2 w = *(const uint2 *)((const unsigned short *)row + i);
-    const int t = bf16 ? ACT_BF16 : ACT_F16;
-    return make_float4(widen_act(w.x & 0xffff, t), widen_act(w.x >> 16, t), widen_act(w.y & 0xffff, t), widen_act(w.y >> 16, t));
+namespace pa {
+
+using namespace pipe;
+
+constexpr int KEYS = PAGED_SMALL_KEYS, ROWS = PAGED_SMALL_ROWS;
+constexpr int WARPS = 4, THREADS = 32 * (WARPS + 1);  // and the producer
+constexpr int CHUNK = 32, PITCH = 40;                 // columns of the accumulators that meet in shared memory at a time; a pitch without bank conflicts
+constexpr uint32_t SPIN_LIMIT = 1u << 19;            // a wait gives up after some two seconds
+
+template <int DP> struct Cfg {
+    static constexpr int HALVES = DP / 64;                  // a copied row is 64 elements wide: the width of a 128-byte swizzled row
+    static constexpr int PART = KEYS * 128;                 // bytes of one half of a step's keys (or values)
+    static constexpr int STAGE = 2 * HALVES * PART;
+    static constexpr int STAGES = 3 * 128 / DP;
+    static constexpr int SMEM = STAGES * STAGE + WARPS * ROWS * PITCH * 4 + 2 * WARPS * ROWS * 4 + 16 * STAGES + 16 + 1024;
+};
+
+template <bool BF16> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); }
+
+// Where a CTA is in the sequence of steps
+struct Walk {
+    uint32_t r, head, tile, tiles, n, kv, q0;
+    PagedTile t;
+};
+__device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
+    w.q0 = p.plan[p.l.q_start + w.r];
+    w.n = p.plan[p.l.q_start + w.r + 1] - w.q0;
+    w.kv = p.plan[p.l.kv_len + w.r];
+    w.tiles = paged_tiles(p.s, w.n, ROWS);
+}
+__device__ __forceinline__ void load_tile(const PagedAttnArgs &p, Walk &w) { w.t = paged_tile(p.s, w.n, w.kv, w.tile, ROWS, KEYS); }
+__device__ __forceinline__ void next_tile(const PagedAttnArgs &p, Walk &w) {
+    if (++w.tile == w.tiles) {
+        w.tile = 0;
+        if (++w.head == p.s.hkv) {
+            w.head = 0;
+            do {
+                w.r++;
+                load_request(p, w);
+            } while (w.n == 0 || !paged_is_small(p.s, w.n));
+        }
+    }
+    load_tile(p, w);
 }
 
-__global__ void __launch_bounds__(256) paged_attn_simple_kernel(PagedAttnArgs p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const PagedShape &s = p.s;
-    if (p.plan[PLAN_STAMP] != p.stamp) {
-        if (threadIdx.x == 0 && blockIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
+__device__ __forceinline__ void store_half4(unsigned short *row, uint32_t col, uint32_t d, float4 v, bool bf16, bool vec) {
+    if (vec && col + 4 <= d) {
+        *(uint2 *)(row + col) = bf16 ? make_uint2(pack<true>(v.x, v.y), pack<true>(v.z, v.w)) : make_uint2(pack<false>(v.x, v.y), pack<false>(v.z, v.w));
         return;
     }
-    const uint32_t lane = threadIdx.x & 31, tokens = p.plan[PLAN_TOKENS];
-    const bool has = 4 * lane < s.d;
-    for (uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < (uint64_t)tokens * s.hq; w += (uint64_t)gridDim.x * 8) {
-        const uint32_t t = (uint32_t)(w / s.hq), h = (uint32_t)(w % s.hq), kvh = h / s.g;
-        uint32_t r = 0, top = s.requests;
-        while (top - r > 1) {
-            const uint32_t mid = (r + top) >> 1;
-            if (p.plan[p.l.q_start + mid] <= t) r = mid;
-            else top = mid;
-        }
-        const uint32_t q0 = p.plan[p.l.q_start + r], n = p.plan[p.l.q_start + r + 1] - q0, kv = p.plan[p.l.kv_len + r];
-        const uint32_t hi = paged_hi(s, n, kv, t - q0), lo = paged_lo(s, hi);
-        const unsigned short *qrow = (const unsigned short *)p.q + p.qv.off + (uint64_t)t * p.qv.token + (uint64_t)h * p.qv.head;
-        const int at = s.bf16 ? ACT_BF16 : ACT_F16;
-        float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o = q;
-        if (has) q = make_float4(load_act(qrow, 4 * lane, at), load_act(qrow, 4 * lane + 1, at), load_act(qrow, 4 * lane + 2, at), load_act(qrow, 4 * lane + 3, at));
-        float m = -INFINITY, l = 0.0f;
-        bool bad = false;
-        for (uint32_t j = lo; j < hi; j++) {
-            const int32_t page = p.table[(size_t)r * s.max_blocks + j / s.page];
-            const bool ok = page >= 0 && (uint32_t)page < s.pages;
-            bad |= !ok;
-            const size_t at_row = (((size_t)(ok ? page : 0) * s.hkv + kvh) * s.page + j % s.page) * s.d;
-            float4 k = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = k;
-            if (ok && has) k = load_half4((const unsigned short *)p.k_cache + at_row, 4 * lane, s.bf16), v = load_half4((const unsigned short *)p.v_cache + at_row, 4 * lane, s.bf16);
-            float x = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
+    const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-            x *= s.scale;
-            const float top_m = fmaxf(m, x), base = top_m == -INFINITY ? 0.0f : top_m, keep = expf(m - base), e = expf(x - base);
-            m = top_m;
-            l = fmaf(l, keep, e);
-            o = make_float4(fmaf(o.x, keep, e * v.x), fmaf(o.y, keep, e * v.y), fmaf(o.z, keep, e * v.z), fmaf(o.w, keep, e * v.w));
-        }
-        if (bad && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)t * p.ov.token + (uint64_t)h * p.ov.head;
-        if (has) {
-            const float f[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-            for (int i = 0; i < 4; i++) {
-                if (s.bf16) ((__nv_bfloat16 *)orow)[4 * lane + i] = __float2bfloat16_rn(f[i]);
-                else ((__half *)orow)[4 * lane + i] = __float2half_rn(f[i]);
-            }
-        }
-        if (p.lse && lane == 0) p.lse[(size_t)t * s.hq + h] = l > 0.0f || l != l ? m + logf(l) : -INFINITY;
-    }
+    for (uint32_t i = 0; i < 4; i++)
+        if (col + i < d) row[col + i] = (unsigned short)(bf16 ? pack<true>(f[i], 0.0f) : pack<false>(f[i], 0.0f));
 }
 
-uint32_t paged_attn_small_ctas(int sm_count) { return (uint32_t)sm_count; }
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PagedAttnArgs p) {
+    using C = Cfg<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((0u - s32(smem_raw)) & 1023u);
+    float *meet = (float *)(smem + C::STAGES * C::STAGE);                  // [warp][row][PITCH]
+    float *meet_m = meet + WARPS * ROWS * PITCH, *meet_l = meet_m + WARPS * ROWS;
+    uint64_t *full = (uint64_t *)(meet_l + WARPS * ROWS), *empty = full + C::STAGES;
+    volatile uint32_t *is_last = (volatile uint32_t *)(empty + C::STAGES);
+    const PagedShape &s = p.s;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, WARPS);
+        }
+        mbar_fence_init();
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (p.plan[PLAN_STAMP] != p.stamp) {
+        if (threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
+        return;
+    }
+    const uint32_t units = p.plan[PLAN_UNITS_SMALL], ctas = p.plan[PLAN_CTAS_SMALL], b = blockIdx.x;
+    if (b >= ctas) return;
+    const uint4 at = ((const uint4 *)(p.plan + p.l.start_small))[b];
+    const uint32_t u0 = paged_span(units, ctas, b), u1 = paged_span(units, ctas, b + 1);
+    Walk w;
+    w.r = at.x, w.head = at.y, w.tile = at.z;
+    load_request(p, w);
+    load_tile(p, w);
+    uint32_t step = at.w;  // of the tile
+    bool healthy = true;
+
+    if (warp == WARPS) {
+        // ---------------- producer: lane i copies one part of a page, half of the keys or values
+        const uint32_t box = s.page < KEYS ? s.page : KEYS, boxes = KEYS / box;  // rows of a copy, copies of a step
+        const uint32_t mine = lane % (boxes * C::HALVES), which = lane / (boxes * C::HALVES);  // 0: keys, 1: values
+        const uint32_t half = mine / boxes, part = mine % boxes;
+        const bool copies = which < 2;
+        const int outside = (int)(s.pages * s.hkv * s.page);  // a row behind the cache: such a copy is filled with zeros
+        uint32_t stage = 0, ph = 1;
+        bool bad = false;
+        for (uint32_t u = u0; u < u1; u++) {
+            const uint32_t key = (w.t.first + step) * KEYS + part * box, block = key / s.page;
+            int row = outside;
+            if (copies && key < w.t.hi) {
+                const int32_t page = p.table[(size_t)w.r * s.max_blocks + block];
+                if (page >= 0 && (uint32_t)page < s.pages) row = (int)(((uint32_t)page * s.hkv + w.head) * s.page + key % s.page);
+                else if ((block + 1) * s.page > paged_lo(s, paged_hi(s, w.n, w.kv, w.tile * ROWS / s.g))) bad = true;
+            }
+            if (++step == w.t.steps && u + 1 < u1) {
+                step = 0;
+                next_tile(p, w);
+            }
+            if (healthy) healthy = __all_sync(0xffffffffu, mbar_wait(empty + stage, ph, SPIN_LIMIT));
+            if (!healthy) break;
+            if (lane == 0) mbar_expect_tx(full + stage, C::STAGE);
+            __syncwarp();
+            uint8_t *to = smem + stage * C::STAGE + (which * C::HALVES + half) * C::PART + part * box * 128;
+            if (copies) tma_load_2d(to, which ? &map_v : &map_k, 64 * (int)half, row, full + stage);
+            if (++stage == C::STAGES) stage = 0, ph ^= 1;
+        }
+        if (bad && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
+        // the copies in flight have to land before the CTA leaves
+        for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < stage ? ph ^ 1 : ph, SPIN_LIMIT);
+        if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
+        return;
+    }
+
+    // ---------------- four warps, 16 keys of each step
+    const uint32_t quad = lane >> 2, pair = 2 * (lane & 3);
+    const float c = s.scale * 1.4426950408889634f;  // exponentials to base 2
+    const bool q2 = ((uintptr_t)p.q & 3) == 0 && ((p.qv.off | p.qv.head | p.qv.token) & 1) == 0;
+    const bool out4 = ((uintptr_t)p.out & 7) == 0 && ((p.ov.off | p.ov.head | p.ov.token) & 3) == 0;
+    const uint32_t tid = threadIdx.x, my_row = tid / 8, my_col = 4 * (tid % 8);  // of the results
+    // ldmatrix: lane i gives row (i & 7) of matrix i / 8; keys: matrices (keys 0-7, 8-15) of two chunks of 8 elements; values the same, transposed
+    const uint32_t k_row = warp * 16 + (lane & 7) + ((lane >> 4) << 3), k_chunk = (lane >> 3) & 1;
+    const uint32_t v_row = warp * 16 + (lane & 15), v_chunk = lane >> 4;
+    uint32_t stage = 0, ph = 0;
+    uint32_t u = u0;
+    while (u < u1) {
+        const uint32_t steps = min(w.t.steps - step, u1 - u);  // of this tile in this span
+        // rows and what they see
+        uint32_t lo[2], hi[2];
+        uint32_t aq[DP / 16][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t row = w.tile * ROWS + quad + 8 * h, token = row / s.g;
+            const bool real = token < w.n;
+            hi[h] = real ? paged_hi(s, w.n, w.kv, token) : 0u;
+            lo[h] = paged_lo(s, hi[h]);
+            const unsigned short *q = (const unsigned short *)p.q + p.qv.off + (uint64_t)(w.q0 + token) * p.qv.token + (uint64_t)(w.head * s.g + row % s.g) * p.qv.head;
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t col = 16 * ks + 8 * j + pair;
+                    uint32_t x = 0;
+                    if (real && col < s.d) x = q2 ? *(const uint32_t *)(q + col) : (uint32_t)q[col] | ((uint32_t)q[col + 1] << 16);
+                    aq[ks][2 * j + h] = x;
+                }
+        }
+        const uint32_t tile_lo = paged_lo(s, paged_hi(s, w.n, w.kv, w.tile * ROWS / s.g));
+        float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (uint32_t i = 0; i < steps; i++) {
+            if (healthy) healthy = __all_sync(0xffffffffu, mbar_wait(full + stage, ph, SPIN_LIMIT));
+            if (!healthy) break;
+            const uint32_t kb = s32(smem + stage * C::STAGE), vb = kb + C::HALVES * C::PART;
+            float sc[2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ks++) {
+                uint32_t f[4];
+                ldmatrix4<false>(f, kb + (ks / 4) * C::PART + k_row * 128 + (((2 * (ks & 3) + k_chunk) ^ (k_row & 7)) << 4));
+                mma16816<BF16>(sc[0], aq[ks], f[0], f[1]);
+                mma16816<BF16>(sc[1], aq[ks], f[2], f[3]);
+            }
+            const uint32_t key0 = (w.t.first + step + i) * KEYS + warp * 16;
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t key = key0 + 8 * t + pair + (e & 1);
+                    sc[t][e] = key >= lo[e >> 1] && key < hi[e >> 1] ? sc[t][e] * c : -INFINITY;
+                    top[e >> 1] = fmaxf(top[e >> 1], sc[t][e]);
+                }
+            float base[2], keep[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                const float mn = fmaxf(m[h], top[h]);
+                base[h] = mn == -INFINITY ? 0.0f : mn;
+                keep[h] = exp2_fast(m[h] - base[h]);
+                if (mn == m[h]) keep[h] = 1.0f;
+                m[h] = mn;
+                l[h] *= keep[h];
+            }
+            if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++) o[n][0] *= keep[0], o[n][1] *= keep[0], o[n][2] *= keep[1], o[n][3] *= keep[1];
+            }
+            uint32_t ap[4];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float x = exp2_fast(sc[t][2 * h] - base[h]), y = exp2_fast(sc[t][2 * h + 1] - base[h]);
+                    l[h] += x + y;
+                    ap[2 * t + h] = pack<BF16>(x, y);
+                }
+            // values of keys outside the tile's are whatever the page holds: 0 times that must be 0
+            uint32_t keep_v[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const uint32_t key = key0 + 8 * t + pair;
+                keep_v[t] = (key >= tile_lo && key < w.t.hi ? 0xffffu : 0u) | (key + 1 >= tile_lo && key + 1 < w.t.hi ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 16; n++) {
+                uint32_t f[4];
+                ldmatrix4<true>(f, vb + (n / 4) * C::PART + v_row * 128 + (((2 * (n & 3) + v_chunk) ^ (v_row & 7)) << 4));
+                mma16816<BF16>(o[2 * n], ap, f[0] & keep_v[0], f[1] & keep_v[1]);
+                mma16816<BF16>(o[2 * n + 1], ap, f[2] & keep_v[0], f[3] & keep_v[1]);
+            }
+            // (behind the products: a load may be carried out late, and would read what the next copy brings)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + stage);
+            if (++stage == C::STAGES) stage = 0, ph ^= 1;
+        }
+        // ---- the four warps' results meet
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        }
+        if ((lane & 3) == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) meet_m[warp * ROWS + quad + 8 * h] = m[h], meet_l[warp * ROWS + quad + 8 * h] = l[h];
+        }
+        warps_sync();
+        float f[WARPS], big = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WARPS; k++) big = fmaxf(big, meet_m[k * ROWS + my_row]);
+        const float base = big == -INFINITY ? 0.0f : big;
+#pragma unroll
+        for (int k = 0; k < WARPS; k++) {
+            f[k] = exp2_fast(meet_m[k * ROWS + my_row] - base);
+            sum = fmaf(meet_l[k * ROWS + my_row], f[k], sum);
+        }
+        const bool whole = step == 0 && steps == w.t.steps;
+        const uint32_t i0 = u - step, i1 = i0 + w.t.steps;  // the tile's place in the sequence
+        float *part = (float *)((uint8_t *)p.plan + p.l.part_small);
+        const uint32_t pf = ROWS * (DP + 2);
+        const uint32_t slot = 2 * b + (i0 < u0 ? 0 : 1);
+        const uint32_t row = w.tile * ROWS + my_row, token = row / s.g, qh = w.head * s.g + row % s.g;
+        const bool real = token < w.n;
+        unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int ch = 0; ch < DP / CHUNK; ch++) {
+#pragma unroll
+            for (int n = 0; n < CHUNK / 8; n++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    *(float2 *)(meet + (warp * ROWS + quad + 8 * h) * PITCH + 8 * n + pair) = make_float2(o[ch * (CHUNK / 8) + n][2 * h], o[ch * (CHUNK / 8) + n][2 * h + 1]);
+            warps_sync();
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < WARPS; k++) {
+                const float4 x = *(const float4 *)(meet + (k * ROWS + my_row) * PITCH + my_col);
+                v = make_float4(fmaf(x.x, f[k], v.x), fmaf(x.y, f[k], v.y), fmaf(x.z, f[k], v.z), fmaf(x.w, f[k], v.w));
+            }
+            if (!whole) *(float4 *)(part + (size_t)slot * pf + my_row * DP + ch * CHUNK + my_col) = v;
+            else if (real) store_half4(orow, ch * CHUNK + my_col, s.d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), BF16, out4);
+            warps_sync();
+        }
+        auto finish_lse = [&](float mm, float ss) {
+            if (p.lse && real && tid % 8 == 0) p.lse[(size_t)(w.q0 + token) * s.hq + qh] = ss == 0.0f ? -INFINITY : (mm + log2f(ss)) * 0.6931471805599453f;
+        };
+        if (whole) {
+            finish_lse(big, sum);
+        } else {
+            if (tid % 8 == 0) {
+                part[(size_t)slot * pf + ROWS * DP + my_row] = big;
+                part[(size_t)slot * pf + ROWS * (DP + 1) + my_row] = sum;
+            }
+            const uint32_t first = paged_holder(units, ctas, i0), last = paged_holder(units, ctas, i1 - 1);
+            warps_sync();
+            if (tid == 0) {
+                __threadfence();
+                uint32_t *count = p.plan + p.l.count_small + first;
+                const bool end = atomicAdd(count, 1u) == last - first;
+                if (end) *count = 0;  // for the next launch
+                __threadfence();
+                *is_last = end;
+            }
+            warps_sync();
+            if (*is_last) {
+                float mm = -INFINITY, ss = 0.0f;
+                float4 v[DP / CHUNK];
+                for (uint32_t k = first; k <= last; k++) {
+                    const float *src = part + (size_t)(2 * k + (k == first ? 1 : 0)) * pf;
+                    mm = fmaxf(mm, __ldcg(src + ROWS * DP + my_row));
+                }
+                const float mb = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+                for (int ch = 0; ch < DP / CHUNK; ch++) v[ch] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                for (uint32_t k = first; k <= last; k++) {
+                    // (a tile's first piece is the end of its CTA's span, the others are the beginning of theirs)
+                    const float *src = part + (size_t)(2 * k + (k == first ? 1 : 0)) * pf;
+                    const float e = exp2_fast(__ldcg(src + ROWS * DP + my_row) - mb);
+                    ss = fmaf(__ldcg(src + ROWS * (DP + 1) + my_row), e, ss);
+#pragma unroll
+                    for (int ch = 0; ch < DP / CHUNK; ch++) {
+                        const float4 x = __ldcg((const float4 *)(src + my_row * DP + ch * CHUNK + my_col));
+                        v[ch] = make_float4(fmaf(x.x, e, v[ch].x), fmaf(x.y, e, v[ch].y), fmaf(x.z, e, v[ch].z), fmaf(x.w, e, v[ch].w));
+                    }
+                }
+                const float r = ss == 0.0f ? 0.0f : 1.0f / ss;
+#pragma unroll
+                for (int ch = 0; ch < DP / CHUNK; ch++)
+                    if (real) store_half4(orow, ch * CHUNK + my_col, s.d, make_float4(v[ch].x * r, v[ch].y * r, v[ch].z * r, v[ch].w * r), BF16, out4);
+                finish_lse(mm, ss);
+            }
+        }
+        u += steps;
+        step = 0;
+        if (u < u1) next_tile(p, w);
+    }
+    if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+}  // namespace pa
+
+// A cache as a matrix [pages * heads * page][d]; boxes of 64 elements (those behind d are filled with zeros) by `rows` rows.
+bool paged_cache_map(const PagedShape &s, const void *cache, uint32_t rows, CUtensorMap &map) {
+    static const pa::EncodeTiledFn fn = [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (pa::EncodeTiledFn)ptr : nullptr;
+    }();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {s.d, (cuuint64_t)s.pages * s.hkv * s.page}, strides[1] = {(cuuint64_t)s.d * 2};
+    const cuuint32_t box[2] = {64, rows}, ones[2] = {1, 1};
+    return fn(&map, s.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void *)cache, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+uint32_t paged_attn_small_ctas(int sm_count) { return 2 * (uint32_t)sm_count; }
 uint32_t paged_attn_large_ctas(int sm_count) { return (uint32_t)sm_count; }
 
-cudaError_t launch_paged_attn_small(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
-    const uint64_t warps = (uint64_t)a.s.tokens * a.s.hq, want = (warps + 7) / 8, cap = (uint64_t)sm_count * 64;
+template <int DP, bool BF16> static cudaError_t small_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sm_count, bool pdl, cudaStream_t stream) {
+    auto *kernel = pa::paged_attn_small_kernel<DP, BF16>;
+    constexpr int SMEM = pa::Cfg<DP>::SMEM;
+    static std::once_flag once[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::call_once(once[dev & 63], [&] { e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3((unsigned)(want < cap ? want : cap));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(paged_attn_small_ctas(sm_count));
+    cfg.blockDim = dim3(pa::THREADS);
+    cfg.dynamicSmemBytes = SMEM;
     cfg.stream = stream;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, paged_attn_simple_kernel, a);
+    return cudaLaunchKernelEx(&cfg, kernel, mk, mv, a);
+}
+
+cudaError_t launch_paged_attn_small(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
+    CUtensorMap mk, mv;
+    const uint32_t rows = a.s.page < PAGED_SMALL_KEYS ? a.s.page : PAGED_SMALL_KEYS;
+    if (!paged_cache_map(a.s, a.k_cache, rows, mk) || !paged_cache_map(a.s, a.v_cache, rows, mv)) return cudaErrorInvalidValue;
+    if (a.s.d > 64) return a.s.bf16 ? small_launch<128, true>(a, mk, mv, sm_count, pdl, stream) : small_launch<128, false>(a, mk, mv, sm_count, pdl, stream);
+    return a.s.bf16 ? small_launch<64, true>(a, mk, mv, sm_count, pdl, stream) : small_launch<64, false>(a, mk, mv, sm_count, pdl, stream);
 }
 cudaError_t launch_paged_attn_large(const PagedAttnArgs &, int, bool, cudaStream_t) { return cudaSuccess; }
 
