@@ -41,6 +41,7 @@ SOURCES = {
     "moe.cu": [],
     "paged.cu": [],
     "paged_attn.cu": [],
+    "paged_attn_tc.cu": [],
     "tp_allreduce.cu": [],
     "backend.cc": ["-x", "cu"],
 }

@@ -392,7 +392,7 @@ cudaError_t launch_silu_mul(const float *gate, const float *up, float *out, uint
 // ---- paged.cu, paged_attn.cu, paged_attn_tc.cu: the paged key/value cache and the attention over it
 constexpr uint32_t PAGED_FULL = 0, PAGED_CAUSAL = 1, PAGED_CROSS = 2;  // LAPID_B200_MASK_*
 constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile and step of the kernel for few rows
-constexpr uint32_t PAGED_SMALL_LIMIT = 1u << 30;                             // requests of at most so many packed rows go to it
+constexpr uint32_t PAGED_SMALL_LIMIT = 16;                             // requests of at most so many packed rows go to it
 constexpr uint32_t PAGED_LARGE_ROWS = 256, PAGED_LARGE_KEYS = 128;     // tile and step of the tensor-memory kernel
 constexpr uint32_t PAGED_SMALL_MIN = 4, PAGED_LARGE_MIN = 2;             // fewest steps worth a CTA of its own
 constexpr uint32_t PAGED_MAX_SMS = 160;

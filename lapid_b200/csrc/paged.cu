@@ -39,7 +39,7 @@ PagedPlanLayout paged_plan_layout(const PagedShape &s) {
     l.start_small = take(4 * cs);
     l.start_large = take(4 * cl);
     l.count_small = take(cs);
-    l.count_large = take(cl);
+    l.count_large = take(2 * cl);  // (for each of a tile's two halves)
     l.part_small = (size_t)w * 4;
     l.part_large = l.part_small + (size_t)cs * 2 * paged_part_floats(s, PAGED_SMALL_ROWS) * 4;
     l.bytes = l.part_large + (size_t)cl * 2 * paged_part_floats(s, PAGED_LARGE_ROWS) * 4;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
         *a.used = (int32_t)taken;
     }
     for (uint32_t b = tid; b < a.ctas_small; b += PLAN_THREADS) a.plan[a.l.count_small + b] = 0;
-    for (uint32_t b = tid; b < a.ctas_large; b += PLAN_THREADS) a.plan[a.l.count_large + b] = 0;
+    for (uint32_t b = tid; b < 2 * a.ctas_large; b += PLAN_THREADS) a.plan[a.l.count_large + b] = 0;
     __syncthreads();
     if (small) cut_units(a, small, cs, a.plan + a.l.units_small, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS);
     if (large) cut_units(a, large, cl, a.plan + a.l.units_large, a.plan + a.l.start_large, PAGED_LARGE_ROWS, PAGED_LARGE_KEYS);

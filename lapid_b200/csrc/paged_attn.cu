@@ -402,7 +402,6 @@ bool paged_cache_map(const PagedShape &s, const void *cache, uint32_t rows, CUte
 }
 
 uint32_t paged_attn_small_ctas(int sm_count) { return 2 * (uint32_t)sm_count; }
-uint32_t paged_attn_large_ctas(int sm_count) { return (uint32_t)sm_count; }
 
 template <int DP, bool BF16> static cudaError_t small_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sm_count, bool pdl, cudaStream_t stream) {
     auto *kernel = pa::paged_attn_small_kernel<DP, BF16>;
@@ -433,6 +432,5 @@ cudaError_t launch_paged_attn_small(const PagedAttnArgs &a, int sm_count, bool p
     if (a.s.d > 64) return a.s.bf16 ? small_launch<128, true>(a, mk, mv, sm_count, pdl, stream) : small_launch<128, false>(a, mk, mv, sm_count, pdl, stream);
     return a.s.bf16 ? small_launch<64, true>(a, mk, mv, sm_count, pdl, stream) : small_launch<64, false>(a, mk, mv, sm_count, pdl, stream);
 }
-cudaError_t launch_paged_attn_large(const PagedAttnArgs &, int, bool, cudaStream_t) { return cudaSuccess; }
 
 }  // namespace lb
