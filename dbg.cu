@@ -1,0 +1,682 @@
+// Attention over the pages for requests of many rows: whole prompts and chunks of them, on the 5th-generation tensor cores.
+//
+//   S = Q K^T;  m = max(scale S), P = exp(scale S - m), l = sum P;  O = sum over the steps of P V;  out = O / l
+//
+// in one pass over the keys a request's rows may see, 128 at a time. A CTA holds two tiles of up to 128 packed rows (token, query head of the group),
+// each with its scores S (f32), its weights P (16 bits, in the columns of the scores they come from) and its
+// accumulator O (f32) in tensor memory, so that one tile's products run while the other's exponentials are formed:
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread is a row. S comes from tensor memory into registers 64 keys at a time, P goes back: the A operand of
+//              the second product may lie there, and that product starts on the first 64 keys while the others' weights are formed. The weights are
+//              taken relative to the last maximum that was looked up, and the maximum of the new scores is formed beside them: only where one
+//              is more than 2^8 times larger are the weights formed again and O and l rescaled (until then the weights are at most 2^8 and
+//              nothing is lost; l and O carry the same factor). Some exponentials are polynomials: see exp2_poly.
+//   warp 8     allocates tensor memory; one lane issues `tcgen05.mma`: S = Q K^T (both from shared memory) and O += P V (V as it lies in the
+//              pages: its rows are the keys, so the descriptor takes it as the transposed operand)
+//   warp 9     copies the pages' keys and values into a ring by TMA
+//   warps 10-11 bring the next tile's rows of Q: one box of whole tokens by TMA, or 16 bytes (2, where they are not aligned) a thread
+// The steps of all requests, heads and tiles are one sequence cut into equal spans, one a CTA (paged.cuh): causal tiles of any length keep every SM
+// busy, few rows over many keys spread over all. A tile that a span's end cuts is left in the plan buffer by each of its CTAs; the one
+// that comes last adds the pieces up in the order of the keys.
+//
+// Every mbarrier wait is bounded: one that gives up sets a bit in the status word, the roles fall through to the end, tensor memory is released.
+#include <cuda.h>
+#include <cstdio>
+#include <cuda_bf16.h>
+
+#include "/root/repo/lapid_b200/csrc/common.cuh"
+#include "/root/repo/lapid_b200/csrc/paged.cuh"
+#include "/root/repo/lapid_b200/csrc/pipe.cuh"
+
+namespace lb {
+
+bool paged_cache_map(const PagedShape &s, const void *cache, uint32_t rows, CUtensorMap &map);
+bool paged_q_map(const PagedAttnArgs &a, CUtensorMap &map);
+
+namespace pt {
+
+using pipe::add2;
+using pipe::fma2;
+using pipe::mbar_arrive;
+using pipe::mbar_expect_tx;
+using pipe::mbar_fence_init;
+using pipe::mbar_init;
+using pipe::pack2;
+using pipe::s32;
+using pipe::tma_load_2d;
+using pipe::unpack2;
+
+constexpr int KEYS = PAGED_LARGE_KEYS, ROWS = PAGED_LARGE_ROWS, TILE = 128;
+constexpr int MMA_WARP = 8, LOAD_WARP = 9, Q_WARP = 10, THREADS = 384;
+constexpr int HALF = 128 * 128;  // bytes of 128 rows of 64 elements
+constexpr int SUB = 64;          // keys whose weights are formed and handed on together
+// Registers: 384 x 168 at launch = 256 x 208 + 128 x 88
+constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88;
+constexpr float LAZY = 8.0f;
+constexpr int POLY = 2;  // pairs of every eight whose exponentials are polynomials
+constexpr uint32_t WAIT_NS = 8000, SPIN_LIMIT = 1u << 17;  // a wait gives up after some two seconds
+
+template <int DP> struct Cfg {
+    static constexpr int HALVES = DP / 64;
+    static constexpr int STAGE = HALVES * HALF;  // keys or values of a step
+    static constexpr int Q_BYTES = 2 * HALVES * HALF;
+    static constexpr int STAGES = (224 * 1024 - Q_BYTES) / STAGE;
+    static constexpr int SMEM = Q_BYTES + STAGES * STAGE + 512 + 1024;
+    static constexpr int O_COL = 256;  // tensor memory: S of tile t at 128 t, O at O_COL + DP t
+};
+
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
+    for (uint32_t spin = 0; spin < SPIN_LIMIT; spin++) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(s32(bar)), "r"(parity), "r"(WAIT_NS)
+                     : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+__device__ __noinline__ void gave(int line, uint32_t parity){ printf("gave up: line %d parity %u block %d warp %d lane %d\n", line, parity, blockIdx.x, threadIdx.x>>5, threadIdx.x&31);}
+__device__ __forceinline__ bool warp_wait_dbg(int line, uint64_t*bar, uint32_t parity){ bool ok=__all_sync(0xffffffffu, mbar_wait(bar, parity)); if(!ok && (threadIdx.x&31)==0) gave(line,parity); return ok; }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+// Operands in shared memory, 128-byte swizzle. K-major: rows of 128 bytes, 8-row groups 1024 bytes apart. Transposed (rows are the K dimension): 8-row
+// groups 1024 bytes apart, the next 64 elements of a row one HALF further.
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_t(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(HALF >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t *r, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Behind a wait for loads from tensor memory: nothing may use the registers before it.
+template <int N> __device__ __forceinline__ void loaded(uint32_t (&x)[N]) {
+    ld_wait();
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(x[i]));
+}
+// max.NaN: a NaN among the scores stays
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a minimax polynomial in f (found by Remez's exchange; relative error 7.5e-5 at
+// degree 3, 2.6e-6 at degree 4: below half a unit of the weights' type, 2^-9 or 2^-12), n added to the exponent. For x <= 100; below -125 it stays 2^-125. The special-function unit forms
+// 16 exponentials a cycle on an SM, and 128 x 128 of them take as long as the two products of 128 x 128 x 128: what it is relieved of here costs
+// five issue slots an element that the schedulers have.
+template <int DEGREE> __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
+    float a, b;
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
+    const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));  // 1.5 2^23: n in the low bits
+    const uint64_t f = add2(x, pipe::mul2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f)));
+    uint64_t y;
+    if constexpr (DEGREE == 3) {
+        y = fma2(f, pack2(0.0551716685f, 0.0551716685f), pack2(0.242611125f, 0.242611125f));
+        y = fma2(f, y, pack2(0.693260968f, 0.693260968f));
+        y = fma2(f, y, pack2(0.999928057f, 0.999928057f));
+    } else {
+        y = fma2(f, pack2(0.00957010221f, 0.00957010221f), pack2(0.0559178591f, 0.0559178591f));
+        y = fma2(f, y, pack2(0.240247443f, 0.240247443f));
+        y = fma2(f, y, pack2(0.693121791f, 0.693121791f));
+        y = fma2(f, y, pack2(0.999999285f, 0.999999285f));
+    }
+    float y0, y1, t0, t1;
+    unpack2(y, y0, y1);
+    unpack2(t, t0, t1);
+    r0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+    r1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
+}
+// The weights of 64 scores, their sums (added to l) and the largest score. POLY of every 8 pairs are polynomials.
+template <bool BF16, int POLY> __device__ __forceinline__ float weights(const uint32_t (&x)[SUB], uint64_t c2, uint64_t b2, uint32_t (&w)[SUB / 2], uint64_t &l0, uint64_t &l1) {
+    float top[4];
+#pragma unroll
+    for (int i = 0; i < SUB / 2; i++) {
+        const float x0 = __uint_as_float(x[2 * i]), x1 = __uint_as_float(x[2 * i + 1]);
+        if (i < 4) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top[i]) : "f"(x0), "f"(x1));
+        else top[i & 3] = max3(top[i & 3], x0, x1);
+        const uint64_t y = fma2(pack2(x0, x1), c2, b2);
+        float e0, e1;
+        if ((i & 7) < POLY) {
+            exp2_poly<BF16 ? 3 : 4>(y, e0, e1);
+        } else {
+            unpack2(y, e0, e1);
+            e0 = exp2_fast(e0), e1 = exp2_fast(e1);
+        }
+        if (i & 1) l1 = add2(l1, pack2(e0, e1));
+        else l0 = add2(l0, pack2(e0, e1));
+        w[i] = pack<BF16>(e0, e1);
+    }
+    return max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+}
+
+struct Walk {
+    uint32_t r, head, tile, tiles, n, kv, q0;
+    PagedTile t;
+    uint32_t u, u1, step, steps;  // place in the sequence, end of the span; first step of the tile here, and how many
+    bool two;                     // the second tile of 128 has rows
+};
+__device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
+    w.q0 = p.plan[p.l.q_start + w.r];
+    w.n = p.plan[p.l.q_start + w.r + 1] - w.q0;
+    w.kv = p.plan[p.l.kv_len + w.r];
+    w.tiles = paged_tiles(p.s, w.n, paged_large_rows(p.s));
+}
+__device__ __forceinline__ void load_tile(const PagedAttnArgs &p, Walk &w) {
+    w.t = paged_tile(p.s, w.n, w.kv, w.tile, paged_large_rows(p.s), KEYS);
+    w.two = (2 * w.tile + 1) * p.s.tt < w.n;
+    w.steps = min(w.t.steps - w.step, w.u1 - w.u);
+}
+// The next piece of work of the span; false: none
+__device__ __forceinline__ bool next_piece(const PagedAttnArgs &p, Walk &w) {
+    w.u += w.steps;
+    if (w.u >= w.u1) return false;
+    w.step = 0;
+    if (++w.tile == w.tiles) {
+        w.tile = 0;
+        if (++w.head == p.s.hkv) {
+            w.head = 0;
+            do {
+                w.r++;
+                load_request(p, w);
+            } while (w.n == 0 || paged_is_small(p.s, w.n));
+        }
+    }
+    load_tile(p, w);
+    return true;
+}
+__device__ __forceinline__ uint32_t tile_low(const PagedAttnArgs &p, const Walk &w) { return paged_lo(p.s, paged_hi(p.s, w.n, w.kv, 2 * w.tile * p.s.tt)); }
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(s32(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z),
+                 "r"(s32(bar))
+                 : "memory");
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q, PagedAttnArgs p, bool q_boxes) {
+    using C = Cfg<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((0u - s32(smem_raw)) & 1023u);
+    uint8_t *ring = smem + C::Q_BYTES;
+    uint64_t *full = (uint64_t *)(ring + C::STAGES * C::STAGE), *empty = full + C::STAGES;
+    uint64_t *q_full = empty + C::STAGES, *q_empty = q_full + 2, *s_full = q_empty + 2, *p_full = s_full + 2, *o_full = p_full + 2;
+    uint32_t *tmem_slot = (uint32_t *)(o_full + 2);
+    volatile uint32_t *is_last = tmem_slot + 1;
+    const PagedShape &s = p.s;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int t = 0; t < 2; t++) {
+            mbar_init(q_full + t, q_boxes ? 1 : 2);
+            mbar_init(q_empty + t, 1);
+            mbar_init(s_full + t, 1);
+            mbar_init(p_full + t, 4);
+            mbar_init(o_full + t, 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t b = blockIdx.x;
+    const PagedStart at = paged_load_start(p.plan + p.l.start_large + b * (sizeof(PagedStart) / 4));
+    const bool stale = at.stamp != p.stamp;
+    if (stale && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
+    const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0;
+    bool work = !stale && at.u0 < at.u1, healthy = true;
+    Walk w{};
+    if (work) {
+        w.u = u0, w.u1 = at.u1, w.r = at.r, w.head = at.head, w.tile = at.tile, w.step = at.step, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
+        w.tiles = paged_tiles(s, w.n, paged_large_rows(s));
+        load_tile(p, w);
+    }
+
+    if (warp >= MMA_WARP) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
+        if (warp == MMA_WARP) {
+            // ---------------- products
+            // D f32, A and B f16 (0) or bf16 (1); S: both K-major, N = 128, A negated for a negative scale; O: B transposed, N = DP
+            constexpr uint32_t TYPE = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((uint32_t)(TILE >> 4) << 24);
+            const uint32_t idesc_s = TYPE | ((uint32_t)(KEYS >> 3) << 17) | (s.scale < 0.0f ? 1u << 13 : 0u);
+            constexpr uint32_t idesc_o = TYPE | ((uint32_t)(DP >> 3) << 17) | (1u << 16);
+            uint32_t st = 0, ph = 0;                    // ring
+            uint32_t piece[2] = {0, 0};                 // pieces of each tile so far
+            auto advance = [&]() {
+                if (++st == C::STAGES) st = 0, ph ^= 1;
+            };
+            auto scores = [&](int t, bool last_use, bool last_step) {
+                if (elect_one()) {
+                    const uint64_t a = desc_k(s32(smem) + t * C::HALVES * HALF), bk = desc_k(s32(ring) + st * C::STAGE);
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++) mma_ss(tmem + TILE * t, a + (i / 4) * (HALF >> 4) + 2 * (i & 3), bk + (i / 4) * (HALF >> 4) + 2 * (i & 3), idesc_s, i ? 1u : 0u);
+                    commit(s_full + t);
+                    if (last_step) commit(q_empty + t);
+                    if (last_use) commit(empty + st);
+                }
+                __syncwarp();
+            };
+            // the first scores of a piece
+            auto first_scores = [&](const Walk &x, int t) {
+                healthy = warp_wait_dbg(315, q_full + t, piece[t] & 1);
+                piece[t]++;
+                if (!healthy) return;
+                fence_after();
+                scores(t, t == (x.two ? 1 : 0), x.steps == 1);
+            };
+            if (work) {
+                healthy = warp_wait_dbg(322, full + st, ph);
+                for (int t = 0; t < (w.two ? 2 : 1) && healthy; t++) first_scores(w, t);
+                advance();
+            }
+            while (work && healthy) {
+                const int tiles = w.two ? 2 : 1;
+                const uint32_t low = tile_low(p, w);
+                Walk next = w;
+                const bool follows = next_piece(p, next);
+                for (uint32_t j = 0; j < w.steps && healthy; j++) {
+                    const uint32_t v_stage = st, v_phase = ph;
+                    advance();
+                    // the products that follow: the next step's scores, or the next piece's first
+                    const bool more = j + 1 < w.steps, any = more || follows;
+                    const int after = more ? tiles : follows ? (next.two ? 2 : 1) : 0;
+                    if (!(healthy = warp_wait_dbg(337, full + v_stage, v_phase))) break;
+                    // values of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0
+                    const uint32_t key0 = (w.t.first + w.step + j) * KEYS, lo = low > key0 ? min(low - key0, (uint32_t)KEYS) : 0u, hi = w.t.hi > key0 ? min(w.t.hi - key0, (uint32_t)KEYS) : 0u;
+                    if (lo > 0 || hi < KEYS) {
+                        for (uint32_t i = lane; i < KEYS * (DP / 8); i += 32) {
+                            const uint32_t key = i / (DP / 8), ch = i % (DP / 8);
+                            if (key < lo || key >= hi) *(uint4 *)(ring + v_stage * C::STAGE + (ch / 8) * HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    if (any && !(healthy = warp_wait_dbg(348, full + st, ph))) break;
+                    const uint64_t bv = desc_t(s32(ring) + v_stage * C::STAGE);
+                    for (int t = 0; t < 2 && healthy; t++) {
+                        if (t < tiles) {
+#pragma unroll
+                            for (int h = 0; h < KEYS / SUB; h++) {
+                                if (!(healthy = warp_wait_dbg(354, p_full + t, h))) break;
+                                fence_after();
+                                if (elect_one()) {
+#pragma unroll
+                                    for (int i = 0; i < SUB / 16; i++)
+                                        mma_ts(tmem + C::O_COL + DP * t, tmem + TILE * t + (SUB / 2) * h + 8 * i, bv + (h * (SUB / 16) + i) * (2048 >> 4), idesc_o, (j | h | i) ? 1u : 0u);
+                                    commit(o_full + t);
+                                    if (t == tiles - 1 && h == KEYS / SUB - 1) commit(empty + v_stage);
+                                }
+                                __syncwarp();
+                            }
+                            if (!healthy) break;
+                        }
+                        if (t < after) {
+                            if (more) scores(t, t == after - 1, j + 2 == w.steps);
+                            else first_scores(next, t);
+                        }
+                    }
+                    if (any) advance();
+                }
+                w = next;
+                work = follows;
+            }
+            if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
+        } else if (warp == LOAD_WARP) {
+            // ---------------- pages: lane i copies one part of a page, half of the keys or values; keys, then values of every step
+            const uint32_t box = min(s.page, (uint32_t)KEYS), boxes = KEYS / box;
+            const bool copies = lane < boxes * C::HALVES;
+            const uint32_t half = lane / boxes, part = lane % boxes;
+            const int outside = (int)(s.pages * s.hkv * s.page);  // a row behind the cache: such a copy is filled with zeros
+            uint32_t st = 0, ph = 1;
+            bool bad = false;
+            while (work && healthy) {
+                const uint32_t low = tile_low(p, w);
+                auto row_of = [&](uint32_t j) -> int {
+                    const uint32_t key = (w.t.first + w.step + j) * KEYS + part * box, block = key / s.page;
+                    if (!copies || key >= w.t.hi) return outside;
+                    const int32_t page = p.table[(size_t)w.r * s.max_blocks + block];
+                    if (page >= 0 && (uint32_t)page < s.pages) return (int)(((uint32_t)page * s.hkv + w.head) * s.page);
+                    if ((block + 1) * s.page > low) bad = true;
+                    return outside;
+                };
+                int row = row_of(0);
+                for (uint32_t j = 0; j < w.steps && healthy; j++) {
+                    const int now = row;
+                    if (j + 1 < w.steps) row = row_of(j + 1);
+                    for (int v = 0; v < 2; v++) {
+                        if (!(healthy = warp_wait_dbg(401, empty + st, ph))) break;
+                        if (lane == 0) mbar_expect_tx(full + st, C::STAGE);
+                        __syncwarp();
+                        if (copies) tma_load_2d(ring + st * C::STAGE + half * HALF + part * box * 128, v ? &map_v : &map_k, 64 * (int)half, now, full + st);
+                        if (++st == C::STAGES) st = 0, ph ^= 1;
+                    }
+                }
+                if (healthy) work = next_piece(p, w);
+            }
+            if (bad && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
+            // the copies in flight have to land before the CTA leaves
+            for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < st ? ph ^ 1 : ph);
+            if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
+        } else {
+            // ---------------- rows of Q, 16 bytes a thread and copy
+            const uint32_t tid = threadIdx.x - 32 * Q_WARP, tile_rows = s.tt * s.g;
+            const bool vec = ((uintptr_t)p.q & 15) == 0 && ((p.qv.off | p.qv.head | p.qv.token) & 7) == 0;
+            uint32_t piece[2] = {0, 0};
+            if (q_boxes && warp != Q_WARP) work = false;
+            while (work && healthy) {
+                for (int t = 0; t < (w.two ? 2 : 1) && healthy; t++) {
+                    if (piece[t] && !(healthy = warp_wait_dbg(422, q_empty + t, (piece[t] - 1) & 1))) break;
+                    piece[t]++;
+                    const uint32_t token0 = (2 * w.tile + t) * s.tt;
+                    uint8_t *const dst0 = smem + t * C::HALVES * HALF;
+                    if (q_boxes) {  // (tokens behind the request's are some other's, or zeros: such rows go nowhere)
+                        if (elect_one()) {
+                            mbar_expect_tx(q_full + t, C::HALVES * tile_rows * 128);
+                            for (int h = 0; h < C::HALVES; h++) tma_load_3d(dst0 + h * HALF, &map_q, 64 * h, (int)(w.head * s.g), (int)(w.q0 + token0), q_full + t);
+                        }
+                        __syncwarp();
+                        continue;
+                    }
+                    for (uint32_t i = tid; i < tile_rows * (DP / 8); i += 64) {
+                        const uint32_t row = i / (DP / 8), ch = i % (DP / 8), local = row / s.g, token = token0 + local;
+                        const bool real = token < w.n && 8 * ch < s.d;
+                        const unsigned short *src = (const unsigned short *)p.q;
+                        if (real) src += p.qv.off + (uint64_t)(w.q0 + token) * p.qv.token + (uint64_t)(w.head * s.g + (row - local * s.g)) * p.qv.head + 8 * ch;
+                        uint8_t *dst = dst0 + (ch / 8) * HALF + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+                        if (vec) {
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s32(dst)), "l"(src), "r"(real ? 16u : 0u) : "memory");
+                        } else {
+                            uint32_t x[4] = {0, 0, 0, 0};
+                            if (real)
+                                for (int e = 0; e < 4; e++) x[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+                            *(uint4 *)dst = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(q_full + t);
+                }
+                if (healthy) work = next_piece(p, w);
+            }
+            // (copies in flight when another role gave up)
+            if (q_boxes && warp == Q_WARP)
+                for (int t = 0; t < 2; t++)
+                    if (piece[t]) mbar_wait(q_full + t, (piece[t] - 1) & 1);
+            if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
+        }
+    } else {
+        // ---------------- softmax: tile t, a thread a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+        const uint32_t t = warp >> 2, row = threadIdx.x & 127, lanes = (32 * (warp & 3)) << 16;
+        const uint32_t s_col = tmem + TILE * t + lanes, o_col = tmem + C::O_COL + DP * t + lanes;
+        const float c = fabsf(s.scale) * 1.4426950408889634f;  // exponentials to base 2
+        const bool vec = ((uintptr_t)p.out & 15) == 0 && ((p.ov.off | p.ov.head | p.ov.token) & 7) == 0, wide = ((uintptr_t)p.out & 31) == 0 && ((p.ov.off | p.ov.head | p.ov.token | s.d) & 15) == 0;
+        float *const parts = (float *)((uint8_t *)p.plan + p.l.part_large);
+        constexpr uint32_t PF = ROWS * (DP + 2);
+        auto tile_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); };
+        uint32_t k = 0;  // halves of steps so far
+        for (; work; work = next_piece(p, w)) {
+            if (t == 1 && !w.two) continue;
+            const uint32_t local = row / s.g, token = (2 * w.tile + t) * s.tt + local, qh = w.head * s.g + (row - local * s.g);
+            const bool real = local < s.tt && token < w.n;
+            // (rows that are none see everything: their results go nowhere, and they ask for no mask)
+            const uint32_t hi = real ? paged_hi(s, w.n, w.kv, token) : ~0u, lo = real ? paged_lo(s, hi) : 0u;
+            float m = -INFINITY, base = 0.0f;  // the maximum that the weights refer to
+            uint64_t l0 = 0, l1 = 0;           // two pairs of sums
+            const uint64_t c2 = pack2(c, c);
+            for (uint32_t j = 0; j < w.steps && healthy; j++) {
+                if (!(healthy = warp_wait_dbg(483, s_full + t, (k >> 1) & 1))) break;
+                fence_after();
+                const uint32_t key0 = (w.t.first + w.step + j) * KEYS;
+                const bool masked = __any_sync(0xffffffffu, (real && key0 + KEYS > hi) || key0 < lo);
+                const uint32_t from = lo > key0 ? lo - key0 : 0u, to = hi > key0 ? hi - key0 : 0u;  // of the columns
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t x[SUB];
+                    tmem_ld32(x, s_col + SUB * h);
+                    tmem_ld32(x + 32, s_col + SUB * h + 32);
+                    loaded(x);
+                    if (masked) {
+#pragma unroll
+                        for (uint32_t i = 0; i < SUB; i++)
+                            if (SUB * h + i < from || SUB * h + i >= to) x[i] = 0xff800000u;
+                    }
+                    uint32_t w16[SUB / 2];
+                    uint64_t n0 = l0, n1 = l1;
+                    float top = weights<BF16, POLY>(x, c2, pack2(-base, -base), w16, n0, n1);
+                    const bool sound = top < INFINITY;  // (false for NaN and +inf: such a row is NaN)
+                    top *= c;
+                    if (__any_sync(0xffffffffu, real && top > m + LAZY)) {
+                        const float mn = fmaxf(m, top), bn = mn == -INFINITY ? 0.0f : mn, keep = exp2_fast(m - bn);
+                        m = mn, base = bn;
+                        const uint64_t k2 = pack2(keep, keep);
+                        n0 = pipe::mul2(l0, k2), n1 = pipe::mul2(l1, k2);
+                        if (j | h) {
+                            if (!(healthy = warp_wait_dbg(510, o_full + t, (k - 1) & 1))) break;
+                            fence_after();
+#pragma unroll 1
+                            for (int i = 0; i < DP / 32; i++) {
+                                uint32_t o[32];
+                                tmem_ld32(o, o_col + 32 * i);
+                                loaded(o);
+#pragma unroll
+                                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                                tmem_st32(o_col + 32 * i, o);
+                            }
+                        }
+                        weights<BF16, POLY>(x, c2, pack2(-base, -base), w16, n0, n1);
+                    }
+                    l0 = n0, l1 = n1;
+                    if (!sound) l0 = pack2(NAN, NAN);
+                    tmem_st32(s_col + (SUB / 2) * h, w16);
+                    st_wait();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + t);
+                    k++;
+                }
+            }
+            // ---- the piece is done: O is complete behind its last product
+            float a0, a1, a2, a3;
+            unpack2(l0, a0, a1);
+            unpack2(l1, a2, a3);
+            float l = m == -INFINITY ? 0.0f : (a0 + a1) + (a2 + a3);  // (no keys: polynomials of nothing)
+            if (a0 != a0) l = NAN;
+            if (healthy) healthy = warp_wait_dbg(540, o_full + t, (k - 1) & 1);
+            fence_after();
+            const bool whole = w.step == 0 && w.steps == w.t.steps;
+            const uint32_t i0 = w.u - w.step, i1 = i0 + w.t.steps;
+            unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
+            auto store32 = [&](const float *v, uint32_t col) {  // 32 columns of the row
+                if (!real) return;
+                if (wide) {  // (32 bytes a thread: every store touches 32 rows, so half as many of them)
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; e += 16)
+                        if (col + e < s.d)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(orow + col + e), "r"(pack<BF16>(v[e], v[e + 1])), "r"(pack<BF16>(v[e + 2], v[e + 3])),
+                                         "r"(pack<BF16>(v[e + 4], v[e + 5])), "r"(pack<BF16>(v[e + 6], v[e + 7])), "r"(pack<BF16>(v[e + 8], v[e + 9])), "r"(pack<BF16>(v[e + 10], v[e + 11])),
+                                         "r"(pack<BF16>(v[e + 12], v[e + 13])), "r"(pack<BF16>(v[e + 14], v[e + 15]))
+                                         : "memory");
+                    return;
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 32; e += 8) {
+                    if (col + e >= s.d) break;
+                    const uint4 y = make_uint4(pack<BF16>(v[e], v[e + 1]), pack<BF16>(v[e + 2], v[e + 3]), pack<BF16>(v[e + 4], v[e + 5]), pack<BF16>(v[e + 6], v[e + 7]));
+                    if (vec) {
+                        *(uint4 *)(orow + col + e) = y;
+                    } else {
+                        const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) orow[col + e + 2 * i] = (unsigned short)z[i], orow[col + e + 2 * i + 1] = (unsigned short)(z[i] >> 16);
+                    }
+                }
+            };
+            auto store_lse = [&](float mm, float ll) {
+                if (p.lse && real) p.lse[(size_t)(w.q0 + token) * s.hq + qh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+            };
+            float *mine = parts + (size_t)(2 * b + (i0 < u0 ? 0 : 1)) * PF + t * TILE + row;  // [column][row], then m, l
+            const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+#pragma unroll 1
+            for (int i = 0; i < DP / 32; i++) {
+                uint32_t o[32];
+                tmem_ld32(o, o_col + 32 * i);
+                loaded(o);
+                float v[32];
+#pragma unroll
+                for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * inv;
+                if (whole) {
+                    store32(v, 32 * i);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) mine[(size_t)(32 * i + e) * ROWS] = v[e];
+                }
+            }
+            fence_before();
+            if (whole) {
+                store_lse(m, l);
+                continue;
+            }
+            mine[(size_t)DP * ROWS] = m;
+            mine[(size_t)(DP + 1) * ROWS] = l;
+            const uint32_t first = paged_holder(units, ctas, i0), last = paged_holder(units, ctas, i1 - 1);
+            tile_sync();
+            if (row == 0) {
+                __threadfence();
+                uint32_t *count = p.plan + p.l.count_large + 2 * first + t;
+                const bool end = atomicAdd(count, 1u) == last - first;
+                if (end) *count = 0;  // for the next launch
+                __threadfence();
+                is_last[t] = end;
+            }
+            tile_sync();
+            if (is_last[t]) {
+                // (a tile's first piece is the end of its CTA's span, the others are the beginning of theirs)
+                auto piece = [&](uint32_t i) -> const float * { return parts + (size_t)(2 * i + (i == first ? 1 : 0)) * PF + t * TILE + row; };
+                float mm = -INFINITY, ll = 0.0f;
+                for (uint32_t i = first; i <= last; i++) mm = fmaxf(mm, __ldcg(piece(i) + (size_t)DP * ROWS));
+                const float mb = mm == -INFINITY ? 0.0f : mm;
+                for (uint32_t i = first; i <= last; i++) ll = fmaf(__ldcg(piece(i) + (size_t)(DP + 1) * ROWS), exp2_fast(__ldcg(piece(i) + (size_t)DP * ROWS) - mb), ll);
+                const float il = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll 1
+                for (int ch = 0; ch < DP / 32; ch++) {
+                    float v[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = 0.0f;
+                    for (uint32_t i = first; i <= last; i++) {
+                        const float *src = piece(i);
+                        const float f = exp2_fast(__ldcg(src + (size_t)DP * ROWS) - mb);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = fmaf(__ldcg(src + (size_t)(32 * ch + e) * ROWS), f, v[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] *= il;
+                    store32(v, 32 * ch);
+                }
+                store_lse(mm, ll);
+            }
+            tile_sync();
+        }
+        if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace pt
+
+uint32_t paged_attn_large_ctas(int sm_count) { return (uint32_t)sm_count; }
+
+template <int DP, bool BF16> static cudaError_t large_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, bool boxes, int sm_count, bool pdl, cudaStream_t stream) {
+    auto *kernel = pt::paged_attn_large_kernel<DP, BF16>;
+    constexpr int SMEM = pt::Cfg<DP>::SMEM;
+    static std::once_flag once[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::call_once(once[dev & 63], [&] { e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(paged_attn_large_ctas(sm_count));
+    cfg.blockDim = dim3(pt::THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, mk, mv, mq, a, boxes);
+}
+
+cudaError_t launch_paged_attn_large(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
+    CUtensorMap mk, mv, mq{};
+    const uint32_t rows = a.s.page < PAGED_LARGE_KEYS ? a.s.page : PAGED_LARGE_KEYS;
+    if (!paged_cache_map(a.s, a.k_cache, rows, mk) || !paged_cache_map(a.s, a.v_cache, rows, mv)) return cudaErrorInvalidValue;
+    const bool boxes = paged_q_map(a, mq);
+    if (a.s.d > 64) return a.s.bf16 ? large_launch<128, true>(a, mk, mv, mq, boxes, sm_count, pdl, stream) : large_launch<128, false>(a, mk, mv, mq, boxes, sm_count, pdl, stream);
+    return a.s.bf16 ? large_launch<64, true>(a, mk, mv, mq, boxes, sm_count, pdl, stream) : large_launch<64, false>(a, mk, mv, mq, boxes, sm_count, pdl, stream);
+}
+
+}  // namespace lb

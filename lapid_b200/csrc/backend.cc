@@ -1616,6 +1616,8 @@ lb::PagedShape paged_shape(const lapid_b200_paged *d) {
     s.max_new = (uint32_t)d->max_new;
     s.mask = (uint32_t)d->mask;
     s.window = (uint32_t)d->window;
+    s.tt = lb::PAGED_LARGE_ROWS / 2 / s.g;
+    s.large_keys = s.d > 64 ? 80 : 96;
     s.scale = scale;
     return s;
 }
@@ -2405,7 +2407,7 @@ lapid_b200_status lapid_b200_paged_plan(lapid_b200_device *dev, const lapid_b200
         a.stamp = lb::paged_stamp(a.s);
         const int sms = paged_sms(dev);
         a.ctas_small = lb::paged_attn_small_ctas(sms);
-        a.ctas_large = a.s.max_new * (uint64_t)a.s.g > lb::PAGED_SMALL_LIMIT ? lb::paged_attn_large_ctas(sms) : 0;
+        a.ctas_large = lb::paged_has_large(a.s) ? lb::paged_attn_large_ctas(sms) : 0;
         cuda_check(lb::launch_paged_plan(a, sms, dev->pdl, dev->stream), "paged_plan launch");
         dev->launches++;
     });
@@ -2510,7 +2512,7 @@ lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *dev, const lapid
         a.lse = lse ? (float *)lse->ptr : nullptr;
         a.status = dev->status_dev;
         // requests of many rows first: their CTAs run longest
-        if (a.s.max_new * (uint64_t)a.s.g > lb::PAGED_SMALL_LIMIT) {
+        if (lb::paged_has_large(a.s)) {
             cuda_check(lb::launch_paged_attn_large(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
             dev->launches++;
         }

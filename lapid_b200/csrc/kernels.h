@@ -393,12 +393,14 @@ cudaError_t launch_silu_mul(const float *gate, const float *up, float *out, uint
 constexpr uint32_t PAGED_FULL = 0, PAGED_CAUSAL = 1, PAGED_CROSS = 2;  // LAPID_B200_MASK_*
 constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile and step of the kernel for few rows
 constexpr uint32_t PAGED_SMALL_LIMIT = 16;                             // requests of at most so many packed rows go to it
-constexpr uint32_t PAGED_LARGE_ROWS = 256, PAGED_LARGE_KEYS = 128;     // tile and step of the tensor-memory kernel
+constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
 constexpr uint32_t PAGED_SMALL_MIN = 4, PAGED_LARGE_MIN = 2;             // fewest steps worth a CTA of its own
 constexpr uint32_t PAGED_MAX_SMS = 160;
 struct PagedShape {
     int bf16;  // cache, q and out: bf16, else f16
     uint32_t hq, hkv, g, d, page, pages, requests, tokens, max_blocks, max_new, mask, window;
+    uint32_t tt;          // whole tokens (of g rows) in 128 rows; 0: none
+    uint32_t large_keys;  // step of the tensor-memory kernel (paged_attn_tc.cu says why): 80 keys where head_dim is above 64, else 96
     float scale;
 };
 // Places in a plan buffer (32-bit words; the partial results behind them at byte offsets)
@@ -408,6 +410,7 @@ struct PagedPlanLayout {
 };
 PagedPlanLayout paged_plan_layout(const PagedShape &s);
 uint32_t paged_stamp(const PagedShape &s);  // what a plan was made for
+bool paged_has_large(const PagedShape &s);  // some request may go to the kernel for many rows
 uint32_t paged_part_floats(const PagedShape &s, uint32_t rows);
 struct PagedPlanArgs {
     PagedShape s;

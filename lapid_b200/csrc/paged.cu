@@ -5,8 +5,8 @@
 //         free_pages[first[r]...] in the requests' order, so the result does not depend on timing. The plan also cuts the work of
 //         the attention launches that follow (paged.cuh): which request, head, tile and step each CTA begins with. That is
 //         done once a step, and every layer's launch reads it.
-//         What bounds it is latency: one launch, two scans over the requests, a search a token. Every CTA scans the lengths
-//         itself (1024 requests at a time) so that nothing passes between CTAs; CTA 0 cuts the work, the others fill tokens and blocks.
+//         What bounds it is latency: one launch, four scans over the requests, a search a token and a search a start. Every CTA scans the
+//         lengths itself (1024 requests at a time) so that nothing passes between CTAs, and takes its share of the tokens, blocks and starts.
 // append  (x, y) -> (x cos - y sin, y cos + x sin) in f32 for the rotary pairs of q and k, one rounding to the cache's type; k and v go
 //         to their slots. Bound by memory: each element is read once and written once; a thread keeps the angles of its
 //         four pairs in registers over the heads of a token.
@@ -24,20 +24,19 @@ uint32_t paged_part_floats(const PagedShape &s, uint32_t rows) { return rows * (
 
 PagedPlanLayout paged_plan_layout(const PagedShape &s) {
     PagedPlanLayout l{};
-    uint32_t w = PLAN_HEADER;
+    uint32_t w = 0;
     auto take = [&](uint32_t n) {
         const uint32_t at = w;
         w = words_up(w + n);
         return at;
     };
-    const bool large = (uint64_t)s.max_new * s.g > PAGED_SMALL_LIMIT;
-    const uint32_t cs = paged_attn_small_ctas(PAGED_MAX_SMS), cl = large ? paged_attn_large_ctas(PAGED_MAX_SMS) : 0;
+    const uint32_t cs = paged_attn_small_ctas(PAGED_MAX_SMS), cl = paged_has_large(s) ? paged_attn_large_ctas(PAGED_MAX_SMS) : 0;
     l.q_start = take(s.requests + 1);
     l.kv_len = take(s.requests);
     l.units_small = take(s.requests + 1);
     l.units_large = take(s.requests + 1);
-    l.start_small = take(4 * cs);
-    l.start_large = take(4 * cl);
+    l.start_small = take(sizeof(PagedStart) / 4 * cs);
+    l.start_large = take(sizeof(PagedStart) / 4 * cl);
     l.count_small = take(cs);
     l.count_large = take(2 * cl);  // (for each of a tile's two halves)
     l.part_small = (size_t)w * 4;
@@ -45,6 +44,8 @@ PagedPlanLayout paged_plan_layout(const PagedShape &s) {
     l.bytes = l.part_large + (size_t)cl * 2 * paged_part_floats(s, PAGED_LARGE_ROWS) * 4;
     return l;
 }
+
+bool paged_has_large(const PagedShape &s) { return (uint64_t)s.max_new * s.g > PAGED_SMALL_LIMIT && s.tt > 0; }
 
 uint32_t paged_stamp(const PagedShape &s) {
     uint32_t h = 2166136261u;  // (Fowler, Noll and Vo's hash over the words a plan depends on)
@@ -59,6 +60,7 @@ constexpr uint32_t PLAN_THREADS = 1024;
 struct PlanShared {
     uint32_t warp_sum[32];
     uint32_t start[PLAN_THREADS + 1], first[PLAN_THREADS + 1], cached[PLAN_THREADS], have[PLAN_THREADS];
+    uint32_t small[PLAN_THREADS + 1], large[PLAN_THREADS + 1];  // units before the request
 };
 
 // Sum over the threads before this one; `total`: over all
@@ -111,34 +113,48 @@ __device__ uint32_t head_steps(const PagedShape &s, uint32_t n, uint32_t kv, uin
     return sum;
 }
 
-// Where CTA b begins: {request, head, tile, step of the tile}; a warp for each CTA
-__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, const uint32_t *prefix, uint32_t *starts, uint32_t rows, uint32_t keys) {
+// What each CTA of an attention launch begins with: warp `worker` of `workers` takes every workers-th of them. `prefix`: units before each request, `q0` first row.
+__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, const uint32_t *q0, uint32_t *starts, uint32_t rows, uint32_t keys,
+                          uint32_t worker, uint32_t workers) {
     const uint32_t lane = threadIdx.x & 31;
-    for (uint32_t b = threadIdx.x >> 5; b < ctas; b += PLAN_THREADS / 32) {
-        const uint32_t x = paged_span(units, ctas, b);
-        const uint32_t r = last_at_most(prefix, a.s.requests, x);
-        const uint32_t per_head = (prefix[r + 1] - prefix[r]) / a.s.hkv, off = x - prefix[r], head = off / per_head;
-        uint32_t rem = off - head * per_head;
-        const uint32_t n = a.plan[a.l.q_start + r + 1] - a.plan[a.l.q_start + r], kv = a.plan[a.l.kv_len + r], tiles = paged_tiles(a.s, n, rows);
-        uint32_t tile = 0;
-        for (uint32_t i0 = 0; i0 < tiles; i0 += 32) {
-            const uint32_t mine = i0 + lane < tiles ? paged_tile(a.s, n, kv, i0 + lane, rows, keys).steps : 0;
-            uint32_t inc = mine;
+    for (uint32_t b = worker; b < all; b += workers) {
+        PagedStart x{};
+        x.stamp = a.stamp, x.units = units, x.ctas = ctas;
+        if (b < ctas) {
+            x.u0 = paged_span(units, ctas, b), x.u1 = paged_span(units, ctas, b + 1);
+            const uint32_t r = last_at_most(prefix, a.s.requests, x.u0);
+            x.r = r, x.q0 = q0[r], x.n = q0[r + 1] - x.q0;
+            const uint32_t c = (uint32_t)a.cached[r];
+            x.kv = a.s.mask == PAGED_CROSS ? c : c + x.n;
+            const uint32_t per_head = (prefix[r + 1] - prefix[r]) / a.s.hkv, off = x.u0 - prefix[r], tiles = paged_tiles(a.s, x.n, rows);
+            x.head = off / per_head;
+            uint32_t rem = off - x.head * per_head;
+            for (uint32_t i0 = 0; i0 < tiles; i0 += 32) {
+                const uint32_t mine = i0 + lane < tiles ? paged_tile(a.s, x.n, x.kv, i0 + lane, rows, keys).steps : 0;
+                uint32_t inc = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += v;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += v;
+                }
+                const uint32_t behind = __ballot_sync(0xffffffffu, inc > rem);
+                if (behind) {
+                    const int who = __ffs(behind) - 1;
+                    x.tile = i0 + who;
+                    rem -= __shfl_sync(0xffffffffu, inc - mine, who);
+                    break;
+                }
+                rem -= __shfl_sync(0xffffffffu, inc, 31);
             }
-            const uint32_t behind = __ballot_sync(0xffffffffu, inc > rem);
-            if (behind) {
-                const int who = __ffs(behind) - 1;
-                tile = i0 + who;
-                rem -= __shfl_sync(0xffffffffu, inc - mine, who);
-                break;
-            }
-            rem -= __shfl_sync(0xffffffffu, inc, 31);
+            x.step = rem;
         }
-        if (lane == 0) ((uint4 *)starts)[b] = make_uint4(r, head, tile, rem);
+        const uint32_t w[12] = {x.stamp, x.units, x.ctas, x.u0, x.u1, x.r, x.head, x.tile, x.step, x.q0, x.n, x.kv};
+        if (lane < 3) {
+            uint4 v = make_uint4(w[0], w[1], w[2], w[3]);
+            if (lane == 1) v = make_uint4(w[4], w[5], w[6], w[7]);
+            if (lane == 2) v = make_uint4(w[8], w[9], w[10], w[11]);
+            ((uint4 *)starts)[b * (sizeof(PagedStart) / 16) + lane] = v;
+        }
     }
 }
 
@@ -147,8 +163,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ PlanShared sh;
     const PagedShape &s = a.s;
-    const uint32_t tid = threadIdx.x, workers = gridDim.x > 1 ? gridDim.x - 1 : 1, worker = gridDim.x > 1 ? blockIdx.x - 1 : 0;
-    const bool cuts = blockIdx.x == 0, fills = gridDim.x == 1 || blockIdx.x > 0;
+    const uint32_t tid = threadIdx.x, worker = blockIdx.x, workers = gridDim.x;
+    const bool one = s.requests <= PLAN_THREADS;  // chunk: what the searches for the starts need stays in shared memory
+    const bool counts = one || blockIdx.x == 0, writes = blockIdx.x == 0;
     uint32_t base = 0, taken = 0, small = 0, large = 0;  // tokens, pages and units of the chunks before
     uint32_t bad = 0;
     for (uint32_t r0 = 0; r0 < s.requests; r0 += PLAN_THREADS) {
@@ -177,73 +194,71 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
         sh.have[tid] = have;
         const uint32_t end_n = min(base + total_n, s.tokens), end_p = taken + total_p;
         if (tid == 0) sh.start[count] = end_n, sh.first[count] = end_p;  // (count < PLAN_THREADS: the thread of that place writes the same)
-        if (cuts) {
-            const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
+        const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
+        if (counts) {
             const bool few = paged_is_small(s, n);
             const uint32_t us = head_steps(s, n, kv, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, few) * s.hkv;
-            const uint32_t ul = head_steps(s, n, kv, PAGED_LARGE_ROWS, PAGED_LARGE_KEYS, !few) * s.hkv;
-            uint32_t total_s, total_l;
-            const uint32_t at_s = small + block_scan(us, sh, total_s), at_l = large + block_scan(ul, sh, total_l);
-            if (r < s.requests) {
-                a.plan[a.l.q_start + r] = lo;
-                a.plan[a.l.kv_len + r] = kv;
+            const uint32_t ul = a.ctas_large ? head_steps(s, n, kv, paged_large_rows(s), s.large_keys, !few) * s.hkv : 0;
+            uint32_t total_s, total_l = 0;
+            const uint32_t at_s = small + block_scan(us, sh, total_s), at_l = a.ctas_large ? large + block_scan(ul, sh, total_l) : 0;
+            small += total_s, large += total_l;
+            if (one) {
+                sh.small[tid] = at_s, sh.large[tid] = at_l;
+                if (tid == 0) sh.small[count] = small, sh.large[count] = large;
+            } else if (r < s.requests) {
                 a.plan[a.l.units_small + r] = at_s;
                 a.plan[a.l.units_large + r] = at_l;
-                a.kv_lens[r] = (int32_t)kv;
             }
-            small += total_s, large += total_l;
+        }
+        if (writes && r < s.requests) {
+            a.plan[a.l.q_start + r] = lo;
+            a.plan[a.l.kv_len + r] = kv;
+            a.kv_lens[r] = (int32_t)kv;
         }
         __syncthreads();
-        if (fills) {
-            for (uint32_t j = taken + worker * PLAN_THREADS + tid; j < end_p; j += workers * PLAN_THREADS) {
-                const uint32_t i = last_at_most(sh.first, count, j);
-                int32_t page = -1;
-                if (j >= a.n_free) bad |= PAGED_STATUS_PAGES;
-                else if ((page = a.free_pages[j]) < 0 || (uint32_t)page >= s.pages) page = -1, bad |= PAGED_STATUS_INDEX;
-                a.table[(size_t)(r0 + i) * s.max_blocks + sh.have[i] + (j - sh.first[i])] = page;
-            }
-            for (uint32_t t = base + worker * PLAN_THREADS + tid; t < end_n; t += workers * PLAN_THREADS) {
-                const uint32_t i = last_at_most(sh.start, count, t), pos = sh.cached[i] + (t - sh.start[i]), block = pos / s.page;
-                int32_t slot = -1;
-                if (s.mask != PAGED_CROSS) {
-                    int32_t page = -1;
-                    if (block < sh.have[i]) page = a.table[(size_t)(r0 + i) * s.max_blocks + block];
-                    else if (sh.first[i] + (block - sh.have[i]) < a.n_free) page = a.free_pages[sh.first[i] + (block - sh.have[i])];
-                    if (page >= 0 && (uint32_t)page < s.pages) slot = (int32_t)((uint32_t)page * s.page + pos % s.page);
-                    else if (block < sh.have[i]) bad |= PAGED_STATUS_INDEX;
-                }
-                a.slots[t] = slot;
-                a.positions[t] = (int32_t)pos;
-            }
+        for (uint32_t j = taken + worker * PLAN_THREADS + tid; j < end_p; j += workers * PLAN_THREADS) {
+            const uint32_t i = last_at_most(sh.first, count, j);
+            int32_t page = -1;
+            if (j >= a.n_free) bad |= PAGED_STATUS_PAGES;
+            else if ((page = a.free_pages[j]) < 0 || (uint32_t)page >= s.pages) page = -1, bad |= PAGED_STATUS_INDEX;
+            a.table[(size_t)(r0 + i) * s.max_blocks + sh.have[i] + (j - sh.first[i])] = page;
         }
-        base += total_n;
-        if (base > s.tokens) base = s.tokens;
+        for (uint32_t t = base + worker * PLAN_THREADS + tid; t < end_n; t += workers * PLAN_THREADS) {
+            const uint32_t i = last_at_most(sh.start, count, t), pos = sh.cached[i] + (t - sh.start[i]), block = pos / s.page;
+            int32_t slot = -1;
+            if (s.mask != PAGED_CROSS) {
+                int32_t page = -1;
+                if (block < sh.have[i]) page = a.table[(size_t)(r0 + i) * s.max_blocks + block];
+                else if (sh.first[i] + (block - sh.have[i]) < a.n_free) page = a.free_pages[sh.first[i] + (block - sh.have[i])];
+                if (page >= 0 && (uint32_t)page < s.pages) slot = (int32_t)((uint32_t)page * s.page + pos % s.page);
+                else if (block < sh.have[i]) bad |= PAGED_STATUS_INDEX;
+            }
+            a.slots[t] = slot;
+            a.positions[t] = (int32_t)pos;
+        }
+        base = end_n;
         taken = end_p;
-        __syncthreads();  // the tables of this chunk are read
+        if (!one) __syncthreads();  // the tables of this chunk are read
     }
-    if (fills)
-        for (uint32_t t = base + worker * PLAN_THREADS + tid; t < s.tokens; t += workers * PLAN_THREADS) a.slots[t] = a.positions[t] = -1;
+    for (uint32_t t = base + worker * PLAN_THREADS + tid; t < s.tokens; t += workers * PLAN_THREADS) a.slots[t] = a.positions[t] = -1;
     if (bad && a.status) atomicOr(a.status, (int)bad);
-    if (!cuts) return;
+    if (writes) {
+        if (tid == 0) {
+            a.plan[a.l.q_start + s.requests] = base;
+            *a.used = (int32_t)taken;
+            if (!one) a.plan[a.l.units_small + s.requests] = small, a.plan[a.l.units_large + s.requests] = large;
+        }
+        for (uint32_t b = tid; b < a.ctas_small; b += PLAN_THREADS) a.plan[a.l.count_small + b] = 0;
+        for (uint32_t b = tid; b < 2 * a.ctas_large; b += PLAN_THREADS) a.plan[a.l.count_large + b] = 0;
+    }
+    if (!counts) return;
+    __syncthreads();
     const uint32_t cs = small < a.ctas_small * PAGED_SMALL_MIN ? (small + PAGED_SMALL_MIN - 1) / PAGED_SMALL_MIN : a.ctas_small;
     const uint32_t cl = large < a.ctas_large * PAGED_LARGE_MIN ? (large + PAGED_LARGE_MIN - 1) / PAGED_LARGE_MIN : a.ctas_large;
-    if (tid == 0) {
-        a.plan[PLAN_STAMP] = a.stamp;
-        a.plan[PLAN_TOKENS] = base;
-        a.plan[PLAN_UNITS_SMALL] = small;
-        a.plan[PLAN_CTAS_SMALL] = cs;
-        a.plan[PLAN_UNITS_LARGE] = large;
-        a.plan[PLAN_CTAS_LARGE] = cl;
-        a.plan[a.l.q_start + s.requests] = base;
-        a.plan[a.l.units_small + s.requests] = small;
-        a.plan[a.l.units_large + s.requests] = large;
-        *a.used = (int32_t)taken;
-    }
-    for (uint32_t b = tid; b < a.ctas_small; b += PLAN_THREADS) a.plan[a.l.count_small + b] = 0;
-    for (uint32_t b = tid; b < 2 * a.ctas_large; b += PLAN_THREADS) a.plan[a.l.count_large + b] = 0;
-    __syncthreads();
-    if (small) cut_units(a, small, cs, a.plan + a.l.units_small, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS);
-    if (large) cut_units(a, large, cl, a.plan + a.l.units_large, a.plan + a.l.start_large, PAGED_LARGE_ROWS, PAGED_LARGE_KEYS);
+    const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start;
+    const uint32_t warp = worker * (PLAN_THREADS / 32) + tid / 32, warps = (one ? workers : 1) * (PLAN_THREADS / 32);
+    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, warp, warps);
+    if (a.ctas_large) cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, warp, warps);
 }
 
 static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim3 grid, unsigned threads, size_t smem, bool pdl, cudaStream_t stream) {
@@ -259,10 +274,11 @@ static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim
 }
 
 cudaError_t launch_paged_plan(const PagedPlanArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
-    const uint32_t want = (a.s.tokens + PLAN_THREADS - 1) / PLAN_THREADS;
+    // a CTA for 1024 tokens, and for 32 starts (a warp each)
+    const uint32_t starts = (a.ctas_small + a.ctas_large + 31) / 32, tokens = (a.s.tokens + PLAN_THREADS - 1) / PLAN_THREADS, want = starts > tokens ? starts : tokens;
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[1];
-    paged_config(cfg, attr, dim3(1 + (want < (uint32_t)sm_count - 1 ? want : (uint32_t)sm_count - 1)), PLAN_THREADS, 0, pdl, stream);
+    paged_config(cfg, attr, dim3(want < (uint32_t)sm_count ? want : (uint32_t)sm_count), PLAN_THREADS, 0, pdl, stream);
     return cudaLaunchKernelEx(&cfg, paged_plan_kernel, a);
 }
 

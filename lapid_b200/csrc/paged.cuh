@@ -2,8 +2,8 @@
 // a row, a tile of rows, a unit of work, and where the words of a plan buffer lie.
 //
 // The query heads of one key/value head read the same keys, so they are rows of one tile: packed row p = token * g + head
-// of the group (g = q_heads / kv_heads). A tile is PAGED_SMALL_ROWS or PAGED_LARGE_ROWS consecutive packed rows of one request and one
-// key/value head; it walks the keys that any of its rows may see in steps of PAGED_SMALL_KEYS or PAGED_LARGE_KEYS: the units.
+// of the group (g = q_heads / kv_heads). A tile is PAGED_SMALL_ROWS consecutive packed rows of one request and one key/value head, or twice the whole
+// tokens that fit 128 rows (PagedShape::tt of them); it walks the keys that any of its rows may see in steps of PAGED_SMALL_KEYS or PagedShape::large_keys: the units.
 // All units of a launch form one sequence (request, head, tile, step), cut into equal spans, one per CTA, whatever the lengths are.
 // A tile cut by the end of a span is joined from its pieces.
 #pragma once
@@ -40,10 +40,24 @@ __host__ __device__ inline PagedTile paged_tile(const PagedShape &s, uint32_t n,
 }
 __host__ __device__ inline uint32_t paged_tiles(const PagedShape &s, uint32_t n, uint32_t rows) { return (n * s.g + rows - 1) / rows; }
 // Requests of few rows go to one kernel, the others to the other
-__host__ __device__ inline bool paged_is_small(const PagedShape &s, uint32_t n) { return n * s.g <= PAGED_SMALL_LIMIT; }
+__host__ __device__ inline bool paged_is_small(const PagedShape &s, uint32_t n) { return n * s.g <= PAGED_SMALL_LIMIT || s.tt == 0; }
+__host__ __device__ inline uint32_t paged_large_rows(const PagedShape &s) { return 2 * s.tt * s.g; }
 
-// Words of a plan's header
-constexpr uint32_t PLAN_STAMP = 0, PLAN_TOKENS = 1, PLAN_UNITS_SMALL = 2, PLAN_CTAS_SMALL = 3, PLAN_UNITS_LARGE = 4, PLAN_CTAS_LARGE = 5, PLAN_HEADER = 64;
+// What a CTA of an attention launch begins with (one 64-byte line of the plan, so that one load brings it all); u0 == u1: it has nothing to do
+struct alignas(16) PagedStart {
+    uint32_t stamp, units, ctas, u0;  // what the plan was made for; the launch's steps and CTAs; this one's span [u0, u1)
+    uint32_t u1, r, head, tile;
+    uint32_t step, q0, n, kv;         // step of the tile; the request's first row of q, new tokens and keys
+    uint32_t unused[4];
+};
+__device__ inline PagedStart paged_load_start(const uint32_t *words) {
+    PagedStart x;
+    const uint4 *src = (const uint4 *)words;
+    *(uint4 *)&x.stamp = src[0];
+    *(uint4 *)&x.u1 = src[1];
+    *(uint4 *)&x.step = src[2];
+    return x;
+}
 
 // Span of CTA b of c over u units, and the CTA whose span holds unit x
 __host__ __device__ inline uint32_t paged_span(uint32_t u, uint32_t c, uint32_t b) { return (uint32_t)((uint64_t)u * b / c); }

@@ -124,19 +124,19 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (p.plan[PLAN_STAMP] != p.stamp) {
+    const uint32_t b = blockIdx.x;
+    const PagedStart at = paged_load_start(p.plan + p.l.start_small + b * (sizeof(PagedStart) / 4));
+    if (at.stamp != p.stamp) {
         if (threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
         return;
     }
-    const uint32_t units = p.plan[PLAN_UNITS_SMALL], ctas = p.plan[PLAN_CTAS_SMALL], b = blockIdx.x;
-    if (b >= ctas) return;
-    const uint4 at = ((const uint4 *)(p.plan + p.l.start_small))[b];
-    const uint32_t u0 = paged_span(units, ctas, b), u1 = paged_span(units, ctas, b + 1);
+    const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0, u1 = at.u1;
+    if (u0 == u1) return;
     Walk w;
-    w.r = at.x, w.head = at.y, w.tile = at.z;
-    load_request(p, w);
+    w.r = at.r, w.head = at.head, w.tile = at.tile, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
+    w.tiles = paged_tiles(s, w.n, ROWS);
     load_tile(p, w);
-    uint32_t step = at.w;  // of the tile
+    uint32_t step = at.step;  // of the tile
     bool healthy = true;
 
     if (warp == WARPS) {
@@ -387,18 +387,36 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
 
 }  // namespace pa
 
-// A cache as a matrix [pages * heads * page][d]; boxes of 64 elements (those behind d are filled with zeros) by `rows` rows.
-bool paged_cache_map(const PagedShape &s, const void *cache, uint32_t rows, CUtensorMap &map) {
+static pa::EncodeTiledFn encode_fn() {
     static const pa::EncodeTiledFn fn = [] {
         void *ptr = nullptr;
         cudaDriverEntryPointQueryResult q;
         return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (pa::EncodeTiledFn)ptr : nullptr;
     }();
-    if (!fn) return false;
+    return fn;
+}
+static bool encode(const PagedShape &s, const void *base, uint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box, CUtensorMap &map) {
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const pa::EncodeTiledFn fn = encode_fn();
+    return fn && fn(&map, s.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, (void *)base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// A cache as a matrix [pages * heads * page][d]; boxes of 64 elements (those behind d are filled with zeros) by `rows` rows.
+bool paged_cache_map(const PagedShape &s, const void *cache, uint32_t rows, CUtensorMap &map) {
     const cuuint64_t dims[2] = {s.d, (cuuint64_t)s.pages * s.hkv * s.page}, strides[1] = {(cuuint64_t)s.d * 2};
-    const cuuint32_t box[2] = {64, rows}, ones[2] = {1, 1};
-    return fn(&map, s.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void *)cache, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t box[2] = {64, rows};
+    return encode(s, cache, 2, dims, strides, box, map);
+}
+// q as [tokens][heads][d]; boxes of 64 elements by the heads of a group by the whole tokens that fit 128 rows: a tile's packed rows in their
+// order. False where the view does not allow it (starts and strides of 16 bytes).
+bool paged_q_map(const PagedAttnArgs &a, CUtensorMap &map) {
+    const PagedShape &s = a.s;
+    const char *base = (const char *)a.q + a.qv.off * 2;
+    const uint64_t most = 1ull << 40, head = s.hq > 1 ? a.qv.head * 2 : s.d * 2, token = s.tokens > 1 ? a.qv.token * 2 : s.hq * head;
+    if (((uintptr_t)base & 15) || head % 16 || token % 16 || head == 0 || token == 0 || head >= most || token >= most || s.tt == 0) return false;
+    const cuuint64_t dims[3] = {s.d, s.hq, s.tokens}, strides[2] = {head, token};
+    const cuuint32_t box[3] = {64, s.g, s.tt};
+    return encode(s, base, 3, dims, strides, box, map);
 }
 
 uint32_t paged_attn_small_ctas(int sm_count) { return 2 * (uint32_t)sm_count; }

@@ -2,16 +2,21 @@
 //
 //   S = Q K^T;  m = max(scale S), P = exp(scale S - m), l = sum P;  O = sum over the steps of P V;  out = O / l
 //
-// in one pass over the keys a request's rows may see, 128 at a time. A CTA holds 256 packed rows (token, query head of the group): two tiles
-// of 128, each with its scores S (f32), its weights P (16 bits, in the columns of the scores they come from) and its
-// accumulator O (f32) in tensor memory, so that one tile's products run while the other's exponentials are formed:
-//   warps 0-3, 4-7  softmax of tile 0, 1: a thread is a row. S comes from tensor memory into registers, P goes back: the A operand of the second product
-//              may lie there. O is rescaled only when a row's maximum has grown by more than 2^8 since the last time: until then
-//              the weights are at most 2^8 and nothing is lost (l and O carry the same factor); the first step of a tile writes O.
-//   warp 8     allocates tensor memory; one lane issues `tcgen05.mma`: S = Q K^T (both from shared memory) and O += P V (V as it lies in the
-//              pages: its rows are the keys, so the descriptor takes it as the transposed operand)
-//   warp 9     copies the pages' keys and values into a ring by TMA
-//   warps 10-11 bring the next tile's rows of Q
+// in one pass over the keys a request's rows may see. A CTA holds two tiles of up to 128 packed rows (token, query head of the group), each with
+// its scores S (f32), its weights P (16 bits) and its accumulator O (f32) in tensor memory, so that one tile's products run while the other's
+// exponentials are formed. A step is 80 keys (head_dim above 64; else 96): then S, P and O of both tiles fit the 512 columns beside each other,
+// and the next step's scores are formed while this one's weights still are. (128 keys with P in S's columns: the next scores wait for the weights' product;
+// a step of 128 keys took 3850 cycles, of which the products are 2048.)
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread is a row. S comes from tensor memory into registers, P goes back: the A operand of the second
+//              product may lie there. The weights are
+//              taken relative to the last maximum that was looked up, and the maximum of the new scores is formed beside them: only where one
+//              is more than 2^8 times larger are the weights formed again and O and l rescaled (until then the weights are at most 2^8 and
+//              nothing is lost; l and O carry the same factor). Some exponentials are polynomials: see exp2_poly.
+//   warps 8, 9 issue `tcgen05.mma` for tile 0, 1: S = Q K^T (both from shared memory) and O += P V (V as it lies in the pages: its rows are
+//              the keys, so the descriptor takes it as the transposed operand). A wait costs such a warp, which the softmax leaves few issue slots, 100 cycles and more
+//              also when it is over at once: a step has three. (One warp for both tiles spent more time between the products than in them.)
+//   warp 10    copies the pages' keys into a ring by TMA
+//   warp 11    copies the values, and the next tiles' rows of Q: one box of whole tokens by TMA, or 16 bytes (2, where they are not aligned) a thread
 // The steps of all requests, heads and tiles are one sequence cut into equal spans, one a CTA (paged.cuh): causal tiles of any length keep every SM
 // busy, few rows over many keys spread over all. A tile that a span's end cuts is left in the plan buffer by each of its CTAs; the one
 // that comes last adds the pieces up in the order of the keys.
@@ -27,6 +32,7 @@
 namespace lb {
 
 bool paged_cache_map(const PagedShape &s, const void *cache, uint32_t rows, CUtensorMap &map);
+bool paged_q_map(const PagedAttnArgs &a, CUtensorMap &map);
 
 namespace pt {
 
@@ -41,33 +47,38 @@ using pipe::s32;
 using pipe::tma_load_2d;
 using pipe::unpack2;
 
-constexpr int KEYS = PAGED_LARGE_KEYS, ROWS = PAGED_LARGE_ROWS, TILE = 128;
-constexpr int MMA_WARP = 8, LOAD_WARP = 9, Q_WARP = 10, THREADS = 384;
-constexpr int HALF = 128 * 128;  // bytes of 128 rows of 64 elements
+constexpr int TILE = 128, ROWS = PAGED_LARGE_ROWS;
+constexpr int MMA_WARP = 8, K_WARP = 10, V_WARP = 11, THREADS = 384;
+constexpr int Q_HALF = TILE * 128;  // bytes of 128 rows of 64 elements
 // Registers: 384 x 168 at launch = 256 x 208 + 128 x 88
 constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88;
 constexpr float LAZY = 8.0f;
+constexpr int POLY = 2;  // pairs of every eight whose exponentials are polynomials
 constexpr uint32_t WAIT_NS = 8000, SPIN_LIMIT = 1u << 19;  // a wait gives up after some two seconds
 
 template <int DP> struct Cfg {
     static constexpr int HALVES = DP / 64;
-    static constexpr int STAGE = HALVES * HALF;  // keys or values of a step
-    static constexpr int Q_BYTES = 2 * HALVES * HALF;
-    static constexpr int STAGES = (224 * 1024 - Q_BYTES) / STAGE;
-    static constexpr int SMEM = Q_BYTES + STAGES * STAGE + 512 + 1024;
-    static constexpr int O_COL = 256;  // tensor memory: S of tile t at 128 t, O at O_COL + DP t
+    static constexpr int KEYS = DP > 64 ? 80 : 96;             // PagedShape::large_keys
+    static constexpr int HALF = KEYS * 128;                    // bytes of 64 elements of a step's keys (or values)
+    static constexpr int STAGE = HALVES * HALF;
+    static constexpr int Q_BYTES = 2 * HALVES * Q_HALF;
+    static constexpr int STAGES = (224 * 1024 - Q_BYTES) / (2 * STAGE);  // of keys, and as many of values
+    static constexpr int SMEM = Q_BYTES + 2 * STAGES * STAGE + 512 + 1024;
+    // tensor memory: O of tile t at DP t, S at T_COL + T_STEP t, P behind it
+    static constexpr int T_COL = 2 * DP, T_STEP = (512 - T_COL) / 2;
+    static_assert(KEYS + KEYS / 2 <= T_STEP && KEYS % 16 == 0, "tensor memory");
 };
 
+// Bounded wait. What is waited for is there already, more often than not: the first attempt has no time to sleep (44 cycles, with one 69).
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
-    for (uint32_t spin = 0; spin < SPIN_LIMIT; spin++) {
-        uint32_t ok;
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(s32(bar)), "r"(parity) : "memory");
+    for (uint32_t spin = 0; !ok && spin < SPIN_LIMIT; spin++)
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok)
                      : "r"(s32(bar)), "r"(parity), "r"(WAIT_NS)
                      : "memory");
-        if (ok) return true;
-    }
-    return false;
+    return ok;
 }
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 __device__ __forceinline__ bool elect_one() {
@@ -76,12 +87,12 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 // Operands in shared memory, 128-byte swizzle. K-major: rows of 128 bytes, 8-row groups 1024 bytes apart. Transposed (rows are the K dimension): 8-row
-// groups 1024 bytes apart, the next 64 elements of a row one HALF further.
+// groups 1024 bytes apart, the next 64 elements of a row `half` bytes further.
 __device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_t(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(HALF >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint64_t desc_t(uint32_t saddr, uint32_t half) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(half >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
@@ -115,11 +126,33 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
         "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t *r, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+                   "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
         "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
         : "memory");
+}
+// The 80 or 96 columns of a step's scores; 40 or 48 columns of weights
+template <int N> __device__ __forceinline__ void load_scores(uint32_t (&x)[N], uint32_t addr) {
+#pragma unroll
+    for (int i = 0; i + 32 <= N; i += 32) tmem_ld32(x + i, addr + i);
+    if constexpr (N % 32 == 16) tmem_ld16(x + N - 16, addr + N - 16);
+}
+template <int N> __device__ __forceinline__ void store_weights(uint32_t addr, const uint32_t (&w)[N]) {
+    tmem_st32(addr, w);
+    if constexpr (N % 32 == 16) tmem_st16(addr + 32, w + 32);
+    if constexpr (N % 32 == 8) tmem_st8(addr + 32, w + 32);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
@@ -133,6 +166,68 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack(float lo, float hi
     return r;
 }
 
+// Behind a wait for loads from tensor memory: nothing may use the registers before it.
+template <int N> __device__ __forceinline__ void loaded(uint32_t (&x)[N]) {
+    ld_wait();
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(x[i]));
+}
+// max.NaN: a NaN among the scores stays
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a minimax polynomial in f (found by Remez's exchange; relative error 7.5e-5 at
+// degree 3, 2.6e-6 at degree 4: below half a unit of the weights' type, 2^-9 or 2^-12), n added to the exponent. For x <= 100; below -125 it stays 2^-125. The special-function unit forms
+// 16 exponentials a cycle on an SM, and 128 x 128 of them take as long as the two products of 128 x 128 x 128: what it is relieved of here costs
+// five issue slots an element that the schedulers have.
+template <int DEGREE> __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
+    float a, b;
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
+    const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));  // 1.5 2^23: n in the low bits
+    const uint64_t f = add2(x, pipe::mul2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f)));
+    uint64_t y;
+    if constexpr (DEGREE == 3) {
+        y = fma2(f, pack2(0.0551716685f, 0.0551716685f), pack2(0.242611125f, 0.242611125f));
+        y = fma2(f, y, pack2(0.693260968f, 0.693260968f));
+        y = fma2(f, y, pack2(0.999928057f, 0.999928057f));
+    } else {
+        y = fma2(f, pack2(0.00957010221f, 0.00957010221f), pack2(0.0559178591f, 0.0559178591f));
+        y = fma2(f, y, pack2(0.240247443f, 0.240247443f));
+        y = fma2(f, y, pack2(0.693121791f, 0.693121791f));
+        y = fma2(f, y, pack2(0.999999285f, 0.999999285f));
+    }
+    float y0, y1, t0, t1;
+    unpack2(y, y0, y1);
+    unpack2(t, t0, t1);
+    r0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+    r1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
+}
+// The weights of N scores, their sums (added to l) and the largest score.
+template <bool BF16, int N> __device__ __forceinline__ float weights(const uint32_t (&x)[N], uint64_t c2, uint64_t b2, uint32_t (&w)[N / 2], uint64_t &l0, uint64_t &l1) {
+    float top[4];
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+        const float x0 = __uint_as_float(x[2 * i]), x1 = __uint_as_float(x[2 * i + 1]);
+        if (i < 4) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top[i]) : "f"(x0), "f"(x1));
+        else top[i & 3] = max3(top[i & 3], x0, x1);
+        const uint64_t y = fma2(pack2(x0, x1), c2, b2);
+        float e0, e1;
+        if ((i & 7) < POLY) {
+            exp2_poly<BF16 ? 3 : 4>(y, e0, e1);
+        } else {
+            unpack2(y, e0, e1);
+            e0 = exp2_fast(e0), e1 = exp2_fast(e1);
+        }
+        if (i & 1) l1 = add2(l1, pack2(e0, e1));
+        else l0 = add2(l0, pack2(e0, e1));
+        w[i] = pack<BF16>(e0, e1);
+    }
+    return max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+}
+
 struct Walk {
     uint32_t r, head, tile, tiles, n, kv, q0;
     PagedTile t;
@@ -143,11 +238,11 @@ __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
     w.q0 = p.plan[p.l.q_start + w.r];
     w.n = p.plan[p.l.q_start + w.r + 1] - w.q0;
     w.kv = p.plan[p.l.kv_len + w.r];
-    w.tiles = paged_tiles(p.s, w.n, ROWS);
+    w.tiles = paged_tiles(p.s, w.n, paged_large_rows(p.s));
 }
 __device__ __forceinline__ void load_tile(const PagedAttnArgs &p, Walk &w) {
-    w.t = paged_tile(p.s, w.n, w.kv, w.tile, ROWS, KEYS);
-    w.two = w.tile * ROWS + TILE < w.n * p.s.g;
+    w.t = paged_tile(p.s, w.n, w.kv, w.tile, paged_large_rows(p.s), p.s.large_keys);
+    w.two = (2 * w.tile + 1) * p.s.tt < w.n;
     w.steps = min(w.t.steps - w.step, w.u1 - w.u);
 }
 // The next piece of work of the span; false: none
@@ -168,30 +263,41 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &p, Walk &w) {
     load_tile(p, w);
     return true;
 }
+__device__ __forceinline__ uint32_t tile_low(const PagedAttnArgs &p, const Walk &w) { return paged_lo(p.s, paged_hi(p.s, w.n, w.kv, 2 * w.tile * p.s.tt)); }
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(s32(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z),
+                 "r"(s32(bar))
+                 : "memory");
+}
 
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PagedAttnArgs p) {
+__global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q, PagedAttnArgs p, bool q_boxes) {
     using C = Cfg<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((0u - s32(smem_raw)) & 1023u);
-    uint8_t *ring = smem + C::Q_BYTES;
-    uint64_t *full = (uint64_t *)(ring + C::STAGES * C::STAGE), *empty = full + C::STAGES;
-    uint64_t *q_full = empty + C::STAGES, *q_empty = q_full + 2, *s_full = q_empty + 2, *p_full = s_full + 2, *o_full = p_full + 2;
-    uint32_t *tmem_slot = (uint32_t *)(o_full + 2);
+    uint8_t *k_ring = smem + C::Q_BYTES, *v_ring = k_ring + C::STAGES * C::STAGE;
+    // full[i]: the keys of the CTA's step i and the values of step i - 1 are in place: all that the products behind the scores of step i - 1 read
+    uint64_t *full = (uint64_t *)(v_ring + C::STAGES * C::STAGE), *k_empty = full + C::STAGES, *v_empty = k_empty + C::STAGES;
+    // of each tile: Q in place, read; scores there, read; weights there; their product done
+    uint64_t *q_full = v_empty + C::STAGES, *q_empty = q_full + 2, *s_full = q_empty + 2, *s_empty = s_full + 2, *p_full = s_empty + 2, *o_full = p_full + 2, *drained = o_full + 2;
+    uint32_t *tmem_slot = (uint32_t *)(drained + 2);
     volatile uint32_t *is_last = tmem_slot + 1;
     const PagedShape &s = p.s;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
-            mbar_init(full + i, 1);
-            mbar_init(empty + i, 1);
+            mbar_init(full + i, 2);     // both loaders
+            mbar_init(k_empty + i, 2);  // both tiles' warps
+            mbar_init(v_empty + i, 2);
         }
         for (int t = 0; t < 2; t++) {
-            mbar_init(q_full + t, 2);
+            mbar_init(q_full + t, 1);
             mbar_init(q_empty + t, 1);
             mbar_init(s_full + t, 1);
+            mbar_init(s_empty + t, 4);
             mbar_init(p_full + t, 4);
             mbar_init(o_full + t, 1);
+            mbar_init(drained + t, 1);
         }
         mbar_fence_init();
     }
@@ -205,147 +311,148 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
     const uint32_t tmem = *tmem_slot;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const bool stale = p.plan[PLAN_STAMP] != p.stamp;
+    const uint32_t b = blockIdx.x;
+    const PagedStart at = paged_load_start(p.plan + p.l.start_large + b * (sizeof(PagedStart) / 4));
+    const bool stale = at.stamp != p.stamp;
     if (stale && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
-    const uint32_t units = stale ? 0 : p.plan[PLAN_UNITS_LARGE], ctas = stale ? 0 : p.plan[PLAN_CTAS_LARGE], b = blockIdx.x;
-    bool work = b < ctas, healthy = true;
+    const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0;
+    bool work = !stale && at.u0 < at.u1, healthy = true;
     Walk w{};
     if (work) {
-        const uint4 at = ((const uint4 *)(p.plan + p.l.start_large))[b];
-        w.u = paged_span(units, ctas, b), w.u1 = paged_span(units, ctas, b + 1);
-        w.r = at.x, w.head = at.y, w.tile = at.z, w.step = at.w;
-        load_request(p, w);
+        w.u = u0, w.u1 = at.u1, w.r = at.r, w.head = at.head, w.tile = at.tile, w.step = at.step, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
+        w.tiles = paged_tiles(s, w.n, paged_large_rows(s));
         load_tile(p, w);
     }
-    const uint32_t u0 = w.u;
 
     if (warp >= MMA_WARP) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
-        if (warp == MMA_WARP) {
-            // ---------------- products
-            // D f32, A and B f16 (0) or bf16 (1); S: both K-major, N = 128, A negated for a negative scale; O: B transposed, N = DP
+        if (warp < K_WARP) {
+            // ---------------- products of tile t
+            // D f32, A and B f16 (0) or bf16 (1); S: both K-major, N = KEYS, A negated for a negative scale; O: B transposed, N = DP
+            const uint32_t t = warp - MMA_WARP;
             constexpr uint32_t TYPE = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((uint32_t)(TILE >> 4) << 24);
-            const uint32_t idesc_s = TYPE | ((uint32_t)(KEYS >> 3) << 17) | (s.scale < 0.0f ? 1u << 13 : 0u);
+            const uint32_t idesc_s = TYPE | ((uint32_t)(C::KEYS >> 3) << 17) | (s.scale < 0.0f ? 1u << 13 : 0u);
             constexpr uint32_t idesc_o = TYPE | ((uint32_t)(DP >> 3) << 17) | (1u << 16);
-            uint32_t st = 0, ph = 0;                 // ring
-            uint32_t piece[2] = {0, 0}, k[2] = {0, 0};  // pieces and steps of each tile so far
-            auto advance = [&]() {
-                if (++st == C::STAGES) st = 0, ph ^= 1;
-            };
-            auto scores = [&](int t, uint32_t stage, bool last_use, bool last_step) {
+            const uint32_t s_col = tmem + C::T_COL + C::T_STEP * t, p_col = s_col + C::KEYS, o_col = tmem + DP * t;
+            const uint64_t q_desc = desc_k(s32(smem) + t * C::HALVES * Q_HALF);
+            uint32_t st = 0, nst = 0, nph = 0;  // ring: this step's stage; the next one's and its phase
+            uint32_t piece = 0, done = 0;       // pieces and steps of this tile so far
+            auto scores = [&](uint32_t stage, bool last) {
                 if (elect_one()) {
-                    const uint64_t a = desc_k(s32(smem) + t * C::HALVES * HALF), bk = desc_k(s32(ring) + stage * C::STAGE);
+                    const uint64_t kd = desc_k(s32(k_ring) + stage * C::STAGE);
 #pragma unroll
-                    for (int i = 0; i < DP / 16; i++) mma_ss(tmem + TILE * t, a + (i / 4) * (HALF >> 4) + 2 * (i & 3), bk + (i / 4) * (HALF >> 4) + 2 * (i & 3), idesc_s, i ? 1u : 0u);
+                    for (int i = 0; i < DP / 16; i++) mma_ss(s_col, q_desc + (i / 4) * (Q_HALF >> 4) + 2 * (i & 3), kd + (i / 4) * (C::HALF >> 4) + 2 * (i & 3), idesc_s, i ? 1u : 0u);
                     commit(s_full + t);
-                    if (last_step) commit(q_empty + t);
-                    if (last_use) commit(empty + stage);
+                    commit(k_empty + stage);
+                    if (last) commit(q_empty + t);
                 }
                 __syncwarp();
             };
+            auto first_scores = [&](const Walk &x, uint32_t stage) {
+                if (!(healthy = warp_wait(q_full + t, piece & 1))) return;
+                piece++;
+                fence_after();
+                scores(stage, x.steps == 1);
+            };
+            auto next_stage = [&]() {  // (waits for what it holds)
+                st = nst;
+                if (++nst == C::STAGES) nst = 0, nph ^= 1;
+                return warp_wait(full + nst, nph);
+            };
+            bool begun = false;  // the piece's first scores are under way
+            if (work) healthy = warp_wait(full, 0);
             while (work && healthy) {
-                const int tiles = w.two ? 2 : 1;
-                const uint32_t tile_lo = paged_lo(s, paged_hi(s, w.n, w.kv, w.tile * ROWS / s.g));
-                // the first scores
-                if (!(healthy = warp_wait(full + st, ph))) break;
-                for (int t = 0; t < tiles && healthy; t++) {
-                    healthy = warp_wait(q_full + t, piece[t] & 1);
-                    piece[t]++;
-                    if (!healthy) break;
-                    fence_after();
-                    scores(t, st, t == tiles - 1, w.steps == 1);
+                Walk next = w;
+                const bool follows = next_piece(p, next);
+                if (t == 1 && !w.two) {  // the other tile's alone
+                    for (uint32_t j = 0; j < w.steps && healthy; j++) {
+                        if (lane == 0) mbar_arrive(k_empty + nst);
+                        if (!(healthy = next_stage())) break;
+                        if (lane == 0) mbar_arrive(v_empty + st);
+                    }
+                    w = next, work = follows;
+                    continue;
                 }
-                if (!healthy) break;
-                advance();
+                const bool next_mine = follows && (t == 0 || next.two);
+                const uint32_t low = tile_low(p, w);
+                if (!begun) first_scores(w, nst);
                 for (uint32_t j = 0; j < w.steps && healthy; j++) {
-                    const uint32_t v_stage = st, v_phase = ph;
-                    advance();
-                    const bool more = j + 1 < w.steps;
-                    if (!(healthy = warp_wait(full + v_stage, v_phase))) break;
-                    // values of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0
-                    const uint32_t key0 = (w.t.first + w.step + j) * KEYS, lo = tile_lo > key0 ? min(tile_lo - key0, (uint32_t)KEYS) : 0u, hi = w.t.hi > key0 ? min(w.t.hi - key0, (uint32_t)KEYS) : 0u;
-                    if (lo > 0 || hi < KEYS) {
-                        for (uint32_t i = lane; i < KEYS * (DP / 8); i += 32) {
+                    if (!(healthy = next_stage())) break;
+                    // values of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0 (both warps do it: zeros twice)
+                    const uint32_t key0 = (w.t.first + w.step + j) * C::KEYS;
+                    if (key0 < low || key0 + C::KEYS > w.t.hi) {
+                        for (uint32_t i = lane; i < C::KEYS * (DP / 8); i += 32) {
                             const uint32_t key = i / (DP / 8), ch = i % (DP / 8);
-                            if (key < lo || key >= hi) *(uint4 *)(ring + v_stage * C::STAGE + (ch / 8) * HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            if (key0 + key < low || key0 + key >= w.t.hi) *(uint4 *)(v_ring + st * C::STAGE + (ch / 8) * C::HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
-                    for (int t = 0; t < tiles; t++) {
-                        if (!(healthy = warp_wait(p_full + t, k[t] & 1))) break;
-                        k[t]++;
+                    const bool more = j + 1 < w.steps;
+                    if (more || next_mine) {
+                        if (!(healthy = warp_wait(s_empty + t, done & 1))) break;
                         fence_after();
-                        if (elect_one()) {
-                            const uint64_t bv = desc_t(s32(ring) + v_stage * C::STAGE);
-#pragma unroll
-                            for (int i = 0; i < KEYS / 16; i++) mma_ts(tmem + C::O_COL + DP * t, tmem + TILE * t + 8 * i, bv + i * (2048 >> 4), idesc_o, (j | i) ? 1u : 0u);
-                            commit(o_full + t);
-                            if (t == tiles - 1) commit(empty + v_stage);
-                        }
-                        __syncwarp();
-                        if (more) {
-                            if (t == 0 && !(healthy = warp_wait(full + st, ph))) break;
-                            scores(t, st, t == tiles - 1, j + 2 == w.steps);
-                        }
+                        if (more) scores(nst, j + 2 == w.steps);
+                        else first_scores(next, nst);
+                        if (!healthy) break;
                     }
-                    if (more) advance();
+                    if (!(healthy = warp_wait(p_full + t, done & 1))) break;
+                    fence_after();
+                    if (elect_one()) {
+                        const uint64_t vd = desc_t(s32(v_ring) + st * C::STAGE, C::HALF);
+#pragma unroll
+                        for (int i = 0; i < C::KEYS / 16; i++) mma_ts(o_col, p_col + 8 * i, vd + i * (2048 >> 4), idesc_o, (j | i) ? 1u : 0u);
+                        commit(o_full + t);
+                        commit(v_empty + st);
+                    }
+                    __syncwarp();
+                    done++;
                 }
-                if (healthy) work = next_piece(p, w);
+                begun = next_mine;
+                w = next, work = follows;
             }
+            // no product may be under way when tensor memory is released, and nothing may arrive in this CTA's shared memory behind its end
+            if (elect_one()) commit(drained + t);
+            __syncwarp();
+            mbar_wait(drained + t, 0);
             if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
-        } else if (warp == LOAD_WARP) {
-            // ---------------- pages: lane i copies one part of a page, half of the keys or values; keys, then values of every step
-            const uint32_t box = min(s.page, (uint32_t)KEYS), boxes = KEYS / box;
+        } else {
+            // ---------------- pages: lane i copies one part of a page, half of the keys (warp 10) or values (warp 11)
+            const bool values = warp == V_WARP;
+            uint8_t *const ring = values ? v_ring : k_ring;
+            uint64_t *const empty = values ? v_empty : k_empty;
+            const CUtensorMap *const map = values ? &map_v : &map_k;
+            constexpr uint32_t box = 16, boxes = C::KEYS / box;  // (rows that every page size and the step are multiples of)
             const bool copies = lane < boxes * C::HALVES;
             const uint32_t half = lane / boxes, part = lane % boxes;
             const int outside = (int)(s.pages * s.hkv * s.page);  // a row behind the cache: such a copy is filled with zeros
-            uint32_t st = 0, ph = 1;
+            // the stage, its empty phase; whose barrier the copies report to
+            uint32_t st = 0, ph = 1, to = values ? 1 : 0, tph = 0, piece[2] = {0, 0};
             bool bad = false;
-            while (work && healthy) {
-                const uint32_t tile_lo = paged_lo(s, paged_hi(s, w.n, w.kv, w.tile * ROWS / s.g));
-                auto row_of = [&](uint32_t j) -> int {
-                    const uint32_t key = (w.t.first + w.step + j) * KEYS + part * box, block = key / s.page;
-                    if (!copies || key >= w.t.hi) return outside;
-                    const int32_t page = p.table[(size_t)w.r * s.max_blocks + block];
-                    if (page >= 0 && (uint32_t)page < s.pages) return (int)(((uint32_t)page * s.hkv + w.head) * s.page);
-                    if ((block + 1) * s.page > tile_lo) bad = true;
-                    return outside;
-                };
-                int row = row_of(0);
-                for (uint32_t j = 0; j < w.steps && healthy; j++) {
-                    const int now = row;
-                    if (j + 1 < w.steps) row = row_of(j + 1);
-                    for (int v = 0; v < 2; v++) {
-                        if (!(healthy = warp_wait(empty + st, ph))) break;
-                        if (lane == 0) mbar_expect_tx(full + st, C::STAGE);
-                        __syncwarp();
-                        if (copies) tma_load_2d(ring + st * C::STAGE + half * HALF + part * box * 128, v ? &map_v : &map_k, 64 * (int)half, now, full + st);
-                        if (++st == C::STAGES) st = 0, ph ^= 1;
-                    }
-                }
-                if (healthy) work = next_piece(p, w);
-            }
-            if (bad && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
-            // the copies in flight have to land before the CTA leaves
-            for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < st ? ph ^ 1 : ph);
-            if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
-        } else {
-            // ---------------- rows of Q, 16 bytes a thread and copy
-            const uint32_t tid = threadIdx.x - 32 * Q_WARP;
+            if (values && work && lane == 0) mbar_arrive(full);  // (no values in front of the first keys)
+            // the rows of Q of a piece, when the scores of the one before have read theirs
+            const uint32_t tile_rows = s.tt * s.g;
             const bool vec = ((uintptr_t)p.q & 15) == 0 && ((p.qv.off | p.qv.head | p.qv.token) & 7) == 0;
-            uint32_t piece[2] = {0, 0};
-            while (work && healthy) {
-                const uint32_t rows = w.n * s.g;
-                for (int t = 0; t < (w.two ? 2 : 1) && healthy; t++) {
-                    if (piece[t] && !(healthy = warp_wait(q_empty + t, (piece[t] - 1) & 1))) break;
+            auto load_q = [&]() {
+                for (int t = 0; t < (w.two ? 2 : 1); t++) {
+                    if (piece[t] && !(healthy = warp_wait(q_empty + t, (piece[t] - 1) & 1))) return;
                     piece[t]++;
-                    for (uint32_t i = tid; i < TILE * (DP / 8); i += 64) {
-                        const uint32_t row = i / (DP / 8), ch = i % (DP / 8), pr = w.tile * ROWS + t * TILE + row, token = pr / s.g;
-                        const bool real = pr < rows && 8 * ch < s.d;
+                    const uint32_t token0 = (2 * w.tile + t) * s.tt;
+                    uint8_t *const dst0 = smem + t * C::HALVES * Q_HALF;
+                    if (q_boxes) {  // (tokens behind the request's are some other's, or zeros: such rows go nowhere)
+                        if (elect_one()) {
+                            mbar_expect_tx(q_full + t, C::HALVES * tile_rows * 128);
+                            for (int h = 0; h < C::HALVES; h++) tma_load_3d(dst0 + h * Q_HALF, &map_q, 64 * h, (int)(w.head * s.g), (int)(w.q0 + token0), q_full + t);
+                        }
+                        __syncwarp();
+                        continue;
+                    }
+                    for (uint32_t i = lane; i < tile_rows * (DP / 8); i += 32) {
+                        const uint32_t row = i / (DP / 8), ch = i % (DP / 8), local = row / s.g, token = token0 + local;
+                        const bool real = token < w.n && 8 * ch < s.d;
                         const unsigned short *src = (const unsigned short *)p.q;
-                        if (real) src += p.qv.off + (uint64_t)(w.q0 + token) * p.qv.token + (uint64_t)(w.head * s.g + (pr - token * s.g)) * p.qv.head + 8 * ch;
-                        uint8_t *dst = smem + t * C::HALVES * HALF + (ch / 8) * HALF + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+                        if (real) src += p.qv.off + (uint64_t)(w.q0 + token) * p.qv.token + (uint64_t)(w.head * s.g + (row - local * s.g)) * p.qv.head + 8 * ch;
+                        uint8_t *dst = dst0 + (ch / 8) * Q_HALF + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
                         if (vec) {
                             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s32(dst)), "l"(src), "r"(real ? 16u : 0u) : "memory");
                         } else {
@@ -360,90 +467,108 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                     __syncwarp();
                     if (lane == 0) mbar_arrive(q_full + t);
                 }
+            };
+            while (work && healthy) {
+                const uint32_t low = tile_low(p, w);
+                auto row_of = [&](uint32_t j) -> int {
+                    const uint32_t key = (w.t.first + w.step + j) * C::KEYS + part * box, block = key / s.page;
+                    if (!copies || key >= w.t.hi) return outside;
+                    const int32_t page = p.table[(size_t)w.r * s.max_blocks + block];
+                    if (page >= 0 && (uint32_t)page < s.pages) return (int)(((uint32_t)page * s.hkv + w.head) * s.page + key % s.page);
+                    if ((block + 1) * s.page > low) bad = true;
+                    return outside;
+                };
+                int row = row_of(0);
+                if (values) load_q();
+                for (uint32_t j = 0; j < w.steps && healthy; j++) {
+                    const int now = row;
+                    if (j + 1 < w.steps) row = row_of(j + 1);
+                    if (!(healthy = warp_wait(empty + st, ph))) break;
+                    // (the barrier's last phase is over: else these would count for it. From the second lap on the stage's own wait implies it.)
+                    if (values && to == 0 && !(healthy = warp_wait(full, tph ^ 1))) break;
+                    if (lane == 0) mbar_expect_tx(full + to, C::STAGE);
+                    __syncwarp();
+                    if (copies) tma_load_2d(ring + st * C::STAGE + half * C::HALF + part * box * 128, map, 64 * (int)half, now, full + to);
+                    if (++st == C::STAGES) st = 0, ph ^= 1;
+                    if (++to == C::STAGES) to = 0, tph ^= 1;
+                }
                 if (healthy) work = next_piece(p, w);
             }
+            if (!values && u0 < at.u1 && !stale && healthy && (healthy = warp_wait(empty + st, ph)) && lane == 0) mbar_arrive(full + to);  // (no keys behind the last values)
+            if (bad && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
+            // the copies in flight have to land before the CTA leaves
+            if (values && u0 < at.u1 && !stale)  // (they are the last to land)
+                for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < to ? tph : tph ^ 1);
+            if (values)
+                for (int t = 0; t < 2; t++)
+                    if (piece[t]) mbar_wait(q_full + t, (piece[t] - 1) & 1);
             if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
         }
     } else {
         // ---------------- softmax: tile t, a thread a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
         const uint32_t t = warp >> 2, row = threadIdx.x & 127, lanes = (32 * (warp & 3)) << 16;
-        const uint32_t s_col = tmem + TILE * t + lanes, o_col = tmem + C::O_COL + DP * t + lanes;
+        const uint32_t s_col = tmem + C::T_COL + C::T_STEP * t + lanes, p_col = s_col + C::KEYS, o_col = tmem + DP * t + lanes;
         const float c = fabsf(s.scale) * 1.4426950408889634f;  // exponentials to base 2
-        const bool vec = ((uintptr_t)p.out & 15) == 0 && ((p.ov.off | p.ov.head | p.ov.token) & 7) == 0;
+        const bool vec = ((uintptr_t)p.out & 15) == 0 && ((p.ov.off | p.ov.head | p.ov.token) & 7) == 0, wide = ((uintptr_t)p.out & 31) == 0 && ((p.ov.off | p.ov.head | p.ov.token | s.d) & 15) == 0;
         float *const parts = (float *)((uint8_t *)p.plan + p.l.part_large);
         constexpr uint32_t PF = ROWS * (DP + 2);
         auto tile_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); };
         uint32_t k = 0;  // steps so far
         for (; work; work = next_piece(p, w)) {
             if (t == 1 && !w.two) continue;
-            const uint32_t pr = w.tile * ROWS + t * TILE + row, token = pr / s.g, qh = w.head * s.g + (pr - token * s.g);
-            const bool real = token < w.n;
+            const uint32_t local = row / s.g, token = (2 * w.tile + t) * s.tt + local, qh = w.head * s.g + (row - local * s.g);
+            const bool real = local < s.tt && token < w.n;
             // (rows that are none see everything: their results go nowhere, and they ask for no mask)
             const uint32_t hi = real ? paged_hi(s, w.n, w.kv, token) : ~0u, lo = real ? paged_lo(s, hi) : 0u;
             float m = -INFINITY, base = 0.0f;  // the maximum that the weights refer to
             uint64_t l0 = 0, l1 = 0;           // two pairs of sums
-            for (uint32_t j = 0; j < w.steps; j++) {
-                if (healthy) healthy = warp_wait(s_full + t, k & 1);
-                if (!healthy) break;
+            const uint64_t c2 = pack2(c, c);
+            for (uint32_t j = 0; j < w.steps && healthy; j++) {
+                if (!(healthy = warp_wait(s_full + t, k & 1))) break;
                 fence_after();
-                uint32_t x[128];
-#pragma unroll
-                for (int i = 0; i < 4; i++) tmem_ld32(x + 32 * i, s_col + 32 * i);
-                ld_wait();
-                const uint32_t key0 = (w.t.first + w.step + j) * KEYS;
-                if (__any_sync(0xffffffffu, (real && key0 + KEYS > hi) || key0 < lo)) {
+                uint32_t x[C::KEYS];
+                load_scores(x, s_col);
+                loaded(x);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_empty + t);  // the next scores may come
+                const uint32_t key0 = (w.t.first + w.step + j) * C::KEYS;
+                if (__any_sync(0xffffffffu, (real && key0 + C::KEYS > hi) || key0 < lo)) {
                     const uint32_t from = lo > key0 ? lo - key0 : 0u, to = hi > key0 ? hi - key0 : 0u;  // of the columns
 #pragma unroll
-                    for (uint32_t i = 0; i < 128; i++)
+                    for (uint32_t i = 0; i < (uint32_t)C::KEYS; i++)
                         if (i < from || i >= to) x[i] = 0xff800000u;
                 }
-                float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 128; i += 4) {
-                    t0 = fmaxf(t0, __uint_as_float(x[i]));
-                    t1 = fmaxf(t1, __uint_as_float(x[i + 1]));
-                    t2 = fmaxf(t2, __uint_as_float(x[i + 2]));
-                    t3 = fmaxf(t3, __uint_as_float(x[i + 3]));
-                }
-                const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * c;
-                if (j == 0) {
-                    m = top;
-                    base = m == -INFINITY ? 0.0f : m;
-                } else if (__any_sync(0xffffffffu, top > m + LAZY)) {
+                uint32_t wt[C::KEYS / 2];
+                uint64_t n0 = l0, n1 = l1;
+                float top = weights<BF16>(x, c2, pack2(-base, -base), wt, n0, n1);
+                const bool sound = top < INFINITY;  // (false for NaN and +inf: such a row is NaN)
+                top *= c;
+                // the product of the step before is done: P's columns are free, O may change
+                if (k > 0 && !(healthy = warp_wait(o_full + t, (k - 1) & 1))) break;
+                if (__any_sync(0xffffffffu, real && top > m + LAZY)) {
                     const float mn = fmaxf(m, top), bn = mn == -INFINITY ? 0.0f : mn, keep = exp2_fast(m - bn);
                     m = mn, base = bn;
                     const uint64_t k2 = pack2(keep, keep);
-                    l0 = pipe::mul2(l0, k2), l1 = pipe::mul2(l1, k2);
-                    healthy = warp_wait(o_full + t, (k - 1) & 1);
-                    if (!healthy) break;
-                    fence_after();
+                    n0 = pipe::mul2(l0, k2), n1 = pipe::mul2(l1, k2);
+                    if (j) {
+                        fence_after();
 #pragma unroll 1
-                    for (int i = 0; i < DP / 32; i++) {
-                        uint32_t o[32];
-                        tmem_ld32(o, o_col + 32 * i);
-                        ld_wait();
+                        for (int i = 0; i < DP / 32; i++) {
+                            uint32_t o[32];
+                            tmem_ld32(o, o_col + 32 * i);
+                            loaded(o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                        tmem_st32(o_col + 32 * i, o);
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st32(o_col + 32 * i, o);
+                        }
                     }
+                    weights<BF16>(x, c2, pack2(-base, -base), wt, n0, n1);
                 }
-                const uint64_t c2 = pack2(c, c), b2 = pack2(-base, -base);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t w16[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const uint64_t y = fma2(pack2(__uint_as_float(x[32 * q + 2 * i]), __uint_as_float(x[32 * q + 2 * i + 1])), c2, b2);
-                        float e0, e1;
-                        unpack2(y, e0, e1);
-                        e0 = exp2_fast(e0), e1 = exp2_fast(e1);
-                        if (i & 1) l1 = add2(l1, pack2(e0, e1));
-                        else l0 = add2(l0, pack2(e0, e1));
-                        w16[i] = pack<BF16>(e0, e1);
-                    }
-                    tmem_st16(s_col + 16 * q, w16);
-                }
+                l0 = n0, l1 = n1;
+                if (!sound) l0 = pack2(NAN, NAN);
+                store_weights(p_col, wt);
                 st_wait();
                 fence_before();
                 __syncwarp();
@@ -454,7 +579,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             float a0, a1, a2, a3;
             unpack2(l0, a0, a1);
             unpack2(l1, a2, a3);
-            float l = (a0 + a1) + (a2 + a3);
+            float l = m == -INFINITY ? 0.0f : (a0 + a1) + (a2 + a3);  // (no keys: polynomials of nothing)
+            if (a0 != a0) l = NAN;
             if (healthy) healthy = warp_wait(o_full + t, (k - 1) & 1);
             fence_after();
             const bool whole = w.step == 0 && w.steps == w.t.steps;
@@ -462,6 +588,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
             auto store32 = [&](const float *v, uint32_t col) {  // 32 columns of the row
                 if (!real) return;
+                if (wide) {  // (32 bytes a thread: every store touches 32 rows, so half as many of them)
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; e += 16)
+                        if (col + e < s.d)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(orow + col + e), "r"(pack<BF16>(v[e], v[e + 1])), "r"(pack<BF16>(v[e + 2], v[e + 3])),
+                                         "r"(pack<BF16>(v[e + 4], v[e + 5])), "r"(pack<BF16>(v[e + 6], v[e + 7])), "r"(pack<BF16>(v[e + 8], v[e + 9])), "r"(pack<BF16>(v[e + 10], v[e + 11])),
+                                         "r"(pack<BF16>(v[e + 12], v[e + 13])), "r"(pack<BF16>(v[e + 14], v[e + 15]))
+                                         : "memory");
+                    return;
+                }
 #pragma unroll
                 for (uint32_t e = 0; e < 32; e += 8) {
                     if (col + e >= s.d) break;
@@ -484,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             for (int i = 0; i < DP / 32; i++) {
                 uint32_t o[32];
                 tmem_ld32(o, o_col + 32 * i);
-                ld_wait();
+                loaded(o);
                 float v[32];
 #pragma unroll
                 for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * inv;
@@ -554,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
 
 uint32_t paged_attn_large_ctas(int sm_count) { return (uint32_t)sm_count; }
 
-template <int DP, bool BF16> static cudaError_t large_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sm_count, bool pdl, cudaStream_t stream) {
+template <int DP, bool BF16> static cudaError_t large_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, bool boxes, int sm_count, bool pdl, cudaStream_t stream) {
     auto *kernel = pt::paged_attn_large_kernel<DP, BF16>;
     constexpr int SMEM = pt::Cfg<DP>::SMEM;
     static std::once_flag once[64];
@@ -573,15 +709,16 @@ template <int DP, bool BF16> static cudaError_t large_launch(const PagedAttnArgs
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, mk, mv, a);
+    return cudaLaunchKernelEx(&cfg, kernel, mk, mv, mq, a, boxes);
 }
 
 cudaError_t launch_paged_attn_large(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
-    CUtensorMap mk, mv;
-    const uint32_t rows = a.s.page < PAGED_LARGE_KEYS ? a.s.page : PAGED_LARGE_KEYS;
+    CUtensorMap mk, mv, mq{};
+    constexpr uint32_t rows = 16;
     if (!paged_cache_map(a.s, a.k_cache, rows, mk) || !paged_cache_map(a.s, a.v_cache, rows, mv)) return cudaErrorInvalidValue;
-    if (a.s.d > 64) return a.s.bf16 ? large_launch<128, true>(a, mk, mv, sm_count, pdl, stream) : large_launch<128, false>(a, mk, mv, sm_count, pdl, stream);
-    return a.s.bf16 ? large_launch<64, true>(a, mk, mv, sm_count, pdl, stream) : large_launch<64, false>(a, mk, mv, sm_count, pdl, stream);
+    const bool boxes = paged_q_map(a, mq);
+    if (a.s.d > 64) return a.s.bf16 ? large_launch<128, true>(a, mk, mv, mq, boxes, sm_count, pdl, stream) : large_launch<128, false>(a, mk, mv, mq, boxes, sm_count, pdl, stream);
+    return a.s.bf16 ? large_launch<64, true>(a, mk, mv, mq, boxes, sm_count, pdl, stream) : large_launch<64, false>(a, mk, mv, mq, boxes, sm_count, pdl, stream);
 }
 
 }  // namespace lb

@@ -225,6 +225,29 @@ def test_chunks_behind_a_context(be, page, new, cached):
     R.Step(be, new, cached, hq=8, hkv=2, d=128, page=page, seed=len(new)).run()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,hkv,d,new,cached", [(8, 8, 128, [900, 1400], [0, 300]), (16, 8, 64, [1, 1500, 700, 60], [50, 0, 900, 2000]), (24, 8, 128, [1300, 40], [77, 1500])])
+def test_many_steps_a_cta(be, dtype, hq, hkv, d, new, cached):
+    """Enough work that each SM walks several tiles and every ring several times (checked on rows picked at random)."""
+    s = R.Step(be, new, cached, hq=hq, hkv=hkv, d=d, dtype=dtype, page=32, seed=d).upload()
+    s.make_plan()
+    s.attend()
+    be.synchronize()
+    out, lse = s.outputs()
+    rng, at = np.random.default_rng(3), 0
+    for r, n in enumerate(new):
+        for t in {0, n - 1, *rng.integers(0, n, 12).tolist()}:
+            end = cached[r] + t + 1
+            o, l, size = R.attention(s.q[at + t:at + t + 1], s.k[r][:end], s.v[r][:end], s.g, s.mask, 0, s.scale, 1, end)
+            assert np.all(np.abs(out[at + t] - o[0]) <= R.bound(dtype, o[0], size[0], end, 6.0)), (r, t)
+            assert np.all(np.abs(lse[at + t] - l[0]) <= 1.5e-4 + 1e-6 * np.abs(l[0])), (r, t)
+        at += n
+    first = s.b["out"].download().copy()
+    s.attend()
+    be.synchronize()
+    assert np.array_equal(first, s.b["out"].download())
+
+
 @pytest.mark.parametrize("window", [1, 17, 64, 128, 200])
 @pytest.mark.parametrize("d", [64, 128])
 def test_sliding_window(be, window, d):
