@@ -394,7 +394,8 @@ constexpr uint32_t PAGED_FULL = 0, PAGED_CAUSAL = 1, PAGED_CROSS = 2;  // LAPID_
 constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile and step of the kernel for few rows
 constexpr uint32_t PAGED_SMALL_LIMIT = 16;                             // requests of at most so many packed rows go to it
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
-constexpr uint32_t PAGED_SMALL_MIN = 4, PAGED_LARGE_MIN = 2;             // fewest steps worth a CTA of its own
+constexpr uint32_t PAGED_LARGE_EXTRA = 3;                              // steps that beginning and ending one of its tiles takes as long as
+constexpr uint32_t PAGED_SMALL_MIN = 4, PAGED_LARGE_MIN = 6;             // fewest units worth a CTA of its own
 constexpr uint32_t PAGED_MAX_SMS = 160;
 struct PagedShape {
     int bf16;  // cache, q and out: bf16, else f16

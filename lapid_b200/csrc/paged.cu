@@ -96,17 +96,17 @@ template <class T> __device__ __forceinline__ uint32_t last_at_most(const T *a, 
     return lo;
 }
 
-// Steps of all tiles of a request and one key/value head; long requests are shared by the warp (every lane of a warp calls it)
-__device__ uint32_t head_steps(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t rows, uint32_t keys, bool mine) {
+// Units of all tiles of a request and one key/value head; long requests are shared by the warp (every lane of a warp calls it)
+__device__ uint32_t head_units(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t rows, uint32_t keys, uint32_t extra, bool mine) {
     const uint32_t lane = threadIdx.x & 31, tiles = mine && n ? paged_tiles(s, n, rows) : 0;
     uint32_t sum = 0;
     if (tiles <= 16)
-        for (uint32_t i = 0; i < tiles; i++) sum += paged_tile(s, n, kv, i, rows, keys).steps;
+        for (uint32_t i = 0; i < tiles; i++) sum += paged_tile(s, n, kv, i, rows, keys).steps + extra;
     for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 16); many; many &= many - 1) {
         const int who = __ffs(many) - 1;
         const uint32_t n1 = __shfl_sync(0xffffffffu, n, who), kv1 = __shfl_sync(0xffffffffu, kv, who), t1 = __shfl_sync(0xffffffffu, tiles, who);
         uint32_t part = 0;
-        for (uint32_t i = lane; i < t1; i += 32) part += paged_tile(s, n1, kv1, i, rows, keys).steps;
+        for (uint32_t i = lane; i < t1; i += 32) part += paged_tile(s, n1, kv1, i, rows, keys).steps + extra;
         part = __reduce_add_sync(0xffffffffu, part);
         if ((int)lane == who) sum = part;
     }
@@ -115,7 +115,7 @@ __device__ uint32_t head_steps(const PagedShape &s, uint32_t n, uint32_t kv, uin
 
 // What each CTA of an attention launch begins with: warp `worker` of `workers` takes every workers-th of them. `prefix`: units before each request, `q0` first row.
 __device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, const uint32_t *q0, uint32_t *starts, uint32_t rows, uint32_t keys,
-                          uint32_t worker, uint32_t workers) {
+                          uint32_t extra, uint32_t worker, uint32_t workers) {
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t b = worker; b < all; b += workers) {
         PagedStart x{};
@@ -130,7 +130,7 @@ __device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas,
             x.head = off / per_head;
             uint32_t rem = off - x.head * per_head;
             for (uint32_t i0 = 0; i0 < tiles; i0 += 32) {
-                const uint32_t mine = i0 + lane < tiles ? paged_tile(a.s, x.n, x.kv, i0 + lane, rows, keys).steps : 0;
+                const uint32_t mine = i0 + lane < tiles ? paged_tile(a.s, x.n, x.kv, i0 + lane, rows, keys).steps + extra : 0;
                 uint32_t inc = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -146,9 +146,9 @@ __device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas,
                 }
                 rem -= __shfl_sync(0xffffffffu, inc, 31);
             }
-            x.step = rem;
+            x.place = rem;
         }
-        const uint32_t w[12] = {x.stamp, x.units, x.ctas, x.u0, x.u1, x.r, x.head, x.tile, x.step, x.q0, x.n, x.kv};
+        const uint32_t w[12] = {x.stamp, x.units, x.ctas, x.u0, x.u1, x.r, x.head, x.tile, x.place, x.q0, x.n, x.kv};
         if (lane < 3) {
             uint4 v = make_uint4(w[0], w[1], w[2], w[3]);
             if (lane == 1) v = make_uint4(w[4], w[5], w[6], w[7]);
@@ -197,8 +197,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
         const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
         if (counts) {
             const bool few = paged_is_small(s, n);
-            const uint32_t us = head_steps(s, n, kv, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, few) * s.hkv;
-            const uint32_t ul = a.ctas_large ? head_steps(s, n, kv, paged_large_rows(s), s.large_keys, !few) * s.hkv : 0;
+            const uint32_t us = head_units(s, n, kv, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, few) * s.hkv;
+            const uint32_t ul = a.ctas_large ? head_units(s, n, kv, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, !few) * s.hkv : 0;
             uint32_t total_s, total_l = 0;
             const uint32_t at_s = small + block_scan(us, sh, total_s), at_l = a.ctas_large ? large + block_scan(ul, sh, total_l) : 0;
             small += total_s, large += total_l;
@@ -257,8 +257,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     const uint32_t cl = large < a.ctas_large * PAGED_LARGE_MIN ? (large + PAGED_LARGE_MIN - 1) / PAGED_LARGE_MIN : a.ctas_large;
     const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start;
     const uint32_t warp = worker * (PLAN_THREADS / 32) + tid / 32, warps = (one ? workers : 1) * (PLAN_THREADS / 32);
-    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, warp, warps);
-    if (a.ctas_large) cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, warp, warps);
+    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);
+    if (a.ctas_large) cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, warp, warps);
 }
 
 static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim3 grid, unsigned threads, size_t smem, bool pdl, cudaStream_t stream) {

@@ -5,7 +5,8 @@
 // of the group (g = q_heads / kv_heads). A tile is PAGED_SMALL_ROWS consecutive packed rows of one request and one key/value head, or twice the whole
 // tokens that fit 128 rows (PagedShape::tt of them); it walks the keys that any of its rows may see in steps of PAGED_SMALL_KEYS or PagedShape::large_keys: the units.
 // All units of a launch form one sequence (request, head, tile, step), cut into equal spans, one per CTA, whatever the lengths are.
-// A tile cut by the end of a span is joined from its pieces.
+// A tile cut by the end of a span is joined from its pieces. A tile of many rows counts PAGED_LARGE_EXTRA units more than its steps, in front of them:
+// what its beginning and its end cost.
 #pragma once
 #include <stdint.h>
 
@@ -47,7 +48,7 @@ __host__ __device__ inline uint32_t paged_large_rows(const PagedShape &s) { retu
 struct alignas(16) PagedStart {
     uint32_t stamp, units, ctas, u0;  // what the plan was made for; the launch's steps and CTAs; this one's span [u0, u1)
     uint32_t u1, r, head, tile;
-    uint32_t step, q0, n, kv;         // step of the tile; the request's first row of q, new tokens and keys
+    uint32_t place, q0, n, kv;        // units of the tile in front of u0; the request's first row of q, new tokens and keys
     uint32_t unused[4];
 };
 __device__ inline PagedStart paged_load_start(const uint32_t *words) {
@@ -55,7 +56,7 @@ __device__ inline PagedStart paged_load_start(const uint32_t *words) {
     const uint4 *src = (const uint4 *)words;
     *(uint4 *)&x.stamp = src[0];
     *(uint4 *)&x.u1 = src[1];
-    *(uint4 *)&x.step = src[2];
+    *(uint4 *)&x.place = src[2];
     return x;
 }
 

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
     w.r = at.r, w.head = at.head, w.tile = at.tile, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
     w.tiles = paged_tiles(s, w.n, ROWS);
     load_tile(p, w);
-    uint32_t step = at.step;  // of the tile
+    uint32_t step = at.place;  // of the tile
     bool healthy = true;
 
     if (warp == WARPS) {

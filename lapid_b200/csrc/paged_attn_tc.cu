@@ -231,8 +231,9 @@ template <bool BF16, int N> __device__ __forceinline__ float weights(const uint3
 struct Walk {
     uint32_t r, head, tile, tiles, n, kv, q0;
     PagedTile t;
-    uint32_t u, u1, step, steps;  // place in the sequence, end of the span; first step of the tile here, and how many
-    bool two;                     // the second tile of 128 has rows
+    uint32_t i0, u1;         // units: where the tile begins, where the span ends
+    uint32_t step, steps;    // first step of the tile here, and how many
+    bool two;                // the second tile of 128 has rows
 };
 __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
     w.q0 = p.plan[p.l.q_start + w.r];
@@ -240,15 +241,18 @@ __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
     w.kv = p.plan[p.l.kv_len + w.r];
     w.tiles = paged_tiles(p.s, w.n, paged_large_rows(p.s));
 }
-__device__ __forceinline__ void load_tile(const PagedAttnArgs &p, Walk &w) {
+// (steps 0: the span ends in what the tile counts in front of its steps)
+__device__ __forceinline__ bool load_tile(const PagedAttnArgs &p, Walk &w) {
     w.t = paged_tile(p.s, w.n, w.kv, w.tile, paged_large_rows(p.s), p.s.large_keys);
     w.two = (2 * w.tile + 1) * p.s.tt < w.n;
-    w.steps = min(w.t.steps - w.step, w.u1 - w.u);
+    const uint32_t begin = w.i0 + PAGED_LARGE_EXTRA, end = w.u1 > begin ? min(w.t.steps, w.u1 - begin) : 0u;
+    w.steps = end > w.step ? end - w.step : 0u;
+    return w.steps > 0;
 }
 // The next piece of work of the span; false: none
 __device__ __forceinline__ bool next_piece(const PagedAttnArgs &p, Walk &w) {
-    w.u += w.steps;
-    if (w.u >= w.u1) return false;
+    w.i0 += PAGED_LARGE_EXTRA + w.t.steps;
+    if (w.i0 + PAGED_LARGE_EXTRA >= w.u1) return false;
     w.step = 0;
     if (++w.tile == w.tiles) {
         w.tile = 0;
@@ -260,8 +264,7 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &p, Walk &w) {
             } while (w.n == 0 || paged_is_small(p.s, w.n));
         }
     }
-    load_tile(p, w);
-    return true;
+    return load_tile(p, w);
 }
 __device__ __forceinline__ uint32_t tile_low(const PagedAttnArgs &p, const Walk &w) { return paged_lo(p.s, paged_hi(p.s, w.n, w.kv, 2 * w.tile * p.s.tt)); }
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
@@ -276,17 +279,18 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((0u - s32(smem_raw)) & 1023u);
     uint8_t *k_ring = smem + C::Q_BYTES, *v_ring = k_ring + C::STAGES * C::STAGE;
-    // full[i]: the keys of the CTA's step i and the values of step i - 1 are in place: all that the products behind the scores of step i - 1 read
-    uint64_t *full = (uint64_t *)(v_ring + C::STAGES * C::STAGE), *k_empty = full + C::STAGES, *v_empty = k_empty + C::STAGES;
-    // of each tile: Q in place, read; scores there, read; weights there; their product done
-    uint64_t *q_full = v_empty + C::STAGES, *q_empty = q_full + 2, *s_full = q_empty + 2, *s_empty = s_full + 2, *p_full = s_empty + 2, *o_full = p_full + 2, *drained = o_full + 2;
+    uint64_t *k_full = (uint64_t *)(v_ring + C::STAGES * C::STAGE), *k_empty = k_full + C::STAGES, *v_full = k_empty + C::STAGES, *v_empty = v_full + C::STAGES;
+    // of each tile: Q in place, read; scores there; scores read and the weights before them there ([event & 1][tile]: the softmax may be at the event behind
+    // a piece's last scores before the one in front of it was looked at); product of the weights done; all done
+    uint64_t *q_full = v_empty + C::STAGES, *q_empty = q_full + 2, *s_full = q_empty + 2, *ready = s_full + 2, *o_full = ready + 4, *drained = o_full + 2;
     uint32_t *tmem_slot = (uint32_t *)(drained + 2);
     volatile uint32_t *is_last = tmem_slot + 1;
     const PagedShape &s = p.s;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
-            mbar_init(full + i, 2);     // both loaders
+            mbar_init(k_full + i, 1);
+            mbar_init(v_full + i, 1);
             mbar_init(k_empty + i, 2);  // both tiles' warps
             mbar_init(v_empty + i, 2);
         }
@@ -294,8 +298,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             mbar_init(q_full + t, 1);
             mbar_init(q_empty + t, 1);
             mbar_init(s_full + t, 1);
-            mbar_init(s_empty + t, 4);
-            mbar_init(p_full + t, 4);
+            mbar_init(ready + t, 4);
+            mbar_init(ready + 2 + t, 4);
             mbar_init(o_full + t, 1);
             mbar_init(drained + t, 1);
         }
@@ -316,12 +320,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
     const bool stale = at.stamp != p.stamp;
     if (stale && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
     const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0;
-    bool work = !stale && at.u0 < at.u1, healthy = true;
+    bool work = !stale && u0 < at.u1, healthy = true;
     Walk w{};
-    if (work) {
-        w.u = u0, w.u1 = at.u1, w.r = at.r, w.head = at.head, w.tile = at.tile, w.step = at.step, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
+    if (work) {  // (a span may hold nothing but the front of a tile)
+        w.i0 = u0 - at.place, w.u1 = at.u1, w.r = at.r, w.head = at.head, w.tile = at.tile, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
+        w.step = at.place > PAGED_LARGE_EXTRA ? at.place - PAGED_LARGE_EXTRA : 0u;
         w.tiles = paged_tiles(s, w.n, paged_large_rows(s));
-        load_tile(p, w);
+        work = load_tile(p, w);
     }
 
     if (warp >= MMA_WARP) {
@@ -335,78 +340,84 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             constexpr uint32_t idesc_o = TYPE | ((uint32_t)(DP >> 3) << 17) | (1u << 16);
             const uint32_t s_col = tmem + C::T_COL + C::T_STEP * t, p_col = s_col + C::KEYS, o_col = tmem + DP * t;
             const uint64_t q_desc = desc_k(s32(smem) + t * C::HALVES * Q_HALF);
-            uint32_t st = 0, nst = 0, nph = 0;  // ring: this step's stage; the next one's and its phase
-            uint32_t piece = 0, done = 0;       // pieces and steps of this tile so far
-            auto scores = [&](uint32_t stage, bool last) {
+            uint32_t ks = 0, kph = 0, vs = 0, vph = 0;  // rings
+            uint32_t piece = 0, events = 0;             // pieces of this tile, and times that its softmax was ready
+            auto scores = [&](bool last) {
                 if (elect_one()) {
-                    const uint64_t kd = desc_k(s32(k_ring) + stage * C::STAGE);
+                    const uint64_t kd = desc_k(s32(k_ring) + ks * C::STAGE);
 #pragma unroll
                     for (int i = 0; i < DP / 16; i++) mma_ss(s_col, q_desc + (i / 4) * (Q_HALF >> 4) + 2 * (i & 3), kd + (i / 4) * (C::HALF >> 4) + 2 * (i & 3), idesc_s, i ? 1u : 0u);
                     commit(s_full + t);
-                    commit(k_empty + stage);
+                    commit(k_empty + ks);
                     if (last) commit(q_empty + t);
                 }
                 __syncwarp();
-            };
-            auto first_scores = [&](const Walk &x, uint32_t stage) {
-                if (!(healthy = warp_wait(q_full + t, piece & 1))) return;
-                piece++;
-                fence_after();
-                scores(stage, x.steps == 1);
-            };
-            auto next_stage = [&]() {  // (waits for what it holds)
-                st = nst;
-                if (++nst == C::STAGES) nst = 0, nph ^= 1;
-                return warp_wait(full + nst, nph);
+                if (++ks == C::STAGES) ks = 0, kph ^= 1;
             };
             bool begun = false;  // the piece's first scores are under way
-            if (work) healthy = warp_wait(full, 0);
             while (work && healthy) {
                 Walk next = w;
                 const bool follows = next_piece(p, next);
                 if (t == 1 && !w.two) {  // the other tile's alone
                     for (uint32_t j = 0; j < w.steps && healthy; j++) {
-                        if (lane == 0) mbar_arrive(k_empty + nst);
-                        if (!(healthy = next_stage())) break;
-                        if (lane == 0) mbar_arrive(v_empty + st);
+                        if (!(healthy = warp_wait(k_full + ks, kph) && warp_wait(v_full + vs, vph))) break;
+                        if (lane == 0) mbar_arrive(k_empty + ks), mbar_arrive(v_empty + vs);
+                        if (++ks == C::STAGES) ks = 0, kph ^= 1;
+                        if (++vs == C::STAGES) vs = 0, vph ^= 1;
                     }
                     w = next, work = follows;
                     continue;
                 }
                 const bool next_mine = follows && (t == 0 || next.two);
                 const uint32_t low = tile_low(p, w);
-                if (!begun) first_scores(w, nst);
-                for (uint32_t j = 0; j < w.steps && healthy; j++) {
-                    if (!(healthy = next_stage())) break;
-                    // values of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0 (both warps do it: zeros twice)
-                    const uint32_t key0 = (w.t.first + w.step + j) * C::KEYS;
-                    if (key0 < low || key0 + C::KEYS > w.t.hi) {
-                        for (uint32_t i = lane; i < C::KEYS * (DP / 8); i += 32) {
-                            const uint32_t key = i / (DP / 8), ch = i % (DP / 8);
-                            if (key0 + key < low || key0 + key >= w.t.hi) *(uint4 *)(v_ring + st * C::STAGE + (ch / 8) * C::HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                    }
-                    const bool more = j + 1 < w.steps;
-                    if (more || next_mine) {
-                        if (!(healthy = warp_wait(s_empty + t, done & 1))) break;
-                        fence_after();
-                        if (more) scores(nst, j + 2 == w.steps);
-                        else first_scores(next, nst);
-                        if (!healthy) break;
-                    }
-                    if (!(healthy = warp_wait(p_full + t, done & 1))) break;
+                if (!begun) {
+                    if (!(healthy = warp_wait(k_full + ks, kph) && warp_wait(q_full + t, piece & 1))) break;
+                    piece++;
                     fence_after();
-                    if (elect_one()) {
-                        const uint64_t vd = desc_t(s32(v_ring) + st * C::STAGE, C::HALF);
-#pragma unroll
-                        for (int i = 0; i < C::KEYS / 16; i++) mma_ts(o_col, p_col + 8 * i, vd + i * (2048 >> 4), idesc_o, (j | i) ? 1u : 0u);
-                        commit(o_full + t);
-                        commit(v_empty + st);
+                    scores(w.steps == 1);
+                }
+                // Event j: the scores of step j have been read, and the weights of step j - 1 are there. Then the scores behind them may be formed, of step
+                // j + 1 or of the next piece's first, and the weights multiplied. (Event `steps`: the last weights are there.)
+                for (uint32_t j = 0; j <= w.steps && healthy; j++) {
+                    const bool more = j + 1 < w.steps, first = j + 1 == w.steps && next_mine;
+                    if (more || first) {
+                        if (!(healthy = warp_wait(k_full + ks, kph))) break;
+                        if (first && !(healthy = warp_wait(q_full + t, piece & 1))) break;
                     }
-                    __syncwarp();
-                    done++;
+                    if (j) {
+                        if (!(healthy = warp_wait(v_full + vs, vph))) break;
+                        // values of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0 (both warps do it: zeros twice)
+                        const uint32_t key0 = (w.t.first + w.step + j - 1) * C::KEYS;
+                        if (key0 < low || key0 + C::KEYS > w.t.hi) {
+                            for (uint32_t i = lane; i < C::KEYS * (DP / 8); i += 32) {
+                                const uint32_t key = i / (DP / 8), ch = i % (DP / 8);
+                                if (key0 + key < low || key0 + key >= w.t.hi)
+                                    *(uint4 *)(v_ring + vs * C::STAGE + (ch / 8) * C::HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                        }
+                    }
+                    if (!(healthy = warp_wait(ready + 2 * (events & 1) + t, (events >> 1) & 1))) break;
+                    events++;
+                    fence_after();
+                    if (more) {
+                        scores(j + 2 == w.steps);
+                    } else if (first) {
+                        piece++;
+                        scores(next.steps == 1);
+                    }
+                    if (j) {
+                        if (elect_one()) {
+                            const uint64_t vd = desc_t(s32(v_ring) + vs * C::STAGE, C::HALF);
+#pragma unroll
+                            for (int i = 0; i < C::KEYS / 16; i++) mma_ts(o_col, p_col + 8 * i, vd + i * (2048 >> 4), idesc_o, (j > 1 || i) ? 1u : 0u);
+                            commit(o_full + t);
+                            commit(v_empty + vs);
+                        }
+                        __syncwarp();
+                        if (++vs == C::STAGES) vs = 0, vph ^= 1;
+                    }
                 }
                 begun = next_mine;
                 w = next, work = follows;
@@ -420,16 +431,14 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             // ---------------- pages: lane i copies one part of a page, half of the keys (warp 10) or values (warp 11)
             const bool values = warp == V_WARP;
             uint8_t *const ring = values ? v_ring : k_ring;
-            uint64_t *const empty = values ? v_empty : k_empty;
+            uint64_t *const full = values ? v_full : k_full, *const empty = values ? v_empty : k_empty;
             const CUtensorMap *const map = values ? &map_v : &map_k;
             constexpr uint32_t box = 16, boxes = C::KEYS / box;  // (rows that every page size and the step are multiples of)
             const bool copies = lane < boxes * C::HALVES;
             const uint32_t half = lane / boxes, part = lane % boxes;
             const int outside = (int)(s.pages * s.hkv * s.page);  // a row behind the cache: such a copy is filled with zeros
-            // the stage, its empty phase; whose barrier the copies report to
-            uint32_t st = 0, ph = 1, to = values ? 1 : 0, tph = 0, piece[2] = {0, 0};
+            uint32_t st = 0, ph = 1, piece[2] = {0, 0};
             bool bad = false;
-            if (values && work && lane == 0) mbar_arrive(full);  // (no values in front of the first keys)
             // the rows of Q of a piece, when the scores of the one before have read theirs
             const uint32_t tile_rows = s.tt * s.g;
             const bool vec = ((uintptr_t)p.q & 15) == 0 && ((p.qv.off | p.qv.head | p.qv.token) & 7) == 0;
@@ -484,21 +493,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                     const int now = row;
                     if (j + 1 < w.steps) row = row_of(j + 1);
                     if (!(healthy = warp_wait(empty + st, ph))) break;
-                    // (the barrier's last phase is over: else these would count for it. From the second lap on the stage's own wait implies it.)
-                    if (values && to == 0 && !(healthy = warp_wait(full, tph ^ 1))) break;
-                    if (lane == 0) mbar_expect_tx(full + to, C::STAGE);
+                    if (lane == 0) mbar_expect_tx(full + st, C::STAGE);
                     __syncwarp();
-                    if (copies) tma_load_2d(ring + st * C::STAGE + half * C::HALF + part * box * 128, map, 64 * (int)half, now, full + to);
+                    if (copies) tma_load_2d(ring + st * C::STAGE + half * C::HALF + part * box * 128, map, 64 * (int)half, now, full + st);
                     if (++st == C::STAGES) st = 0, ph ^= 1;
-                    if (++to == C::STAGES) to = 0, tph ^= 1;
                 }
                 if (healthy) work = next_piece(p, w);
             }
-            if (!values && u0 < at.u1 && !stale && healthy && (healthy = warp_wait(empty + st, ph)) && lane == 0) mbar_arrive(full + to);  // (no keys behind the last values)
             if (bad && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
             // the copies in flight have to land before the CTA leaves
-            if (values && u0 < at.u1 && !stale)  // (they are the last to land)
-                for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < to ? tph : tph ^ 1);
+            for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < st ? ph ^ 1 : ph);
             if (values)
                 for (int t = 0; t < 2; t++)
                     if (piece[t]) mbar_wait(q_full + t, (piece[t] - 1) & 1);
@@ -514,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
         float *const parts = (float *)((uint8_t *)p.plan + p.l.part_large);
         constexpr uint32_t PF = ROWS * (DP + 2);
         auto tile_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); };
-        uint32_t k = 0;  // steps so far
+        uint32_t k = 0, events = 0;  // steps so far, and times that it was ready
         for (; work; work = next_piece(p, w)) {
             if (t == 1 && !w.two) continue;
             const uint32_t local = row / s.g, token = (2 * w.tile + t) * s.tt + local, qh = w.head * s.g + (row - local * s.g);
@@ -524,21 +528,45 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             float m = -INFINITY, base = 0.0f;  // the maximum that the weights refer to
             uint64_t l0 = 0, l1 = 0;           // two pairs of sums
             const uint64_t c2 = pack2(c, c);
-            for (uint32_t j = 0; j < w.steps && healthy; j++) {
-                if (!(healthy = warp_wait(s_full + t, k & 1))) break;
+            uint32_t x[C::KEYS];
+            auto next_scores = [&](uint32_t step) -> bool {
+                if (!warp_wait(s_full + t, step & 1)) return false;
                 fence_after();
-                uint32_t x[C::KEYS];
                 load_scores(x, s_col);
-                loaded(x);
+                return true;
+            };
+            auto say_ready = [&]() {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(s_empty + t);  // the next scores may come
+                if (lane == 0) mbar_arrive(ready + 2 * (events & 1) + t);
+                events++;
+            };
+            if (healthy && (healthy = next_scores(k))) {
+                loaded(x);
+                say_ready();
+            }
+            for (uint32_t j = 0; j < w.steps && healthy; j++) {
                 const uint32_t key0 = (w.t.first + w.step + j) * C::KEYS;
                 if (__any_sync(0xffffffffu, (real && key0 + C::KEYS > hi) || key0 < lo)) {
-                    const uint32_t from = lo > key0 ? lo - key0 : 0u, to = hi > key0 ? hi - key0 : 0u;  // of the columns
+                    // a bit for each column that the row sees
+                    const uint32_t from = lo > key0 ? min(lo - key0, (uint32_t)C::KEYS) : 0u, to = hi > key0 ? min(hi - key0, (uint32_t)C::KEYS) : 0u;
 #pragma unroll
-                    for (uint32_t i = 0; i < (uint32_t)C::KEYS; i++)
-                        if (i < from || i >= to) x[i] = 0xff800000u;
+                    for (uint32_t g = 0; g < (uint32_t)C::KEYS; g += 32) {
+                        const uint32_t below = to > g ? (to - g >= 32 ? ~0u : (1u << (to - g)) - 1) : 0u, out = from > g ? (from - g >= 32 ? ~0u : (1u << (from - g)) - 1) : 0u;
+                        const uint32_t bits = below & ~out;
+#pragma unroll
+                        for (uint32_t i = 0; i < 32 && g + i < (uint32_t)C::KEYS; i++)
+                            if (!(bits & (1u << i))) x[g + i] = 0xff800000u;
+                    }
+                }
+                if (j == 0) {  // no maximum as yet: the scores' own
+                    float a4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) a4[i] = fmaxf(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+#pragma unroll
+                    for (int i = 8; i < C::KEYS; i += 2) a4[(i / 2) & 3] = fmaxf(fmaxf(a4[(i / 2) & 3], __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
+                    m = fmaxf(fmaxf(a4[0], a4[1]), fmaxf(a4[2], a4[3])) * c;
+                    base = m == -INFINITY ? 0.0f : m;
                 }
                 uint32_t wt[C::KEYS / 2];
                 uint64_t n0 = l0, n1 = l1;
@@ -569,11 +597,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 l0 = n0, l1 = n1;
                 if (!sound) l0 = pack2(NAN, NAN);
                 store_weights(p_col, wt);
-                st_wait();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + t);
                 k++;
+                if (j + 1 < w.steps && !(healthy = next_scores(k))) break;
+                st_wait();
+                if (j + 1 < w.steps) loaded(x);
+                say_ready();
             }
             // ---- the piece is done: O is complete behind its last product
             float a0, a1, a2, a3;
@@ -583,8 +611,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             if (a0 != a0) l = NAN;
             if (healthy) healthy = warp_wait(o_full + t, (k - 1) & 1);
             fence_after();
-            const bool whole = w.step == 0 && w.steps == w.t.steps;
-            const uint32_t i0 = w.u - w.step, i1 = i0 + w.t.steps;
+            const bool whole = w.steps == w.t.steps;
+            const uint32_t first_unit = w.i0 + PAGED_LARGE_EXTRA;
             unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
             auto store32 = [&](const float *v, uint32_t col) {  // 32 columns of the row
                 if (!real) return;
@@ -614,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             auto store_lse = [&](float mm, float ll) {
                 if (p.lse && real) p.lse[(size_t)(w.q0 + token) * s.hq + qh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
             };
-            float *mine = parts + (size_t)(2 * b + (i0 < u0 ? 0 : 1)) * PF + t * TILE + row;  // [column][row], then m, l
+            float *mine = parts + (size_t)(2 * b + (w.step ? 0 : 1)) * PF + t * TILE + row;  // [column][row], then m, l
             const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
 #pragma unroll 1
             for (int i = 0; i < DP / 32; i++) {
@@ -638,7 +666,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             }
             mine[(size_t)DP * ROWS] = m;
             mine[(size_t)(DP + 1) * ROWS] = l;
-            const uint32_t first = paged_holder(units, ctas, i0), last = paged_holder(units, ctas, i1 - 1);
+            const uint32_t first = paged_holder(units, ctas, first_unit), last = paged_holder(units, ctas, first_unit + w.t.steps - 1);
             tile_sync();
             if (row == 0) {
                 __threadfence();
@@ -658,19 +686,23 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 for (uint32_t i = first; i <= last; i++) ll = fmaf(__ldcg(piece(i) + (size_t)(DP + 1) * ROWS), exp2_fast(__ldcg(piece(i) + (size_t)DP * ROWS) - mb), ll);
                 const float il = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll 1
-                for (int ch = 0; ch < DP / 32; ch++) {
-                    float v[32];
+                for (int ch = 0; ch < DP / 64; ch++) {  // (64 loads in flight)
+                    float v[64];
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = 0.0f;
+                    for (int e = 0; e < 64; e++) v[e] = 0.0f;
                     for (uint32_t i = first; i <= last; i++) {
                         const float *src = piece(i);
                         const float f = exp2_fast(__ldcg(src + (size_t)DP * ROWS) - mb);
+                        float y[64];
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = fmaf(__ldcg(src + (size_t)(32 * ch + e) * ROWS), f, v[e]);
+                        for (int e = 0; e < 64; e++) y[e] = __ldcg(src + (size_t)(64 * ch + e) * ROWS);
+#pragma unroll
+                        for (int e = 0; e < 64; e++) v[e] = fmaf(y[e], f, v[e]);
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] *= il;
-                    store32(v, 32 * ch);
+                    for (int e = 0; e < 64; e++) v[e] *= il;
+                    store32(v, 64 * ch);
+                    store32(v + 32, 64 * ch + 32);
                 }
                 store_lse(mm, ll);
             }
