@@ -228,6 +228,10 @@ template <bool BF16, int N> __device__ __forceinline__ float weights(const uint3
     return max3(max3(top[0], top[1], top[2]), top[3], top[3]);
 }
 
+// The same value in all lanes, and the compiler knows it: what the tensor instructions take then stays in uniform registers (a step of 80 keys took
+// 2055 cycles without, 1716 with).
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 struct Walk {
     uint32_t r, head, tile, tiles, n, kv, q0;
     PagedTile t;
@@ -236,9 +240,9 @@ struct Walk {
     bool two;                // the second tile of 128 has rows
 };
 __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
-    w.q0 = p.plan[p.l.q_start + w.r];
-    w.n = p.plan[p.l.q_start + w.r + 1] - w.q0;
-    w.kv = p.plan[p.l.kv_len + w.r];
+    w.q0 = uniform(p.plan[p.l.q_start + w.r]);
+    w.n = uniform(p.plan[p.l.q_start + w.r + 1]) - w.q0;
+    w.kv = uniform(p.plan[p.l.kv_len + w.r]);
     w.tiles = paged_tiles(p.s, w.n, paged_large_rows(p.s));
 }
 // (steps 0: the span ends in what the tile counts in front of its steps)
@@ -286,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
     uint32_t *tmem_slot = (uint32_t *)(drained + 2);
     volatile uint32_t *is_last = tmem_slot + 1;
     const PagedShape &s = p.s;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
             mbar_init(k_full + i, 1);
@@ -312,19 +316,19 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t b = blockIdx.x;
     const PagedStart at = paged_load_start(p.plan + p.l.start_large + b * (sizeof(PagedStart) / 4));
-    const bool stale = at.stamp != p.stamp;
+    const bool stale = uniform(at.stamp) != p.stamp;
     if (stale && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
-    const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0;
-    bool work = !stale && u0 < at.u1, healthy = true;
+    const uint32_t units = uniform(at.units), ctas = uniform(at.ctas), u0 = uniform(at.u0), u1 = uniform(at.u1), place = uniform(at.place);
+    bool work = !stale && u0 < u1, healthy = true;
     Walk w{};
     if (work) {  // (a span may hold nothing but the front of a tile)
-        w.i0 = u0 - at.place, w.u1 = at.u1, w.r = at.r, w.head = at.head, w.tile = at.tile, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
-        w.step = at.place > PAGED_LARGE_EXTRA ? at.place - PAGED_LARGE_EXTRA : 0u;
+        w.i0 = u0 - place, w.u1 = u1, w.r = uniform(at.r), w.head = uniform(at.head), w.tile = uniform(at.tile), w.q0 = uniform(at.q0), w.n = uniform(at.n), w.kv = uniform(at.kv);
+        w.step = place > PAGED_LARGE_EXTRA ? place - PAGED_LARGE_EXTRA : 0u;
         w.tiles = paged_tiles(s, w.n, paged_large_rows(s));
         work = load_tile(p, w);
     }
