@@ -53,7 +53,7 @@ constexpr int Q_HALF = TILE * 128;  // bytes of 128 rows of 64 elements
 // Registers: 384 x 168 at launch = 256 x 208 + 128 x 88
 constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88;
 constexpr float LAZY = 8.0f;
-constexpr int POLY = 2;  // pairs of every eight whose exponentials are polynomials
+constexpr int POLY = 1;  // pairs of every eight whose exponentials are polynomials
 constexpr uint32_t WAIT_NS = 8000, SPIN_LIMIT = 1u << 19;  // a wait gives up after some two seconds
 
 template <int DP> struct Cfg {
@@ -179,26 +179,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 // 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a minimax polynomial in f (found by Remez's exchange; relative error 7.5e-5 at
-// degree 3, 2.6e-6 at degree 4: below half a unit of the weights' type, 2^-9 or 2^-12), n added to the exponent. For x <= 100; below -125 it stays 2^-125. The special-function unit forms
+// degree 3: below half a unit of the weights' type, 2^-9 or 2^-12), n added to the exponent. For x <= 100; below -125 it stays 2^-125. The special-function unit forms
 // 16 exponentials a cycle on an SM, and 128 x 128 of them take as long as the two products of 128 x 128 x 128: what it is relieved of here costs
 // five issue slots an element that the schedulers have.
-template <int DEGREE> __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
+__device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
     float a, b;
     unpack2(x, a, b);
     x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
     const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));  // 1.5 2^23: n in the low bits
-    const uint64_t f = add2(x, pipe::mul2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f)));
-    uint64_t y;
-    if constexpr (DEGREE == 3) {
-        y = fma2(f, pack2(0.0551716685f, 0.0551716685f), pack2(0.242611125f, 0.242611125f));
-        y = fma2(f, y, pack2(0.693260968f, 0.693260968f));
-        y = fma2(f, y, pack2(0.999928057f, 0.999928057f));
-    } else {
-        y = fma2(f, pack2(0.00957010221f, 0.00957010221f), pack2(0.0559178591f, 0.0559178591f));
-        y = fma2(f, y, pack2(0.240247443f, 0.240247443f));
-        y = fma2(f, y, pack2(0.693121791f, 0.693121791f));
-        y = fma2(f, y, pack2(0.999999285f, 0.999999285f));
-    }
+    const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
+    uint64_t y = fma2(f, pack2(0.0551716685f, 0.0551716685f), pack2(0.242611125f, 0.242611125f));
+    y = fma2(f, y, pack2(0.693260968f, 0.693260968f));
+    y = fma2(f, y, pack2(0.999928057f, 0.999928057f));
     float y0, y1, t0, t1;
     unpack2(y, y0, y1);
     unpack2(t, t0, t1);
@@ -216,7 +208,7 @@ template <bool BF16, int N> __device__ __forceinline__ float weights(const uint3
         const uint64_t y = fma2(pack2(x0, x1), c2, b2);
         float e0, e1;
         if ((i & 7) < POLY) {
-            exp2_poly<BF16 ? 3 : 4>(y, e0, e1);
+            exp2_poly(y, e0, e1);
         } else {
             unpack2(y, e0, e1);
             e0 = exp2_fast(e0), e1 = exp2_fast(e1);
@@ -405,6 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                     if (!(healthy = warp_wait(ready + 2 * (events & 1) + t, (events >> 1) & 1))) break;
                     events++;
                     fence_after();
+                    // (the scores first: the softmax waits for them sooner)
                     if (more) {
                         scores(j + 2 == w.steps);
                     } else if (first) {
@@ -533,10 +526,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             uint64_t l0 = 0, l1 = 0;           // two pairs of sums
             const uint64_t c2 = pack2(c, c);
             uint32_t x[C::KEYS];
-            auto next_scores = [&](uint32_t step) -> bool {
+            auto wait_scores = [&](uint32_t step) -> bool {
                 if (!warp_wait(s_full + t, step & 1)) return false;
                 fence_after();
-                load_scores(x, s_col);
                 return true;
             };
             auto say_ready = [&]() {
@@ -545,7 +537,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 if (lane == 0) mbar_arrive(ready + 2 * (events & 1) + t);
                 events++;
             };
-            if (healthy && (healthy = next_scores(k))) {
+            if (healthy && (healthy = wait_scores(k))) {
+                load_scores(x, s_col);
                 loaded(x);
                 say_ready();
             }
@@ -602,9 +595,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 if (!sound) l0 = pack2(NAN, NAN);
                 store_weights(p_col, wt);
                 k++;
-                if (j + 1 < w.steps && !(healthy = next_scores(k))) break;
+                const bool more = j + 1 < w.steps;
+                if (more && !(healthy = wait_scores(k))) break;
+                if (more) load_scores(x, s_col);
                 st_wait();
-                if (j + 1 < w.steps) loaded(x);
+                if (more) loaded(x);
                 say_ready();
             }
             // ---- the piece is done: O is complete behind its last product
