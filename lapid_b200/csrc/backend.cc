@@ -2513,6 +2513,7 @@ lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *dev, const lapid
         a.status = dev->status_dev;
         // requests of many rows first: their CTAs run longest
         if (lb::paged_has_large(a.s)) {
+            a.behind = true;
             cuda_check(lb::launch_paged_attn_large(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
             dev->launches++;
         }

@@ -396,6 +396,9 @@ constexpr uint32_t PAGED_SMALL_LIMIT = 16;                             // reques
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
 constexpr uint32_t PAGED_LARGE_EXTRA = 3;                              // steps that beginning and ending one of its tiles takes as long as
 constexpr uint32_t PAGED_SMALL_MIN = 4, PAGED_LARGE_MIN = 6;             // fewest units worth a CTA of its own
+// What a unit of either kernel takes of an SM, in ns, at 128 / 64 elements a head: of the kernel for few rows when it shares the chip with the other (alone
+// it is bound by all SMs' common memory, here by what one SM can have in flight)
+constexpr uint32_t PAGED_SMALL_NS_128 = 360, PAGED_SMALL_NS_64 = 180, PAGED_LARGE_NS_128 = 1000, PAGED_LARGE_NS_64 = 1350;
 constexpr uint32_t PAGED_MAX_SMS = 160;
 struct PagedShape {
     int bf16;  // cache, q and out: bf16, else f16
@@ -449,6 +452,7 @@ struct PagedAttnArgs {
     void *out;
     float *lse;
     int *status;
+    bool behind;  // the kernel for few rows: the one for many is in front of it, and nothing it needs comes from there
 };
 uint32_t paged_attn_small_ctas(int sm_count);
 uint32_t paged_attn_large_ctas(int sm_count);

@@ -253,8 +253,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
     }
     if (!counts) return;
     __syncthreads();
-    const uint32_t cs = small < a.ctas_small * PAGED_SMALL_MIN ? (small + PAGED_SMALL_MIN - 1) / PAGED_SMALL_MIN : a.ctas_small;
-    const uint32_t cl = large < a.ctas_large * PAGED_LARGE_MIN ? (large + PAGED_LARGE_MIN - 1) / PAGED_LARGE_MIN : a.ctas_large;
+    uint32_t cs = small < a.ctas_small * PAGED_SMALL_MIN ? (small + PAGED_SMALL_MIN - 1) / PAGED_SMALL_MIN : a.ctas_small;
+    uint32_t cl = large < a.ctas_large * PAGED_LARGE_MIN ? (large + PAGED_LARGE_MIN - 1) / PAGED_LARGE_MIN : a.ctas_large;
+    if (small && large) {
+        // Both kernels have work, one bound by memory, the other by its products: they run side by side, on as many SMs as their shares of the work
+        // (a chunk of 512 tokens beside 11 tokens of other requests, 3000 keys each: one after the other 83 us, side by side 62). Every CTA of the kernel for many rows holds an SM; the other's come, two to an SM,
+        // where one of those had nothing to do.
+        const uint64_t ts = (uint64_t)small * (s.d > 64 ? PAGED_SMALL_NS_128 : PAGED_SMALL_NS_64), tl = (uint64_t)large * (s.d > 64 ? PAGED_LARGE_NS_128 : PAGED_LARGE_NS_64);
+        const uint32_t sms = a.ctas_large, share = (uint32_t)(sms * tl / (ts + tl));
+        cl = min(cl, max(share, 1u));
+        cs = min(cs, max(a.ctas_small / sms * (sms - cl), 1u));
+    }
     const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start;
     const uint32_t warp = worker * (PLAN_THREADS / 32) + tid / 32, warps = (one ? workers : 1) * (PLAN_THREADS / 32);
     cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);

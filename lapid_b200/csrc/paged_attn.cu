@@ -122,16 +122,19 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
         mbar_fence_init();
     }
     __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // Behind the kernel for many rows nothing needs to be waited for: it let this one start when all that was in front of it was over, and the two share no
+    // memory that either writes. But this grid's end has to mean that one's too: its first CTA waits before it leaves.
+    const bool holds = p.behind && blockIdx.x == 0;
+    if (!p.behind) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t b = blockIdx.x;
     const PagedStart at = paged_load_start(p.plan + p.l.start_small + b * (sizeof(PagedStart) / 4));
-    if (at.stamp != p.stamp) {
-        if (threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
+    if (at.stamp != p.stamp && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
+    const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0, u1 = at.u1;
+    if (at.stamp != p.stamp || u0 == u1) {
+        if (holds) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
-    const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0, u1 = at.u1;
-    if (u0 == u1) return;
     Walk w;
     w.r = at.r, w.head = at.head, w.tile = at.tile, w.q0 = at.q0, w.n = at.n, w.kv = at.kv;
     w.tiles = paged_tiles(s, w.n, ROWS);
@@ -172,6 +175,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
         // the copies in flight have to land before the CTA leaves
         for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < stage ? ph ^ 1 : ph, SPIN_LIMIT);
         if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
+        if (holds) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 

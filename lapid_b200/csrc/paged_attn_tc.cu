@@ -81,6 +81,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
     return ok;
 }
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// Whether the phase is over now
+__device__ __forceinline__ bool warp_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(s32(bar)), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, ok);
+}
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
@@ -373,13 +379,12 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                     scores(w.steps == 1);
                 }
                 // Event j: the scores of step j have been read, and the weights of step j - 1 are there. Then the scores behind them may be formed, of step
-                // j + 1 or of the next piece's first, and the weights multiplied. (Event `steps`: the last weights are there.)
+                // j + 1 or of the next piece's first, and the weights multiplied. (Event `steps`: the last weights are there.) The next piece's Q comes
+                // when these scores have read theirs: if it is not there at event `steps` - 1, its scores are left until the last weights are multiplied.
+                begun = false;
                 for (uint32_t j = 0; j <= w.steps && healthy; j++) {
-                    const bool more = j + 1 < w.steps, first = j + 1 == w.steps && next_mine;
-                    if (more || first) {
-                        if (!(healthy = warp_wait(k_full + ks, kph))) break;
-                        if (first && !(healthy = warp_wait(q_full + t, piece & 1))) break;
-                    }
+                    const bool more = j + 1 < w.steps, first = j + 1 == w.steps && next_mine && warp_test(k_full + ks, kph) && warp_test(q_full + t, piece & 1);
+                    if (more && !(healthy = warp_wait(k_full + ks, kph))) break;
                     if (j) {
                         if (!(healthy = warp_wait(v_full + vs, vph))) break;
                         // values of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0 (both warps do it: zeros twice)
@@ -402,6 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                         scores(j + 2 == w.steps);
                     } else if (first) {
                         piece++;
+                        begun = true;
                         scores(next.steps == 1);
                     }
                     if (j) {
@@ -416,7 +422,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                         if (++vs == C::STAGES) vs = 0, vph ^= 1;
                     }
                 }
-                begun = next_mine;
                 w = next, work = follows;
             }
             // no product may be under way when tensor memory is released, and nothing may arrive in this CTA's shared memory behind its end
