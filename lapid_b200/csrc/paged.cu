@@ -5,8 +5,9 @@
 //         free_pages[first[r]...] in the requests' order, so the result does not depend on timing. The plan also cuts the work of
 //         the attention launches that follow (paged.cuh): which request, head, tile and step each CTA begins with. That is
 //         done once a step, and every layer's launch reads it.
-//         What bounds it is latency: one launch, four scans over the requests, a search a token and a search a start. Every CTA scans the
-//         lengths itself (1024 requests at a time) so that nothing passes between CTAs, and takes its share of the tokens, blocks and starts.
+//         What bounds it is latency: one launch, two scans over the requests, a search a token and a search a start. Every CTA scans the
+//         lengths itself so that nothing passes between CTAs, and takes its share of the tokens, blocks and starts. 64 requests of one token 4.2 us, 48
+//         prompts (65520 tokens) 8.1.
 // append  (x, y) -> (x cos - y sin, y cos + x sin) in f32 for the rotary pairs of q and k, one rounding to the cache's type; k and v go
 //         to their slots. Bound by memory: each element is read once and written once; a thread keeps the angles of its
 //         four pairs in registers over the heads of a token.
@@ -55,38 +56,40 @@ uint32_t paged_stamp(const PagedShape &s) {
 }
 
 // ------------------------------------------------------------------ plan
-constexpr uint32_t PLAN_THREADS = 1024;
-
-struct PlanShared {
-    uint32_t warp_sum[32];
-    uint32_t start[PLAN_THREADS + 1], first[PLAN_THREADS + 1], cached[PLAN_THREADS], have[PLAN_THREADS];
-    uint32_t small[PLAN_THREADS + 1], large[PLAN_THREADS + 1];  // units before the request
+// T threads take T requests at a time: 256 where there are no more (64 requests: 4.2 us, with 1024 threads and a scan for each sum 6.7), else 1024.
+template <uint32_t T> struct PlanShared {
+    uint64_t warp_sum[T / 32];
+    uint32_t start[T + 1], first[T + 1], cached[T], have[T], kv[T];
+    uint32_t small[T + 1], large[T + 1];    // units before the request
+    uint32_t tiles[T + 1], steps[T];        // of many rows: tiles before the request, units of its tiles for one head
 };
 
-// Sum over the threads before this one; `total`: over all
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, PlanShared &sh, uint32_t &total) {
+// Two sums at once (low and high half) over the threads before this one; `total`: over all
+template <uint32_t T> __device__ __forceinline__ uint64_t block_scan(uint64_t v, PlanShared<T> &sh, uint64_t &total) {
+    constexpr uint32_t WARPS = T / 32;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t inc = v;
+    uint64_t inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        const uint64_t x = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += x;
     }
     __syncthreads();  // the sums of the scan before have been read
     if (lane == 31) sh.warp_sum[warp] = inc;
     __syncthreads();
-    uint32_t w = sh.warp_sum[lane], winc = w;
+    uint64_t w = lane < WARPS ? sh.warp_sum[lane] : 0, winc = w;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, winc, o);
+    for (int o = 1; o < (int)WARPS; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(0xffffffffu, winc, o);
         if (lane >= o) winc += x;
     }
-    total = __shfl_sync(0xffffffffu, winc, 31);
+    total = __shfl_sync(0xffffffffu, winc, WARPS - 1);
     return __shfl_sync(0xffffffffu, winc - w, warp) + inc - v;
 }
+__device__ __forceinline__ uint64_t both(uint32_t lo, uint32_t hi) { return lo | (uint64_t)hi << 32; }
 
 // The last i < n with a[i] <= x (a rises, a[0] <= x)
-template <class T> __device__ __forceinline__ uint32_t last_at_most(const T *a, uint32_t n, uint32_t x) {
+__device__ __forceinline__ uint32_t last_at_most(const uint32_t *a, uint32_t n, uint32_t x) {
     uint32_t lo = 0, hi = n;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
@@ -96,36 +99,20 @@ template <class T> __device__ __forceinline__ uint32_t last_at_most(const T *a, 
     return lo;
 }
 
-// Units of all tiles of a request and one key/value head; long requests are shared by the warp (every lane of a warp calls it)
-__device__ uint32_t head_units(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t rows, uint32_t keys, uint32_t extra, bool mine) {
-    const uint32_t lane = threadIdx.x & 31, tiles = mine && n ? paged_tiles(s, n, rows) : 0;
-    uint32_t sum = 0;
-    if (tiles <= 16)
-        for (uint32_t i = 0; i < tiles; i++) sum += paged_tile(s, n, kv, i, rows, keys).steps + extra;
-    for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 16); many; many &= many - 1) {
-        const int who = __ffs(many) - 1;
-        const uint32_t n1 = __shfl_sync(0xffffffffu, n, who), kv1 = __shfl_sync(0xffffffffu, kv, who), t1 = __shfl_sync(0xffffffffu, tiles, who);
-        uint32_t part = 0;
-        for (uint32_t i = lane; i < t1; i += 32) part += paged_tile(s, n1, kv1, i, rows, keys).steps + extra;
-        part = __reduce_add_sync(0xffffffffu, part);
-        if ((int)lane == who) sum = part;
-    }
-    return sum;
-}
-
-// What each CTA of an attention launch begins with: warp `worker` of `workers` takes every workers-th of them. `prefix`: units before each request, `q0` first row.
-__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, const uint32_t *q0, uint32_t *starts, uint32_t rows, uint32_t keys,
-                          uint32_t extra, uint32_t worker, uint32_t workers) {
+// What each CTA of an attention launch begins with: warp `worker` of `workers` takes every workers-th of them. `prefix`: units before each request, `q0` its first
+// row, `kv` its keys.
+__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, const uint32_t *q0, const uint32_t *kv, uint32_t *starts, uint32_t rows,
+                          uint32_t keys, uint32_t extra, uint32_t worker, uint32_t workers) {
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t b = worker; b < all; b += workers) {
         PagedStart x{};
         x.stamp = a.stamp, x.units = units, x.ctas = ctas;
         if (b < ctas) {
-            x.u0 = paged_span(units, ctas, b), x.u1 = paged_span(units, ctas, b + 1);
+            x.u0 = paged_span(units, ctas, b + (lane & 1));  // (an even lane: where the span begins, an odd one: where it ends)
+            x.u1 = __shfl_sync(0xffffffffu, x.u0, 1);
+            x.u0 = __shfl_sync(0xffffffffu, x.u0, 0);
             const uint32_t r = last_at_most(prefix, a.s.requests, x.u0);
-            x.r = r, x.q0 = q0[r], x.n = q0[r + 1] - x.q0;
-            const uint32_t c = (uint32_t)a.cached[r];
-            x.kv = a.s.mask == PAGED_CROSS ? c : c + x.n;
+            x.r = r, x.q0 = q0[r], x.n = q0[r + 1] - x.q0, x.kv = kv[r];
             const uint32_t per_head = (prefix[r + 1] - prefix[r]) / a.s.hkv, off = x.u0 - prefix[r], tiles = paged_tiles(a.s, x.n, rows);
             x.head = off / per_head;
             uint32_t rem = off - x.head * per_head;
@@ -148,89 +135,100 @@ __device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas,
             }
             x.place = rem;
         }
-        const uint32_t w[12] = {x.stamp, x.units, x.ctas, x.u0, x.u1, x.r, x.head, x.tile, x.place, x.q0, x.n, x.kv};
         if (lane < 3) {
-            uint4 v = make_uint4(w[0], w[1], w[2], w[3]);
-            if (lane == 1) v = make_uint4(w[4], w[5], w[6], w[7]);
-            if (lane == 2) v = make_uint4(w[8], w[9], w[10], w[11]);
+            uint4 v = make_uint4(x.stamp, x.units, x.ctas, x.u0);
+            if (lane == 1) v = make_uint4(x.u1, x.r, x.head, x.tile);
+            if (lane == 2) v = make_uint4(x.place, x.q0, x.n, x.kv);
             ((uint4 *)starts)[b * (sizeof(PagedStart) / 16) + lane] = v;
         }
     }
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs a) {
+template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(PagedPlanArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ PlanShared sh;
+    __shared__ PlanShared<T> sh;
     const PagedShape &s = a.s;
-    const uint32_t tid = threadIdx.x, worker = blockIdx.x, workers = gridDim.x;
-    const bool one = s.requests <= PLAN_THREADS;  // chunk: what the searches for the starts need stays in shared memory
+    const uint32_t tid = threadIdx.x, worker = blockIdx.x, workers = gridDim.x, shift = 31 - __clz(s.page);  // (page sizes are powers of two)
+    const bool one = s.requests <= T;  // chunk: what the searches for the starts need stays in shared memory
     const bool counts = one || blockIdx.x == 0, writes = blockIdx.x == 0;
     uint32_t base = 0, taken = 0, small = 0, large = 0;  // tokens, pages and units of the chunks before
     uint32_t bad = 0;
-    for (uint32_t r0 = 0; r0 < s.requests; r0 += PLAN_THREADS) {
-        const uint32_t r = r0 + tid, count = min(PLAN_THREADS, s.requests - r0);
+    for (uint32_t r0 = 0; r0 < s.requests; r0 += T) {
+        const uint32_t r = r0 + tid, count = min(T, s.requests - r0);
         uint32_t n = 0, c = 0, have = 0, need = 0;
         if (r < s.requests) {
             const int32_t n0 = a.new_lens[r], c0 = a.cached[r];
-            const int64_t blocks = ((int64_t)c0 + (s.mask == PAGED_CROSS ? 0 : n0) + s.page - 1) / s.page;
-            if (n0 < 0 || c0 < 0 || n0 > (int64_t)s.max_new || blocks > (int64_t)s.max_blocks) {
+            const uint64_t blocks = ((uint64_t)(uint32_t)c0 + (s.mask == PAGED_CROSS ? 0u : (uint32_t)n0) + s.page - 1) >> shift;
+            if (n0 < 0 || c0 < 0 || (uint32_t)n0 > s.max_new || blocks > s.max_blocks) {
                 bad |= PAGED_STATUS_LENGTHS;  // such a request takes no part
             } else {
                 n = (uint32_t)n0, c = (uint32_t)c0;
-                have = (c + s.page - 1) / s.page;
+                have = (c + s.page - 1) >> shift;
                 need = (uint32_t)blocks;
             }
         }
-        uint32_t total_n, total_p;
-        const uint32_t at_n = base + block_scan(n, sh, total_n), at_p = taken + block_scan(need - have, sh, total_p);
+        uint64_t total;
+        uint64_t at = block_scan<T>(both(n, need - have), sh, total);
         // (rows behind the last one of q: such tokens take no part)
-        const uint32_t lo = min(at_n, s.tokens), hi = min(at_n + n, s.tokens);
+        const uint32_t at_n = base + (uint32_t)at, lo = min(at_n, s.tokens), hi = min(at_n + n, s.tokens), at_p = taken + (uint32_t)(at >> 32);
+        const uint32_t end_n = min(base + (uint32_t)total, s.tokens), end_p = taken + (uint32_t)(total >> 32);
         if (hi - lo != n) bad |= PAGED_STATUS_LENGTHS;
         n = hi - lo;
+        const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
         sh.start[tid] = lo;
         sh.first[tid] = at_p;
         sh.cached[tid] = c;
         sh.have[tid] = have;
-        const uint32_t end_n = min(base + total_n, s.tokens), end_p = taken + total_p;
-        if (tid == 0) sh.start[count] = end_n, sh.first[count] = end_p;  // (count < PLAN_THREADS: the thread of that place writes the same)
-        const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
+        sh.kv[tid] = kv;
+        if (tid == 0) sh.start[count] = end_n, sh.first[count] = end_p;  // (count < T: the thread of that place writes the same)
         if (counts) {
             const bool few = paged_is_small(s, n);
-            const uint32_t us = head_units(s, n, kv, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, few) * s.hkv;
-            const uint32_t ul = a.ctas_large ? head_units(s, n, kv, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, !few) * s.hkv : 0;
-            uint32_t total_s, total_l = 0;
-            const uint32_t at_s = small + block_scan(us, sh, total_s), at_l = a.ctas_large ? large + block_scan(ul, sh, total_l) : 0;
-            small += total_s, large += total_l;
-            if (one) {
-                sh.small[tid] = at_s, sh.large[tid] = at_l;
-                if (tid == 0) sh.small[count] = small, sh.large[count] = large;
-            } else if (r < s.requests) {
-                a.plan[a.l.units_small + r] = at_s;
-                a.plan[a.l.units_large + r] = at_l;
+            uint32_t us = 0, ul = 0;
+            if (few && n)
+                for (uint32_t i = 0; i < paged_tiles(s, n, PAGED_SMALL_ROWS); i++) us += paged_tile(s, n, kv, i, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS).steps;
+            if (a.ctas_large) {  // all tiles of many rows, a thread each (they add whole numbers: in whatever order)
+                const uint32_t rows = paged_large_rows(s), tiles = few ? 0 : paged_tiles(s, n, rows);
+                const uint32_t before = (uint32_t)block_scan<T>(tiles, sh, total);
+                sh.tiles[tid] = before;
+                sh.steps[tid] = 0;
+                if (tid == 0) sh.tiles[count] = (uint32_t)total;
+                __syncthreads();
+                for (uint32_t i = tid; i < (uint32_t)total; i += T) {
+                    const uint32_t q = last_at_most(sh.tiles, count, i);
+                    atomicAdd(&sh.steps[q], paged_tile(s, sh.start[q + 1] - sh.start[q], sh.kv[q], i - sh.tiles[q], rows, s.large_keys).steps + PAGED_LARGE_EXTRA);
+                }
+                __syncthreads();
+                ul = sh.steps[tid];
             }
+            at = block_scan<T>(both(us * s.hkv, ul * s.hkv), sh, total);
+            sh.small[tid] = small + (uint32_t)at, sh.large[tid] = large + (uint32_t)(at >> 32);
+            small += (uint32_t)total, large += (uint32_t)(total >> 32);
+            if (tid == 0) sh.small[count] = small, sh.large[count] = large;
         }
         if (writes && r < s.requests) {
             a.plan[a.l.q_start + r] = lo;
             a.plan[a.l.kv_len + r] = kv;
             a.kv_lens[r] = (int32_t)kv;
+            if (!one) a.plan[a.l.units_small + r] = sh.small[tid], a.plan[a.l.units_large + r] = sh.large[tid];
         }
         __syncthreads();
-        for (uint32_t j = taken + worker * PLAN_THREADS + tid; j < end_p; j += workers * PLAN_THREADS) {
+        for (uint32_t j = taken + worker * T + tid; j < end_p; j += workers * T) {
             const uint32_t i = last_at_most(sh.first, count, j);
             int32_t page = -1;
             if (j >= a.n_free) bad |= PAGED_STATUS_PAGES;
             else if ((page = a.free_pages[j]) < 0 || (uint32_t)page >= s.pages) page = -1, bad |= PAGED_STATUS_INDEX;
             a.table[(size_t)(r0 + i) * s.max_blocks + sh.have[i] + (j - sh.first[i])] = page;
         }
-        for (uint32_t t = base + worker * PLAN_THREADS + tid; t < end_n; t += workers * PLAN_THREADS) {
-            const uint32_t i = last_at_most(sh.start, count, t), pos = sh.cached[i] + (t - sh.start[i]), block = pos / s.page;
+        // (the last CTA begins: the first one has the pages)
+        for (uint32_t t = base + (workers - 1 - worker) * T + tid; t < end_n; t += workers * T) {
+            const uint32_t i = last_at_most(sh.start, count, t), pos = sh.cached[i] + (t - sh.start[i]), block = pos >> shift;
             int32_t slot = -1;
             if (s.mask != PAGED_CROSS) {
                 int32_t page = -1;
                 if (block < sh.have[i]) page = a.table[(size_t)(r0 + i) * s.max_blocks + block];
                 else if (sh.first[i] + (block - sh.have[i]) < a.n_free) page = a.free_pages[sh.first[i] + (block - sh.have[i])];
-                if (page >= 0 && (uint32_t)page < s.pages) slot = (int32_t)((uint32_t)page * s.page + pos % s.page);
+                if (page >= 0 && (uint32_t)page < s.pages) slot = (int32_t)(((uint32_t)page << shift) + (pos & (s.page - 1)));
                 else if (block < sh.have[i]) bad |= PAGED_STATUS_INDEX;
             }
             a.slots[t] = slot;
@@ -240,7 +238,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
         taken = end_p;
         if (!one) __syncthreads();  // the tables of this chunk are read
     }
-    for (uint32_t t = base + worker * PLAN_THREADS + tid; t < s.tokens; t += workers * PLAN_THREADS) a.slots[t] = a.positions[t] = -1;
+    for (uint32_t t = base + worker * T + tid; t < s.tokens; t += workers * T) a.slots[t] = a.positions[t] = -1;
     if (bad && a.status) atomicOr(a.status, (int)bad);
     if (writes) {
         if (tid == 0) {
@@ -248,11 +246,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
             *a.used = (int32_t)taken;
             if (!one) a.plan[a.l.units_small + s.requests] = small, a.plan[a.l.units_large + s.requests] = large;
         }
-        for (uint32_t b = tid; b < a.ctas_small; b += PLAN_THREADS) a.plan[a.l.count_small + b] = 0;
-        for (uint32_t b = tid; b < 2 * a.ctas_large; b += PLAN_THREADS) a.plan[a.l.count_large + b] = 0;
+        for (uint32_t b = tid; b < a.ctas_small; b += T) a.plan[a.l.count_small + b] = 0;
+        for (uint32_t b = tid; b < 2 * a.ctas_large; b += T) a.plan[a.l.count_large + b] = 0;
     }
     if (!counts) return;
-    __syncthreads();
+    if (!one) __syncthreads();  // (the tables in the plan are read)
     uint32_t cs = small < a.ctas_small * PAGED_SMALL_MIN ? (small + PAGED_SMALL_MIN - 1) / PAGED_SMALL_MIN : a.ctas_small;
     uint32_t cl = large < a.ctas_large * PAGED_LARGE_MIN ? (large + PAGED_LARGE_MIN - 1) / PAGED_LARGE_MIN : a.ctas_large;
     if (small && large) {
@@ -264,10 +262,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PagedPlanArgs 
         cl = min(cl, max(share, 1u));
         cs = min(cs, max(a.ctas_small / sms * (sms - cl), 1u));
     }
-    const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start;
-    const uint32_t warp = worker * (PLAN_THREADS / 32) + tid / 32, warps = (one ? workers : 1) * (PLAN_THREADS / 32);
-    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);
-    if (a.ctas_large) cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, warp, warps);
+    const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start, *kv = one ? sh.kv : a.plan + a.l.kv_len;
+    const uint32_t warp = worker * (T / 32) + tid / 32, warps = (one ? workers : 1) * (T / 32);
+    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, kv, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);
+    // (from the other end: a warp has a start of one kind or of the other)
+    if (a.ctas_large)
+        cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, kv, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, warps - 1 - warp, warps);
 }
 
 static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim3 grid, unsigned threads, size_t smem, bool pdl, cudaStream_t stream) {
@@ -283,12 +283,13 @@ static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim
 }
 
 cudaError_t launch_paged_plan(const PagedPlanArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
-    // a CTA for 1024 tokens, and for 32 starts (a warp each)
-    const uint32_t starts = (a.ctas_small + a.ctas_large + 31) / 32, tokens = (a.s.tokens + PLAN_THREADS - 1) / PLAN_THREADS, want = starts > tokens ? starts : tokens;
+    const uint32_t T = a.s.requests <= 256 ? 256 : 1024;
+    // a thread for each token, a warp for each start
+    const uint32_t starts = (a.ctas_small + a.ctas_large + T / 32 - 1) / (T / 32), tokens = (a.s.tokens + T - 1) / T, want = starts > tokens ? starts : tokens;
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[1];
-    paged_config(cfg, attr, dim3(want < (uint32_t)sm_count ? want : (uint32_t)sm_count), PLAN_THREADS, 0, pdl, stream);
-    return cudaLaunchKernelEx(&cfg, paged_plan_kernel, a);
+    paged_config(cfg, attr, dim3(want < (uint32_t)sm_count ? want : (uint32_t)sm_count), T, 0, pdl, stream);
+    return T == 256 ? cudaLaunchKernelEx(&cfg, paged_plan_kernel<256>, a) : cudaLaunchKernelEx(&cfg, paged_plan_kernel<1024>, a);
 }
 
 // ------------------------------------------------------------------ append

@@ -74,6 +74,18 @@ def test_plan_says_when_the_free_pages_run_out(be):
     be.synchronize()
 
 
+def test_plan_refuses_lengths_whose_sum_passes_32_bits(be):
+    s = R.Step(be, [1], [4]).upload()
+    spec = PagedSpec(dtype=BF16, q_heads=1, kv_heads=1, head_dim=16, page_size=16, pages=4, requests=1, tokens=4, max_blocks=4, max_new=2 ** 31 - 1)
+    big = np.array([2 ** 31 - 1], np.int32)
+    z = lambda n: be.upload(np.zeros(n, np.int32))
+    table, used = z(4), z(1)
+    be.paged_plan(spec, be.upload(big), be.upload(big), table, z(4), z(4), z(1), used, be.alloc(plan_bytes(spec)), free_pages=s.b["free"], n_free=1)
+    with pytest.raises(lp.LapidError) as e:
+        be.synchronize()
+    assert e.value.code == "shape_mismatch" and not used.download().any() and not table.download().any()
+
+
 @pytest.mark.parametrize("new,cached", [([1, -1, 2], [4, 4, 4]), ([1, 2, 2], [4, -3, 4]), ([1, 9, 2], [4, 4, 4]), ([1, 1, 2], [4, 1000, 4]), ([8, 8, 8], [0, 0, 0])])
 def test_plan_refuses_lengths_outside_the_bounds(be, new, cached):
     s = R.Step(be, [1, 3, 2], [4, 4, 4], max_new=8).upload()
