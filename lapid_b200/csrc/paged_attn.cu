@@ -14,6 +14,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged.cuh"
 #include "pipe.cuh"
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
                 const float4 x = *(const float4 *)(meet + (k * ROWS + my_row) * PITCH + my_col);
                 v = make_float4(fmaf(x.x, f[k], v.x), fmaf(x.y, f[k], v.y), fmaf(x.z, f[k], v.z), fmaf(x.w, f[k], v.w));
             }
-            if (!whole) *(float4 *)(part + (size_t)slot * pf + my_row * DP + ch * CHUNK + my_col) = v;
+            if (!whole && real) *(float4 *)(part + (size_t)slot * pf + my_row * DP + ch * CHUNK + my_col) = v;
             else if (real) store_half4(orow, ch * CHUNK + my_col, s.d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), BF16, out4);
             warps_sync();
         }
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
         if (whole) {
             finish_lse(big, sum);
         } else {
-            if (tid % 8 == 0) {
+            if (tid % 8 == 0 && real) {
                 part[(size_t)slot * pf + ROWS * DP + my_row] = big;
                 part[(size_t)slot * pf + ROWS * (DP + 1) + my_row] = sum;
             }
@@ -351,32 +353,60 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
             }
             warps_sync();
             if (*is_last) {
-                float mm = -INFINITY, ss = 0.0f;
-                float4 v[DP / CHUNK];
-                for (uint32_t k = first; k <= last; k++) {
-                    const float *src = part + (size_t)(2 * k + (k == first ? 1 : 0)) * pf;
-                    mm = fmaxf(mm, __ldcg(src + ROWS * DP + my_row));
-                }
-                const float mb = mm == -INFINITY ? 0.0f : mm;
+                // (a tile's first piece is the end of its CTA's span, the others are the beginning of theirs)
+                auto piece = [&](uint32_t k) -> const float * { return part + (size_t)(2 * k + (k == first ? 1 : 0)) * pf; };
+                const uint32_t quads = min(w.n * s.g - w.tile * ROWS, (uint32_t)ROWS) * (DP / 4);  // four columns of one of the rows that there are
+                // a thread has N of them, and B pieces of each in flight: what this takes is the way to memory, and with few rows once
+                auto join = [&](auto count, auto batch) {
+                    constexpr int N = decltype(count)::value, B = decltype(batch)::value;
+                    float rm[N], rl[N];
+                    float4 v[N];
 #pragma unroll
-                for (int ch = 0; ch < DP / CHUNK; ch++) v[ch] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                for (uint32_t k = first; k <= last; k++) {
-                    // (a tile's first piece is the end of its CTA's span, the others are the beginning of theirs)
-                    const float *src = part + (size_t)(2 * k + (k == first ? 1 : 0)) * pf;
-                    const float e = exp2_fast(__ldcg(src + ROWS * DP + my_row) - mb);
-                    ss = fmaf(__ldcg(src + ROWS * (DP + 1) + my_row), e, ss);
+                    for (int i = 0; i < N; i++) rm[i] = -INFINITY, rl[i] = 0.0f, v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (uint32_t k0 = first; k0 <= last; k0 += B) {
+                        float mk[B][N], lk[B][N];
+                        float4 x[B][N];
 #pragma unroll
-                    for (int ch = 0; ch < DP / CHUNK; ch++) {
-                        const float4 x = __ldcg((const float4 *)(src + my_row * DP + ch * CHUNK + my_col));
-                        v[ch] = make_float4(fmaf(x.x, e, v[ch].x), fmaf(x.y, e, v[ch].y), fmaf(x.z, e, v[ch].z), fmaf(x.w, e, v[ch].w));
+                        for (int k = 0; k < B; k++)
+#pragma unroll
+                            for (int i = 0; i < N; i++) {
+                                const uint32_t q = tid + 32 * WARPS * i;
+                                const bool there = k0 + k <= last && q < quads;
+                                const float *src = piece(there ? k0 + k : first);
+                                mk[k][i] = there ? __ldcg(src + ROWS * DP + q / (DP / 4)) : -INFINITY;
+                                lk[k][i] = there ? __ldcg(src + ROWS * (DP + 1) + q / (DP / 4)) : 0.0f;
+                                x[k][i] = there ? __ldcg((const float4 *)src + q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            }
+#pragma unroll
+                        for (int i = 0; i < N; i++) {
+                            float mm = rm[i];
+#pragma unroll
+                            for (int k = 0; k < B; k++) mm = fmaxf(mm, mk[k][i]);
+                            const float mb = mm == -INFINITY ? 0.0f : mm, keep = exp2_fast(rm[i] - mb);
+                            rm[i] = mm;
+                            rl[i] *= keep;
+                            v[i] = make_float4(v[i].x * keep, v[i].y * keep, v[i].z * keep, v[i].w * keep);
+#pragma unroll
+                            for (int k = 0; k < B; k++) {
+                                const float e = exp2_fast(mk[k][i] - mb);
+                                rl[i] = fmaf(lk[k][i], e, rl[i]);
+                                v[i] = make_float4(fmaf(x[k][i].x, e, v[i].x), fmaf(x[k][i].y, e, v[i].y), fmaf(x[k][i].z, e, v[i].z), fmaf(x[k][i].w, e, v[i].w));
+                            }
+                        }
                     }
-                }
-                const float r = ss == 0.0f ? 0.0f : 1.0f / ss;
 #pragma unroll
-                for (int ch = 0; ch < DP / CHUNK; ch++)
-                    if (real) store_half4(orow, ch * CHUNK + my_col, s.d, make_float4(v[ch].x * r, v[ch].y * r, v[ch].z * r, v[ch].w * r), BF16, out4);
-                finish_lse(mm, ss);
+                    for (int i = 0; i < N; i++) {
+                        const uint32_t q = tid + 32 * WARPS * i;
+                        if (q >= quads) break;
+                        const uint32_t pr = w.tile * ROWS + q / (DP / 4), tok = pr / s.g, col = 4 * (q % (DP / 4)), head = w.head * s.g + (pr - tok * s.g);
+                        unsigned short *to = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + tok) * p.ov.token + (uint64_t)head * p.ov.head;
+                        const float r = rl[i] == 0.0f ? 0.0f : 1.0f / rl[i];
+                        store_half4(to, col, s.d, make_float4(v[i].x * r, v[i].y * r, v[i].z * r, v[i].w * r), BF16, out4);
+                        if (p.lse && col == 0) p.lse[(size_t)(w.q0 + tok) * s.hq + head] = rl[i] == 0.0f ? -INFINITY : (rm[i] + log2f(rl[i])) * 0.6931471805599453f;
+                    }
+                };
+                if (quads <= 32 * WARPS) join(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
+                else join(std::integral_constant<int, DP / CHUNK>(), std::integral_constant<int, 4>());
             }
         }
         u += steps;
