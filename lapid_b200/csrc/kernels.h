@@ -395,7 +395,7 @@ constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile a
 constexpr uint32_t PAGED_SMALL_LIMIT = 16;                             // requests of at most so many packed rows go to it
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
 constexpr uint32_t PAGED_LARGE_EXTRA = 3;                              // steps that beginning and ending one of its tiles takes as long as
-constexpr uint32_t PAGED_SMALL_MIN = 4, PAGED_LARGE_MIN = 6;             // fewest units worth a CTA of its own
+constexpr uint32_t PAGED_SMALL_MIN = 2, PAGED_LARGE_MIN = 6;             // fewest units worth a CTA of its own
 // What a unit of either kernel takes of an SM, in ns, at 128 / 64 elements a head: of the kernel for few rows when it shares the chip with the other (alone
 // it is bound by all SMs' common memory, here by what one SM can have in flight)
 constexpr uint32_t PAGED_SMALL_NS_128 = 360, PAGED_SMALL_NS_64 = 180, PAGED_LARGE_NS_128 = 1000, PAGED_LARGE_NS_64 = 1350;

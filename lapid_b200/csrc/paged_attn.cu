@@ -28,7 +28,7 @@ using namespace pipe;
 
 constexpr int KEYS = PAGED_SMALL_KEYS, ROWS = PAGED_SMALL_ROWS;
 constexpr int WARPS = 4, THREADS = 32 * (WARPS + 1);  // and the producer
-constexpr int CHUNK = 32, PITCH = 40;                 // columns of the accumulators that meet in shared memory at a time; a pitch without bank conflicts
+constexpr int CHUNK = 32, MEET = WARPS * ROWS * (CHUNK + 8);  // the accumulators meet in shared memory 32 columns of 16 rows at a time, or more of fewer; the pitch avoids bank conflicts
 constexpr uint32_t SPIN_LIMIT = 1u << 19;            // a wait gives up after some two seconds
 
 template <int DP> struct Cfg {
@@ -36,7 +36,7 @@ template <int DP> struct Cfg {
     static constexpr int PART = KEYS * 128;                 // bytes of one half of a step's keys (or values)
     static constexpr int STAGE = 2 * HALVES * PART;
     static constexpr int STAGES = 3 * 128 / DP;
-    static constexpr int SMEM = STAGES * STAGE + WARPS * ROWS * PITCH * 4 + 2 * WARPS * ROWS * 4 + 16 * STAGES + 16 + 1024;
+    static constexpr int SMEM = STAGES * STAGE + MEET * 4 + 2 * WARPS * ROWS * 4 + 16 * STAGES + 16 + 1024;
 };
 
 template <bool BF16> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
     using C = Cfg<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((0u - s32(smem_raw)) & 1023u);
-    float *meet = (float *)(smem + C::STAGES * C::STAGE);                  // [warp][row][PITCH]
-    float *meet_m = meet + WARPS * ROWS * PITCH, *meet_l = meet_m + WARPS * ROWS;
+    float *meet = (float *)(smem + C::STAGES * C::STAGE);                  // [warp][row][columns]
+    float *meet_m = meet + MEET, *meet_l = meet_m + WARPS * ROWS;
     uint64_t *full = (uint64_t *)(meet_l + WARPS * ROWS), *empty = full + C::STAGES;
     volatile uint32_t *is_last = (volatile uint32_t *)(empty + C::STAGES);
     const PagedShape &s = p.s;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
     const float c = s.scale * 1.4426950408889634f;  // exponentials to base 2
     const bool q2 = ((uintptr_t)p.q & 3) == 0 && ((p.qv.off | p.qv.head | p.qv.token) & 1) == 0;
     const bool out4 = ((uintptr_t)p.out & 7) == 0 && ((p.ov.off | p.ov.head | p.ov.token) & 3) == 0;
-    const uint32_t tid = threadIdx.x, my_row = tid / 8, my_col = 4 * (tid % 8);  // of the results
+    const uint32_t tid = threadIdx.x;
     // ldmatrix: lane i gives row (i & 7) of matrix i / 8; keys: matrices (keys 0-7, 8-15) of two chunks of 8 elements; values the same, transposed
     const uint32_t k_row = warp * 16 + (lane & 7) + ((lane >> 4) << 3), k_chunk = (lane >> 3) & 1;
     const uint32_t v_row = warp * 16 + (lane & 15), v_chunk = lane >> 4;
@@ -295,60 +295,64 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
             for (int h = 0; h < 2; h++) meet_m[warp * ROWS + quad + 8 * h] = m[h], meet_l[warp * ROWS + quad + 8 * h] = l[h];
         }
         warps_sync();
-        float f[WARPS], big = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < WARPS; k++) big = fmaxf(big, meet_m[k * ROWS + my_row]);
-        const float base = big == -INFINITY ? 0.0f : big;
-#pragma unroll
-        for (int k = 0; k < WARPS; k++) {
-            f[k] = exp2_fast(meet_m[k * ROWS + my_row] - base);
-            sum = fmaf(meet_l[k * ROWS + my_row], f[k], sum);
-        }
         const bool whole = step == 0 && steps == w.t.steps;
         const uint32_t i0 = u - step, i1 = i0 + w.t.steps;  // the tile's place in the sequence
-        float *part = (float *)((uint8_t *)p.plan + p.l.part_small);
-        const uint32_t pf = ROWS * (DP + 2);
-        const uint32_t slot = 2 * b + (i0 < u0 ? 0 : 1);
-        const uint32_t row = w.tile * ROWS + my_row, token = row / s.g, qh = w.head * s.g + row % s.g;
-        const bool real = token < w.n;
-        unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const uint32_t pf = ROWS * (DP + 2), rows = min(w.n * s.g - w.tile * ROWS, (uint32_t)ROWS);  // (rows that there are)
+        float *part = (float *)((uint8_t *)p.plan + p.l.part_small), *mine = part + (size_t)(2 * b + (i0 < u0 ? 0 : 1)) * pf;
+        // NR rows of C columns at a time, a thread has four columns of one row: with four rows all columns at once
+        auto meeting = [&](auto count) {
+            constexpr int NR = decltype(count)::value, C = 512 / NR < DP ? 512 / NR : DP, PITCH = C + 8;
+            static_assert(WARPS * NR * PITCH <= MEET, "shared memory");
+            const uint32_t row = tid / (C / 4), col = 4 * (tid % (C / 4)), pr = w.tile * ROWS + row, token = pr / s.g, head = w.head * s.g + (pr - token * s.g);
+            const bool real = row < rows;
+            float f[WARPS], big = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int ch = 0; ch < DP / CHUNK; ch++) {
-#pragma unroll
-            for (int n = 0; n < CHUNK / 8; n++)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    *(float2 *)(meet + (warp * ROWS + quad + 8 * h) * PITCH + 8 * n + pair) = make_float2(o[ch * (CHUNK / 8) + n][2 * h], o[ch * (CHUNK / 8) + n][2 * h + 1]);
-            warps_sync();
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int k = 0; k < WARPS; k++) big = fmaxf(big, meet_m[k * ROWS + row % ROWS]);
+            const float base = big == -INFINITY ? 0.0f : big;
 #pragma unroll
             for (int k = 0; k < WARPS; k++) {
-                const float4 x = *(const float4 *)(meet + (k * ROWS + my_row) * PITCH + my_col);
-                v = make_float4(fmaf(x.x, f[k], v.x), fmaf(x.y, f[k], v.y), fmaf(x.z, f[k], v.z), fmaf(x.w, f[k], v.w));
+                f[k] = exp2_fast(meet_m[k * ROWS + row % ROWS] - base);
+                sum = fmaf(meet_l[k * ROWS + row % ROWS], f[k], sum);
             }
-            if (!whole && real) *(float4 *)(part + (size_t)slot * pf + my_row * DP + ch * CHUNK + my_col) = v;
-            else if (real) store_half4(orow, ch * CHUNK + my_col, s.d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), BF16, out4);
-            warps_sync();
-        }
-        auto finish_lse = [&](float mm, float ss) {
-            if (p.lse && real && tid % 8 == 0) p.lse[(size_t)(w.q0 + token) * s.hq + qh] = ss == 0.0f ? -INFINITY : (mm + log2f(ss)) * 0.6931471805599453f;
+            unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)head * p.ov.head;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int c0 = 0; c0 < DP; c0 += C) {
+#pragma unroll
+                for (int n = 0; n < C / 8; n++)
+#pragma unroll
+                    for (int h = 0; h < (NR > 8 ? 2 : 1); h++)
+                        if (NR >= 8 || quad < NR)
+                            *(float2 *)(meet + (warp * NR + quad + 8 * h) * PITCH + 8 * n + pair) = make_float2(o[c0 / 8 + n][2 * h], o[c0 / 8 + n][2 * h + 1]);
+                warps_sync();
+                if (real) {
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int k = 0; k < WARPS; k++) {
+                        const float4 x = *(const float4 *)(meet + (k * NR + row) * PITCH + col);
+                        v = make_float4(fmaf(x.x, f[k], v.x), fmaf(x.y, f[k], v.y), fmaf(x.z, f[k], v.z), fmaf(x.w, f[k], v.w));
+                    }
+                    if (!whole) *(float4 *)(mine + row * DP + c0 + col) = v;
+                    else store_half4(orow, c0 + col, s.d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), BF16, out4);
+                }
+                warps_sync();
+            }
+            if (real && col == 0) {
+                if (!whole) mine[ROWS * DP + row] = big, mine[ROWS * (DP + 1) + row] = sum;
+                else if (p.lse) p.lse[(size_t)(w.q0 + token) * s.hq + head] = sum == 0.0f ? -INFINITY : (big + log2f(sum)) * 0.6931471805599453f;
+            }
         };
-        if (whole) {
-            finish_lse(big, sum);
-        } else {
-            if (tid % 8 == 0 && real) {
-                part[(size_t)slot * pf + ROWS * DP + my_row] = big;
-                part[(size_t)slot * pf + ROWS * (DP + 1) + my_row] = sum;
-            }
+        if (rows <= 4) meeting(std::integral_constant<int, 4>());
+        else if (rows <= 8) meeting(std::integral_constant<int, 8>());
+        else meeting(std::integral_constant<int, 16>());
+        if (!whole) {
             const uint32_t first = paged_holder(units, ctas, i0), last = paged_holder(units, ctas, i1 - 1);
             warps_sync();
             if (tid == 0) {
-                __threadfence();
-                uint32_t *count = p.plan + p.l.count_small + first;
-                const bool end = atomicAdd(count, 1u) == last - first;
+                uint32_t *count = p.plan + p.l.count_small + first, before;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+                const bool end = before == last - first;
                 if (end) *count = 0;  // for the next launch
-                __threadfence();
                 *is_last = end;
             }
             warps_sync();

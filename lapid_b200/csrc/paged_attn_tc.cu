@@ -673,11 +673,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             const uint32_t first = paged_holder(units, ctas, first_unit), last = paged_holder(units, ctas, first_unit + w.t.steps - 1);
             tile_sync();
             if (row == 0) {
-                __threadfence();
-                uint32_t *count = p.plan + p.l.count_large + 2 * first + t;
-                const bool end = atomicAdd(count, 1u) == last - first;
+                uint32_t *count = p.plan + p.l.count_large + 2 * first + t, before;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+                const bool end = before == last - first;
                 if (end) *count = 0;  // for the next launch
-                __threadfence();
                 is_last[t] = end;
             }
             tile_sync();
