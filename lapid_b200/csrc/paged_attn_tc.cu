@@ -184,8 +184,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a minimax polynomial in f (found by Remez's exchange; relative error 7.5e-5 at
-// degree 3: below half a unit of the weights' type, 2^-9 or 2^-12), n added to the exponent. For x <= 100; below -125 it stays 2^-125. The special-function unit forms
+// 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a minimax polynomial in f (found by Remez's exchange; relative error 2.6e-6 at
+// degree 4; at degree 3, 7.5e-5, which the weights' type would hide but not the logarithm of their sum), n added to the exponent. For x <= 100; below -125 it stays 2^-125. The special-function unit forms
 // 16 exponentials a cycle on an SM, and 128 x 128 of them take as long as the two products of 128 x 128 x 128: what it is relieved of here costs
 // five issue slots an element that the schedulers have.
 __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
@@ -194,9 +194,10 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
     x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
     const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));  // 1.5 2^23: n in the low bits
     const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
-    uint64_t y = fma2(f, pack2(0.0551716685f, 0.0551716685f), pack2(0.242611125f, 0.242611125f));
-    y = fma2(f, y, pack2(0.693260968f, 0.693260968f));
-    y = fma2(f, y, pack2(0.999928057f, 0.999928057f));
+    uint64_t y = fma2(f, pack2(0.00957010221f, 0.00957010221f), pack2(0.0559178591f, 0.0559178591f));
+    y = fma2(f, y, pack2(0.240247443f, 0.240247443f));
+    y = fma2(f, y, pack2(0.693121791f, 0.693121791f));
+    y = fma2(f, y, pack2(0.999999285f, 0.999999285f));
     float y0, y1, t0, t1;
     unpack2(y, y0, y1);
     unpack2(t, t0, t1);
