@@ -392,7 +392,9 @@ cudaError_t launch_silu_mul(const float *gate, const float *up, float *out, uint
 // ---- paged.cu, paged_attn.cu, paged_attn_tc.cu: the paged key/value cache and the attention over it
 constexpr uint32_t PAGED_FULL = 0, PAGED_CAUSAL = 1, PAGED_CROSS = 2;  // LAPID_B200_MASK_*
 constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile and step of the kernel for few rows
-constexpr uint32_t PAGED_SMALL_LIMIT = 16;                             // requests of at most so many packed rows go to it
+// Requests of at most so many packed rows go to it: its tile. Two such tiles read the keys twice: 32 rows (eight tokens of four heads) take with a limit of 16
+// and of 32 47.8 and 63.3 us at 16 requests over 2048 to 4096 keys, 19.1 and 21.0 at one over 8192, 56.0 and 76.1 at 64 over 512 to 1024; at d = 64 22.7 and 25.5.
+constexpr uint32_t PAGED_SMALL_LIMIT = 16;
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
 constexpr uint32_t PAGED_LARGE_EXTRA = 3;                              // steps that beginning and ending one of its tiles takes as long as
 constexpr uint32_t PAGED_SMALL_MIN = 2, PAGED_LARGE_MIN = 6;             // fewest units worth a CTA of its own
