@@ -14,7 +14,7 @@ the block table names. A step of a layer stack, with everything on the device::
         be.paged_attention(spec, plan, q_half, layer.k, layer.v, table, mixed)
         ...                                                     # o projection, a_dtype = DType.BF16
 
-``tp.PagedLayers`` is that loop over whole decoder layers.
+``tp.PagedLayers`` is that step over whole decoder layers.
 """
 from __future__ import annotations
 

@@ -327,6 +327,7 @@ class GpuTpLayers:
                       "act": wrap(self.act)}
         self._keep = []
         self.steps = []
+        o_in, o_dtype = self._o_operand()
         # fuse_act: the glue kernels also write x and act as the quantized operand of the decode GEMVs that
         # read them (no pre-pass kernel in front of q/k/v, gate/up and down); per layer, the layout of the
         # phase's first projection is used, a projection that wants another one keeps the f32 operand
@@ -337,7 +338,7 @@ class GpuTpLayers:
         self._glue["qx"], self._glue["qact"] = wrap(self.qx), wrap(self.qact)
         self.act_layouts = []   # per weight set: layout codes for (q/k/v phase, gate/up phase, down), None = not fused
         for w, f in zip(weights, formats):
-            bufs = [wrap(self.x), wrap(self.outs["q"]), wrap(self.act)]                 # 0 x, 1 q_out, 2 act
+            bufs = [wrap(self.x), wrap(o_in), wrap(self.act)]                           # 0 x, 1 what o reads, 2 act
             order = ["q", "k", "v", "o", "gate", "up", "down"]
             bufs += [wrap(w[n_]) for n_ in order]                                       # 3..9 weights
             bufs += [wrap(self.outs[n_]) for n_ in order]                               # 10..16 outputs
@@ -346,7 +347,8 @@ class GpuTpLayers:
 
             def launch(name, a_id, quantized=False):
                 n, k = proj[name]
-                return matmul_launch(f[name], m, n, k, inputs=(a_id, 3 + idx[name]), output=10 + idx[name], a_quantized=quantized)
+                kw = {"a_dtype": o_dtype} if name == "o" else {}
+                return matmul_launch(f[name], m, n, k, inputs=(a_id, 3 + idx[name]), output=10 + idx[name], a_quantized=quantized, **kw)
 
             def layout_of(name, holder):
                 if not self.fuse_act:
@@ -375,6 +377,14 @@ class GpuTpLayers:
             self.steps.append(step)
             self._keep.append(bufs)
 
+    def _o_operand(self):
+        """The tensor that the o projection reads, and its type: q's output (the attention itself is outside this path)."""
+        from .backend import DType
+        return self.outs["q"], DType.F32
+
+    def _mix(self, i: int):
+        """What a layer does between its q / k / v and its o projection."""
+
     def all_reduce(self, name):
         if self.world == 1 or self.skip_collective:
             return
@@ -395,6 +405,7 @@ class GpuTpLayers:
         qkv, o, _, _ = self.steps[i % len(self.steps)]
         lay_gu = self.act_layouts[i % len(self.steps)][1]
         qkv()
+        self._mix(i)
         o()
         if self.fused:
             self.peer.rms_norm(w["x"], m, d, residual=res, sum_out=w["hw"], **self._q_of(lay_gu, "qx"))
@@ -439,3 +450,66 @@ class GpuTpLayers:
         self.be.rms_norm(w["h"], w["x"], self.m, self.shape.d_model, **self._q_of(self.act_layouts[0][0], "qx"))
         self._attention_half(0, w["h"])
         return self.hw
+
+
+class PagedLayers(GpuTpLayers):
+    """Decoder layers that serve many requests from a paged key/value cache: ``GpuTpLayers`` with rotary embedding, cache and
+    attention between q / k / v and o (lapid-nn's ``Attention`` and ``KvCache``, crates/lapid-nn, hold one request).
+
+    `spec` describes a step on this rank (its heads are the rank's share; `spec.tokens` rows of `h`). `caches` are a layer's
+    (keys, values), CUDA tensors of `spec.cache_bytes()` each; a step of n layers takes the first n. `table` (i32 [requests, max_blocks]), `free` (i32, page
+    numbers) and `rope` (f32 [rows, rot], `paged.rope_table`; None: no embedding) are CUDA tensors too; objects for prompts and for single tokens share
+    all of them. Before a step the caller fills `h`, `new` and `cached` (i32 [requests]; `kv` of the step before is the next step's
+    `cached`) and drops the pages that the step before `used` from the front of `free`; all of it may happen on the device, so that a captured step can be replayed
+    while the requests grow.
+    """
+
+    def __init__(self, backend, shape: LayerShape, spec, weights: list, formats: list, caches: list, table, free, rope=None, neighbours: bool = False,
+                 world: int = 1, rank: int = 0, group=None, peer_all_reduce=None, fuse_act: bool = True):
+        import torch
+        from .backend import DType
+        from .paged import plan_bytes
+        if (spec.q_heads * world, spec.kv_heads * world, spec.head_dim) != (shape.n_heads, shape.n_kv_heads, shape.head_dim):
+            raise ValueError(f"{spec.q_heads} / {spec.kv_heads} heads of {spec.head_dim} on each of {world} ranks are not the layer's {shape.n_heads} / {shape.n_kv_heads} of {shape.head_dim}")
+        if tuple(table.shape) != (spec.requests, spec.max_blocks) or table.dtype != torch.int32 or free.dtype != torch.int32:
+            raise ValueError(f"the block table and the free pages must be i32, the table {spec.requests} x {spec.max_blocks}")
+        if rope is not None and (rope.dim() != 2 or rope.dtype != torch.float32):
+            raise ValueError("rope must be an f32 matrix, a row a position")
+        self.spec, dev = spec, weights[0]["q"].device
+        self.half = torch.bfloat16 if spec.dtype == DType.BF16 else torch.float16
+        self.mixed = torch.zeros(spec.tokens, spec.q_heads * spec.head_dim, dtype=self.half, device=dev)
+        super().__init__(backend, shape, world, rank, spec.tokens, weights, formats, group=group, peer_all_reduce=peer_all_reduce, fuse_act=fuse_act)
+        i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=dev)
+        self.table, self.free, self.rope = table, free, rope
+        self.new, self.cached, self.kv, self.used = i32(spec.requests), i32(spec.requests), i32(spec.requests), i32(1)
+        self.slots, self.positions = i32(spec.tokens), i32(spec.tokens)
+        self.q_half = torch.zeros_like(self.mixed)
+        self.plan = torch.zeros(plan_bytes(spec), dtype=torch.uint8, device=dev)
+        torch.cuda.synchronize(dev)
+        w = {n_: backend.wrap_tensor(getattr(self, n_)) for n_ in ("new", "cached", "table", "slots", "positions", "kv", "used", "plan", "q_half", "mixed")}
+        w["free"] = backend.wrap_tensor(free) if free.numel() else None
+        rot = {} if rope is None else {"rope": backend.wrap_tensor(rope), "rope_rows": rope.shape[0], "rot": rope.shape[1], "neighbours": neighbours}
+        q, k, v = (backend.wrap_tensor(self.outs[n_]) for n_ in ("q", "k", "v"))
+        self._plan_step = backend.packed_paged_plan(spec, w["new"], w["cached"], w["table"], w["slots"], w["positions"], w["kv"], w["used"], w["plan"],
+                                                    free_pages=w["free"], n_free=free.numel())
+        self._mixes = []
+        for keys, values in caches:
+            kc, vc = backend.wrap_tensor(keys), backend.wrap_tensor(values)
+            self._mixes.append((backend.packed_paged_append(spec, DType.F32, q, k, v, w["slots"], w["positions"], kc, vc, w["q_half"], **rot),
+                                backend.packed_paged_attention(spec, w["plan"], w["q_half"], kc, vc, w["table"], w["mixed"])))
+
+    def _o_operand(self):
+        return self.mixed, self.spec.dtype
+
+    def _mix(self, i: int):
+        append, attend = self._mixes[i]
+        append()
+        attend()
+
+    def token(self, n_layers: int):
+        """Queues a step of `n_layers` layers on the current stream: the plan, then the layers. Returns the residual stream behind the
+        last one, a row a new token, the requests' tokens behind each other (rows behind the last token mean nothing)."""
+        if n_layers > len(self._mixes):
+            raise ValueError(f"{n_layers} layers, but caches for {len(self._mixes)}")
+        self._plan_step()
+        return super().token(n_layers)
