@@ -29,15 +29,19 @@ __host__ __device__ inline uint32_t paged_hi(const PagedShape &s, uint32_t n, ui
 }
 __host__ __device__ inline uint32_t paged_lo(const PagedShape &s, uint32_t hi) { return s.window && hi > s.window ? hi - s.window : 0u; }
 
-// Tile i of a request: at least one step, so that rows without keys are written too
-__host__ __device__ inline PagedTile paged_tile(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t i, uint32_t rows, uint32_t keys) {
-    const uint32_t p0 = i * rows, p1 = p0 + rows < n * s.g ? p0 + rows : n * s.g;  // packed rows
+// The tile of a request's new tokens [t0, t1]: at least one step, so that rows without keys are written too
+__host__ __device__ inline PagedTile paged_tile_of(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t t0, uint32_t t1, uint32_t keys) {
     PagedTile t;
-    t.hi = paged_hi(s, n, kv, (p1 - 1) / s.g);
-    t.first = paged_lo(s, paged_hi(s, n, kv, p0 / s.g)) / keys;
+    t.hi = paged_hi(s, n, kv, t1);
+    t.first = paged_lo(s, paged_hi(s, n, kv, t0)) / keys;
     const uint32_t end = (t.hi + keys - 1) / keys;
     t.steps = end > t.first ? end - t.first : 1u;
     return t;
+}
+// Tile i of a request
+__host__ __device__ inline PagedTile paged_tile(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t i, uint32_t rows, uint32_t keys) {
+    const uint32_t p0 = i * rows, p1 = p0 + rows < n * s.g ? p0 + rows : n * s.g;  // packed rows
+    return paged_tile_of(s, n, kv, p0 / s.g, (p1 - 1) / s.g, keys);
 }
 __host__ __device__ inline uint32_t paged_tiles(const PagedShape &s, uint32_t n, uint32_t rows) { return (n * s.g + rows - 1) / rows; }
 // Requests of few rows go to one kernel, the others to the other

@@ -245,15 +245,16 @@ __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
     w.tiles = paged_tiles(p.s, w.n, paged_large_rows(p.s));
 }
 // (steps 0: the span ends in what the tile counts in front of its steps)
-__device__ __forceinline__ bool load_tile(const PagedAttnArgs &p, Walk &w) {
-    w.t = paged_tile(p.s, w.n, w.kv, w.tile, paged_large_rows(p.s), p.s.large_keys);
-    w.two = (2 * w.tile + 1) * p.s.tt < w.n;
+template <int KEYS> __device__ __forceinline__ bool load_tile(const PagedAttnArgs &p, Walk &w) {
+    const uint32_t token0 = 2 * w.tile * p.s.tt;
+    w.t = paged_tile_of(p.s, w.n, w.kv, token0, min(token0 + 2 * p.s.tt, w.n) - 1, KEYS);
+    w.two = token0 + p.s.tt < w.n;
     const uint32_t begin = w.i0 + PAGED_LARGE_EXTRA, end = w.u1 > begin ? min(w.t.steps, w.u1 - begin) : 0u;
     w.steps = end > w.step ? end - w.step : 0u;
     return w.steps > 0;
 }
 // The next piece of work of the span; false: none
-__device__ __forceinline__ bool next_piece(const PagedAttnArgs &p, Walk &w) {
+template <int KEYS> __device__ __forceinline__ bool next_piece(const PagedAttnArgs &p, Walk &w) {
     w.i0 += PAGED_LARGE_EXTRA + w.t.steps;
     if (w.i0 + PAGED_LARGE_EXTRA >= w.u1) return false;
     w.step = 0;
@@ -267,7 +268,7 @@ __device__ __forceinline__ bool next_piece(const PagedAttnArgs &p, Walk &w) {
             } while (w.n == 0 || paged_is_small(p.s, w.n));
         }
     }
-    return load_tile(p, w);
+    return load_tile<KEYS>(p, w);
 }
 __device__ __forceinline__ uint32_t tile_low(const PagedAttnArgs &p, const Walk &w) { return paged_lo(p.s, paged_hi(p.s, w.n, w.kv, 2 * w.tile * p.s.tt)); }
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
         w.i0 = u0 - place, w.u1 = u1, w.r = uniform(at.r), w.head = uniform(at.head), w.tile = uniform(at.tile), w.q0 = uniform(at.q0), w.n = uniform(at.n), w.kv = uniform(at.kv);
         w.step = place > PAGED_LARGE_EXTRA ? place - PAGED_LARGE_EXTRA : 0u;
         w.tiles = paged_tiles(s, w.n, paged_large_rows(s));
-        work = load_tile(p, w);
+        work = load_tile<C::KEYS>(p, w);
     }
 
     if (warp >= MMA_WARP) {
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             bool begun = false;  // the piece's first scores are under way
             while (work && healthy) {
                 Walk next = w;
-                const bool follows = next_piece(p, next);
+                const bool follows = next_piece<C::KEYS>(p, next);
                 if (t == 1 && !w.two) {  // the other tile's alone
                     for (uint32_t j = 0; j < w.steps && healthy; j++) {
                         if (!(healthy = warp_wait(k_full + ks, kph) && warp_wait(v_full + vs, vph))) break;
@@ -491,6 +492,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                             __syncwarp();
                         }
+                    }
+                    // (Q comes some 1200 cycles behind its read of the one before, the last weights some 2000: the softmax finds its next scores behind its end)
+                    if (j == w.steps && next_mine && !begun) {
+                        if (!(healthy = warp_wait(k_full + ks, kph) && warp_wait(q_full + t, piece & 1))) break;
+                        piece++;
+                        begun = true;
+                        scores(next.steps == 1);
                     }
                     if (!(healthy = warp_wait(ready + 2 * (events & 1) + t, (events >> 1) & 1))) break;
                     events++;
@@ -532,6 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             const bool copies = lane < boxes * C::HALVES;
             const uint32_t half = lane / boxes, part = lane % boxes;
             const int outside = (int)(s.pages * s.hkv * s.page);  // a row behind the cache: such a copy is filled with zeros
+            const uint32_t shift = 31 - __clz(s.page);  // (page sizes are powers of two)
             uint32_t st = 0, ph = 1, piece[2] = {0, 0};
             bool bad = false;
             // the rows of Q of a piece, when the scores of the one before have read theirs
@@ -575,10 +584,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             while (work && healthy) {
                 const uint32_t low = tile_low(p, w);
                 auto row_of = [&](uint32_t j) -> int {
-                    const uint32_t key = (w.t.first + w.step + j) * C::KEYS + part * box, block = key / s.page;
+                    const uint32_t key = (w.t.first + w.step + j) * C::KEYS + part * box, block = key >> shift;
                     if (!copies || key >= w.t.hi) return outside;
                     const int32_t page = p.table[(size_t)w.r * s.max_blocks + block];
-                    if (page >= 0 && (uint32_t)page < s.pages) return (int)(((uint32_t)page * s.hkv + w.head) * s.page + key % s.page);
+                    if (page >= 0 && (uint32_t)page < s.pages) return (int)(((uint32_t)page * s.hkv + w.head) * s.page + (key & (s.page - 1)));
                     if ((block + 1) * s.page > low) bad = true;
                     return outside;
                 };
@@ -593,7 +602,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                     if (copies) tma_load_2d(ring + st * C::STAGE + half * C::HALF + part * box * 128, map, 64 * (int)half, now, full + st);
                     if (++st == C::STAGES) st = 0, ph ^= 1;
                 }
-                if (healthy) work = next_piece(p, w);
+                if (healthy) work = next_piece<C::KEYS>(p, w);
             }
             if (bad && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
             // the copies in flight have to land before the CTA leaves
@@ -614,9 +623,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
         constexpr uint32_t PF = ROWS * (DP + 2);
         auto tile_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); };
         uint32_t k = 0, events = 0;  // steps so far, and times that it was ready
-        for (; work; work = next_piece(p, w)) {
+        const uint32_t local = row / s.g, member = row - local * s.g;
+        for (; work; work = next_piece<C::KEYS>(p, w)) {
             if (t == 1 && !w.two) continue;
-            const uint32_t local = row / s.g, token = (2 * w.tile + t) * s.tt + local, qh = w.head * s.g + (row - local * s.g);
+            const uint32_t token = (2 * w.tile + t) * s.tt + local, qh = w.head * s.g + member;
             const bool real = local < s.tt && token < w.n;
             // (rows that are none see everything: their results go nowhere, and they ask for no mask)
             const uint32_t hi = real ? paged_hi(s, w.n, w.kv, token) : ~0u, lo = real ? paged_lo(s, hi) : 0u;
