@@ -396,10 +396,14 @@ constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile a
 // and of 32 47.8 and 63.3 us at 16 requests over 2048 to 4096 keys, 19.1 and 21.0 at one over 8192, 56.0 and 76.1 at 64 over 512 to 1024; at d = 64 22.7 and 25.5.
 constexpr uint32_t PAGED_SMALL_LIMIT = 16;
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
-constexpr uint32_t PAGED_LARGE_EXTRA = 3;                              // steps that beginning and ending one of its tiles takes as long as
-constexpr uint32_t PAGED_SMALL_MIN = 2, PAGED_LARGE_MIN = 6;             // fewest units worth a CTA of its own
+// Steps that beginning and ending one of its tiles takes as long as. (With 2 in place of 3: four prompts of up to 4096 tokens 428 instead of 418 us, other cases the same.)
+constexpr uint32_t PAGED_LARGE_EXTRA = 3;
+// Fewest units worth a CTA of its own. With 1, 2, 3, 4 and 6: 64 tokens 9.2, 9.1, 9.0, 8.9, 14.6 us; 64 behind 1024 keys 34.6, 24.9, 24.0, 22.8, 25.3; 200 tokens 18.7, 18.0, 12.1,
+// 18.0, 16.4; 512 tokens 21.3, 21.4, 21.3, 21.4, 30.4. (The kernel for few rows: paged_plan_kernel.)
+constexpr uint32_t PAGED_LARGE_MIN = 3;
 // What a unit of either kernel takes of an SM, in ns, at 128 / 64 elements a head: of the kernel for few rows when it shares the chip with the other (alone
-// it is bound by all SMs' common memory, here by what one SM can have in flight)
+// it is bound by all SMs' common memory, here by what one SM can have in flight). With 700, 1000 and 1400 ns for the other: 512 tokens beside 11 single ones over
+// up to 4096 keys 52.3, 48.4 and 47.7 us, beside 39 over up to 8192 161.9, 148.0 and 154.2.
 constexpr uint32_t PAGED_SMALL_NS_128 = 360, PAGED_SMALL_NS_64 = 180, PAGED_LARGE_NS_128 = 1000, PAGED_LARGE_NS_64 = 1350;
 constexpr uint32_t PAGED_MAX_SMS = 160;
 struct PagedShape {

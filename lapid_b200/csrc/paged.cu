@@ -251,7 +251,9 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
     }
     if (!counts) return;
     if (!one) __syncthreads();  // (the tables in the plan are read)
-    uint32_t cs = small < a.ctas_small * PAGED_SMALL_MIN ? (small + PAGED_SMALL_MIN - 1) / PAGED_SMALL_MIN : a.ctas_small;
+    // Few rows: a step a CTA where every CTA then has an SM of its own, else two. (One token over 48, 192, 512, 1024 keys and 8 heads: with a step 5.7, 6.7, 6.9, 7.4 us, with
+    // two 7.5, 10.5, 7.7, 9.4, over 128 keys 6.7 and 5.8; over 4096 keys, where there are more steps than SMs, 11.5 and 10.5.)
+    uint32_t cs = small <= a.ctas_small / 2 ? small : min((small + 1) / 2, a.ctas_small);
     uint32_t cl = large < a.ctas_large * PAGED_LARGE_MIN ? (large + PAGED_LARGE_MIN - 1) / PAGED_LARGE_MIN : a.ctas_large;
     if (small && large) {
         // Both kernels have work, one bound by memory, the other by its products: they run side by side, on as many SMs as their shares of the work

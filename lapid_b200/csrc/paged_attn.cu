@@ -11,6 +11,10 @@
 // lengths keep every SM busy to the end. A producer warp fills a ring of steps with TMA copies of (parts of) pages, four warps take 16
 // keys of every step each, with maxima, sums and accumulators of their own, which meet at the end of a tile. A tile that a span's end
 // cuts is left in the plan buffer by each of its CTAs; the one that comes last adds the pieces up, in the order of the keys.
+//
+// Measured: 64 requests of one token over 820 to 8192 keys, 32 query and 8 key heads of 128, 187 us for 1.18 GB (6.3 TB/s, 0.96 of the measured copy rate); two over 118 to
+// 131 thousand keys, 64 query heads, 165 us (0.94); one over 4096 keys 10.5 us, of which 2.6 are its bytes: four trips to memory one after the other
+// (start, page number, page, pieces of the other CTAs) and the launch. Two CTAs of 110 KB an SM: one's end is the other's work.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
