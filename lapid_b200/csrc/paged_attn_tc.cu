@@ -726,7 +726,36 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             };
             const uint32_t prow = t * TILE + row;
             float *mine = parts + (size_t)(2 * b + (w.step ? 0 : 1)) * PF;
-            const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            // A cut tile's first piece is the end of a span, its others are the beginnings of theirs. When they are there as the first is done they are added here, so that
+            // the first need not go through memory. It is worth a look when the second of two is well shorter than the span, and when there are three (of few rows join_pieces is quicker).
+            // 2048 tokens 59.1 -> 52.4 us, 512 beside 11 requests' single ones 48.6 -> 45.4.
+            const uint32_t first = whole ? b : paged_holder(units, ctas, first_unit), last = whole ? b : paged_holder(units, ctas, first_unit + w.t.steps - 1);
+            uint32_t *const count = p.plan + p.l.count_large + 2 * first + t;
+            uint32_t others = 0;
+            if (b == first && !whole && ((last == first + 2 && (w.n - 2 * w.tile * s.tt) * s.g > 64) || (last == first + 1 && w.t.steps - w.steps + 2 * PAGED_LARGE_EXTRA <= u1 - u0))) {
+                if (row == 0) {
+                    uint32_t there;
+                    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(count) : "memory");
+                    there = there == last - first ? there : 0;
+                    if (there) *count = 0;  // for the next launch
+                    is_last[t] = there;
+                }
+                tile_sync();
+                others = is_last[t];
+                tile_sync();
+            }
+            const bool here = whole || others;
+            const float *const theirs = parts + (size_t)2 * (first + 1) * PF;  // and 2 PF behind it
+            float keep = 1.0f, add[2] = {0.0f, 0.0f};
+            if (others) {
+                const float m1 = __ldcg(theirs + DP * ROWS + prow), m2 = others > 1 ? __ldcg(theirs + (DP + 2 * (DP + 2)) * ROWS + prow) : -INFINITY;
+                const float mm = fmaxf(fmaxf(m, m1), m2), mb = mm == -INFINITY ? 0.0f : mm;
+                keep = exp2_fast(m - mb), add[0] = exp2_fast(m1 - mb), add[1] = exp2_fast(m2 - mb);
+                m = mm;
+                l = fmaf(__ldcg(theirs + (DP + 1) * ROWS + prow), add[0], l * keep);
+                if (others > 1) l = fmaf(__ldcg(theirs + (DP + 1 + 2 * (DP + 2)) * ROWS + prow), add[1], l);
+            }
+            const float inv = here ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
 #pragma unroll 1
             for (int i = 0; i < DP / 32; i++) {
                 uint32_t o[32];
@@ -734,8 +763,25 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 loaded(o);
                 float v[32];
 #pragma unroll
-                for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * inv;
-                if (whole) {
+                for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * keep;
+#pragma unroll 1
+                for (uint32_t k = 0; k < others; k++) {
+                    const float4 *src = (const float4 *)(theirs + (size_t)k * 2 * PF) + 8 * i * ROWS + prow;
+                    const float f = k ? add[1] : add[0];
+                    float4 y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = __ldcg(src + e * ROWS);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        v[4 * e] = fmaf(y[e].x, f, v[4 * e]);
+                        v[4 * e + 1] = fmaf(y[e].y, f, v[4 * e + 1]);
+                        v[4 * e + 2] = fmaf(y[e].z, f, v[4 * e + 2]);
+                        v[4 * e + 3] = fmaf(y[e].w, f, v[4 * e + 3]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e++) v[e] *= inv;
+                if (here) {
                     if (real) store32<BF16>(orow, v, 32 * i, s.d, vec, wide);
                 } else if (real) {
 #pragma unroll
@@ -743,15 +789,14 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 }
             }
             fence_before();
-            if (whole) {
+            if (here) {
                 store_lse(m, l);
                 continue;
             }
             if (real) mine[DP * ROWS + prow] = m, mine[(DP + 1) * ROWS + prow] = l;
-            const uint32_t first = paged_holder(units, ctas, first_unit), last = paged_holder(units, ctas, first_unit + w.t.steps - 1);
             tile_sync();
             if (row == 0) {
-                uint32_t *count = p.plan + p.l.count_large + 2 * first + t, before;
+                uint32_t before;
                 asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
                 const bool end = before == last - first;
                 if (end) *count = 0;  // for the next launch
