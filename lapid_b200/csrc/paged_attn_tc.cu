@@ -716,16 +716,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             unpack2(l1, a2, a3);
             float l = m == -INFINITY ? 0.0f : (a0 + a1) + (a2 + a3);  // (no keys: polynomials of nothing)
             if (a0 != a0) l = NAN;
-            if (healthy) healthy = warp_wait(o_full + t, (k - 1) & 1);
-            fence_after();
             const bool whole = w.steps == w.t.steps;
             const uint32_t first_unit = w.i0 + PAGED_LARGE_EXTRA;
-            unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
-            auto store_lse = [&](float mm, float ll) {
-                if (p.lse && real) p.lse[(size_t)(w.q0 + token) * s.hq + qh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
-            };
-            const uint32_t prow = t * TILE + row;
-            float *mine = parts + (size_t)(2 * b + (w.step ? 0 : 1)) * PF;
             // A cut tile's first piece is the end of a span, its others are the beginnings of theirs. When they are there as the first is done they are added here, so that
             // the first need not go through memory. It is worth a look when the second of two is well shorter than the span, and when there are three (of few rows join_pieces is quicker).
             // 2048 tokens 59.1 -> 52.4 us, 512 beside 11 requests' single ones 48.6 -> 45.4.
@@ -744,6 +736,14 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 others = is_last[t];
                 tile_sync();
             }
+            if (healthy) healthy = warp_wait(o_full + t, (k - 1) & 1);
+            fence_after();
+            unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
+            auto store_lse = [&](float mm, float ll) {
+                if (p.lse && real) p.lse[(size_t)(w.q0 + token) * s.hq + qh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+            };
+            const uint32_t prow = t * TILE + row;
+            float *mine = parts + (size_t)(2 * b + (w.step ? 0 : 1)) * PF;
             const bool here = whole || others;
             const float *const theirs = parts + (size_t)2 * (first + 1) * PF;  // and 2 PF behind it
             float keep = 1.0f, add[2] = {0.0f, 0.0f};

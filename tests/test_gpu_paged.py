@@ -518,3 +518,20 @@ def test_refusals_of_buffers(be):
         with pytest.raises(lp.LapidError) as e:
             append(**kw)
         assert e.value.code == code, kw
+
+
+@pytest.mark.parametrize("new,cached,hq,hkv,d,mask,window", [
+    ([700], [0], 16, 8, 64, Mask.CAUSAL, 0),          # spans of several tiles: a cut tile's first piece finds the second there
+    ([130], [900], 64, 16, 64, Mask.CAUSAL, 0),       # tiles longer than a span: two to three pieces
+    ([90, 3, 90], [700, 5, 650], 32, 8, 128, Mask.FULL, 0),
+    ([400], [300], 14, 2, 64, Mask.CAUSAL, 200),
+])
+def test_cut_tiles_are_added_up_alike_whoever_does_it(be, new, cached, hq, hkv, d, mask, window):
+    """The formula, and the same bits in every run: which CTA adds a cut tile's pieces up depends on timing, the sum's order must not."""
+    s = R.Step(be, new, cached, hq=hq, hkv=hkv, d=d, mask=mask, window=window, seed=12).run()
+    first = [s.b[n].download().copy() for n in ("out", "lse")]
+    for _ in range(30):
+        s.attend()
+        be.synchronize()
+        for a, n in zip(first, ("out", "lse")):
+            assert np.array_equal(a, s.b[n].download())
