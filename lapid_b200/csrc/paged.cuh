@@ -5,7 +5,7 @@
 // of the group (g = q_heads / kv_heads). A tile is PAGED_SMALL_ROWS consecutive packed rows of one request and one key/value head, or twice the whole
 // tokens that fit 128 rows (PagedShape::tt of them); it walks the keys that any of its rows may see in steps of PAGED_SMALL_KEYS or PagedShape::large_keys: the units.
 // All units of a launch form one sequence (request, head, tile, step), cut into equal spans, one per CTA, whatever the lengths are.
-// A tile cut by the end of a span is joined from its pieces. A tile of many rows counts PAGED_LARGE_EXTRA units more than its steps, in front of them:
+// A tile cut by the end of a span is added up from its pieces. A tile of many rows counts PAGED_LARGE_EXTRA units more than its steps, in front of them:
 // what its beginning and its end cost.
 #pragma once
 #include <stdint.h>
