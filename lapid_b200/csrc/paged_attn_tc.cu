@@ -483,55 +483,60 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 }
                 // Event j: the scores of step j have been read, and the weights of step j - 1 are there. Then the scores behind them may be formed, of step
                 // j + 1 or of the next piece's first, and the weights multiplied. (Event `steps`: the last weights are there.) The next piece's Q comes
-                // when these scores have read theirs: if it is not there at event `steps` - 1, its scores are left until the last weights are multiplied.
+                // when these scores have read theirs: if it is not there at event `steps` - 1 it is looked for until the last weights are.
                 begun = false;
-                for (uint32_t j = 0; j <= w.steps && healthy; j++) {
-                    const bool more = j + 1 < w.steps, first = j + 1 == w.steps && next_mine && warp_test(k_full + ks, kph) && warp_test(q_full + t, piece & 1);
-                    if (more && !(healthy = warp_wait(k_full + ks, kph))) break;
-                    if (j) {
-                        if (!(healthy = warp_wait(v_full + vs, vph))) break;
-                        // values of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0 (both warps do it: zeros twice)
-                        const uint32_t key0 = (w.t.first + w.step + j - 1) * C::KEYS;
-                        if (key0 < low || key0 + C::KEYS > w.t.hi) {
-                            for (uint32_t i = lane; i < C::KEYS * (DP / 8); i += 32) {
-                                const uint32_t key = i / (DP / 8), ch = i % (DP / 8);
-                                if (key0 + key < low || key0 + key >= w.t.hi)
-                                    *(uint4 *)(v_ring + vs * C::STAGE + (ch / 8) * C::HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-                            }
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
+                // the values of step j are there; those of keys that no row of the tile sees are whatever the page holds: 0 times that must be 0 (both warps do it: zeros twice)
+                auto values = [&](uint32_t j) -> bool {
+                    if (!warp_wait(v_full + vs, vph)) return false;
+                    const uint32_t key0 = (w.t.first + w.step + j) * C::KEYS;
+                    if (key0 < low || key0 + C::KEYS > w.t.hi) {
+                        for (uint32_t i = lane; i < C::KEYS * (DP / 8); i += 32) {
+                            const uint32_t key = i / (DP / 8), ch = i % (DP / 8);
+                            if (key0 + key < low || key0 + key >= w.t.hi)
+                                *(uint4 *)(v_ring + vs * C::STAGE + (ch / 8) * C::HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
                     }
-                    // (Q comes some 1200 cycles behind its read of the one before, the last weights some 2000: the softmax finds its next scores behind its end)
-                    if (j == w.steps && next_mine && !begun) {
-                        if (!(healthy = warp_wait(k_full + ks, kph) && warp_wait(q_full + t, piece & 1))) break;
-                        piece++;
-                        begun = true;
-                        scores(next.steps == 1);
+                    return true;
+                };
+                auto multiply = [&](uint32_t j) {
+                    if (elect_one()) {
+                        const uint64_t vd = desc_t(s32(v_ring) + vs * C::STAGE, C::HALF);
+#pragma unroll
+                        for (int i = 0; i < C::KEYS / 16; i++) mma_ts(o_col, p_col + 8 * i, vd + i * (2048 >> 4), idesc_o, (j || i) ? 1u : 0u);
+                        commit(o_full + t);
+                        commit(v_empty + vs);
                     }
-                    if (!(healthy = warp_wait(ready + 2 * (events & 1) + t, (events >> 1) & 1))) break;
+                    __syncwarp();
+                    if (++vs == C::STAGES) vs = 0, vph ^= 1;
+                };
+                auto event = [&]() -> bool {
+                    if (!warp_wait(ready + 2 * (events & 1) + t, (events >> 1) & 1)) return false;
                     events++;
                     fence_after();
+                    return true;
+                };
+                auto ahead = [&]() {  // the next piece's first scores
+                    piece++;
+                    begun = true;
+                    scores(next.steps == 1);
+                };
+                for (uint32_t j = 0; j < w.steps; j++) {
+                    const bool more = j + 1 < w.steps, first = !more && next_mine && warp_test(k_full + ks, kph) && warp_test(q_full + t, piece & 1);
+                    if (!(healthy = (!more || warp_wait(k_full + ks, kph)) && (!j || values(j - 1)) && event())) break;
                     // (the scores first: the softmax waits for them sooner)
-                    if (more) {
-                        scores(j + 2 == w.steps);
-                    } else if (first) {
-                        piece++;
-                        begun = true;
-                        scores(next.steps == 1);
-                    }
-                    if (j) {
-                        if (elect_one()) {
-                            const uint64_t vd = desc_t(s32(v_ring) + vs * C::STAGE, C::HALF);
-#pragma unroll
-                            for (int i = 0; i < C::KEYS / 16; i++) mma_ts(o_col, p_col + 8 * i, vd + i * (2048 >> 4), idesc_o, (j > 1 || i) ? 1u : 0u);
-                            commit(o_full + t);
-                            commit(v_empty + vs);
-                        }
-                        __syncwarp();
-                        if (++vs == C::STAGES) vs = 0, vph ^= 1;
-                    }
+                    if (more) scores(j + 2 == w.steps);
+                    else if (first) ahead();
+                    if (j) multiply(j - 1);
                 }
+                if (!healthy || !(healthy = values(w.steps - 1))) break;
+                // (Q comes some 1200 cycles and more behind its read of the one before, the last weights some 2000: whichever is first)
+                if (next_mine)
+                    for (uint32_t spin = 0; !begun && spin < SPIN_LIMIT && !warp_test(ready + 2 * (events & 1) + t, (events >> 1) & 1); spin++)
+                        if (warp_test(k_full + ks, kph) && warp_test(q_full + t, piece & 1)) ahead();
+                if (!(healthy = event())) break;
+                multiply(w.steps - 1);
                 w = next, work = follows;
             }
             // no product may be under way when tensor memory is released, and nothing may arrive in this CTA's shared memory behind its end
