@@ -25,10 +25,10 @@
 // all of them up, in the order of the keys either way and with the same roundings.
 //
 // What bounds it: a softmax warp's own chain, two warps a scheduler. A step of 96 keys takes 2050 to 2400 cycles: exponentials 1345 (the special-function unit 47 % busy over
-// the kernel), loads, stores and two waits 540, the more of it hidden the further the two tiles are apart; products 26 % of the time. The end of a tile costs some 7000 cycles more (its
-// last product, 64 KB of rows written, the walk), a cut one 9000. Long work runs into the power limit: 512 tokens over 32768 keys, 64 query and 8 key heads of 128, 545 to 575 us
-// (0.95 to 1.0 PFLOP/s, the clock at 1.2 to 1.4 GHz); four prompts of up to 4096 tokens, 32 query heads, 381 to 415 us, about as much; three of up to 3001 through a window of 1024 keys, 14 heads
-// of 64, 61.6 us.
+// the kernel), loads, stores and two waits 540, the more of it hidden the further the two tiles are apart; products 26 % of the time. From tile to tile some 6300 cycles pass (heads of 64: 4600), for
+// the last product, the rows' stores and the walk; a cut tile's later piece costs 9000, its first 8000 behind the span. Long work runs into the power limit: 512 tokens over
+// 32768 keys, 64 query and 8 key heads of 128, 546 to 580 us (0.94 to 1.0 PFLOP/s, the clock at 1.2 to 1.4 GHz); four prompts of up to 4096 tokens, 32 query heads, 373 to 392 us; one of 2048 47.1 us;
+// three of up to 3001 through a window of 1024 keys, 14 heads of 64, 61.5 us.
 //
 // Every mbarrier wait is bounded: one that gives up sets a bit in the status word, the roles fall through to the end, tensor memory is released.
 #include <cuda.h>
@@ -62,7 +62,7 @@ constexpr int Q_HALF = TILE * 128;  // bytes of 128 rows of 64 elements
 // Registers: 384 x 168 at launch = 256 x 208 + 128 x 88
 constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88;
 constexpr float LAZY = 8.0f;
-constexpr int POLY = 1;  // pairs of every eight whose exponentials are polynomials
+constexpr int POLY = 1;  // pairs of every eight whose exponentials are polynomials (with 0, 1, 2 prompts through a window 63.8, 61.5, 66.3 us, 512 tokens over 32768 keys 584, 553, 583)
 constexpr uint32_t WAIT_NS = 8000, SPIN_LIMIT = 1u << 19;  // a wait gives up after some two seconds
 
 template <int DP> struct Cfg {
