@@ -535,3 +535,15 @@ def test_cut_tiles_are_added_up_alike_whoever_does_it(be, new, cached, hq, hkv, 
         be.synchronize()
         for a, n in zip(first, ("out", "lse")):
             assert np.array_equal(a, s.b[n].download())
+
+
+@pytest.mark.parametrize("new,cached", [([1, 3], [10, 100]), ([20], [70])])
+@pytest.mark.parametrize("hq,d", [(128, 64), (136, 64), (200, 128)])
+def test_more_heads_of_a_key_head_than_a_tile_has_rows(be, new, cached, hq, d):
+    R.Step(be, new, cached, hq=hq, hkv=1, d=d, seed=21).run()
+
+
+@pytest.mark.parametrize("d", [16, 24, 40, 104, 120])
+@pytest.mark.parametrize("new,cached", [([1, 2], [33, 0]), ([70, 1], [20, 99])])
+def test_odd_head_sizes(be, d, new, cached):
+    R.Step(be, new, cached, hq=6, hkv=2, d=d, dtype=F16, seed=22).run()
