@@ -396,7 +396,8 @@ constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile a
 // and of 32 47.8 and 63.3 us at 16 requests over 2048 to 4096 keys, 19.1 and 21.0 at one over 8192, 56.0 and 76.1 at 64 over 512 to 1024; at d = 64 22.7 and 25.5.
 constexpr uint32_t PAGED_SMALL_LIMIT = 16;
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
-// Steps that beginning and ending one of its tiles takes as long as. (With 2 in place of 3: four prompts of up to 4096 tokens 428 instead of 418 us, other cases the same.)
+// Steps that beginning and ending one of its tiles takes as long as. (With 2 in place of 3: 200 tokens 17.0 instead of 10.9 us, 2048 46.2 instead of 47.0, the others
+// within 1 %.)
 constexpr uint32_t PAGED_LARGE_EXTRA = 3;
 // Fewest units worth a CTA of its own. With 1, 2, 3, 4 and 6: 64 tokens 9.2, 9.1, 9.0, 8.9, 14.6 us; 64 behind 1024 keys 34.6, 24.9, 24.0, 22.8, 25.3; 200 tokens 18.7, 18.0, 12.1,
 // 18.0, 16.4; 512 tokens 21.3, 21.4, 21.3, 21.4, 30.4. (The kernel for few rows: paged_plan_kernel.)
