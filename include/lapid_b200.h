@@ -417,7 +417,7 @@ typedef struct lapid_b200_paged {
     uint32_t page_size;  /* tokens in a page: 16, 32, 64 or 128 */
     int32_t mask;        /* LAPID_B200_MASK_* */
     uint64_t pages;      /* of the cache; pages * page_size < 2^31 */
-    uint64_t requests;   /* rows of the block table */
+    uint64_t requests;   /* rows of the block table; at most 2^28 */
     uint64_t tokens;     /* rows of q, k, v and out: the sum of the new lengths, or more (rows behind the sum are left alone) */
     uint64_t max_blocks; /* columns of the block table */
     uint64_t max_new;    /* no request has more new tokens */

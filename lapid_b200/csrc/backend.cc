@@ -1594,7 +1594,9 @@ lb::PagedShape paged_shape(const lapid_b200_paged *d) {
     const uint64_t most = (1ull << 31) - 1, g = d->q_heads / d->kv_heads;
     auto product_ok = [&](uint64_t x, uint64_t y) { return y == 0 || x <= most / y; };
     if (!product_ok(d->pages, d->page_size) || !product_ok(d->pages * d->page_size, d->kv_heads)) fail("too_large", "paged cache: pages * kv_heads * page_size must be below 2^31");
-    if (d->requests > most || !product_ok(d->requests, d->max_blocks) || !product_ok(d->requests, d->max_new) || !product_ok(d->max_blocks, d->page_size))
+    // (the plan holds a few words a request, at places of 32 bits)
+    if (d->requests > 1ull << 28) fail("too_large", "paged cache: at most 2^28 requests, got " + std::to_string(d->requests));
+    if (!product_ok(d->requests, d->max_blocks) || !product_ok(d->requests, d->max_new) || !product_ok(d->max_blocks, d->page_size))
         fail("too_large", "paged cache: requests * max_blocks, requests * max_new and max_blocks * page_size must be below 2^31");
     if (d->tokens > most || !product_ok(d->tokens, d->q_heads) || !product_ok(d->max_new, g)) fail("too_large", "paged cache: tokens * q_heads must be below 2^31");
     // units of work: (tiles of rows) x heads x (steps of 64 keys), with the smaller tile
