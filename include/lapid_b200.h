@@ -430,7 +430,7 @@ LAPID_B200_API lapid_b200_status lapid_b200_paged_plan_bytes(const lapid_b200_pa
  * need beyond ceil(cached / page_size) are taken from free_pages (i32 [n_free], in order, requests in order; NULL with
  * n_free 0 when none are needed) and entered in its row of block_table (i32 [requests, max_blocks]; entries of cached tokens are
  * read, others left alone). Out: slots and positions i32 [tokens] (page * page_size + place, and the token's index in its request;
- * -1 behind the last token), kv_lens i32 [requests] (what the next step passes as cached_lens), used i32 [1]
+ * -1 behind the last token), kv_lens i32 [requests] (what the next step passes as cached_lens; of a request that takes no part, its cached length), used i32 [1]
  * (how many free pages the step takes, also when there are fewer), plan. Running it again on the same inputs gives the same result. */
 LAPID_B200_API lapid_b200_status lapid_b200_paged_plan(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *new_lens,
                                                        const lapid_b200_buffer *cached_lens, const lapid_b200_buffer *free_pages, uint64_t n_free,

@@ -160,10 +160,11 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
         if (r < s.requests) {
             const int32_t n0 = a.new_lens[r], c0 = a.cached[r];
             const uint64_t blocks = ((uint64_t)(uint32_t)c0 + (s.mask == PAGED_CROSS ? 0u : (uint32_t)n0) + s.page - 1) >> shift;
+            c = (uint32_t)c0;
             if (n0 < 0 || c0 < 0 || (uint32_t)n0 > s.max_new || blocks > s.max_blocks) {
-                bad |= PAGED_STATUS_LENGTHS;  // such a request takes no part
+                bad |= PAGED_STATUS_LENGTHS;  // such a request takes no part: it keeps the length that it has
             } else {
-                n = (uint32_t)n0, c = (uint32_t)c0;
+                n = (uint32_t)n0;
                 have = (c + s.page - 1) >> shift;
                 need = (uint32_t)blocks;
             }
