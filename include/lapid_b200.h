@@ -402,7 +402,7 @@ LAPID_B200_API lapid_b200_status lapid_b200_silu_mul_act(lapid_b200_device *dev,
  * None of them allocates or waits, so a step can be captured in a graph; lengths are read on the device, so a captured
  * step serves whatever lengths fit the bounds below. What a kernel finds wrong on the device is reported by the next call that
  * waits (execute, device_synchronize): "shape_mismatch" (a length is negative, or outside max_new, max_blocks or tokens: such a request
- * takes no part), "out_of_memory" (the list of free pages ran out), "index_out_of_range" (a page, slot or position outside
+ * takes no part; its rows of q and out, as many as its new length where that is from 0 to max_new, are left alone, and the other requests' stay where they are), "out_of_memory" (the list of free pages ran out), "index_out_of_range" (a page, slot or position outside
  * its range; it is not read or written), "invalid_launch" (the plan was made for another description).
  *
  * lapid_b200_paged describes a step; zero-fill it first. */

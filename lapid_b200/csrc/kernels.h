@@ -416,7 +416,7 @@ struct PagedShape {
 };
 // Places in a plan buffer (32-bit words; the partial results behind them at byte offsets)
 struct PagedPlanLayout {
-    uint32_t q_start, kv_len, units_small, units_large, start_small, start_large, count_small, count_large;
+    uint32_t q_start, new_len, kv_len, units_small, units_large, start_small, start_large, count_small, count_large;
     size_t part_small, part_large, bytes;  // part_*: [CTA][2] results of cut tiles: rows x (d padded + 2) f32
 };
 PagedPlanLayout paged_plan_layout(const PagedShape &s);

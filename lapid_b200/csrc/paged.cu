@@ -1,9 +1,9 @@
 // The paged key/value cache: block tables and slot maps from the requests' lengths, and the append of new keys and values.
 //
-// plan    start[r] = sum of the new lengths before r, first[r] = sum of the pages taken before r; token t of r lies at position cached + t,
-//         in block pos / page of its table row, slot = table[r][block] * page + pos % page. New blocks take the pages
-//         free_pages[first[r]...] in the requests' order, so the result does not depend on timing. The plan also cuts the work of
-//         the attention launches that follow (paged.cuh): which request, head, tile and step each CTA begins with. That is
+// plan    start[r] = sum of the new lengths before r (those within bounds, whether their request takes part or not), first[r] = sum of the pages taken
+//         before r; token t of r lies at position cached + t, in block pos / page of its table row, slot = table[r][block] * page + pos % page.
+//         New blocks take the pages free_pages[first[r]...] in the requests' order, so the result does not depend on timing. The plan also cuts the
+//         work of the attention launches that follow (paged.cuh): which request, head, tile and step each CTA begins with. That is
 //         done once a step, and every layer's launch reads it.
 //         What bounds it is latency: one launch, two scans over the requests, a search a token and a search a start. Every CTA scans the
 //         lengths itself so that nothing passes between CTAs, and takes its share of the tokens, blocks and starts. 64 requests of one token 4.2 us, 48
@@ -32,7 +32,8 @@ PagedPlanLayout paged_plan_layout(const PagedShape &s) {
         return at;
     };
     const uint32_t cs = paged_attn_small_ctas(PAGED_MAX_SMS), cl = paged_has_large(s) ? paged_attn_large_ctas(PAGED_MAX_SMS) : 0;
-    l.q_start = take(s.requests + 1);
+    l.q_start = take(s.requests);
+    l.new_len = take(s.requests);
     l.kv_len = take(s.requests);
     l.units_small = take(s.requests + 1);
     l.units_large = take(s.requests + 1);
@@ -59,7 +60,7 @@ uint32_t paged_stamp(const PagedShape &s) {
 // T threads take T requests at a time: 256 where there are no more (64 requests: 4.2 us, with 1024 threads and a scan for each sum 6.7), else 1024.
 template <uint32_t T> struct PlanShared {
     uint64_t warp_sum[T / 32];
-    uint32_t start[T + 1], first[T + 1], cached[T], have[T], kv[T];
+    uint32_t start[T], n[T], first[T], cached[T], have[T], kv[T];  // n: tokens that take part
     uint32_t small[T + 1], large[T + 1];    // units before the request
     uint32_t tiles[T + 1], steps[T];        // of many rows: tiles before the request, units of its tiles for one head
 };
@@ -100,9 +101,9 @@ __device__ __forceinline__ uint32_t last_at_most(const uint32_t *a, uint32_t n, 
 }
 
 // What each CTA of an attention launch begins with: warp `worker` of `workers` takes every workers-th of them. `prefix`: units before each request, `q0` its first
-// row, `kv` its keys.
-__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, const uint32_t *q0, const uint32_t *kv, uint32_t *starts, uint32_t rows,
-                          uint32_t keys, uint32_t extra, uint32_t worker, uint32_t workers) {
+// row, `n` its new tokens, `kv` its keys.
+__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, const uint32_t *q0, const uint32_t *n, const uint32_t *kv,
+                          uint32_t *starts, uint32_t rows, uint32_t keys, uint32_t extra, uint32_t worker, uint32_t workers) {
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t b = worker; b < all; b += workers) {
         PagedStart x{};
@@ -112,7 +113,7 @@ __device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas,
             x.u1 = __shfl_sync(0xffffffffu, x.u0, 1);
             x.u0 = __shfl_sync(0xffffffffu, x.u0, 0);
             const uint32_t r = last_at_most(prefix, a.s.requests, x.u0);
-            x.r = r, x.q0 = q0[r], x.n = q0[r + 1] - x.q0, x.kv = kv[r];
+            x.r = r, x.q0 = q0[r], x.n = n[r], x.kv = kv[r];
             const uint32_t per_head = (prefix[r + 1] - prefix[r]) / a.s.hkv, off = x.u0 - prefix[r], tiles = paged_tiles(a.s, x.n, rows);
             x.head = off / per_head;
             uint32_t rem = off - x.head * per_head;
@@ -156,21 +157,23 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
     uint32_t bad = 0;
     for (uint32_t r0 = 0; r0 < s.requests; r0 += T) {
         const uint32_t r = r0 + tid, count = min(T, s.requests - r0);
-        uint32_t n = 0, c = 0, have = 0, need = 0;
+        uint32_t own = 0, n = 0, c = 0, have = 0, need = 0;  // rows of q, new tokens
         if (r < s.requests) {
             const int32_t n0 = a.new_lens[r], c0 = a.cached[r];
             const uint64_t blocks = ((uint64_t)(uint32_t)c0 + (s.mask == PAGED_CROSS ? 0u : (uint32_t)n0) + s.page - 1) >> shift;
+            const bool counted = n0 >= 0 && (uint32_t)n0 <= s.max_new;
             c = (uint32_t)c0;
-            if (n0 < 0 || c0 < 0 || (uint32_t)n0 > s.max_new || blocks > s.max_blocks) {
-                bad |= PAGED_STATUS_LENGTHS;  // such a request takes no part: it keeps the length that it has
+            if (counted) own = (uint32_t)n0;
+            if (!counted || c0 < 0 || blocks > s.max_blocks) {
+                bad |= PAGED_STATUS_LENGTHS;  // such a request takes no part: it keeps the length that it has, and its rows, so that the others' stay where they are
             } else {
-                n = (uint32_t)n0;
+                n = own;
                 have = (c + s.page - 1) >> shift;
                 need = (uint32_t)blocks;
             }
         }
         uint64_t total;
-        uint64_t at = block_scan<T>(both(n, need - have), sh, total);
+        uint64_t at = block_scan<T>(both(own, need - have), sh, total);
         // (rows behind the last one of q: such tokens take no part)
         const uint32_t at_n = base + (uint32_t)at, lo = min(at_n, s.tokens), hi = min(at_n + n, s.tokens), at_p = taken + (uint32_t)(at >> 32);
         const uint32_t end_n = min(base + (uint32_t)total, s.tokens), end_p = taken + (uint32_t)(total >> 32);
@@ -178,11 +181,11 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
         n = hi - lo;
         const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
         sh.start[tid] = lo;
+        sh.n[tid] = n;
         sh.first[tid] = at_p;
         sh.cached[tid] = c;
         sh.have[tid] = have;
         sh.kv[tid] = kv;
-        if (tid == 0) sh.start[count] = end_n, sh.first[count] = end_p;  // (count < T: the thread of that place writes the same)
         if (counts) {
             const bool few = paged_is_small(s, n);
             uint32_t us = 0, ul = 0;
@@ -197,7 +200,7 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
                 __syncthreads();
                 for (uint32_t i = tid; i < (uint32_t)total; i += T) {
                     const uint32_t q = last_at_most(sh.tiles, count, i);
-                    atomicAdd(&sh.steps[q], paged_tile(s, sh.start[q + 1] - sh.start[q], sh.kv[q], i - sh.tiles[q], rows, s.large_keys).steps + PAGED_LARGE_EXTRA);
+                    atomicAdd(&sh.steps[q], paged_tile(s, sh.n[q], sh.kv[q], i - sh.tiles[q], rows, s.large_keys).steps + PAGED_LARGE_EXTRA);
                 }
                 __syncthreads();
                 ul = sh.steps[tid];
@@ -209,6 +212,7 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
         }
         if (writes && r < s.requests) {
             a.plan[a.l.q_start + r] = lo;
+            a.plan[a.l.new_len + r] = n;
             a.plan[a.l.kv_len + r] = kv;
             a.kv_lens[r] = (int32_t)kv;
             if (!one) a.plan[a.l.units_small + r] = sh.small[tid], a.plan[a.l.units_large + r] = sh.large[tid];
@@ -224,8 +228,9 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
         // (the last CTA begins: the first one has the pages)
         for (uint32_t t = base + (workers - 1 - worker) * T + tid; t < end_n; t += workers * T) {
             const uint32_t i = last_at_most(sh.start, count, t), pos = sh.cached[i] + (t - sh.start[i]), block = pos >> shift;
+            const bool part = t - sh.start[i] < sh.n[i];
             int32_t slot = -1;
-            if (s.mask != PAGED_CROSS) {
+            if (part && s.mask != PAGED_CROSS) {
                 int32_t page = -1;
                 if (block < sh.have[i]) page = a.table[(size_t)(r0 + i) * s.max_blocks + block];
                 else if (sh.first[i] + (block - sh.have[i]) < a.n_free) page = a.free_pages[sh.first[i] + (block - sh.have[i])];
@@ -233,7 +238,7 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
                 else if (block < sh.have[i]) bad |= PAGED_STATUS_INDEX;
             }
             a.slots[t] = slot;
-            a.positions[t] = (int32_t)pos;
+            a.positions[t] = part ? (int32_t)pos : -1;
         }
         base = end_n;
         taken = end_p;
@@ -243,7 +248,6 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
     if (bad && a.status) atomicOr(a.status, (int)bad);
     if (writes) {
         if (tid == 0) {
-            a.plan[a.l.q_start + s.requests] = base;
             *a.used = (int32_t)taken;
             if (!one) a.plan[a.l.units_small + s.requests] = small, a.plan[a.l.units_large + s.requests] = large;
         }
@@ -265,12 +269,12 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
         cl = min(cl, max(share, 1u));
         cs = min(cs, max(a.ctas_small / sms * (sms - cl), 1u));
     }
-    const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start, *kv = one ? sh.kv : a.plan + a.l.kv_len;
+    const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start, *n = one ? sh.n : a.plan + a.l.new_len, *kv = one ? sh.kv : a.plan + a.l.kv_len;
     const uint32_t warp = worker * (T / 32) + tid / 32, warps = (one ? workers : 1) * (T / 32);
-    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, kv, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);
+    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, n, kv, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);
     // (from the other end: a warp has a start of one kind or of the other)
     if (a.ctas_large)
-        cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, kv, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, warps - 1 - warp, warps);
+        cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, n, kv, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, warps - 1 - warp, warps);
 }
 
 static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim3 grid, unsigned threads, size_t smem, bool pdl, cudaStream_t stream) {

@@ -79,7 +79,7 @@ struct Walk {
 };
 __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
     w.q0 = p.plan[p.l.q_start + w.r];
-    w.n = p.plan[p.l.q_start + w.r + 1] - w.q0;
+    w.n = p.plan[p.l.new_len + w.r];
     w.kv = p.plan[p.l.kv_len + w.r];
     w.tiles = paged_tiles(p.s, w.n, ROWS);
 }

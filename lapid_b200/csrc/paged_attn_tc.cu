@@ -249,7 +249,7 @@ struct Walk {
 };
 __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
     w.q0 = uniform(p.plan[p.l.q_start + w.r]);
-    w.n = uniform(p.plan[p.l.q_start + w.r + 1]) - w.q0;
+    w.n = uniform(p.plan[p.l.new_len + w.r]);
     w.kv = uniform(p.plan[p.l.kv_len + w.r]);
     w.tiles = paged_tiles(p.s, w.n, paged_large_rows(p.s));
 }

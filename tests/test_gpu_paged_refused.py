@@ -4,7 +4,9 @@ import numpy as np
 import pytest
 
 import lapid_b200 as lp
+from lapid_b200.paged import Mask
 from tests import paged_ref as R
+from tests.paged_more import plan_with_refusals
 
 pytestmark = pytest.mark.gpu
 
@@ -25,6 +27,19 @@ def i32(buf, n):
     return buf.download().view(np.int32)[:n]
 
 
+def want_of(s, new, cached, table, free):
+    return plan_with_refusals(new, cached, table, free, s.page, s.blocks, s.spec.max_new, s.spec.tokens, s.mask == Mask.CROSS)
+
+
+def check_plan(s, want):
+    b, r = s.b, len(s.new)
+    assert np.array_equal(i32(b["kv"], r), want[3])
+    assert i32(b["used"], 1)[0] == want[4]
+    assert np.array_equal(i32(b["positions"], s.spec.tokens), want[2])
+    assert np.array_equal(i32(b["slots"], s.spec.tokens), want[1])
+    assert np.array_equal(i32(b["table"], want[0].size).reshape(want[0].shape), want[0])
+
+
 @pytest.mark.parametrize("bad", ["blocks", "negative"])
 @pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 2]])
 def test_a_refused_request_keeps_its_length(be, bad, new):
@@ -35,3 +50,39 @@ def test_a_refused_request_keeps_its_length(be, bad, new):
     s.make_plan()
     refused(be)
     assert i32(s.b["kv"], 3).tolist() == [20 + new[0], cached[1], 33 + new[2]]
+
+
+@pytest.mark.parametrize("bad", ["blocks", "negative"])
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [3, 2, 60, 1], [40, 70, 1, 90]])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_the_rows_of_the_others_stay_where_they_are(be, bad, new, which):
+    """The rows of q belong to the requests by the new lengths; one that cannot grow any more does not hand its rows to the next."""
+    s = R.Step(be, new, [20, 40, 33, 90], hq=8, hkv=2, d=64).upload()
+    cached = list(s.cached)
+    cached[which] = s.blocks * s.page if bad == "blocks" else -1
+    s.b["cached"].write(0, np.array(cached, np.int32))
+    s.make_plan()
+    s.attend()
+    refused(be)
+    # (the pages that the refused one does not take go to the requests behind it: their new tokens' keys lie there)
+    want = want_of(s, new, cached, s.table0, s.free)
+    check_plan(s, want)
+    kc, vc = np.full((s.pages, s.hkv, s.page, s.d), np.nan), np.full((s.pages, s.hkv, s.page, s.d), np.nan)
+    for r, x in enumerate(s.kv):
+        if r != which:
+            for j in range(x):
+                p = want[0][r, j // s.page]
+                kc[p, :, j % s.page], vc[p, :, j % s.page] = s.k[r][j], s.v[r][j]
+    s.b["k"].write(0, R.to_half(kc, s.dtype)[1])
+    s.b["v"].write(0, R.to_half(vc, s.dtype)[1])
+    s.attend()
+    be.synchronize()
+    out, lse = s.outputs()
+    raw, at = s.b["out"].download().view(np.int16)[: s.tokens * s.hq * s.d].reshape(s.tokens, -1), 0
+    for r, n in enumerate(new):
+        if r == which:
+            assert np.all(raw[at:at + n] == 0x7e7e) and np.all(lse[at:at + n] == 77.0)
+        else:
+            o, l, size = R.attention(s.q[at:at + n], s.k[r], s.v[r], s.g, s.mask, 0, s.scale, n, s.kv[r])
+            assert np.all(np.abs(out[at:at + n] - o) <= R.bound(s.dtype, o, size, s.kv[r], float(np.abs(s.v[r]).max()))), r
+        at += n
