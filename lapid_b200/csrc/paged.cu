@@ -60,6 +60,7 @@ uint32_t paged_stamp(const PagedShape &s) {
 // T threads take T requests at a time: 256 where there are no more (64 requests: 4.2 us, with 1024 threads and a scan for each sum 6.7), else 1024.
 template <uint32_t T> struct PlanShared {
     uint64_t warp_sum[T / 32];
+    uint32_t end_pages;  // pages taken in front of the request whose rows pass the last one
     uint32_t start[T], n[T], first[T], cached[T], have[T], kv[T];  // n: tokens that take part
     uint32_t small[T + 1], large[T + 1];    // units before the request
     uint32_t tiles[T + 1], steps[T];        // of many rows: tiles before the request, units of its tiles for one head
@@ -172,13 +173,14 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
                 need = (uint32_t)blocks;
             }
         }
+        if (tid == 0) sh.end_pages = ~0u;
         uint64_t total;
         uint64_t at = block_scan<T>(both(own, need - have), sh, total);
-        // (rows behind the last one of q: such tokens take no part)
-        const uint32_t at_n = base + (uint32_t)at, lo = min(at_n, s.tokens), hi = min(at_n + n, s.tokens), at_p = taken + (uint32_t)(at >> 32);
-        const uint32_t end_n = min(base + (uint32_t)total, s.tokens), end_p = taken + (uint32_t)(total >> 32);
-        if (hi - lo != n) bad |= PAGED_STATUS_LENGTHS;
-        n = hi - lo;
+        const uint64_t pages = total;  // (high half)
+        const uint32_t at_n = base + (uint32_t)at, at_p = taken + (uint32_t)(at >> 32), lo = min(at_n, s.tokens), end_n = min(base + (uint32_t)total, s.tokens);
+        // A request whose rows pass the last one of q takes no part either, and none behind it has rows: the pages end where it stands.
+        if (n && at_n + n > s.tokens) bad |= PAGED_STATUS_LENGTHS, n = 0;
+        if (at_n <= s.tokens && at_n + own > s.tokens) sh.end_pages = at_p;
         const uint32_t kv = s.mask == PAGED_CROSS ? c : c + n;
         sh.start[tid] = lo;
         sh.n[tid] = n;
@@ -218,6 +220,7 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
             if (!one) a.plan[a.l.units_small + r] = sh.small[tid], a.plan[a.l.units_large + r] = sh.large[tid];
         }
         __syncthreads();
+        const uint32_t end_p = min(taken + (uint32_t)(pages >> 32), sh.end_pages);
         for (uint32_t j = taken + worker * T + tid; j < end_p; j += workers * T) {
             const uint32_t i = last_at_most(sh.first, count, j);
             int32_t page = -1;

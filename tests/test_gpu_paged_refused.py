@@ -1,5 +1,7 @@
 """Requests that take no part in a step of the paged cache (lengths outside the bounds, rows behind the last one of q): they keep their rows, pages and lengths, and the
 requests beside them are what they would be without the fault. Whole numbers are equal; attention by ``paged_ref.bound``."""
+import dataclasses
+
 import numpy as np
 import pytest
 
@@ -86,3 +88,57 @@ def test_the_rows_of_the_others_stay_where_they_are(be, bad, new, which):
             o, l, size = R.attention(s.q[at:at + n], s.k[r], s.v[r], s.g, s.mask, 0, s.scale, n, s.kv[r])
             assert np.all(np.abs(out[at:at + n] - o) <= R.bound(s.dtype, o, size, s.kv[r], float(np.abs(s.v[r]).max()))), r
         at += n
+
+
+@pytest.mark.parametrize("tokens", [4, 5, 7, 13, 17])
+@pytest.mark.parametrize("mask", [Mask.CAUSAL, Mask.CROSS])
+def test_a_request_whose_rows_pass_the_last_one_is_left_out_whole(be, tokens, mask):
+    """No page taken, none of its tokens stored; and a step of fewer tokens from these lengths goes on where the one before left off."""
+    new, cached = [5, 0, 9, 0, 4, 17], [20, 3, 15, 0, 40, 0]
+    s = R.Step(be, new, cached, mask=mask)
+    s.spec = dataclasses.replace(s.spec, tokens=tokens)
+    s.upload()
+    s.make_plan()
+    refused(be)
+    want = want_of(s, new, cached, s.table0, s.free)
+    assert not all(want[5])
+    check_plan(s, want)
+    # the next step, on the device's own results
+    free, kv, table = s.free[want[4]:], want[3].tolist(), want[0]
+    new = [1, 0, 2, 0, 1, 0]
+    s.b["new"].write(0, np.array(new, np.int32))
+    s.b["cached"].write(0, i32(s.b["kv"], 6).copy())
+    s.b["free"].write(0, np.concatenate([free, np.full(want[4], -1, np.int32)]).astype(np.int32))
+    s.make_plan()
+    be.synchronize()
+    check_plan(s, want_of(s, new, kv, table, free))
+
+
+@pytest.mark.parametrize("requests", [7, 256, 257, 1024, 1500, 2100])
+@pytest.mark.parametrize("mask", [Mask.CAUSAL, Mask.CROSS])
+def test_plans_with_requests_that_take_no_part(be, requests, mask):
+    """Some of many requests, whichever chunk of the scan they lie in, and rows that end somewhere between them."""
+    rng = np.random.default_rng(requests)
+    base, cached = rng.integers(0, 9, requests).tolist(), rng.integers(0, 70, requests).tolist()
+    for share in (0.05, 0.5):
+        s = R.Step(be, base, cached, hq=1, hkv=1, d=16, mask=mask, max_new=9)
+        s.spec = dataclasses.replace(s.spec, tokens=int(sum(base) * (0.7 if share < 0.5 else 0.3)) + 1)
+        s.upload()
+        new, c = list(base), list(cached)
+        for r in np.nonzero(rng.random(requests) < share)[0].tolist():
+            what = int(rng.integers(4))
+            if what == 0:
+                new[r] = -3
+            elif what == 1:
+                new[r] = 10
+            else:
+                c[r] = -1 if what == 2 else s.blocks * s.page + 1
+        s.b["new"].write(0, np.array(new, np.int32))
+        s.b["cached"].write(0, np.array(c, np.int32))
+        s.make_plan()
+        want = want_of(s, new, c, s.table0, s.free)
+        if all(want[5]):
+            be.synchronize()
+        else:
+            refused(be)
+        check_plan(s, want)
