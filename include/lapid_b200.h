@@ -428,10 +428,11 @@ typedef struct lapid_b200_paged {
 LAPID_B200_API lapid_b200_status lapid_b200_paged_plan_bytes(const lapid_b200_paged *desc, uint64_t *bytes);
 /* new_lens, cached_lens: i32 [requests], tokens to append and tokens already there. The pages that a request's new tokens
  * need beyond ceil(cached / page_size) are taken from free_pages (i32 [n_free], in order, requests in order; NULL with
- * n_free 0 when none are needed) and entered in its row of block_table (i32 [requests, max_blocks]; entries of cached tokens are
+ * n_free 0 when none are needed; an entry below 0 is no page, so a list whose length only the device knows is filled up with -1: with those left, pages have
+ * run out; the step can be run again from the same lengths when there are more) and entered in its row of block_table (i32 [requests, max_blocks]; entries of cached tokens are
  * read, others left alone). Out: slots and positions i32 [tokens] (page * page_size + place, and the token's index in its request;
  * -1 behind the last token), kv_lens i32 [requests] (what the next step passes as cached_lens; of a request that takes no part, its cached length), used i32 [1]
- * (how many free pages the step takes, also when there are fewer), plan. Running it again on the same inputs gives the same result. */
+ * (how many free pages the step takes, also when there are fewer; the caller drops as many from the front of the list), plan. Running it again on the same inputs gives the same result. */
 LAPID_B200_API lapid_b200_status lapid_b200_paged_plan(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *new_lens,
                                                        const lapid_b200_buffer *cached_lens, const lapid_b200_buffer *free_pages, uint64_t n_free,
                                                        lapid_b200_buffer *block_table, lapid_b200_buffer *slots, lapid_b200_buffer *positions,

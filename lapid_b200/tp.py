@@ -460,8 +460,9 @@ class PagedLayers(GpuTpLayers):
     (keys, values), CUDA tensors of `spec.cache_bytes()` each; a step of n layers takes the first n. `table` (i32 [requests, max_blocks]), `free` (i32, page
     numbers) and `rope` (f32 [rows, rot], `paged.rope_table`; None: no embedding) are CUDA tensors too; objects for prompts and for single tokens share
     all of them. Before a step the caller fills `h`, `new` and `cached` (i32 [requests]; `kv` of the step before is the next step's
-    `cached`) and drops the pages that the step before `used` from the front of `free`; all of it may happen on the device, so that a captured step can be replayed
-    while the requests grow.
+    `cached`) and drops the pages that the step before `used` from the front of `free` (`drop_used`); all of it may happen on the device, so that a captured step can be
+    replayed while the requests grow. `free` keeps its length: behind the pages that are left it must hold -1, and a step that finds no page there is
+    reported as "out_of_memory". Numbers left standing behind them would be given out a second time, and the requests that own those pages written over.
     """
 
     def __init__(self, backend, shape: LayerShape, spec, weights: list, formats: list, caches: list, table, free, rope=None, neighbours: bool = False,
@@ -483,6 +484,7 @@ class PagedLayers(GpuTpLayers):
         self.table, self.free, self.rope = table, free, rope
         self.new, self.cached, self.kv, self.used = i32(spec.requests), i32(spec.requests), i32(spec.requests), i32(1)
         self.slots, self.positions = i32(spec.tokens), i32(spec.tokens)
+        self._places = torch.arange(free.numel(), dtype=torch.int32, device=dev)
         self.q_half = torch.zeros_like(self.mixed)
         self.plan = torch.zeros(plan_bytes(spec), dtype=torch.uint8, device=dev)
         torch.cuda.synchronize(dev)
@@ -505,6 +507,14 @@ class PagedLayers(GpuTpLayers):
         append, attend = self._mixes[i]
         append()
         attend()
+
+    def drop_used(self):
+        """Queues, behind a step on the current stream, dropping the pages that it took from the front of `free`: the others move up, -1 takes their place at the end.
+        Once a step; part of a captured step where that is to be replayed."""
+        import torch
+        if self.free.numel():
+            at = self._places + self.used
+            self.free.copy_(torch.where(at < self.free.numel(), self.free[at.clamp(max=self.free.numel() - 1).long()], -1))
 
     def token(self, n_layers: int):
         """Queues a step of `n_layers` layers on the current stream: the plan, then the layers. Returns the residual stream behind the

@@ -142,3 +142,24 @@ def test_plans_with_requests_that_take_no_part(be, requests, mask):
         else:
             refused(be)
         check_plan(s, want)
+
+
+def test_free_pages_may_end_in_none(be):
+    """A list whose length only the device knows ends in -1: out of memory, not a bad index, and the pages in front are given out."""
+    s = R.Step(be, [40, 40], [0, 0]).upload()
+    free = s.free.copy()
+    free[4:] = -1
+    s.b["free"].write(0, free)
+    s.make_plan()
+    refused(be, "out_of_memory")
+    want = want_of(s, s.new, s.cached, s.table0, free)
+    assert want[4] == 6
+    check_plan(s, want)
+    # such entries that no request asks for are not looked at
+    s = R.Step(be, [40, 8], [0, 0]).upload()
+    free = s.free.copy()
+    free[4:] = -1
+    s.b["free"].write(0, free)
+    s.make_plan()
+    be.synchronize()
+    check_plan(s, want_of(s, s.new, s.cached, s.table0, free))
