@@ -523,3 +523,7 @@ class PagedLayers(GpuTpLayers):
             raise ValueError(f"{n_layers} layers, but caches for {len(self._mixes)}")
         self._plan_step()
         return super().token(n_layers)
+
+    def first_row_parallel(self):
+        self._plan_step()
+        return super().first_row_parallel()

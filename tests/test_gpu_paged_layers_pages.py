@@ -1,10 +1,10 @@
-"""Decoder layers over a paged cache when the free pages end."""
+"""Decoder layers over a paged cache when the free pages end, and a first exchange by itself."""
 import numpy as np
 import pytest
 
 import lapid_b200 as lp
 
-from .test_gpu_paged_layers import LAYERS, PAGE, Stack
+from .test_gpu_paged_layers import LAYERS, PAGE, SHAPE, Stack
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +75,17 @@ def test_pages_that_run_out_are_said_and_no_ones_keys_are_written_over(captured)
             break
     assert failed == (2, "out_of_memory")
     del graph
+
+
+def test_the_first_row_parallel_result_makes_its_plan():
+    s = Stack(lp.DType.BF16, [20, 3], 0)
+    s.fill(s.prompt, [20, 3], [0, 0])
+    with s.torch.cuda.stream(s.stream):
+        out = s.prompt.first_row_parallel()
+    s.stream.synchronize()
+    s.be.synchronize()
+    assert s.check_attention(s.prompt, 0, [20, 3], [0, 0]) == 23
+    h, o = s.prompt.h.double(), s.prompt.outs["o"].double()
+    assert float(o.abs().max()) > 0
+    assert s.torch.all((out.double() - (h + o)).abs() <= 2.0 ** -22 * (h.abs() + o.abs()))
+    assert out.shape == (23, SHAPE[0])
