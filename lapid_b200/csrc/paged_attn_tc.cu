@@ -194,13 +194,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 // 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a minimax polynomial in f (found by Remez's exchange; relative error 2.6e-6 at
-// degree 4; at degree 3, 7.5e-5, which the weights' type would hide but not the logarithm of their sum), n added to the exponent. For x <= 100; below -125 it stays 2^-125. The special-function unit forms
+// degree 4; at degree 3, 7.5e-5, which the weights' type would hide but not the logarithm of their sum), n added to the exponent. For x <= 100; below -125 it is 0, as it is
+// of a NaN (whose row's sum is one all the same). The special-function unit forms
 // 16 exponentials a cycle on an SM, and 128 x 128 of them take as long as the two products of 128 x 128 x 128: what it is relieved of here costs
 // five issue slots an element that the schedulers have.
 __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
     float a, b;
     unpack2(x, a, b);
-    x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
     const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));  // 1.5 2^23: n in the low bits
     const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
     uint64_t y = fma2(f, pack2(0.00957010221f, 0.00957010221f), pack2(0.0559178591f, 0.0559178591f));
@@ -210,8 +210,8 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
     float y0, y1, t0, t1;
     unpack2(y, y0, y1);
     unpack2(t, t0, t1);
-    r0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
-    r1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
+    r0 = a >= -125.0f ? __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23)) : 0.0f;
+    r1 = b >= -125.0f ? __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)) : 0.0f;
 }
 // The weights of N scores, their sums (added to l) and the largest score.
 template <bool BF16, int N> __device__ __forceinline__ float weights(const uint32_t (&x)[N], uint64_t c2, uint64_t b2, uint32_t (&w)[N / 2], uint64_t &l0, uint64_t &l1) {
@@ -755,8 +755,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             float a0, a1, a2, a3;
             unpack2(l0, a0, a1);
             unpack2(l1, a2, a3);
-            float l = m == -INFINITY ? 0.0f : (a0 + a1) + (a2 + a3);  // (no keys: polynomials of nothing)
-            if (a0 != a0) l = NAN;
+            float l = (a0 + a1) + (a2 + a3);
             const bool whole = w.steps == w.t.steps;
             const uint32_t first_unit = w.i0 + PAGED_LARGE_EXTRA;
             // A cut tile's first piece is the end of a span, its others are the beginnings of theirs. When they are there as the first is done they are added here, so that

@@ -1,0 +1,43 @@
+"""Attention over the paged cache where an error would be small or far away: keys that a mask leaves out, with values of any size."""
+import numpy as np
+import pytest
+
+import lapid_b200 as lp
+from tests import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def be():
+    return lp.Backend(0)
+
+
+@pytest.mark.parametrize("new,cached", [([50], [30]), ([130], [0]), ([3], [70])])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("why", ["causal", "window", "weight"])
+def test_a_key_without_weight_adds_nothing_whatever_its_value(be, new, cached, d, why):
+    """2^120 where a mask, or a score 1000 below the others, leaves a key no weight. Every 16 neighbouring keys in turn: the kernels do not treat them alike."""
+    window = 12 if why == "window" else 0
+    s = R.Step(be, new, cached, hq=8, hkv=2, d=d, window=window, seed=d)
+    n, c, kv = new[0], cached[0], s.kv[0]
+    first = {"causal": kv - min(n - 1, 16), "window": 0, "weight": 2}[why]   # (keys that the first rows, the last rows, no row takes part of)
+    for key in range(first, min(first + 16, kv)):
+        k, v = s.k[0].copy(), s.v[0].copy()
+        v[key] = 2.0 ** 120
+        s.k[0], s.v[0] = k, v
+        if why == "weight":   # q's first element 16, the key's -1000 * sqrt(d) / 16; the others' 0
+            s.q[:, :, 0] = 16.0
+            s.q_bits = R.to_half(s.q, s.dtype)[1]
+            k[:, :, 0] = 0.0
+            k[key, :, 0] = R.to_half(np.array([-1000.0 / (16.0 * s.scale)]), s.dtype)[0][0]
+        s.upload()
+        s.make_plan()
+        s.attend()
+        be.synchronize()
+        out, _ = s.outputs()
+        v[key] = 0.0
+        o, _, size = R.attention(s.q, k, v, s.g, s.mask, window, s.scale, n, kv)
+        rows = [t for t in range(n) if why == "weight" or not R.seen(s.mask, window, n, kv, t)[0] <= key < R.seen(s.mask, window, n, kv, t)[1]]
+        assert rows or why == "window"
+        assert np.all(np.abs(out[rows] - o[rows]) <= R.bound(s.dtype, o[rows], size[rows], kv, 6.0)), key
