@@ -721,13 +721,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 top *= c;
                 // the product of the step before is done: P's columns are free, O may change
                 if (k > 0 && !(healthy = warp_wait(o_full + t, (k - 1) & 1))) break;
+                fence_after();  // (the stores to P's columns and the loads and stores of O come behind that product)
                 if (__any_sync(0xffffffffu, real && top > m + LAZY)) {
                     const float mn = fmaxf(m, top), bn = mn == -INFINITY ? 0.0f : mn, keep = exp2_fast(m - bn);
                     m = mn, base = bn;
                     const uint64_t k2 = pack2(keep, keep);
                     n0 = pipe::mul2(l0, k2), n1 = pipe::mul2(l1, k2);
                     if (j) {
-                        fence_after();
 #pragma unroll 1
                         for (int i = 0; i < DP / 32; i++) {
                             uint32_t o[32];
