@@ -193,25 +193,26 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a minimax polynomial in f (found by Remez's exchange; relative error 2.6e-6 at
-// degree 4; at degree 3, 7.5e-5, which the weights' type would hide but not the logarithm of their sum), n added to the exponent. For x <= 100; below -125 it is 0, as it is
-// of a NaN (whose row's sum is one all the same). The special-function unit forms
-// 16 exponentials a cycle on an SM, and 128 x 128 of them take as long as the two products of 128 x 128 x 128: what it is relieved of here costs
-// five issue slots an element that the schedulers have.
+// 2^x of a pair by Cody and Waite's reduction, x = n + f with |f| <= 1/2, and a polynomial in f, n added to the exponent. The polynomial is 1 at f = 0 and
+// otherwise the minimax one (by linear programming; relative error 2.9e-6 at degree 4, at degree 3 7.5e-5, which the weights' type would hide but not the logarithm of their sum). For
+// x <= 100. What is below -127, the scores that a mask leaves out among them, is taken as -127: n = -127 takes the 1's exponent to nothing, so the weight is +0 without a test
+// (with two tests and selects a pair: window 65.0 instead of 63.6 us). The special-function unit forms 16 exponentials a cycle on an SM, and 128 x 128 of
+// them take as long as the two products of 128 x 128 x 128: what it is relieved of here costs five issue slots an element that the schedulers have.
 __device__ __forceinline__ void exp2_poly(uint64_t x, float &r0, float &r1) {
     float a, b;
     unpack2(x, a, b);
+    x = pack2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
     const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));  // 1.5 2^23: n in the low bits
     const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
-    uint64_t y = fma2(f, pack2(0.00957010221f, 0.00957010221f), pack2(0.0559178591f, 0.0559178591f));
-    y = fma2(f, y, pack2(0.240247443f, 0.240247443f));
-    y = fma2(f, y, pack2(0.693121791f, 0.693121791f));
-    y = fma2(f, y, pack2(0.999999285f, 0.999999285f));
+    uint64_t y = fma2(f, pack2(0.00958285294f, 0.00958285294f), pack2(0.0559064262f, 0.0559064262f));
+    y = fma2(f, y, pack2(0.240240991f, 0.240240991f));
+    y = fma2(f, y, pack2(0.693124175f, 0.693124175f));
+    y = fma2(f, y, pack2(1.0f, 1.0f));
     float y0, y1, t0, t1;
     unpack2(y, y0, y1);
     unpack2(t, t0, t1);
-    r0 = a >= -125.0f ? __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23)) : 0.0f;
-    r1 = b >= -125.0f ? __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)) : 0.0f;
+    r0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+    r1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
 // The weights of N scores, their sums (added to l) and the largest score.
 template <bool BF16, int N> __device__ __forceinline__ float weights(const uint32_t (&x)[N], uint64_t c2, uint64_t b2, uint32_t (&w)[N / 2], uint64_t &l0, uint64_t &l1) {
