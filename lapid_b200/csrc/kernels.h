@@ -414,9 +414,9 @@ struct PagedShape {
     uint32_t large_keys;  // step of the tensor-memory kernel (paged_attn_tc.cu says why): 80 keys where head_dim is above 64, else 96
     float scale;
 };
-// Places in a plan buffer (32-bit words; the partial results behind them at byte offsets)
+// Places in a plan buffer (32-bit words; `request`: the row of q where its tokens begin, the one where they end, its keys, 0; the partial results behind them at byte offsets)
 struct PagedPlanLayout {
-    uint32_t q_start, new_len, kv_len, units_small, units_large, start_small, start_large, count_small, count_large;
+    uint32_t request, units_small, units_large, start_small, start_large, count_small, count_large;
     size_t part_small, part_large, bytes;  // part_*: [CTA][2] results of cut tiles: rows x (d padded + 2) f32
 };
 PagedPlanLayout paged_plan_layout(const PagedShape &s);

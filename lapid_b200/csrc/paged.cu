@@ -32,9 +32,7 @@ PagedPlanLayout paged_plan_layout(const PagedShape &s) {
         return at;
     };
     const uint32_t cs = paged_attn_small_ctas(PAGED_MAX_SMS), cl = paged_has_large(s) ? paged_attn_large_ctas(PAGED_MAX_SMS) : 0;
-    l.q_start = take(s.requests);
-    l.new_len = take(s.requests);
-    l.kv_len = take(s.requests);
+    l.request = take(4 * s.requests);
     l.units_small = take(s.requests + 1);
     l.units_large = take(s.requests + 1);
     l.start_small = take(sizeof(PagedStart) / 4 * cs);
@@ -101,10 +99,11 @@ __device__ __forceinline__ uint32_t last_at_most(const uint32_t *a, uint32_t n, 
     return lo;
 }
 
-// What each CTA of an attention launch begins with: warp `worker` of `workers` takes every workers-th of them. `prefix`: units before each request, `q0` its first
-// row, `n` its new tokens, `kv` its keys.
-__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, const uint32_t *q0, const uint32_t *n, const uint32_t *kv,
-                          uint32_t *starts, uint32_t rows, uint32_t keys, uint32_t extra, uint32_t worker, uint32_t workers) {
+// What each CTA of an attention launch begins with: warp `worker` of `workers` takes every workers-th of them. `prefix`: units before each request, `request`: what the
+// plan holds of one.
+template <class Request>
+__device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas, uint32_t all, const uint32_t *prefix, Request request, uint32_t *starts, uint32_t rows, uint32_t keys,
+                          uint32_t extra, uint32_t worker, uint32_t workers) {
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t b = worker; b < all; b += workers) {
         PagedStart x{};
@@ -114,7 +113,8 @@ __device__ void cut_units(const PagedPlanArgs &a, uint32_t units, uint32_t ctas,
             x.u1 = __shfl_sync(0xffffffffu, x.u0, 1);
             x.u0 = __shfl_sync(0xffffffffu, x.u0, 0);
             const uint32_t r = last_at_most(prefix, a.s.requests, x.u0);
-            x.r = r, x.q0 = q0[r], x.n = n[r], x.kv = kv[r];
+            const uint4 q = request(r);
+            x.r = r, x.q0 = q.x, x.n = q.y - q.x, x.kv = q.z;
             const uint32_t per_head = (prefix[r + 1] - prefix[r]) / a.s.hkv, off = x.u0 - prefix[r], tiles = paged_tiles(a.s, x.n, rows);
             x.head = off / per_head;
             uint32_t rem = off - x.head * per_head;
@@ -213,9 +213,7 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
             if (tid == 0) sh.small[count] = small, sh.large[count] = large;
         }
         if (writes && r < s.requests) {
-            a.plan[a.l.q_start + r] = lo;
-            a.plan[a.l.new_len + r] = n;
-            a.plan[a.l.kv_len + r] = kv;
+            ((uint4 *)(a.plan + a.l.request))[r] = make_uint4(lo, lo + n, kv, 0);
             a.kv_lens[r] = (int32_t)kv;
             if (!one) a.plan[a.l.units_small + r] = sh.small[tid], a.plan[a.l.units_large + r] = sh.large[tid];
         }
@@ -273,12 +271,12 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
         cl = min(cl, max(share, 1u));
         cs = min(cs, max(a.ctas_small / sms * (sms - cl), 1u));
     }
-    const uint32_t *q0 = one ? sh.start : a.plan + a.l.q_start, *n = one ? sh.n : a.plan + a.l.new_len, *kv = one ? sh.kv : a.plan + a.l.kv_len;
+    auto request = [&](uint32_t r) { return one ? make_uint4(sh.start[r], sh.start[r] + sh.n[r], sh.kv[r], 0) : ((const uint4 *)(a.plan + a.l.request))[r]; };
     const uint32_t warp = worker * (T / 32) + tid / 32, warps = (one ? workers : 1) * (T / 32);
-    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, q0, n, kv, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);
+    cut_units(a, small, cs, a.ctas_small, one ? sh.small : a.plan + a.l.units_small, request, a.plan + a.l.start_small, PAGED_SMALL_ROWS, PAGED_SMALL_KEYS, 0, warp, warps);
     // (from the other end: a warp has a start of one kind or of the other)
     if (a.ctas_large)
-        cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, q0, n, kv, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, warps - 1 - warp, warps);
+        cut_units(a, large, cl, a.ctas_large, one ? sh.large : a.plan + a.l.units_large, request, a.plan + a.l.start_large, paged_large_rows(s), s.large_keys, PAGED_LARGE_EXTRA, warps - 1 - warp, warps);
 }
 
 static void paged_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, dim3 grid, unsigned threads, size_t smem, bool pdl, cudaStream_t stream) {

@@ -78,9 +78,8 @@ struct Walk {
     PagedTile t;
 };
 __device__ __forceinline__ void load_request(const PagedAttnArgs &p, Walk &w) {
-    w.q0 = p.plan[p.l.q_start + w.r];
-    w.n = p.plan[p.l.new_len + w.r];
-    w.kv = p.plan[p.l.kv_len + w.r];
+    const uint4 x = ((const uint4 *)(p.plan + p.l.request))[w.r];
+    w.q0 = x.x, w.n = x.y - x.x, w.kv = x.z;
     w.tiles = paged_tiles(p.s, w.n, ROWS);
 }
 __device__ __forceinline__ void load_tile(const PagedAttnArgs &p, Walk &w) { w.t = paged_tile(p.s, w.n, w.kv, w.tile, ROWS, KEYS); }
