@@ -414,9 +414,10 @@ struct PagedShape {
     uint32_t large_keys;  // step of the tensor-memory kernel (paged_attn_tc.cu says why): 80 keys where head_dim is above 64, else 96
     float scale;
 };
-// Places in a plan buffer (32-bit words; `request`: the row of q where its tokens begin, the one where they end, its keys, 0; the partial results behind them at byte offsets)
+// Places in a plan buffer (32-bit words; `past`, at the same place whatever the description: 1 from when the kernel for many rows has waited for what is in front of it until
+// both are over; `request`: the row of q where its tokens begin, the one where they end, its keys, 0; the partial results behind them at byte offsets)
 struct PagedPlanLayout {
-    uint32_t request, units_small, units_large, start_small, start_large, count_small, count_large;
+    uint32_t past, request, units_small, units_large, start_small, start_large, count_small, count_large;
     size_t part_small, part_large, bytes;  // part_*: [CTA][2] results of cut tiles: rows x (d padded + 2) f32
 };
 PagedPlanLayout paged_plan_layout(const PagedShape &s);
@@ -459,7 +460,7 @@ struct PagedAttnArgs {
     void *out;
     float *lse;
     int *status;
-    bool behind;  // the kernel for few rows: the one for many is in front of it, and nothing it needs comes from there
+    bool behind;  // the kernel for few rows: the one for many is in front of it, and nothing it needs is made there
 };
 uint32_t paged_attn_small_ctas(int sm_count);
 uint32_t paged_attn_large_ctas(int sm_count);

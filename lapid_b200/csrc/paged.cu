@@ -32,6 +32,7 @@ PagedPlanLayout paged_plan_layout(const PagedShape &s) {
         return at;
     };
     const uint32_t cs = paged_attn_small_ctas(PAGED_MAX_SMS), cl = paged_has_large(s) ? paged_attn_large_ctas(PAGED_MAX_SMS) : 0;
+    l.past = take(1);  // (the first word: written before it is known whether the plan is one for this description)
     l.request = take(4 * s.requests);
     l.units_small = take(s.requests + 1);
     l.units_large = take(s.requests + 1);
@@ -251,6 +252,7 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
     if (writes) {
         if (tid == 0) {
             *a.used = (int32_t)taken;
+            a.plan[a.l.past] = 0;
             if (!one) a.plan[a.l.units_small + s.requests] = small, a.plan[a.l.units_large + s.requests] = large;
         }
         for (uint32_t b = tid; b < a.ctas_small; b += T) a.plan[a.l.count_small + b] = 0;

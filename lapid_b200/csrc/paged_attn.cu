@@ -126,18 +126,30 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
         }
         mbar_fence_init();
     }
+    // Behind the kernel for many rows this one starts as soon as all that was in front of that is over; the two share no memory that either writes. That what was in front is
+    // visible here comes through a word that the other's first CTA releases behind its own wait; where it is not there the wait for that kernel's end does it.
+    // And this grid's end has to mean that one's too: its first CTA waits before it leaves, and takes the word back.
+    if (p.behind && threadIdx.x == 32) {
+        uint32_t past;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(past) : "l"(p.plan + p.l.past) : "memory");
+        *is_last = past;
+    }
     __syncthreads();
-    // Behind the kernel for many rows nothing needs to be waited for: it let this one start when all that was in front of it was over, and the two share no
-    // memory that either writes. But this grid's end has to mean that one's too: its first CTA waits before it leaves.
-    const bool holds = p.behind && blockIdx.x == 0;
-    if (!p.behind) asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool ahead = p.behind && *is_last, holds = p.behind && blockIdx.x == 0;
+    if (!ahead) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (p.behind) asm volatile("fence.proxy.async.global;" ::: "memory");  // (the pages are read by TMA)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto leave = [&]() {
+        if (!holds) return;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        p.plan[p.l.past] = 0;
+    };
     const uint32_t b = blockIdx.x;
     const PagedStart at = paged_load_start(p.plan + p.l.start_small + b * (sizeof(PagedStart) / 4));
     if (at.stamp != p.stamp && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_PLAN);
     const uint32_t units = at.units, ctas = at.ctas, u0 = at.u0, u1 = at.u1;
     if (at.stamp != p.stamp || u0 == u1) {
-        if (holds) asm volatile("griddepcontrol.wait;" ::: "memory");
+        leave();
         return;
     }
     Walk w;
@@ -180,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
         // the copies in flight have to land before the CTA leaves
         for (uint32_t i = 0; i < C::STAGES; i++) mbar_wait(full + i, i < stage ? ph ^ 1 : ph, SPIN_LIMIT);
         if (!healthy && lane == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_WAIT);
-        if (holds) asm volatile("griddepcontrol.wait;" ::: "memory");
+        leave();
         return;
     }
 

@@ -449,7 +449,12 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
     fence_after();
     const uint32_t tmem = uniform(*tmem_slot);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // (the kernel for few rows, started by the next instruction, reads there that what was written in front of this kernel is visible; by a warp that has time)
+    if (warp == MMA_WARP + 1) {
+        if (lane == 0 && blockIdx.x == 0) asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p.plan + p.l.past), "r"(1u) : "memory");
+        __syncwarp();
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
     const uint32_t b = blockIdx.x;
     const PagedStart at = paged_load_start(p.plan + p.l.start_large + b * (sizeof(PagedStart) / 4));
     const bool stale = uniform(at.stamp) != p.stamp;

@@ -1,4 +1,4 @@
-"""Attention over the paged cache where an error would be small or far away: keys that a mask leaves out, with values of any size."""
+"""Attention over the paged cache where an error would be small or far away: keys that a mask leaves out, with values of any size, and keys appended just before."""
 import numpy as np
 import pytest
 
@@ -6,6 +6,7 @@ import lapid_b200 as lp
 from tests import paged_ref as R
 
 pytestmark = pytest.mark.gpu
+BF16, F32 = lp.DType.BF16, lp.DType.F32
 
 
 @pytest.fixture(scope="module")
@@ -41,3 +42,28 @@ def test_a_key_without_weight_adds_nothing_whatever_its_value(be, new, cached, d
         rows = [t for t in range(n) if why == "weight" or not R.seen(s.mask, window, n, kv, t)[0] <= key < R.seen(s.mask, window, n, kv, t)[1]]
         assert rows or why == "window"
         assert np.all(np.abs(out[rows] - o[rows]) <= R.bound(s.dtype, o[rows], size[rows], kv, 6.0)), key
+
+
+def test_few_rows_beside_many_read_what_was_appended_just_before(be):
+    """Append and attention queued behind each other, other keys and values every time: a prompt's chunk and single tokens, whose kernels run side by side."""
+    new, cached, hq, hkv, d = [1, 70, 1, 1, 2], [200, 40, 63, 31, 500], 8, 2, 64
+    s = R.Step(be, new, cached, hq=hq, hkv=hkv, d=d).upload()
+    rng = np.random.default_rng(7)
+    sets, t = [], s.tokens
+    for _ in range(6):
+        k, v = rng.normal(size=(t, hkv, d)).astype(np.float32), rng.normal(size=(t, hkv, d)).astype(np.float32)
+        sets.append((k, v, be.upload(k), be.upload(v), be.upload(np.zeros(t * hq * d, np.int16)), be.upload(np.zeros(t * hq, np.float32))))
+    b = s.b
+    be.synchronize()
+    for i in range(30):
+        _, _, kb, vb, out, lse = sets[i % 6]
+        s.make_plan()
+        be.paged_append(s.spec, F32, None, kb, vb, b["slots"], b["positions"], b["k"], b["v"], None)
+        be.paged_attention(s.spec, b["plan"], b["q"], b["k"], b["v"], b["table"], out, lse=lse)
+    be.synchronize()
+    for k, v, _, _, out, lse in sets:
+        at = 0
+        for r, n in enumerate(new):
+            s.k[r][cached[r]:], s.v[r][cached[r]:] = R.to_half(k[at:at + n], BF16)[0], R.to_half(v[at:at + n], BF16)[0]
+            at += n
+        s.check((R.from_half(out.download().view(np.int16)[: t * hq * d], BF16).reshape(t, hq, d), lse.download().view(np.float32)[: t * hq].astype(np.float64).reshape(t, hq)))
