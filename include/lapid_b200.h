@@ -408,7 +408,7 @@ LAPID_B200_API lapid_b200_status lapid_b200_silu_mul_act(lapid_b200_device *dev,
  * lapid_b200_paged describes a step; zero-fill it first. */
 #define LAPID_B200_MASK_FULL 0   /* a new token sees all keys, cached and new */
 #define LAPID_B200_MASK_CAUSAL 1 /* ... up to its own; with window > 0 the last `window` of these */
-#define LAPID_B200_MASK_CROSS 2  /* ... the cached ones only: nothing is appended (slots are -1) */
+#define LAPID_B200_MASK_CROSS 2  /* ... the cached ones only: nothing is appended (slots are -1, paged_append takes q alone) */
 typedef struct lapid_b200_paged {
     int32_t dtype;       /* of the cache, q and out: F16 or BF16 */
     uint32_t q_heads;    /* a multiple of kv_heads: query head h reads key/value head h / (q_heads / kv_heads) */
@@ -442,7 +442,8 @@ LAPID_B200_API lapid_b200_status lapid_b200_paged_plan(lapid_b200_device *dev, c
  * of one fused projection's rows. rope (NULL: none): f32 [rope_rows, rot], row p the cosines of position p's rot / 2 angles, then their
  * sines; the first rot (a multiple of 8) elements of each q and k head are turned in pairs (i, i + rot / 2), or with
  * neighbours = 1 (2 i, 2 i + 1), in f32. Results are rounded once to the cache's type: k and v to their slots, q to q_out
- * [tokens, q_heads, head_dim] contiguous (q and q_out NULL: only k and v). Rows with position -1 are skipped, with slot -1 not stored. */
+ * [tokens, q_heads, head_dim] contiguous. q and q_out NULL: only k and v. k, v, k_cache and v_cache NULL: q alone, slots are not read -- what a CROSS step takes, and
+ * a layer that reads another one's cache. Rows with position -1 are skipped, with slot -1 not stored. */
 LAPID_B200_API lapid_b200_status lapid_b200_paged_append(lapid_b200_device *dev, const lapid_b200_paged *desc, int32_t src_dtype,
                                                          const lapid_b200_buffer *q, const lapid_b200_matview *q_view, const lapid_b200_buffer *k,
                                                          const lapid_b200_matview *k_view, const lapid_b200_buffer *v, const lapid_b200_matview *v_view,

@@ -457,8 +457,8 @@ class Backend:
         attention over the SMs into ``plan`` (``lapid_b200_paged_plan``). Arguments: ``packed_paged_plan``."""
         self.packed_paged_plan(*args, **kw)()
 
-    def packed_paged_append(self, spec, src_dtype: DType, q: Optional[Buffer], k: Buffer, v: Buffer, slots: Buffer, positions: Buffer, k_cache: Buffer,
-                            v_cache: Buffer, q_out: Optional[Buffer], *, rope: Optional[Buffer] = None, rope_rows: int = 0, rot: int = 0,
+    def packed_paged_append(self, spec, src_dtype: DType, q: Optional[Buffer], k: Optional[Buffer], v: Optional[Buffer], slots: Optional[Buffer],
+                            positions: Buffer, k_cache: Optional[Buffer], v_cache: Optional[Buffer], q_out: Optional[Buffer], *, rope: Optional[Buffer] = None, rope_rows: int = 0, rot: int = 0,
                             neighbours: bool = False, q_view: Optional[MatView] = None, k_view: Optional[MatView] = None,
                             v_view: Optional[MatView] = None):
         """``paged_append`` as a zero-argument callable."""
@@ -469,7 +469,7 @@ class Backend:
                                  int(bool(neighbours)), *h[4:]), bufs)
 
     def paged_append(self, *args, **kw) -> None:
-        """Rotary embedding of q and k, rounding to the cache's type, k and v to their slots, q to ``q_out``
+        """Rotary embedding of q and k, rounding to the cache's type, k and v to their slots, q to ``q_out``; k and v alone, or q alone (None for the rest)
         (``lapid_b200_paged_append``). A view is a ``MatView``: ``batch_stride`` from head to head, ``row_stride`` from token to token."""
         self.packed_paged_append(*args, **kw)()
 

@@ -2427,21 +2427,28 @@ lapid_b200_status lapid_b200_paged_append(lapid_b200_device *dev, const lapid_b2
         lb::PagedAppendArgs a{};
         a.s = paged_shape(desc);
         if (!is_act_float(src_dtype)) fail("unsupported_dtype", "paged_append: src_dtype must be F32, F16 or BF16, got " + std::to_string(src_dtype));
-        if (a.s.mask == lb::PAGED_CROSS) fail("invalid_launch", "paged_append: a CROSS step appends nothing");
+        const bool stores = k || v || k_cache || v_cache;  // else q alone
+        if (a.s.mask == lb::PAGED_CROSS && stores) fail("invalid_launch", "paged_append: a CROSS step appends nothing: q alone");
         if ((q == nullptr) != (q_out == nullptr)) fail("invalid_argument", "paged_append: q and q_out come together");
+        if (stores && !(k && v && k_cache && v_cache)) fail("invalid_argument", "paged_append: k, v, k_cache and v_cache come together");
+        if (!stores && !q) fail("invalid_argument", "paged_append: neither q nor k and v");
         if ((rope == nullptr) != (rot == 0)) fail("invalid_argument", "paged_append: rope and rot come together");
         if (rot % 8 != 0 || rot > a.s.d) fail("invalid_launch", "paged_append: rot must be a multiple of 8 and at most head_dim, got " + std::to_string(rot));
         if (neighbours != 0 && neighbours != 1) fail("invalid_argument", "paged_append: neighbours must be 0 or 1");
         if (rope_rows >= (1ull << 31)) fail("too_large", "paged_append: rope_rows must be below 2^31");
         const uint64_t T = a.s.tokens, eb = act_elem_size(src_dtype), cache = (uint64_t)a.s.pages * a.s.hkv * a.s.page * a.s.d * 2;
         if (q) a.qv = paged_view(dev, q, q_view, "paged_append: q", T, a.s.hq, a.s.d, eb);
-        a.kv = paged_view(dev, k, k_view, "paged_append: k", T, a.s.hkv, a.s.d, eb);
-        a.vv = paged_view(dev, v, v_view, "paged_append: v", T, a.s.hkv, a.s.d, eb);
+        if (stores) {
+            a.kv = paged_view(dev, k, k_view, "paged_append: k", T, a.s.hkv, a.s.d, eb);
+            a.vv = paged_view(dev, v, v_view, "paged_append: v", T, a.s.hkv, a.s.d, eb);
+            paged_buffer(dev, slots, "paged_append: slots", T * 4);
+            paged_buffer(dev, k_cache, "paged_append: k_cache", cache);
+            paged_buffer(dev, v_cache, "paged_append: v_cache", cache);
+        } else {
+            slots = nullptr;
+        }
         if (rope) paged_buffer(dev, rope, "paged_append: rope", rope_rows * rot * 4);
-        paged_buffer(dev, slots, "paged_append: slots", T * 4);
         paged_buffer(dev, positions, "paged_append: positions", T * 4);
-        paged_buffer(dev, k_cache, "paged_append: k_cache", cache);
-        paged_buffer(dev, v_cache, "paged_append: v_cache", cache);
         if (q_out) paged_buffer(dev, q_out, "paged_append: q_out", T * a.s.hq * a.s.d * 2);
         const lapid_b200_buffer *ins[] = {q, k, v, rope, slots, positions}, *outs[] = {k_cache, v_cache, q_out};
         for (size_t i = 0; i < 3; i++) {
@@ -2449,23 +2456,23 @@ lapid_b200_status lapid_b200_paged_append(lapid_b200_device *dev, const lapid_b2
             for (const lapid_b200_buffer *b : ins)
                 if (b && paged_overlap(b, outs[i])) fail("buffer_aliasing", "paged_append: an output aliases an input");
             for (size_t j = 0; j < i; j++)
-                if (paged_overlap(outs[i], outs[j])) fail("buffer_aliasing", "paged_append: two outputs alias");
+                if (outs[j] && paged_overlap(outs[i], outs[j])) fail("buffer_aliasing", "paged_append: two outputs alias");
         }
         if (T == 0) return;
         std::lock_guard<std::mutex> lock(dev->mu);
         dev->make_current();
         a.src_type = act_type_of(src_dtype);
         a.q = q ? q->ptr : nullptr;
-        a.k = k->ptr;
-        a.v = v->ptr;
+        a.k = k ? k->ptr : nullptr;
+        a.v = v ? v->ptr : nullptr;
         a.rope = rope ? (const float *)rope->ptr : nullptr;
         a.rope_rows = (uint32_t)rope_rows;
         a.rot = rot;
         a.neighbours = (uint32_t)neighbours;
-        a.slots = (const int32_t *)slots->ptr;
+        a.slots = slots ? (const int32_t *)slots->ptr : nullptr;
         a.positions = (const int32_t *)positions->ptr;
-        a.k_cache = k_cache->ptr;
-        a.v_cache = v_cache->ptr;
+        a.k_cache = k_cache ? k_cache->ptr : nullptr;
+        a.v_cache = v_cache ? v_cache->ptr : nullptr;
         a.q_out = q_out ? q_out->ptr : nullptr;
         a.status = dev->status_dev;
         cuda_check(lb::launch_paged_append(a, dev->pdl, dev->stream), "paged_append launch");

@@ -440,7 +440,7 @@ struct PagedView {
 struct PagedAppendArgs {
     PagedShape s;
     int src_type;  // ACT_F32 / ACT_F16 / ACT_BF16
-    const void *q, *k, *v;
+    const void *q, *k, *v;  // q or k and v may be null; without k and v there are no slots and no cache
     PagedView qv, kv, vv;
     const float *rope;  // [rope_rows][rot]: cos, then sin
     uint32_t rope_rows, rot, neighbours;

@@ -334,12 +334,12 @@ template <int SRC, bool VEC> __global__ void __launch_bounds__(APPEND_THREADS) p
     const PagedShape &s = p.s;
     const uint32_t chunks = s.d / 8, lanes = APPEND_THREADS / chunks, c = threadIdx.x % chunks, hl = threadIdx.x / chunks;
     if (hl >= lanes) return;
-    const uint32_t hq = p.q ? s.hq : 0, heads = hq + 2 * s.hkv, half = p.rot / 2;
+    const uint32_t hq = p.q ? s.hq : 0, heads = hq + (p.k ? 2 * s.hkv : 0), half = p.rot / 2;
     const bool turned = c < p.rot / 8;
     const bool bf16 = s.bf16;
     const uint32_t shift = 31 - __clz(s.page);  // (page sizes are powers of two)
     for (uint32_t t = blockIdx.x; t < s.tokens; t += gridDim.x) {
-        const int32_t slot = p.slots[t], pos = p.positions[t];
+        const int32_t slot = p.slots ? p.slots[t] : -1, pos = p.positions[t];
         float4 cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const bool stored = slot >= 0 && (uint32_t)slot < s.pages << shift, sound = pos >= 0 && !(p.rot && (uint32_t)pos >= p.rope_rows) && (slot < 0 || stored);
         bool first = true;
@@ -402,7 +402,7 @@ template <int SRC> static cudaError_t append_src(const PagedAppendArgs &a, bool 
 }
 
 cudaError_t launch_paged_append(const PagedAppendArgs &a, bool pdl, cudaStream_t stream) {
-    const uint32_t eb = act_elem_bytes(a.src_type), per = APPEND_THREADS / (a.s.d / 8) * APPEND_HEADS, heads = (a.q ? a.s.hq : 0) + 2 * a.s.hkv;
+    const uint32_t eb = act_elem_bytes(a.src_type), per = APPEND_THREADS / (a.s.d / 8) * APPEND_HEADS, heads = (a.q ? a.s.hq : 0) + (a.k ? 2 * a.s.hkv : 0);
     bool vec = true;  // every group of four elements starts on a multiple of its size
     auto check = [&](const void *base, const PagedView &v) {
         if (base && (((uintptr_t)base + v.off * eb) % (4 * eb) || v.head % 4 || v.token % 4)) vec = false;

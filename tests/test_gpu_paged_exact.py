@@ -1,12 +1,15 @@
-"""Attention over the paged cache where an error would be small or far away: keys that a mask leaves out, with values of any size, and keys appended just before."""
+"""Attention over the paged cache where an error would be small or far away: keys that a mask leaves out, with values of any size, keys appended just before, and q
+alone (a step that appends nothing)."""
 import numpy as np
 import pytest
 
 import lapid_b200 as lp
+from lapid_b200.backend import MatView
+from lapid_b200.paged import Mask, rope_table
 from tests import paged_ref as R
 
 pytestmark = pytest.mark.gpu
-BF16, F32 = lp.DType.BF16, lp.DType.F32
+BF16, F16, F32 = lp.DType.BF16, lp.DType.F16, lp.DType.F32
 
 
 @pytest.fixture(scope="module")
@@ -67,3 +70,52 @@ def test_few_rows_beside_many_read_what_was_appended_just_before(be):
             s.k[r][cached[r]:], s.v[r][cached[r]:] = R.to_half(k[at:at + n], BF16)[0], R.to_half(v[at:at + n], BF16)[0]
             at += n
         s.check((R.from_half(out.download().view(np.int16)[: t * hq * d], BF16).reshape(t, hq, d), lse.download().view(np.float32)[: t * hq].astype(np.float64).reshape(t, hq)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("mask", [Mask.CROSS, Mask.CAUSAL])
+@pytest.mark.parametrize("rot", [0, 32])
+def test_q_alone(be, dtype, mask, rot):
+    """From f32 projections to the attention over keys that are there already: cross attention, and a layer that reads another one's cache."""
+    new, cached, hq, hkv, d = [5, 1, 40], [100, 33, 64], 8, 2, 64
+    s = R.Step(be, new, cached, hq=hq, hkv=hkv, d=d, dtype=dtype, mask=mask, pad=1).upload()
+    s.make_plan()
+    x = np.random.default_rng(2).normal(size=(s.tokens, hq, d)).astype(np.float32)
+    q_out, table = be.upload(np.full((s.tokens, hq, d), 0x1111, np.int16)), rope_table(128, 32)
+    kc = s.b["k"].download().copy()
+    kw = dict(rope=be.upload(table), rope_rows=128, rot=32) if rot else {}
+    be.paged_append(s.spec, F32, be.upload(x), None, None, None, s.b["positions"], None, None, q_out, **kw)
+    be.paged_attention(s.spec, s.b["plan"], q_out, s.b["k"], s.b["v"], s.b["table"], s.b["out"], lse=s.b["lse"])
+    be.synchronize()
+    assert np.array_equal(kc, s.b["k"].download())
+    bits = q_out.download().view(np.int16).reshape(s.tokens, hq, d)
+    assert np.all(bits[sum(new):] == 0x1111)
+    want, pos = x.astype(np.float64), s.want[2]
+    if rot:
+        c, sn = (table[np.maximum(pos, 0)][:, i * 16:(i + 1) * 16].astype(np.float64)[:, None] for i in (0, 1))
+        a, b = want[..., :16].copy(), want[..., 16:32].copy()
+        want[..., :16], want[..., 16:32] = a * c - b * sn, b * c + a * sn
+    got = R.from_half(bits, dtype).reshape(bits.shape)
+    n = sum(new)
+    assert np.all(np.abs(got[:n] - want[:n]) <= R.U[dtype] * np.abs(want[:n]) + (2.0 ** -25 if dtype == F16 else 0.0) + 2.0 ** -22 * (np.abs(want[:n]) + np.abs(x).max()))
+    s.q[:n] = got[:n]
+    s.check()
+
+
+def test_refusals_of_an_append_of_q_alone(be):
+    s = R.Step(be, [3], [20], hq=4, hkv=2, d=64).upload()
+    c = R.Step(be, [3], [20], hq=4, hkv=2, d=64, mask=Mask.CROSS).upload()
+    b, x = s.b, be.upload(np.zeros(3 * 4 * 64, np.float32))
+    for spec, args, code in ((s.spec, (x, x, None, b["slots"], b["positions"], b["k"], b["v"], b["out"]), "invalid_argument"),
+                             (s.spec, (x, None, x, b["slots"], b["positions"], b["k"], b["v"], b["out"]), "invalid_argument"),
+                             (s.spec, (x, None, None, b["slots"], b["positions"], b["k"], None, b["out"]), "invalid_argument"),
+                             (s.spec, (x, x, x, None, b["positions"], b["k"], b["v"], b["out"]), "invalid_argument"),
+                             (s.spec, (None, None, None, b["slots"], b["positions"], None, None, None), "invalid_argument"),
+                             (s.spec, (x, None, None, None, None, None, None, b["out"]), "invalid_argument"),
+                             (c.spec, (x, x, x, b["slots"], b["positions"], b["k"], b["v"], b["out"]), "invalid_launch")):
+        with pytest.raises(lp.LapidError) as e:
+            be.paged_append(spec, F32, *args)
+        assert e.value.code == code, args
+    with pytest.raises(lp.LapidError) as e:
+        be.paged_append(s.spec, F32, x, None, None, None, b["positions"], None, None, b["out"], q_view=MatView(1, 64, 256))
+    assert e.value.code == "out_of_bounds"
