@@ -223,9 +223,9 @@ template <uint32_t T> __global__ void __launch_bounds__(T) paged_plan_kernel(Pag
         for (uint32_t j = taken + worker * T + tid; j < end_p; j += workers * T) {
             const uint32_t i = last_at_most(sh.first, count, j);
             int32_t page = -1;
-            if (j < a.n_free) page = a.free_pages[j];
-            if (page < 0) page = -1, bad |= PAGED_STATUS_PAGES;  // (the list ends at n_free, or in such entries where only the device knows its length)
-            else if ((uint32_t)page >= s.pages) page = -1, bad |= PAGED_STATUS_INDEX;
+            // (the list ends at n_free, or in entries below 0 where only the device knows its length)
+            if (j >= a.n_free) bad |= PAGED_STATUS_PAGES;
+            else if ((page = a.free_pages[j]) < 0 || (uint32_t)page >= s.pages) bad |= page < 0 ? PAGED_STATUS_PAGES : PAGED_STATUS_INDEX, page = -1;
             a.table[(size_t)(r0 + i) * s.max_blocks + sh.have[i] + (j - sh.first[i])] = page;
         }
         // (the last CTA begins: the first one has the pages)
