@@ -341,7 +341,7 @@ template <int SRC, bool VEC> __global__ void __launch_bounds__(APPEND_THREADS) p
     for (uint32_t t = blockIdx.x; t < s.tokens; t += gridDim.x) {
         const int32_t slot = p.slots ? p.slots[t] : -1, pos = p.positions[t];
         float4 cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const bool stored = slot >= 0 && (uint32_t)slot < s.pages << shift, sound = pos >= 0 && !(p.rot && (uint32_t)pos >= p.rope_rows) && (slot < 0 || stored);
+        const bool stored = slot >= 0 && (uint32_t)slot < s.pages << shift, sound = pos >= 0 && !(p.rot && (uint32_t)pos >= p.rope_rows) && (slot == -1 || stored);
         bool first = true;
         for (uint32_t h0 = blockIdx.y * lanes * APPEND_HEADS; h0 < heads; h0 += gridDim.y * lanes * APPEND_HEADS) {
             // (the rows do not wait for the slot and the position)
@@ -393,7 +393,7 @@ template <int SRC, bool VEC> __global__ void __launch_bounds__(APPEND_THREADS) p
                 }
             }
         }
-        if (!sound && pos >= 0 && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
+        if (!sound && pos != -1 && threadIdx.x == 0 && p.status) atomicOr(p.status, (int)PAGED_STATUS_INDEX);
     }
 }
 

@@ -11,6 +11,7 @@ from tests import paged_ref as R
 from tests.paged_more import plan_with_refusals
 
 pytestmark = pytest.mark.gpu
+F32 = lp.DType.F32
 
 
 @pytest.fixture(scope="module")
@@ -163,3 +164,24 @@ def test_free_pages_may_end_in_none(be):
     s.make_plan()
     be.synchronize()
     check_plan(s, want_of(s, s.new, s.cached, s.table0, free))
+
+
+@pytest.mark.parametrize("slots,positions,code", [([5, -2, 7], [0, 1, 2], "index_out_of_range"), ([5, 6, 7], [0, 1, -2], "index_out_of_range"),
+                                                  ([5, -2 ** 31, 7], [0, 1, 2], "index_out_of_range"), ([5, 6, 7], [0, -2 ** 31, 2], "index_out_of_range"),
+                                                  ([5, -1, 7], [0, 1, -1], None)])
+def test_append_reports_every_slot_and_position_outside_but_minus_one(be, slots, positions, code):
+    s = R.Step(be, [3], [0], hq=2, hkv=2, d=16).upload()
+    x = be.upload(np.ones((3, 2, 16), np.float32))
+    before = s.b["k"].download().view(np.int16).reshape(s.pages, 2, 16, 16).copy()
+    be.paged_append(s.spec, F32, None, x, x, be.upload(np.array(slots, np.int32)), be.upload(np.array(positions, np.int32)), s.b["k"], s.b["v"], None)
+    if code:
+        refused(be, code)
+    else:
+        be.synchronize()
+    after = s.b["k"].download().view(np.int16).reshape(s.pages, 2, 16, 16)
+    stored = [sl for sl, p in zip(slots, positions) if sl >= 0 and p >= 0]
+    touched = np.zeros((s.pages, 16), bool)
+    for sl in stored:
+        touched[sl // 16, sl % 16] = True
+    assert np.array_equal(after.transpose(0, 2, 1, 3)[~touched], before.transpose(0, 2, 1, 3)[~touched])
+    assert np.all(after.transpose(0, 2, 1, 3)[touched] == R.to_half(np.ones(1), s.dtype)[1][0])
