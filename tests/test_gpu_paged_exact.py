@@ -1,5 +1,5 @@
-"""Attention over the paged cache where an error would be small or far away: keys that a mask leaves out, with values of any size, keys appended just before, and q
-alone (a step that appends nothing)."""
+"""Attention over the paged cache where an error would be small or far away: keys that a mask leaves out with values of any size, the logarithm of the sum by what f32 allows,
+plans of more requests than one scan takes, and q alone (a step that appends nothing)."""
 import numpy as np
 import pytest
 
@@ -7,6 +7,7 @@ import lapid_b200 as lp
 from lapid_b200.backend import MatView
 from lapid_b200.paged import Mask, rope_table
 from tests import paged_ref as R
+from tests.paged_more import lse_bound
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = lp.DType.BF16, lp.DType.F16, lp.DType.F32
@@ -45,6 +46,46 @@ def test_a_key_without_weight_adds_nothing_whatever_its_value(be, new, cached, d
         rows = [t for t in range(n) if why == "weight" or not R.seen(s.mask, window, n, kv, t)[0] <= key < R.seen(s.mask, window, n, kv, t)[1]]
         assert rows or why == "window"
         assert np.all(np.abs(out[rows] - o[rows]) <= R.bound(s.dtype, o[rows], size[rows], kv, 6.0)), key
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("new,cached", [([40], [0]), ([1, 1, 2], [0, 1, 37]), ([300], [0]), ([70, 1], [33, 200])])
+def test_the_logarithm_of_the_sum_is_as_close_as_f32_allows(be, dtype, d, new, cached):
+    """q and k are whole numbers, so the scores are exact. The first rows see one key, two keys, ...: there a single exponential's error stands in the result."""
+    s = R.Step(be, new, cached, hq=8, hkv=2, d=d, dtype=dtype, seed=d + len(new))
+    rng = np.random.default_rng(d)
+    s.q = rng.integers(-2, 3, s.q.shape).astype(np.float64)
+    s.q_bits = R.to_half(s.q, dtype)[1]
+    s.k = [rng.integers(-2, 3, x.shape).astype(np.float64) for x in s.k]
+    s.upload()
+    s.make_plan()
+    s.attend()
+    be.synchronize()
+    _, lse = s.outputs()
+    at = 0
+    for r, n in enumerate(new):
+        _, want, _ = R.attention(s.q[at:at + n], s.k[r], s.v[r], s.g, s.mask, 0, s.scale, n, s.kv[r])
+        top = s.scale * max(float(np.abs(s.q[at + t, h] @ s.k[r][:, h // s.g].T).max()) for t in range(n) for h in range(s.hq))
+        keys = cached[r] + 1 + np.arange(n)[:, None]
+        err = np.abs(lse[at:at + n] - want)
+        assert np.all(err <= lse_bound(want, top, keys)), (r, float(err.max()))
+        at += n
+
+
+@pytest.mark.parametrize("requests", [257, 300, 1024, 1025, 1500])
+@pytest.mark.parametrize("most", [3, 30])
+def test_attention_of_many_requests(be, requests, most):
+    """Plans of 1024 threads, and those that take the requests in several chunks and read the cut back from the plan buffer; few rows alone, and both kinds."""
+    rng = np.random.default_rng(requests + most)
+    new = np.where(rng.random(requests) < 0.1, rng.integers(0, most + 1, requests), rng.integers(0, 3, requests)).tolist()
+    cached = np.where(rng.random(requests) < 0.02, rng.integers(0, 400, requests), rng.integers(0, 40, requests)).tolist()
+    new[requests - 1], cached[requests - 1] = most, 70
+    s = R.Step(be, new, cached, hq=2, hkv=1, d=16, seed=most, pad=2).run()
+    first = s.b["out"].download().copy()
+    s.attend()
+    be.synchronize()
+    assert np.array_equal(first, s.b["out"].download())
 
 
 def test_few_rows_beside_many_read_what_was_appended_just_before(be):
