@@ -33,7 +33,7 @@ using namespace pipe;
 constexpr int KEYS = PAGED_SMALL_KEYS, ROWS = PAGED_SMALL_ROWS;
 constexpr int WARPS = 4, THREADS = 32 * (WARPS + 1);  // and the producer
 constexpr int CHUNK = 32, MEET = WARPS * ROWS * (CHUNK + 8);  // the accumulators meet in shared memory 32 columns of 16 rows at a time, or more of fewer; the pitch avoids bank conflicts
-constexpr uint32_t SPIN_LIMIT = 1u << 19;            // a wait gives up after some two seconds
+constexpr uint32_t SPIN_LIMIT = 1u << 19;            // a wait gives up after so many attempts, each as long as the hardware lets one sleep
 
 template <int DP> struct Cfg {
     static constexpr int HALVES = DP / 64;                  // a copied row is 64 elements wide: the width of a 128-byte swizzled row

@@ -63,7 +63,7 @@ constexpr int Q_HALF = TILE * 128;  // bytes of 128 rows of 64 elements
 constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88;
 constexpr float LAZY = 8.0f;
 constexpr int POLY = 1;  // pairs of every eight whose exponentials are polynomials (with 0, 1, 2 prompts through a window 63.8, 61.5, 66.3 us, 512 tokens over 32768 keys 584, 553, 583)
-constexpr uint32_t WAIT_NS = 8000, SPIN_LIMIT = 1u << 19;  // a wait gives up after some two seconds
+constexpr uint32_t WAIT_NS = 8000, SPIN_LIMIT = 1u << 18;  // a wait gives up after at most 2.1 seconds
 
 template <int DP> struct Cfg {
     static constexpr int HALVES = DP / 64;
