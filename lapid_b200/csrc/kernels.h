@@ -396,11 +396,12 @@ constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile a
 // and of 32 47.8 and 63.3 us at 16 requests over 2048 to 4096 keys, 19.1 and 21.0 at one over 8192, 56.0 and 76.1 at 64 over 512 to 1024; at d = 64 22.7 and 25.5.
 constexpr uint32_t PAGED_SMALL_LIMIT = 16;
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
-// Steps that beginning and ending one of its tiles takes as long as. (With 2 in place of 3: 200 tokens 17.0 instead of 10.9 us, 2048 46.2 instead of 47.0, the others
-// within 1 %.)
+// Steps that beginning and ending one of its tiles takes as long as. (With 2 in place of 3: 100 and 200 tokens 13.9 and 16.9 instead of 9.2 and 10.7 us, 2048 44.7 instead of 45.3,
+// the others within 3 %.)
 constexpr uint32_t PAGED_LARGE_EXTRA = 3;
-// Fewest units worth a CTA of its own. With 1, 2, 3, 4 and 6: 64 tokens 9.2, 9.1, 9.0, 8.9, 14.6 us; 64 behind 1024 keys 34.6, 24.9, 24.0, 22.8, 25.3; 200 tokens 18.7, 18.0, 12.1,
-// 18.0, 16.4; 512 tokens 21.3, 21.4, 21.3, 21.4, 30.4. (The kernel for few rows: paged_plan_kernel.)
+// Fewest units worth a CTA of its own. With 1, 2, 3, 4 and 6: 64 tokens 8.5, 8.5, 8.4, 8.5, 12.7 us; 64 behind 1024 keys 35.0, 24.2, 23.5, 23.2, 24.0; 150 tokens 16.1, 16.5, 15.7, 16.3,
+// 20.2; 300 18.7, 18.2, 18.1, 18.3, 23.0; 512 20.4, 20.4, 20.4, 20.7, 25.0. At 100 and 200 tokens the cut lands on tiles' ends with 3 alone (14.0, 14.1, 9.2, 14.2, 13.9 and 17.9, 16.7, 10.7, 16.7,
+// 14.2): what a cut tile costs, not the rule. (The kernel for few rows: paged_plan_kernel.)
 constexpr uint32_t PAGED_LARGE_MIN = 3;
 // What a unit of either kernel takes of an SM, in ns, at 128 / 64 elements a head: of the kernel for few rows when it shares the chip with the other (alone
 // it is bound by all SMs' common memory, here by what one SM can have in flight). With 700, 1000 and 1400 ns for the other: 512 tokens beside 11 single ones over
