@@ -454,9 +454,10 @@ LAPID_B200_API lapid_b200_status lapid_b200_paged_append(lapid_b200_device *dev,
  * [tokens, q_heads, head_dim] through views as above (NULL: contiguous) in the cache's type: what an output projection takes as
  * a_dtype F16 / BF16. lse (or NULL): f32 [tokens, q_heads], the logarithm of the softmax's sum (-inf: no keys), with which
  * results over parts of the keys can be joined. Scores, sums and accumulators are f32; the softmax's weights are rounded to
- * the cache's type for their product with v. What lies in pages behind a request's keys, or in front of its window, may be anything; a value
- * of v that is not finite, though, also reaches rows of the same few tokens that do not see it (0 times infinity). `plan` also holds this call's intermediate results: attention calls with the same
- * plan must not overlap on the GPU (calls on one stream never do). */
+ * the cache's type for their product with v. What lies in pages behind a request's keys, or in front of its window, may be anything, and a finite
+ * value of a key that a row does not see adds nothing to it. A value of v that is not finite, though, also reaches rows that do not see it but share a tile with one that
+ * does (0 times infinity): of a request of at most 16 rows (tokens * q_heads / kv_heads) any, else those of up to 2 * (128 kv_heads / q_heads) tokens, 256 with a key head for each query head. `plan` also holds this call's intermediate results: attention calls with the same
+ * plan must not overlap on the GPU (calls on one stream never do), and after an error "backend" (a wait that gave up) the plan is made again. */
 LAPID_B200_API lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan,
                                                             const lapid_b200_buffer *q, const lapid_b200_matview *q_view,
                                                             const lapid_b200_buffer *k_cache, const lapid_b200_buffer *v_cache,

@@ -7,7 +7,7 @@
 //         done once a step, and every layer's launch reads it.
 //         What bounds it is latency: one launch, two scans over the requests, a search a token and a search a start. Every CTA scans the
 //         lengths itself so that nothing passes between CTAs, and takes its share of the tokens, blocks and starts. 64 requests of one token 4.2 us, 48
-//         prompts (65520 tokens) 8.1.
+//         prompts (65520 tokens) 7.8, 256 requests 9.1, 1024 9.1. Above that one CTA makes all starts, from prefixes in global memory: 1025 requests 36 us, 2048 38.
 // append  (x, y) -> (x cos - y sin, y cos + x sin) in f32 for the rotary pairs of q and k, one rounding to the cache's type; k and v go
 //         to their slots. Bound by memory: each element is read once and written once; a thread keeps the angles of its
 //         four pairs in registers over the heads of a token.
@@ -305,7 +305,7 @@ cudaError_t launch_paged_plan(const PagedPlanArgs &a, int sm_count, bool pdl, cu
 
 // ------------------------------------------------------------------ append
 // Heads whose loads a thread has in flight. 8192 tokens of 48 heads of 128: 47.6 us (0.98 of the measured bandwidth); CTAs of 256 threads 52.8, of 64 49.1, two heads 48.2,
-// four 49.1; with the rows asked for behind slot and position 61.
+// four 49.1; with the rows asked for behind slot and position 61. From f16 or bf16 rows 51.7 for two thirds of the bytes (31.5 us of bandwidth): as many requests, half of the bytes in each.
 constexpr uint32_t APPEND_THREADS = 128, APPEND_HEADS = 3;
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b, bool bf16) {

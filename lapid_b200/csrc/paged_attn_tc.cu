@@ -24,11 +24,12 @@
 // ends with the first piece: that one adds the others to its accumulator. Where they are not there yet, or are many, the CTA that comes last adds
 // all of them up, in the order of the keys either way and with the same roundings.
 //
-// What bounds it: a softmax warp's own chain, two warps a scheduler. A step of 96 keys takes 2050 to 2400 cycles: exponentials 1345 (the special-function unit 47 % busy over
-// the kernel), loads, stores and two waits 540, the more of it hidden the further the two tiles are apart; products 26 % of the time. From tile to tile some 6300 cycles pass (heads of 64: 4600), for
+// What bounds it: a softmax warp's own chain, two warps a scheduler. Heads of 64: a step of 96 keys takes 2050 to 2400 cycles: exponentials 1345 (the special-function unit 47 % busy over
+// the kernel), loads, stores and two waits 540, the more of it hidden the further the two tiles are apart; products 26 % of the time. Heads of 128: a step of 80 keys takes some 1720, of which
+// both tiles' products are 1280 and their exponentials 1120; over four prompts the tensor pipe is busy 59 % of the time, the special-function unit 52 %. From tile to tile some 6300 cycles pass (heads of 64: 4600), for
 // the last product, the rows' stores and the walk; a cut tile's later piece costs 9000, its first 8000 behind the span. Long work runs into the power limit: 512 tokens over
-// 32768 keys, 64 query and 8 key heads of 128, 546 to 580 us (0.94 to 1.0 PFLOP/s, the clock at 1.2 to 1.4 GHz); four prompts of up to 4096 tokens, 32 query heads, 373 to 392 us; one of 2048 47.1 us;
-// three of up to 3001 through a window of 1024 keys, 14 heads of 64, 61.5 us.
+// 32768 keys, 64 query and 8 key heads of 128, 546 to 580 us (0.94 to 1.0 PFLOP/s, the clock at 1.2 to 1.4 GHz); four prompts of up to 4096 tokens, 32 query heads, 306 to 392 us as their lengths fall (0.91 PFLOP/s; when they see all keys 1.06);
+// one of 2048 45.3 us; three of up to 3001 through a window of 1024 keys, 14 heads of 64, 61 to 64 us.
 //
 // Every mbarrier wait is bounded: one that gives up sets a bit in the status word, the roles fall through to the end, tensor memory is released.
 #include <cuda.h>
