@@ -409,6 +409,7 @@ LAPID_B200_API lapid_b200_status lapid_b200_silu_mul_act(lapid_b200_device *dev,
 #define LAPID_B200_MASK_FULL 0   /* a new token sees all keys, cached and new */
 #define LAPID_B200_MASK_CAUSAL 1 /* ... up to its own; with window > 0 the last `window` of these */
 #define LAPID_B200_MASK_CROSS 2  /* ... the cached ones only: nothing is appended (slots are -1, paged_append takes q alone) */
+#define LAPID_B200_MASK_TREE 4   /* ... the cached ones, its ancestors among the new ones and itself (drafted tokens, below); with window > 0 those at the last `window` positions up to its own */
 typedef struct lapid_b200_paged {
     int32_t dtype;       /* of the cache, q and out: F16 or BF16 */
     uint32_t q_heads;    /* a multiple of kv_heads: query head h reads key/value head h / (q_heads / kv_heads) */
@@ -420,8 +421,8 @@ typedef struct lapid_b200_paged {
     uint64_t requests;   /* rows of the block table; at most 2^28 */
     uint64_t tokens;     /* rows of q, k, v and out: the sum of the new lengths, or more (rows behind the sum are left alone) */
     uint64_t max_blocks; /* columns of the block table */
-    uint64_t max_new;    /* no request has more new tokens */
-    uint64_t window;     /* CAUSAL: 0, or how many keys a token sees */
+    uint64_t max_new;    /* no request has more new tokens; TREE: at most 1024 */
+    uint64_t window;     /* CAUSAL, TREE: 0, or how many keys a token sees */
     float scale;         /* of the scores; 0: 1 / sqrt(head_dim) */
 } lapid_b200_paged;
 /* Bytes of the plan buffer of such a step (16-byte aligned; its contents need no clearing). Host only; needs no device. */
@@ -463,6 +464,53 @@ LAPID_B200_API lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *d
                                                             const lapid_b200_buffer *k_cache, const lapid_b200_buffer *v_cache,
                                                             const lapid_b200_buffer *block_table, lapid_b200_buffer *out,
                                                             const lapid_b200_matview *out_view, lapid_b200_buffer *lse);
+
+/* ---- drafted tokens over the paged cache -------------------------------------------------------- */
+/* Speculative decoding: a cheap draft proposes tokens, the model looks at all of them in one step, and those that its probabilities accept are kept. A
+ * request's new tokens are a tree with the mask TREE: the first one is the text's last token (it is not in question), the others are drafted, each the child of one in front of it; a chain with
+ * the mask CAUSAL. A step, queued on the device's stream and not waited for, without an allocation (it can be captured):
+ *   lapid_b200_paged_plan            slots (a drafted token lies where its place among the new ones says), pages, the cut of the attention
+ *   lapid_b200_paged_tree            TREE: positions (cached + the number of ancestors) and every token's ancestors, once a step
+ *   lapid_b200_paged_append, lapid_b200_paged_tree_attention (CAUSAL: paged_attention)       once a layer
+ *   lapid_b200_paged_verify          which path of the tree the logits accept, with given random numbers, and the token behind it
+ *   lapid_b200_paged_commit          the path's keys and values behind the cached ones, in all layers; lengths; the pages not needed go back
+ * All of them read the requests' rows in `plan`. Reported by the next call that waits, beside what is said above: "index_out_of_range" (a parent, drafted token, accepted length
+ * or path out of range), "invalid_argument" (a row of logits that cannot be a distribution). */
+/* Bytes of the tree buffer of such a step: u32 [tokens][1 + ceil(max_new / 32)], of each token how many ancestors it has, then a bit for each of its request's new tokens (bit i of
+ * word w: token 32 w + i) that says whether it is seen: an ancestor or itself, with a window one of those at the last `window` positions. Host only; needs no device. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_tree_bytes(const lapid_b200_paged *desc, uint64_t *bytes);
+/* parents i32 [tokens]: the place of a token's parent among its request's new tokens, smaller than its own, or -1: none (also other ones than the first may have none; a parent out of range is
+ * reported, and counts as none). Behind paged_plan, whose positions it replaces. Rows of positions and tree of tokens that take no part are left alone. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_tree(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan,
+                                                       const lapid_b200_buffer *parents, lapid_b200_buffer *positions, lapid_b200_buffer *tree);
+/* lapid_b200_paged_attention for the mask TREE: what is said there holds here. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_tree_attention(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan,
+                                                                 const lapid_b200_buffer *tree, const lapid_b200_buffer *q, const lapid_b200_matview *q_view,
+                                                                 const lapid_b200_buffer *k_cache, const lapid_b200_buffer *v_cache,
+                                                                 const lapid_b200_buffer *block_table, lapid_b200_buffer *out,
+                                                                 const lapid_b200_matview *out_view, lapid_b200_buffer *lse);
+/* The walk down each request's tree. logits: of type logits_dtype (F32, F16 or BF16), row t (logits_row elements from one to the next, 0: vocab, at most 2^22) those of what follows new token t: with z
+ * the row of node v, P = softmax(z / temperature) (temperature f32 [requests], NULL: 1; 0 or below: 1 for the largest logit, of equal ones the first, else 0; -inf: never). The walk begins at a request's
+ * first token. The children of the node it is at are tried in their order: child c, drafted token x = tokens[c] (i32 [tokens]), is accepted
+ *   with draft (f32, row v, draft_row apart, the probabilities D that v's children were drawn from, independently):  when accept[c] * D(x) < P(x);  else P <- max(P - D, 0), scaled to sum 1
+ *   without (NULL: candidates that were chosen):                                                                      when accept[c] < P(x);         else P(x) <- 0, scaled to sum 1
+ * (where nothing would be left, P stays). The walk goes on at the accepted child. Where none is, next is the first token t with P(0) + .. + P(t) > pick. accept f32 [tokens], pick f32 [requests]: random
+ * numbers in [0, 1). Out: path i32 [requests, max_new], the walk's nodes (the first is 0), -1 behind them; accepted i32 [requests], how many; next i32 [requests], the token behind the last. A
+ * drafted token outside the vocabulary is reported and not accepted; where a row has NaN, +inf or nothing but -inf the walk ends there and next is -1. Of a request without new tokens accepted is 0 and next -1. Weights, sums and
+ * comparisons are 64 bits wide. parents as in paged_tree; NULL with the mask CAUSAL: every token's parent is the one in front of it. At most 1024 new tokens a request. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_verify(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan, int32_t logits_dtype,
+                                                         uint64_t vocab, const lapid_b200_buffer *logits, uint64_t logits_row, const lapid_b200_buffer *draft,
+                                                         uint64_t draft_row, const lapid_b200_buffer *tokens, const lapid_b200_buffer *parents,
+                                                         const lapid_b200_buffer *accept, const lapid_b200_buffer *pick, const lapid_b200_buffer *temperature,
+                                                         lapid_b200_buffer *path, lapid_b200_buffer *accepted, lapid_b200_buffer *next);
+/* Keeps of every request the accepted[r] (0 to its new length) tokens path[r][0 ..) (rising; as verify writes them): in each of the n_caches caches (keys and values of all layers, in any order) what lies at
+ * cached + path[r][i] moves to cached + i. path NULL, with the mask CAUSAL: the first ones, which lie there already. Out: kv_lens (cached + accepted: the next step's cached_lens) and used, in the place of what paged_plan
+ * wrote there, and free_pages: of the pages that the step took (the first ones of the list) the kept ones first, then the others, so that the caller drops `used` of them from the front as behind any step. A request
+ * whose accepted length or path is out of range is reported and keeps nothing. Not to be run twice on one step: what it moves has moved. */
+LAPID_B200_API lapid_b200_status lapid_b200_paged_commit(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan,
+                                                         lapid_b200_buffer *const *caches, uint64_t n_caches, const lapid_b200_buffer *block_table,
+                                                         const lapid_b200_buffer *path, const lapid_b200_buffer *accepted, lapid_b200_buffer *free_pages,
+                                                         uint64_t n_free, lapid_b200_buffer *kv_lens, lapid_b200_buffer *used);
 
 /* ---- decode without allocation ------------------------------------------------------------ */
 /* This entry point has no counterpart in the reference. It exists for hosts that may not allocate

@@ -115,6 +115,11 @@ SYMBOLS = {
     "lapid_b200_paged_append": (C.c_int32, [P, C.POINTER(PagedC), C.c_int32, P, C.POINTER(MatViewC), P, C.POINTER(MatViewC), P, C.POINTER(MatViewC),
                                            P, C.c_uint64, C.c_uint32, C.c_int32, P, P, P, P, P]),
     "lapid_b200_paged_attention": (C.c_int32, [P, C.POINTER(PagedC), P, P, C.POINTER(MatViewC), P, P, P, P, C.POINTER(MatViewC), P]),
+    "lapid_b200_paged_tree_bytes": (C.c_int32, [C.POINTER(PagedC), C.POINTER(C.c_uint64)]),
+    "lapid_b200_paged_tree": (C.c_int32, [P, C.POINTER(PagedC), P, P, P, P]),
+    "lapid_b200_paged_tree_attention": (C.c_int32, [P, C.POINTER(PagedC), P, P, P, C.POINTER(MatViewC), P, P, P, P, C.POINTER(MatViewC), P]),
+    "lapid_b200_paged_verify": (C.c_int32, [P, C.POINTER(PagedC), P, C.c_int32, C.c_uint64, P, C.c_uint64, P, C.c_uint64, P, P, P, P, P, P, P, P]),
+    "lapid_b200_paged_commit": (C.c_int32, [P, C.POINTER(PagedC), P, C.POINTER(P), C.c_uint64, P, P, P, P, C.c_uint64, P, P]),
     "lapid_b200_gemv_q4k_static": (C.c_int32, [C.c_int32, P, P, P, C.c_uint64, P, C.c_uint32, C.c_uint32, C.c_uint32]),
     "lapid_b200_gemv_q4k_static_status": (C.c_int32, [C.c_int32, C.POINTER(C.c_int32)]),
 }

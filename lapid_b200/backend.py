@@ -485,6 +485,53 @@ class Backend:
         """Attention of the new tokens of every request over its pages (``lapid_b200_paged_attention``)."""
         self.packed_paged_attention(*args, **kw)()
 
+    # ---- drafted tokens over the paged cache (queued, not waited for)
+    def packed_paged_tree(self, spec, plan: Buffer, parents: Buffer, positions: Buffer, tree: Buffer):
+        """``paged_tree`` as a zero-argument callable."""
+        bufs = (plan, parents, positions, tree)
+        return self._paged_call(_lib.lib().lapid_b200_paged_tree, spec, tuple(b._h for b in bufs), bufs)
+
+    def paged_tree(self, *args, **kw) -> None:
+        """Positions (in the place of the plan's) and ancestors of a step's drafted tokens, from their parents' places (``lapid_b200_paged_tree``)."""
+        self.packed_paged_tree(*args, **kw)()
+
+    def packed_paged_tree_attention(self, spec, plan: Buffer, tree: Buffer, q: Buffer, k_cache: Buffer, v_cache: Buffer, block_table: Buffer, out: Buffer, *,
+                                    lse: Optional[Buffer] = None, q_view: Optional[MatView] = None, out_view: Optional[MatView] = None):
+        """``paged_tree_attention`` as a zero-argument callable."""
+        bufs = (plan, tree, q, k_cache, v_cache, block_table, out, lse)
+        h = [b._h if b is not None else None for b in bufs]
+        return self._paged_call(_lib.lib().lapid_b200_paged_tree_attention, spec,
+                                (h[0], h[1], h[2], self._view(q_view), h[3], h[4], h[5], h[6], self._view(out_view), h[7]), bufs)
+
+    def paged_tree_attention(self, *args, **kw) -> None:
+        """Attention of the drafted tokens of every request over its cached keys, their ancestors' and their own (``lapid_b200_paged_tree_attention``)."""
+        self.packed_paged_tree_attention(*args, **kw)()
+
+    def packed_paged_verify(self, spec, plan: Buffer, logits_dtype: DType, vocab: int, logits: Buffer, tokens: Buffer, accept: Buffer, pick: Buffer, path: Buffer,
+                            accepted: Buffer, next: Buffer, *, parents: Optional[Buffer] = None, draft: Optional[Buffer] = None, temperature: Optional[Buffer] = None,
+                            logits_row: int = 0, draft_row: int = 0):
+        """``paged_verify`` as a zero-argument callable."""
+        bufs = (plan, logits, draft, tokens, parents, accept, pick, temperature, path, accepted, next)
+        h = [b._h if b is not None else None for b in bufs]
+        return self._paged_call(_lib.lib().lapid_b200_paged_verify, spec, (h[0], int(logits_dtype), vocab, h[1], logits_row, h[2], draft_row, *h[3:]), bufs)
+
+    def paged_verify(self, *args, **kw) -> None:
+        """Which path of each request's drafted tokens the logits accept, with the given random numbers, and the token behind it (``lapid_b200_paged_verify``)."""
+        self.packed_paged_verify(*args, **kw)()
+
+    def packed_paged_commit(self, spec, plan: Buffer, layers: Sequence[tuple], block_table: Buffer, path: Optional[Buffer], accepted: Buffer, kv_lens: Buffer, used: Buffer, *,
+                            free_pages: Optional[Buffer] = None, n_free: int = 0):
+        """``paged_commit`` as a zero-argument callable; ``layers``: the (keys, values) of all layers."""
+        caches = [b for pair in layers for b in pair]
+        arr = (C.c_void_p * max(1, len(caches)))(*[b._h for b in caches])
+        bufs = (plan, block_table, path, accepted, free_pages, kv_lens, used)
+        h = [b._h if b is not None else None for b in bufs]
+        return self._paged_call(_lib.lib().lapid_b200_paged_commit, spec, (h[0], arr, len(caches), h[1], h[2], h[3], h[4], n_free, h[5], h[6]), bufs + tuple(caches))
+
+    def paged_commit(self, *args, **kw) -> None:
+        """Keys and values of the accepted tokens behind the cached ones in every layer, the requests' lengths, and the pages that are not needed back to the list (``lapid_b200_paged_commit``)."""
+        self.packed_paged_commit(*args, **kw)()
+
     def take_launch_count(self) -> int:
         return int(_lib.lib().lapid_b200_take_launch_count(self._h))
 

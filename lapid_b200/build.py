@@ -42,6 +42,8 @@ SOURCES = {
     "paged.cu": [],
     "paged_attn.cu": [],
     "paged_attn_tc.cu": [],
+    "paged_draft.cu": [],
+    "paged_verify.cu": [],
     "tp_allreduce.cu": [],
     "backend.cc": ["-x", "cu"],
 }

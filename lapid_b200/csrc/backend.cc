@@ -16,6 +16,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <algorithm>
+#include <functional>
 #include <map>
 #include <mutex>
 #include <new>
@@ -1128,12 +1129,13 @@ void check_status_word(lapid_b200_device *dev) {
     // a launch that gave up may have left partial sums in the decode workspace
     cudaMemsetAsync(dev->stream_ws.pairs, 0, dev->stream_ws.total_bytes, dev->stream);
     cudaStreamSynchronize(dev->stream);
-    constexpr int BAD_INDEX = 128, PAGED_INDEX = 512, PAGED_PAGES = 1024, PAGED_LENGTHS = 4096, PAGED_PLAN = 8192;
-    if ((st & ~(BAD_INDEX | PAGED_INDEX | PAGED_PAGES | PAGED_LENGTHS | PAGED_PLAN)) == 0) {  // no wait gave up
-        if (st & PAGED_PLAN) fail("invalid_launch", "paged attention: the plan buffer was not made for this description");
+    constexpr int BAD_INDEX = 128, PAGED_INDEX = 512, PAGED_PAGES = 1024, PAGED_LENGTHS = 4096, PAGED_PLAN = 8192, PAGED_LOGITS = 16384;
+    if ((st & ~(BAD_INDEX | PAGED_INDEX | PAGED_PAGES | PAGED_LENGTHS | PAGED_PLAN | PAGED_LOGITS)) == 0) {  // no wait gave up
+        if (st & PAGED_PLAN) fail("invalid_launch", "paged cache: the plan buffer was not made for this description");
         if (st & PAGED_LENGTHS) fail("shape_mismatch", "paged plan: a request's length is negative or outside max_new, max_blocks or tokens; it took no part");
         if (st & PAGED_PAGES) fail("out_of_memory", "paged plan: the list of free pages ran out");
-        if (st & PAGED_INDEX) fail("index_out_of_range", "paged cache: a page, slot or position is out of range; what it names was not read or written");
+        if (st & PAGED_INDEX) fail("index_out_of_range", "paged cache: a page, slot, position, parent, drafted token or path is out of range; what it names was not read or written");
+        if (st & PAGED_LOGITS) fail("invalid_argument", "paged verify: a row of logits has NaN, +inf or nothing but -inf; the walk ended in front of it");
         fail("index_out_of_range", "an index of a gather or an expert id of a matmul_id is out of range; the rows it selects were not computed");
     }
     // (which kernel sets which bit: 1 decode, 2 to 32 the waits of the tensor-core prefill, 64 tensor-parallel exchange, 128 a bad index, 256 exact-f32 GEMM, 2048 paged attention)
@@ -1588,8 +1590,10 @@ lb::PagedShape paged_shape(const lapid_b200_paged *d) {
         fail("unsupported", "paged cache: head_dim must be a multiple of 8 in 16..128, got " + std::to_string(d->head_dim));
     if (d->page_size != 16 && d->page_size != 32 && d->page_size != 64 && d->page_size != 128)
         fail("unsupported", "paged cache: page_size must be 16, 32, 64 or 128, got " + std::to_string(d->page_size));
-    if (d->mask < LAPID_B200_MASK_FULL || d->mask > LAPID_B200_MASK_CROSS) fail("invalid_argument", "paged cache: unknown mask " + std::to_string(d->mask));
-    if (d->window && d->mask != LAPID_B200_MASK_CAUSAL) fail("invalid_argument", "paged cache: a window needs the causal mask");
+    const bool tree = d->mask == LAPID_B200_MASK_TREE;
+    if (!tree && (d->mask < LAPID_B200_MASK_FULL || d->mask > LAPID_B200_MASK_CROSS)) fail("invalid_argument", "paged cache: unknown mask " + std::to_string(d->mask));
+    if (d->window && !tree && d->mask != LAPID_B200_MASK_CAUSAL) fail("invalid_argument", "paged cache: a window needs the causal mask");
+    if (tree && d->max_new > lb::PAGED_TREE_MOST) fail("unsupported", "paged cache: a tree has at most 1024 tokens, max_new is " + std::to_string(d->max_new));
     if (d->pages == 0) fail("invalid_launch", "paged cache: no pages");
     const uint64_t most = (1ull << 31) - 1, g = d->q_heads / d->kv_heads;
     auto product_ok = [&](uint64_t x, uint64_t y) { return y == 0 || x <= most / y; };
@@ -1617,7 +1621,9 @@ lb::PagedShape paged_shape(const lapid_b200_paged *d) {
     s.tokens = (uint32_t)d->tokens;
     s.max_blocks = (uint32_t)d->max_blocks;
     s.max_new = (uint32_t)d->max_new;
-    s.mask = (uint32_t)d->mask;
+    s.mask = tree ? lb::PAGED_CAUSAL : (uint32_t)d->mask;
+    s.tree = tree ? ((uint32_t)d->max_new + 31) / 32 : 0;
+    if (tree && !s.tree) s.tree = 1;  // (no new tokens)
     s.window = (uint32_t)d->window;
     s.tt = lb::PAGED_LARGE_ROWS / 2 / s.g;
     s.large_keys = s.d > 64 ? 80 : 96;
@@ -1645,6 +1651,22 @@ lb::PagedView paged_view(const lapid_b200_device *dev, const lapid_b200_buffer *
 bool paged_overlap(const lapid_b200_buffer *a, const lapid_b200_buffer *b) {
     const char *x = (const char *)a->ptr, *y = (const char *)b->ptr;
     return x < y + b->bytes && y < x + a->bytes;
+}
+// No output shares memory with an input or with another output (any may be NULL). In the order of their addresses: a commit has the caches of all layers.
+void paged_apart(const std::string &call, const std::vector<const lapid_b200_buffer *> &ins, const std::vector<const lapid_b200_buffer *> &outs) {
+    std::vector<std::pair<const lapid_b200_buffer *, bool>> all;
+    for (const lapid_b200_buffer *b : ins)
+        if (b && b->bytes) all.push_back({b, false});
+    for (const lapid_b200_buffer *b : outs)
+        if (b && b->bytes) all.push_back({b, true});
+    std::sort(all.begin(), all.end(), [](const auto &x, const auto &y) { return std::less<const void *>()(x.first->ptr, y.first->ptr); });
+    const char *in_end = nullptr, *out_end = nullptr;  // of those that begin no later
+    for (const auto &[b, out] : all) {
+        const char *begin = (const char *)b->ptr, *end = begin + b->bytes;
+        if (out && begin < out_end) fail("buffer_aliasing", call + ": two outputs alias");
+        if (begin < (out ? in_end : out_end)) fail("buffer_aliasing", call + ": an output aliases an input");
+        (out ? out_end : in_end) = std::max(out ? out_end : in_end, end);
+    }
 }
 int paged_sms(const lapid_b200_device *dev) { return dev->sm_count < (int)lb::PAGED_MAX_SMS ? dev->sm_count : (int)lb::PAGED_MAX_SMS; }
 
@@ -2480,55 +2502,226 @@ lapid_b200_status lapid_b200_paged_append(lapid_b200_device *dev, const lapid_b2
     });
 }
 
+// The attention of a step; `tree`: its tokens' ancestors, where they are drafted ones
+static void paged_attention_impl(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan, const lapid_b200_buffer *tree, const lapid_b200_buffer *q,
+                                 const lapid_b200_matview *q_view, const lapid_b200_buffer *k_cache, const lapid_b200_buffer *v_cache, const lapid_b200_buffer *block_table,
+                                 lapid_b200_buffer *out, const lapid_b200_matview *out_view, lapid_b200_buffer *lse) {
+    need(dev);
+    lb::PagedAttnArgs a{};
+    a.s = paged_shape(desc);
+    if (!tree && a.s.tree) fail("invalid_launch", "paged_attention: the new tokens are a tree: paged_tree_attention");
+    if (tree && !a.s.tree) fail("invalid_launch", "paged_tree_attention: the description's mask is not TREE");
+    a.l = lb::paged_plan_layout(a.s);
+    const uint64_t T = a.s.tokens, cache = (uint64_t)a.s.pages * a.s.hkv * a.s.page * a.s.d * 2;
+    paged_buffer(dev, plan, "paged_attention: plan", a.l.bytes);
+    a.qv = paged_view(dev, q, q_view, "paged_attention: q", T, a.s.hq, a.s.d, 2);
+    paged_buffer(dev, k_cache, "paged_attention: k_cache", cache);
+    paged_buffer(dev, v_cache, "paged_attention: v_cache", cache);
+    paged_buffer(dev, block_table, "paged_attention: block_table", (uint64_t)a.s.requests * a.s.max_blocks * 4);
+    a.ov = paged_view(dev, out, out_view, "paged_attention: out", T, a.s.hq, a.s.d, 2);
+    // each element of out is written by one row only
+    const uint64_t D = a.s.d, H = a.s.hq;
+    const bool heads_inside = a.ov.head >= D && (T <= 1 || a.ov.token >= (H - 1) * a.ov.head + D), tokens_inside = a.ov.token >= D && a.ov.head >= (T - 1) * a.ov.token + D;
+    if (T && !((H == 1 && (T <= 1 || a.ov.token >= D)) || heads_inside || tokens_inside)) fail("invalid_launch", "paged_attention: rows of out overlap");
+    if (lse) paged_buffer(dev, lse, "paged_attention: lse", T * H * 4);
+    if (tree) paged_buffer(dev, tree, "paged_tree_attention: tree", T * (1 + a.s.tree) * 4);
+    const lapid_b200_buffer *ins[] = {q, k_cache, v_cache, block_table, tree}, *outs[] = {plan, out, lse};
+    for (size_t i = 0; i < 3; i++) {
+        if (!outs[i]) continue;
+        for (const lapid_b200_buffer *b : ins)
+            if (b && paged_overlap(b, outs[i])) fail("buffer_aliasing", "paged_attention: an output aliases an input");
+        for (size_t j = 0; j < i; j++)
+            if (paged_overlap(outs[i], outs[j])) fail("buffer_aliasing", "paged_attention: two outputs alias");
+    }
+    if (T == 0 || a.s.requests == 0) return;
+    std::lock_guard<std::mutex> lock(dev->mu);
+    dev->make_current();
+    a.stamp = lb::paged_stamp(a.s);
+    a.plan = (uint32_t *)plan->ptr;
+    a.q = q->ptr;
+    a.k_cache = k_cache->ptr;
+    a.v_cache = v_cache->ptr;
+    a.table = (const int32_t *)block_table->ptr;
+    a.out = out->ptr;
+    a.lse = lse ? (float *)lse->ptr : nullptr;
+    a.tree = tree ? (const uint32_t *)tree->ptr : nullptr;
+    a.status = dev->status_dev;
+    // requests of many rows first: their CTAs run longest
+    if (lb::paged_has_large(a.s)) {
+        a.behind = true;
+        cuda_check(lb::launch_paged_attn_large(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
+        dev->launches++;
+    }
+    cuda_check(lb::launch_paged_attn_small(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
+    dev->launches++;
+}
+
 lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan,
                                              const lapid_b200_buffer *q, const lapid_b200_matview *q_view, const lapid_b200_buffer *k_cache,
                                              const lapid_b200_buffer *v_cache, const lapid_b200_buffer *block_table, lapid_b200_buffer *out,
                                              const lapid_b200_matview *out_view, lapid_b200_buffer *lse) {
+    return guard([&] { paged_attention_impl(dev, desc, plan, nullptr, q, q_view, k_cache, v_cache, block_table, out, out_view, lse); });
+}
+
+lapid_b200_status lapid_b200_paged_tree_attention(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan, const lapid_b200_buffer *tree,
+                                                  const lapid_b200_buffer *q, const lapid_b200_matview *q_view, const lapid_b200_buffer *k_cache,
+                                                  const lapid_b200_buffer *v_cache, const lapid_b200_buffer *block_table, lapid_b200_buffer *out,
+                                                  const lapid_b200_matview *out_view, lapid_b200_buffer *lse) {
     return guard([&] {
         need(dev);
-        lb::PagedAttnArgs a{};
+        if (!tree) fail("invalid_argument", "paged_tree_attention: tree is NULL");
+        paged_attention_impl(dev, desc, plan, tree, q, q_view, k_cache, v_cache, block_table, out, out_view, lse);
+    });
+}
+
+// ------------------------------------------------------------------ drafted tokens
+lapid_b200_status lapid_b200_paged_tree_bytes(const lapid_b200_paged *desc, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) fail("invalid_argument", "bytes is NULL");
+        const lb::PagedShape s = paged_shape(desc);
+        if (!s.tree) fail("invalid_launch", "paged_tree: the description's mask is not TREE");
+        *bytes = (uint64_t)s.tokens * (1 + s.tree) * 4;
+    });
+}
+
+lapid_b200_status lapid_b200_paged_tree(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan, const lapid_b200_buffer *parents,
+                                        lapid_b200_buffer *positions, lapid_b200_buffer *tree) {
+    return guard([&] {
+        need(dev);
+        lb::PagedTreeArgs a{};
         a.s = paged_shape(desc);
-        a.l = lb::paged_plan_layout(a.s);
-        const uint64_t T = a.s.tokens, cache = (uint64_t)a.s.pages * a.s.hkv * a.s.page * a.s.d * 2;
-        paged_buffer(dev, plan, "paged_attention: plan", a.l.bytes);
-        a.qv = paged_view(dev, q, q_view, "paged_attention: q", T, a.s.hq, a.s.d, 2);
-        paged_buffer(dev, k_cache, "paged_attention: k_cache", cache);
-        paged_buffer(dev, v_cache, "paged_attention: v_cache", cache);
-        paged_buffer(dev, block_table, "paged_attention: block_table", (uint64_t)a.s.requests * a.s.max_blocks * 4);
-        a.ov = paged_view(dev, out, out_view, "paged_attention: out", T, a.s.hq, a.s.d, 2);
-        // each element of out is written by one row only
-        const uint64_t D = a.s.d, H = a.s.hq;
-        const bool heads_inside = a.ov.head >= D && (T <= 1 || a.ov.token >= (H - 1) * a.ov.head + D), tokens_inside = a.ov.token >= D && a.ov.head >= (T - 1) * a.ov.token + D;
-        if (T && !((H == 1 && (T <= 1 || a.ov.token >= D)) || heads_inside || tokens_inside)) fail("invalid_launch", "paged_attention: rows of out overlap");
-        if (lse) paged_buffer(dev, lse, "paged_attention: lse", T * H * 4);
-        const lapid_b200_buffer *ins[] = {q, k_cache, v_cache, block_table}, *outs[] = {plan, out, lse};
-        for (size_t i = 0; i < 3; i++) {
-            if (!outs[i]) continue;
-            for (const lapid_b200_buffer *b : ins)
-                if (paged_overlap(b, outs[i])) fail("buffer_aliasing", "paged_attention: an output aliases an input");
-            for (size_t j = 0; j < i; j++)
-                if (paged_overlap(outs[i], outs[j])) fail("buffer_aliasing", "paged_attention: two outputs alias");
-        }
-        if (T == 0 || a.s.requests == 0) return;
+        if (!a.s.tree) fail("invalid_launch", "paged_tree: the description's mask is not TREE");
+        const uint64_t T = a.s.tokens;
+        const lb::PagedPlanLayout l = lb::paged_plan_layout(a.s);
+        paged_buffer(dev, plan, "paged_tree: plan", l.bytes);
+        paged_buffer(dev, parents, "paged_tree: parents", T * 4);
+        paged_buffer(dev, positions, "paged_tree: positions", T * 4);
+        paged_buffer(dev, tree, "paged_tree: tree", T * (1 + a.s.tree) * 4);
+        paged_apart("paged_tree", {plan, parents}, {positions, tree});
+        if (T == 0 || a.s.requests == 0 || a.s.max_new == 0) return;
         std::lock_guard<std::mutex> lock(dev->mu);
         dev->make_current();
+        a.request = (const uint32_t *)plan->ptr + l.request;
+        a.stamped = (const uint32_t *)plan->ptr + l.start_small;
         a.stamp = lb::paged_stamp(a.s);
-        a.plan = (uint32_t *)plan->ptr;
-        a.q = q->ptr;
-        a.k_cache = k_cache->ptr;
-        a.v_cache = v_cache->ptr;
-        a.table = (const int32_t *)block_table->ptr;
-        a.out = out->ptr;
-        a.lse = lse ? (float *)lse->ptr : nullptr;
+        a.parents = (const int32_t *)parents->ptr;
+        a.positions = (int32_t *)positions->ptr;
+        a.tree = (uint32_t *)tree->ptr;
         a.status = dev->status_dev;
-        // requests of many rows first: their CTAs run longest
-        if (lb::paged_has_large(a.s)) {
-            a.behind = true;
-            cuda_check(lb::launch_paged_attn_large(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
-            dev->launches++;
-        }
-        cuda_check(lb::launch_paged_attn_small(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
+        cuda_check(lb::launch_paged_tree(a, dev->sm_count, dev->pdl, dev->stream), "paged_tree launch");
         dev->launches++;
+    });
+}
+
+lapid_b200_status lapid_b200_paged_verify(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan, int32_t logits_dtype, uint64_t vocab,
+                                          const lapid_b200_buffer *logits, uint64_t logits_row, const lapid_b200_buffer *draft, uint64_t draft_row,
+                                          const lapid_b200_buffer *tokens, const lapid_b200_buffer *parents, const lapid_b200_buffer *accept,
+                                          const lapid_b200_buffer *pick, const lapid_b200_buffer *temperature, lapid_b200_buffer *path,
+                                          lapid_b200_buffer *accepted, lapid_b200_buffer *next) {
+    return guard([&] {
+        need(dev);
+        lb::PagedVerifyArgs a{};
+        a.s = paged_shape(desc);
+        if (!a.s.tree && a.s.mask != lb::PAGED_CAUSAL) fail("invalid_launch", "paged_verify: the description's mask must be TREE or CAUSAL");
+        if (a.s.tree ? !parents : parents != nullptr) fail("invalid_argument", "paged_verify: parents come with the mask TREE");
+        if (a.s.max_new > lb::PAGED_TREE_MOST) fail("unsupported", "paged_verify: at most 1024 new tokens a request, max_new is " + std::to_string(a.s.max_new));
+        if (!is_act_float(logits_dtype)) fail("unsupported_dtype", "paged_verify: logits_dtype must be F32, F16 or BF16, got " + std::to_string(logits_dtype));
+        if (vocab == 0 || vocab > lb::PAGED_VERIFY_VOCAB) fail("unsupported", "paged_verify: vocab must be 1 to 2^22, got " + std::to_string(vocab));
+        const uint64_t T = a.s.tokens, R = a.s.requests, most = 1ull << 60;
+        const lb::PagedPlanLayout l = lb::paged_plan_layout(a.s);
+        paged_buffer(dev, plan, "paged_verify: plan", l.bytes);
+        auto rows = [&](const lapid_b200_buffer *b, uint64_t row, uint64_t elem, const char *what) -> uint64_t {
+            if (row == 0) row = vocab;
+            if (row < vocab) fail("invalid_launch", std::string(what) + ": rows overlap");
+            if (T > 1 && row > most / T) fail("too_large", std::string(what) + ": rows overflow");
+            paged_buffer(dev, b, what, T ? ((T - 1) * row + vocab) * elem : 0);
+            return row;
+        };
+        a.logits_row = rows(logits, logits_row, act_elem_size(logits_dtype), "paged_verify: logits");
+        if (draft) a.draft_row = rows(draft, draft_row, 4, "paged_verify: draft");
+        paged_buffer(dev, tokens, "paged_verify: tokens", T * 4);
+        if (parents) paged_buffer(dev, parents, "paged_verify: parents", T * 4);
+        paged_buffer(dev, accept, "paged_verify: accept", T * 4);
+        paged_buffer(dev, pick, "paged_verify: pick", R * 4);
+        if (temperature) paged_buffer(dev, temperature, "paged_verify: temperature", R * 4);
+        paged_buffer(dev, path, "paged_verify: path", R * a.s.max_new * 4);
+        paged_buffer(dev, accepted, "paged_verify: accepted", R * 4);
+        paged_buffer(dev, next, "paged_verify: next", R * 4);
+        paged_apart("paged_verify", {plan, logits, draft, tokens, parents, accept, pick, temperature}, {path, accepted, next});
+        if (R == 0) return;
+        std::lock_guard<std::mutex> lock(dev->mu);
+        dev->make_current();
+        a.request = (const uint32_t *)plan->ptr + l.request;
+        a.stamped = (const uint32_t *)plan->ptr + l.start_small;
+        a.stamp = lb::paged_stamp(a.s);
+        a.vocab = (uint32_t)vocab;
+        a.type = act_type_of(logits_dtype);
+        a.logits = logits->ptr;
+        a.draft = draft ? (const float *)draft->ptr : nullptr;
+        a.tokens = (const int32_t *)tokens->ptr;
+        a.parents = parents ? (const int32_t *)parents->ptr : nullptr;
+        a.accept = (const float *)accept->ptr;
+        a.pick = (const float *)pick->ptr;
+        a.temperature = temperature ? (const float *)temperature->ptr : nullptr;
+        a.path = (int32_t *)path->ptr;
+        a.accepted = (int32_t *)accepted->ptr;
+        a.next = (int32_t *)next->ptr;
+        a.status = dev->status_dev;
+        cuda_check(lb::launch_paged_verify(a, dev->sm_count, dev->pdl, dev->stream), "paged_verify launch");
+        dev->launches++;
+    });
+}
+
+lapid_b200_status lapid_b200_paged_commit(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan, lapid_b200_buffer *const *caches,
+                                          uint64_t n_caches, const lapid_b200_buffer *block_table, const lapid_b200_buffer *path, const lapid_b200_buffer *accepted,
+                                          lapid_b200_buffer *free_pages, uint64_t n_free, lapid_b200_buffer *kv_lens, lapid_b200_buffer *used) {
+    return guard([&] {
+        need(dev);
+        lb::PagedCommitArgs a{};
+        a.s = paged_shape(desc);
+        if (!a.s.tree && a.s.mask != lb::PAGED_CAUSAL) fail("invalid_launch", "paged_commit: the description's mask must be TREE or CAUSAL");
+        if (a.s.tree && !path) fail("invalid_argument", "paged_commit: path is NULL (the accepted tokens of a tree do not lie behind each other)");
+        if (n_free >= (1ull << 31)) fail("too_large", "paged_commit: n_free must be below 2^31");
+        if (n_caches > 1u << 16) fail("too_large", "paged_commit: at most 65536 caches");
+        if (n_caches && !caches) fail("invalid_argument", "paged_commit: caches is NULL");
+        const uint64_t R = a.s.requests, cache = (uint64_t)a.s.pages * a.s.hkv * a.s.page * a.s.d * 2;
+        const lb::PagedPlanLayout l = lb::paged_plan_layout(a.s);
+        paged_buffer(dev, plan, "paged_commit: plan", l.bytes);
+        paged_buffer(dev, block_table, "paged_commit: block_table", R * a.s.max_blocks * 4);
+        if (path) paged_buffer(dev, path, "paged_commit: path", R * a.s.max_new * 4);
+        paged_buffer(dev, accepted, "paged_commit: accepted", R * 4);
+        if (free_pages || n_free) paged_buffer(dev, free_pages, "paged_commit: free_pages", n_free * 4);
+        paged_buffer(dev, kv_lens, "paged_commit: kv_lens", R * 4);
+        paged_buffer(dev, used, "paged_commit: used", 4);
+        std::vector<const lapid_b200_buffer *> outs = {free_pages, kv_lens, used};
+        for (uint64_t i = 0; i < n_caches; i++) {
+            paged_buffer(dev, caches[i], "paged_commit: a cache", cache);
+            outs.push_back(caches[i]);
+        }
+        paged_apart("paged_commit", {plan, block_table, path, accepted}, outs);
+        if (R == 0) n_caches = 0;
+        std::lock_guard<std::mutex> lock(dev->mu);
+        dev->make_current();
+        a.request = (const uint32_t *)plan->ptr + l.request;
+        a.stamped = (const uint32_t *)plan->ptr + l.start_small;
+        a.stamp = lb::paged_stamp(a.s);
+        a.n_free = (uint32_t)n_free;
+        a.table = (const int32_t *)block_table->ptr;
+        a.path = path ? (const int32_t *)path->ptr : nullptr;
+        a.accepted = (const int32_t *)accepted->ptr;
+        a.free_pages = free_pages ? (int32_t *)free_pages->ptr : nullptr;
+        a.kv_lens = (int32_t *)kv_lens->ptr;
+        a.used = (int32_t *)used->ptr;
+        a.status = dev->status_dev;
+        uint64_t done = 0;
+        do {
+            a.pages = done == 0;
+            a.caches = path ? (uint32_t)std::min<uint64_t>(n_caches - done, lb::PAGED_COMMIT_CACHES) : 0u;
+            for (uint32_t i = 0; i < a.caches; i++) a.cache[i] = caches[done + i]->ptr;
+            cuda_check(lb::launch_paged_commit(a, dev->pdl, dev->stream), "paged_commit launch");
+            dev->launches++;
+            done += a.caches;
+        } while (path && done < n_caches);
     });
 }
 

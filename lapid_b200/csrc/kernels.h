@@ -390,7 +390,7 @@ cudaError_t launch_silu_mul(const float *gate, const float *up, float *out, uint
                             bool pdl, cudaStream_t stream);
 
 // ---- paged.cu, paged_attn.cu, paged_attn_tc.cu: the paged key/value cache and the attention over it
-constexpr uint32_t PAGED_FULL = 0, PAGED_CAUSAL = 1, PAGED_CROSS = 2;  // LAPID_B200_MASK_*
+constexpr uint32_t PAGED_FULL = 0, PAGED_CAUSAL = 1, PAGED_CROSS = 2;  // LAPID_B200_MASK_* (TREE: PagedShape::tree)
 constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile and step of the kernel for few rows
 // Requests of at most so many packed rows go to it: its tile. Two such tiles read the keys twice: 32 rows (eight tokens of four heads) take with a limit of 16
 // and of 32 47.8 and 63.3 us at 16 requests over 2048 to 4096 keys, 19.1 and 21.0 at one over 8192, 56.0 and 76.1 at 64 over 512 to 1024; at d = 64 22.7 and 25.5.
@@ -413,6 +413,7 @@ struct PagedShape {
     uint32_t hq, hkv, g, d, page, pages, requests, tokens, max_blocks, max_new, mask, window;
     uint32_t tt;          // whole tokens (of g rows) in 128 rows; 0: none
     uint32_t large_keys;  // step of the tensor-memory kernel (paged_attn_tc.cu says why): 80 keys where head_dim is above 64, else 96
+    uint32_t tree;        // the new tokens are a tree (LAPID_B200_MASK_TREE; mask is CAUSAL then: no token sees one behind it): the words of a token's bits, else 0
     float scale;
 };
 // Places in a plan buffer (32-bit words; `past`, at the same place whatever the description: 1 from when the kernel for many rows has waited for what is in front of it until
@@ -462,11 +463,51 @@ struct PagedAttnArgs {
     float *lse;
     int *status;
     bool behind;  // the kernel for few rows: the one for many is in front of it, and nothing it needs is made there
+    const uint32_t *tree;  // of a tree: [tokens][1 + s.tree], what paged_tree makes
 };
 uint32_t paged_attn_small_ctas(int sm_count);
 uint32_t paged_attn_large_ctas(int sm_count);
 cudaError_t launch_paged_attn_small(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream);
 cudaError_t launch_paged_attn_large(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream);
+
+// ---- paged_draft.cu, paged_verify.cu: drafted tokens over the paged cache
+constexpr uint32_t PAGED_TREE_MOST = 1024;  // new tokens of a request whose tokens are a tree, or are verified
+constexpr uint32_t PAGED_VERIFY_VOCAB = 1u << 22;
+struct PagedTreeArgs {
+    PagedShape s;
+    const uint32_t *request, *stamped;  // of the plan: the requests' records, and a word with its stamp
+    uint32_t stamp;
+    const int32_t *parents;
+    int32_t *positions;
+    uint32_t *tree;
+    int *status;
+};
+cudaError_t launch_paged_tree(const PagedTreeArgs &a, int sm_count, bool pdl, cudaStream_t stream);
+constexpr uint32_t PAGED_COMMIT_CACHES = 256;  // keys and values of at most so many layers' halves in one launch
+struct PagedCommitArgs {
+    PagedShape s;
+    const uint32_t *request, *stamped;
+    uint32_t stamp, caches, n_free;
+    const int32_t *table, *path, *accepted;  // path null: the accepted tokens lie where they belong
+    int32_t *free_pages, *kv_lens, *used;
+    int *status;
+    bool pages;  // the lengths and the list of free pages too (the first launch of a call)
+    void *cache[PAGED_COMMIT_CACHES];
+};
+cudaError_t launch_paged_commit(const PagedCommitArgs &a, bool pdl, cudaStream_t stream);
+struct PagedVerifyArgs {
+    PagedShape s;
+    const uint32_t *request, *stamped;
+    uint32_t stamp, vocab;
+    int type;  // ACT_F32 / ACT_F16 / ACT_BF16, of the logits
+    const void *logits;
+    uint64_t logits_row, draft_row;  // elements from row to row
+    const float *draft, *accept, *pick, *temperature;  // draft and temperature may be null
+    const int32_t *tokens, *parents;                   // parents null: each token's is the one in front of it
+    int32_t *path, *accepted, *next;
+    int *status;
+};
+cudaError_t launch_paged_verify(const PagedVerifyArgs &a, int sm_count, bool pdl, cudaStream_t stream);
 
 // ---- tp_allreduce.cu: one-shot all-reduce over peer-mapped memory
 struct TpAllReduceArgs {

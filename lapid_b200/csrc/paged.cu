@@ -50,7 +50,7 @@ bool paged_has_large(const PagedShape &s) { return (uint64_t)s.max_new * s.g > P
 
 uint32_t paged_stamp(const PagedShape &s) {
     uint32_t h = 2166136261u;  // (Fowler, Noll and Vo's hash over the words a plan depends on)
-    for (uint32_t v : {s.g, s.hkv, s.page, s.requests, s.tokens, s.max_blocks, s.max_new, s.mask, s.window, s.d > 64 ? 128u : 64u})
+    for (uint32_t v : {s.g, s.hkv, s.page, s.requests, s.tokens, s.max_blocks, s.max_new, s.mask, s.window, s.d > 64 ? 128u : 64u, s.tree})
         for (int b = 0; b < 4; b++) h = (h ^ ((v >> (8 * b)) & 0xff)) * 16777619u;
     return h | 1u;  // never what a zeroed buffer holds
 }

@@ -14,7 +14,7 @@
 
 namespace lb {
 
-constexpr uint32_t PAGED_STATUS_INDEX = 512, PAGED_STATUS_PAGES = 1024, PAGED_STATUS_WAIT = 2048, PAGED_STATUS_LENGTHS = 4096, PAGED_STATUS_PLAN = 8192;
+constexpr uint32_t PAGED_STATUS_INDEX = 512, PAGED_STATUS_PAGES = 1024, PAGED_STATUS_WAIT = 2048, PAGED_STATUS_LENGTHS = 4096, PAGED_STATUS_PLAN = 8192, PAGED_STATUS_LOGITS = 16384;
 
 struct PagedTile {
     uint32_t first, steps;  // its steps over the keys: [first, first + steps), in units of `keys`
@@ -28,12 +28,26 @@ __host__ __device__ inline uint32_t paged_hi(const PagedShape &s, uint32_t n, ui
     return kv > back ? kv - back : 0u;
 }
 __host__ __device__ inline uint32_t paged_lo(const PagedShape &s, uint32_t hi) { return s.window && hi > s.window ? hi - s.window : 0u; }
+// The first key that any token from `t0` on may see. Of a tree: where a token that has no ancestor may begin to look, since the tokens' places say nothing of their depth.
+__host__ __device__ inline uint32_t paged_tile_lo(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t t0) { return paged_lo(s, paged_hi(s, n, kv, s.tree ? 0u : t0)); }
+
+// A drafted token's row of the tree buffer: [0] how many ancestors it has, behind it the bits of those and of itself (bit i of word w: token 32 w + i of the request; with a
+// window the near ones). Of the cached keys it sees those from `lo` on.
+__host__ __device__ inline uint32_t paged_tree_lo(const PagedShape &s, uint32_t cached, uint32_t depth) { return paged_lo(s, cached + depth + 1); }
+#ifdef __CUDACC__
+// 32 of its bits, from token i0 on (which may lie in front of the first)
+__device__ __forceinline__ uint32_t paged_tree_bits(const uint32_t *row, uint32_t words, int32_t i0) {
+    const int32_t w = i0 >> 5;
+    const uint32_t a = (uint32_t)w < words ? row[1 + w] : 0u, b = (uint32_t)(w + 1) < words ? row[2 + w] : 0u;
+    return __funnelshift_r(a, b, (uint32_t)i0 & 31);
+}
+#endif
 
 // The tile of a request's new tokens [t0, t1]: at least one step, so that rows without keys are written too
 __host__ __device__ inline PagedTile paged_tile_of(const PagedShape &s, uint32_t n, uint32_t kv, uint32_t t0, uint32_t t1, uint32_t keys) {
     PagedTile t;
     t.hi = paged_hi(s, n, kv, t1);
-    t.first = paged_lo(s, paged_hi(s, n, kv, t0)) / keys;
+    t.first = paged_tile_lo(s, n, kv, t0) / keys;
     const uint32_t end = (t.hi + keys - 1) / keys;
     t.steps = end > t.first ? end - t.first : 1u;
     return t;

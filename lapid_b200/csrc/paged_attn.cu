@@ -108,7 +108,8 @@ __device__ __forceinline__ void store_half4(unsigned short *row, uint32_t col, u
         if (col + i < d) row[col + i] = (unsigned short)(bf16 ? pack<true>(f[i], 0.0f) : pack<false>(f[i], 0.0f));
 }
 
-template <int DP, bool BF16>
+// TREE: the new tokens are a request's drafted ones, and of those a token sees its ancestors and itself
+template <int DP, bool BF16, bool TREE>
 __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PagedAttnArgs p) {
     using C = Cfg<DP>;
     extern __shared__ uint8_t smem_raw[];
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
             if (copies && key < w.t.hi) {
                 const int32_t page = p.table[(size_t)w.r * s.max_blocks + block];
                 if (page >= 0 && (uint32_t)page < s.pages) row = (int)(((uint32_t)page * s.hkv + w.head) * s.page + key % s.page);
-                else if ((block + 1) * s.page > paged_lo(s, paged_hi(s, w.n, w.kv, w.tile * ROWS / s.g))) bad = true;
+                else if ((block + 1) * s.page > paged_tile_lo(s, w.n, w.kv, w.tile * ROWS / s.g)) bad = true;
             }
             if (++step == w.t.steps && u + 1 < u1) {
                 step = 0;
@@ -211,13 +212,20 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
         const uint32_t steps = min(w.t.steps - step, u1 - u);  // of this tile in this span
         // rows and what they see
         uint32_t lo[2], hi[2];
+        const uint32_t *tree[2] = {};
+        const uint32_t cached = w.kv - w.n;
         uint32_t aq[DP / 16][4];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint32_t row = w.tile * ROWS + quad + 8 * h, token = row / s.g;
             const bool real = token < w.n;
             hi[h] = real ? paged_hi(s, w.n, w.kv, token) : 0u;
-            lo[h] = paged_lo(s, hi[h]);
+            if constexpr (TREE) {
+                tree[h] = p.tree + (size_t)(w.q0 + (real ? token : 0u)) * (1 + s.tree);
+                lo[h] = paged_tree_lo(s, cached, *tree[h]);
+            } else {
+                lo[h] = paged_lo(s, hi[h]);
+            }
             const unsigned short *q = (const unsigned short *)p.q + p.qv.off + (uint64_t)(w.q0 + token) * p.qv.token + (uint64_t)(w.head * s.g + row % s.g) * p.qv.head;
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ks++)
@@ -229,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
                     aq[ks][2 * j + h] = x;
                 }
         }
-        const uint32_t tile_lo = paged_lo(s, paged_hi(s, w.n, w.kv, w.tile * ROWS / s.g));
+        const uint32_t tile_lo = paged_tile_lo(s, w.n, w.kv, w.tile * ROWS / s.g);
         float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -247,12 +255,23 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attn_small_kernel(const __gr
             }
             const uint32_t key0 = (w.t.first + step + i) * KEYS + warp * 16;
             float top[2] = {-INFINITY, -INFINITY};
+            uint32_t seen[2];  // of a tree: a bit for each of the 16 keys that the row sees
+            if constexpr (TREE) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t from = lo[h] > key0 ? min(lo[h] - key0, 16u) : 0u, to = cached > key0 ? min(cached - key0, 16u) : 0u;
+                    seen[h] = ((1u << to) - 1) & ~((1u << from) - 1);
+                    if (key0 + 16 > cached) seen[h] |= paged_tree_bits(tree[h], s.tree, (int32_t)(key0 - cached));
+                    if (hi[h] == 0) seen[h] = 0;  // (no row)
+                }
+            }
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t key = key0 + 8 * t + pair + (e & 1);
-                    sc[t][e] = key >= lo[e >> 1] && key < hi[e >> 1] ? sc[t][e] * c : -INFINITY;
+                    const bool sees = TREE ? seen[e >> 1] >> (8 * t + pair + (e & 1)) & 1 : key >= lo[e >> 1] && key < hi[e >> 1];
+                    sc[t][e] = sees ? sc[t][e] * c : -INFINITY;
                     top[e >> 1] = fmaxf(top[e >> 1], sc[t][e]);
                 }
             float base[2], keep[2];
@@ -474,8 +493,8 @@ bool paged_q_map(const PagedAttnArgs &a, CUtensorMap &map) {
 
 uint32_t paged_attn_small_ctas(int sm_count) { return 2 * (uint32_t)sm_count; }
 
-template <int DP, bool BF16> static cudaError_t small_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sm_count, bool pdl, cudaStream_t stream) {
-    auto *kernel = pa::paged_attn_small_kernel<DP, BF16>;
+template <int DP, bool BF16, bool TREE> static cudaError_t small_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sm_count, bool pdl, cudaStream_t stream) {
+    auto *kernel = pa::paged_attn_small_kernel<DP, BF16, TREE>;
     constexpr int SMEM = pa::Cfg<DP>::SMEM;
     static std::once_flag once[64];
     int dev = 0;
@@ -500,8 +519,10 @@ cudaError_t launch_paged_attn_small(const PagedAttnArgs &a, int sm_count, bool p
     CUtensorMap mk, mv;
     const uint32_t rows = a.s.page < PAGED_SMALL_KEYS ? a.s.page : PAGED_SMALL_KEYS;
     if (!paged_cache_map(a.s, a.k_cache, rows, mk) || !paged_cache_map(a.s, a.v_cache, rows, mv)) return cudaErrorInvalidValue;
-    if (a.s.d > 64) return a.s.bf16 ? small_launch<128, true>(a, mk, mv, sm_count, pdl, stream) : small_launch<128, false>(a, mk, mv, sm_count, pdl, stream);
-    return a.s.bf16 ? small_launch<64, true>(a, mk, mv, sm_count, pdl, stream) : small_launch<64, false>(a, mk, mv, sm_count, pdl, stream);
+    auto launch = [&](auto dp, auto bf16, auto tree) { return small_launch<decltype(dp)::value, decltype(bf16)::value, decltype(tree)::value>(a, mk, mv, sm_count, pdl, stream); };
+    auto typed = [&](auto dp, auto tree) { return a.s.bf16 ? launch(dp, std::true_type(), tree) : launch(dp, std::false_type(), tree); };
+    auto sized = [&](auto tree) { return a.s.d > 64 ? typed(std::integral_constant<int, 128>(), tree) : typed(std::integral_constant<int, 64>(), tree); };
+    return a.s.tree ? sized(std::true_type()) : sized(std::false_type());
 }
 
 }  // namespace lb

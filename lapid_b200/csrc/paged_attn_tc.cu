@@ -35,6 +35,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged.cuh"
 #include "pipe.cuh"
@@ -282,7 +284,7 @@ template <int KEYS> __device__ __forceinline__ bool next_piece(const PagedAttnAr
     }
     return load_tile<KEYS>(p, w);
 }
-__device__ __forceinline__ uint32_t tile_low(const PagedAttnArgs &p, const Walk &w) { return paged_lo(p.s, paged_hi(p.s, w.n, w.kv, 2 * w.tile * p.s.tt)); }
+__device__ __forceinline__ uint32_t tile_low(const PagedAttnArgs &p, const Walk &w) { return paged_tile_lo(p.s, w.n, w.kv, 2 * w.tile * p.s.tt); }
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(s32(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z),
                  "r"(s32(bar))
@@ -408,7 +410,8 @@ template <int DP, bool BF16> __device__ __forceinline__ void join_pieces(const P
     }
 }
 
-template <int DP, bool BF16>
+// TREE: the new tokens are a request's drafted ones, and of those a token sees its ancestors and itself
+template <int DP, bool BF16, bool TREE>
 __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q, PagedAttnArgs p, bool q_boxes) {
     using C = Cfg<DP>;
     extern __shared__ uint8_t smem_raw[];
@@ -678,7 +681,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             const uint32_t token = (2 * w.tile + t) * s.tt + local, qh = w.head * s.g + member;
             const bool real = local < s.tt && token < w.n;
             // (rows that are none see everything: their results go nowhere, and they ask for no mask)
-            const uint32_t hi = real ? paged_hi(s, w.n, w.kv, token) : ~0u, lo = real ? paged_lo(s, hi) : 0u;
+            // (of a tree: hi and lo are those of the cached keys)
+            const uint32_t cached = w.kv - w.n;
+            const uint32_t *const tree = TREE ? p.tree + (size_t)(w.q0 + (real ? token : 0u)) * (1 + s.tree) : nullptr;
+            const uint32_t hi = !real ? ~0u : TREE ? cached : paged_hi(s, w.n, w.kv, token), lo = !real ? 0u : TREE ? paged_tree_lo(s, cached, *tree) : paged_lo(s, hi);
             float m = -INFINITY, base = 0.0f;  // the maximum that the weights refer to
             uint64_t l0 = 0, l1 = 0;           // two pairs of sums
             const uint64_t c2 = pack2(c, c);
@@ -707,7 +713,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
 #pragma unroll
                     for (uint32_t g = 0; g < (uint32_t)C::KEYS; g += 32) {
                         const uint32_t below = to > g ? (to - g >= 32 ? ~0u : (1u << (to - g)) - 1) : 0u, out = from > g ? (from - g >= 32 ? ~0u : (1u << (from - g)) - 1) : 0u;
-                        const uint32_t bits = below & ~out;
+                        uint32_t bits = below & ~out;
+                        if constexpr (TREE) {
+                            if (real) bits |= paged_tree_bits(tree, s.tree, (int32_t)(key0 + g - cached));
+                        }
 #pragma unroll
                         for (uint32_t i = 0; i < 32 && g + i < (uint32_t)C::KEYS; i++)
                             if (!(bits & (1u << i))) x[g + i] = 0xff800000u;
@@ -875,8 +884,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
 
 uint32_t paged_attn_large_ctas(int sm_count) { return (uint32_t)sm_count; }
 
-template <int DP, bool BF16> static cudaError_t large_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, bool boxes, int sm_count, bool pdl, cudaStream_t stream) {
-    auto *kernel = pt::paged_attn_large_kernel<DP, BF16>;
+template <int DP, bool BF16, bool TREE> static cudaError_t large_launch(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, bool boxes, int sm_count, bool pdl, cudaStream_t stream) {
+    auto *kernel = pt::paged_attn_large_kernel<DP, BF16, TREE>;
     constexpr int SMEM = pt::Cfg<DP>::SMEM;
     static std::once_flag once[64];
     int dev = 0;
@@ -902,8 +911,10 @@ cudaError_t launch_paged_attn_large(const PagedAttnArgs &a, int sm_count, bool p
     constexpr uint32_t rows = 16;
     if (!paged_cache_map(a.s, a.k_cache, rows, mk) || !paged_cache_map(a.s, a.v_cache, rows, mv)) return cudaErrorInvalidValue;
     const bool boxes = paged_q_map(a, mq);
-    if (a.s.d > 64) return a.s.bf16 ? large_launch<128, true>(a, mk, mv, mq, boxes, sm_count, pdl, stream) : large_launch<128, false>(a, mk, mv, mq, boxes, sm_count, pdl, stream);
-    return a.s.bf16 ? large_launch<64, true>(a, mk, mv, mq, boxes, sm_count, pdl, stream) : large_launch<64, false>(a, mk, mv, mq, boxes, sm_count, pdl, stream);
+    auto launch = [&](auto dp, auto bf16, auto tree) { return large_launch<decltype(dp)::value, decltype(bf16)::value, decltype(tree)::value>(a, mk, mv, mq, boxes, sm_count, pdl, stream); };
+    auto typed = [&](auto dp, auto tree) { return a.s.bf16 ? launch(dp, std::true_type(), tree) : launch(dp, std::false_type(), tree); };
+    auto sized = [&](auto tree) { return a.s.d > 64 ? typed(std::integral_constant<int, 128>(), tree) : typed(std::integral_constant<int, 64>(), tree); };
+    return a.s.tree ? sized(std::true_type()) : sized(std::false_type());
 }
 
 }  // namespace lb

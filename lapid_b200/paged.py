@@ -15,6 +15,19 @@ the block table names. A step of a layer stack, with everything on the device::
         ...                                                     # o projection, a_dtype = DType.BF16
 
 ``tp.PagedLayers`` is that step over whole decoder layers.
+
+Drafted tokens (speculative decoding) are the new tokens of such a step with ``mask=Mask.TREE``: a request's first one is the text's last token, each other one the child of one in front of it::
+
+    tree = be.alloc(tree_bytes(spec))
+    be.paged_plan(...)
+    be.paged_tree(spec, plan, parents, positions, tree)             # positions: cached + number of ancestors
+    for layer in layers:
+        be.paged_append(...); be.paged_tree_attention(spec, plan, tree, q_half, layer.k, layer.v, table, mixed)
+    ...                                                             # logits of every drafted token
+    be.paged_verify(spec, plan, DType.F32, vocab, logits, tokens, accept, pick, path, accepted, next, parents=parents, draft=probabilities)
+    be.paged_commit(spec, plan, [(layer.k, layer.v) for layer in layers], table, path, accepted, kv_lens, used, free_pages=free, n_free=n)
+
+``tp.DraftLayers`` is that step.
 """
 from __future__ import annotations
 
@@ -30,10 +43,11 @@ from .backend import DType
 
 
 class Mask(enum.IntEnum):
-    """Which keys a new token sees: all, those up to its own, or the cached ones only."""
+    """Which keys a new token sees: all, those up to its own, the cached ones only, or the cached ones and its ancestors' (drafted tokens)."""
     FULL = 0
     CAUSAL = 1
     CROSS = 2
+    TREE = 4
 
 
 @dataclass(frozen=True)
@@ -74,6 +88,14 @@ def plan_bytes(spec: PagedSpec) -> int:
     n = C.c_uint64(0)
     c = spec.to_c()
     check(_lib.lib().lapid_b200_paged_plan_bytes(C.byref(c), C.byref(n)))
+    return int(n.value)
+
+
+def tree_bytes(spec: PagedSpec) -> int:
+    """Bytes of the tree buffer of a step of drafted tokens (``lapid_b200_paged_tree_bytes``: u32 ``[tokens][1 + ceil(max_new / 32)]``, ancestors' count and bits); needs no device."""
+    n = C.c_uint64(0)
+    c = spec.to_c()
+    check(_lib.lib().lapid_b200_paged_tree_bytes(C.byref(c), C.byref(n)))
     return int(n.value)
 
 

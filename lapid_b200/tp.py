@@ -492,13 +492,16 @@ class PagedLayers(GpuTpLayers):
         w["free"] = backend.wrap_tensor(free) if free.numel() else None
         rot = {} if rope is None else {"rope": backend.wrap_tensor(rope), "rope_rows": rope.shape[0], "rot": rope.shape[1], "neighbours": neighbours}
         q, k, v = (backend.wrap_tensor(self.outs[n_]) for n_ in ("q", "k", "v"))
+        self._paged, self._caches = w, [(backend.wrap_tensor(keys), backend.wrap_tensor(values)) for keys, values in caches]
         self._plan_step = backend.packed_paged_plan(spec, w["new"], w["cached"], w["table"], w["slots"], w["positions"], w["kv"], w["used"], w["plan"],
                                                     free_pages=w["free"], n_free=free.numel())
-        self._mixes = []
-        for keys, values in caches:
-            kc, vc = backend.wrap_tensor(keys), backend.wrap_tensor(values)
-            self._mixes.append((backend.packed_paged_append(spec, DType.F32, q, k, v, w["slots"], w["positions"], kc, vc, w["q_half"], **rot),
-                                backend.packed_paged_attention(spec, w["plan"], w["q_half"], kc, vc, w["table"], w["mixed"])))
+        self._mixes = [(backend.packed_paged_append(spec, DType.F32, q, k, v, w["slots"], w["positions"], kc, vc, w["q_half"], **rot), self._attention_call(kc, vc))
+                       for kc, vc in self._caches]
+
+    def _attention_call(self, keys, values):
+        """A layer's attention over its cache, packed."""
+        w = self._paged
+        return self.be.packed_paged_attention(self.spec, w["plan"], w["q_half"], keys, values, w["table"], w["mixed"])
 
     def _o_operand(self):
         return self.mixed, self.spec.dtype
@@ -527,3 +530,61 @@ class PagedLayers(GpuTpLayers):
     def first_row_parallel(self):
         self._plan_step()
         return super().first_row_parallel()
+
+
+class DraftLayers(PagedLayers):
+    """``PagedLayers`` for drafted tokens (speculative decoding): a step looks at a tree of them for every request, keeps what the model's probabilities accept, and gives the token behind it.
+
+    `spec.mask` is ``Mask.TREE``. `head` is the quantized output matrix ``[vocab, d_model]`` in `head_format`; `drawn`: the drafted tokens are drawn from a draft model's distributions, which
+    the caller writes to `draft` (f32 [tokens, vocab], row of a node: what its children were drawn from); else they are candidates that were chosen. Before a step the caller fills, besides what ``PagedLayers``
+    takes (`h`: the rows of all new tokens, a request's first one the text's last), `parents`, `drafted` (token ids) and the random numbers `accept` (f32 [tokens]) and `pick` (f32 [requests]);
+    `temperature` (f32 [requests]) is 1 until it is changed. Behind it `path`, `accepted` and `next` say what was kept, `logits` has the rows, and `kv` and `used` are those of the kept tokens: `kv` is the next
+    step's `cached`, `drop_used` as behind any step. On one rank.
+    """
+
+    def __init__(self, backend, shape: LayerShape, spec, weights: list, formats: list, caches: list, table, free, head, head_format: int, vocab: int, rope=None,
+                 neighbours: bool = False, drawn: bool = False, fuse_act: bool = True):
+        import torch
+        from .backend import DType, matmul_launch
+        from .paged import Mask, tree_bytes
+        if spec.mask != Mask.TREE:
+            raise ValueError("the mask of drafted tokens' layers is TREE")
+        dev = weights[0]["q"].device
+        i32, f32 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.float32, device=dev)
+        self.parents, self.drafted = torch.full((spec.tokens,), -1, **i32), torch.zeros(spec.tokens, **i32)
+        self.accept, self.pick, self.temperature = torch.zeros(spec.tokens, **f32), torch.zeros(spec.requests, **f32), torch.ones(spec.requests, **f32)
+        self.path, self.accepted, self.next = torch.full((spec.requests, spec.max_new), -1, **i32), torch.zeros(spec.requests, **i32), torch.zeros(spec.requests, **i32)
+        self.logits = torch.zeros(spec.tokens, vocab, **f32)
+        self.draft = torch.zeros(spec.tokens, vocab, **f32) if drawn else None
+        self.tree = torch.zeros(tree_bytes(spec), dtype=torch.uint8, device=dev)
+        torch.cuda.synchronize(dev)
+        wrap = backend.wrap_tensor
+        self._tree = wrap(self.tree)
+        super().__init__(backend, shape, spec, weights, formats, caches, table, free, rope=rope, neighbours=neighbours, fuse_act=fuse_act)
+        w = self._paged
+        plan, parents, accepted, path = self._plan_step, wrap(self.parents), wrap(self.accepted), wrap(self.path)
+        grow = backend.packed_paged_tree(spec, w["plan"], parents, w["positions"], self._tree)
+
+        def plan_and_tree():
+            plan()
+            grow()
+        self._plan_step = plan_and_tree
+        head_launch = [matmul_launch(head_format, spec.tokens, vocab, shape.d_model)]
+        backend.prepare(head_launch)
+        logits = wrap(self.logits)
+        self._head = backend.packed(head_launch, [wrap(self.x), wrap(head), logits])
+        self._verify = backend.packed_paged_verify(spec, w["plan"], DType.F32, vocab, logits, wrap(self.drafted), wrap(self.accept), wrap(self.pick), path, accepted, wrap(self.next),
+                                                   parents=parents, draft=wrap(self.draft) if drawn else None, temperature=wrap(self.temperature))
+        self._commit = backend.packed_paged_commit(spec, w["plan"], self._caches, w["table"], path, accepted, w["kv"], w["used"], free_pages=w["free"], n_free=free.numel())
+
+    def _attention_call(self, keys, values):
+        w = self._paged
+        return self.be.packed_paged_tree_attention(self.spec, w["plan"], self._tree, w["q_half"], keys, values, w["table"], w["mixed"])
+
+    def step(self):
+        """Queues a whole step on the current stream: plan, layers (all that there are caches for), logits, verification, and what is kept of it. Returns `next`."""
+        self.token(len(self._caches))
+        self._head()
+        self._verify()
+        self._commit()
+        return self.next
