@@ -5,11 +5,13 @@
 // left, max(P - D, 0) / sum of it; without D (candidates that were chosen, not drawn) when u_c < P(x), else x leaves P. An accepted child is the next v; when none is,
 // the token behind the path is the first t with P(0) + .. + P(t) > w. Whatever the drafts are, the tokens are then distributed as the model's own.
 //
-// Decisions are comparisons, so weights and sums are 64 bits wide: a result differs from the definition's only where u or w is within 1e-13 of a border.
+// Decisions are comparisons, so what decides is 64 bits wide: a result differs from the definition's only where u or w is within 1e-12 of a border. A node's sum is formed in 32 bits first,
+// which is off by less than SURE of it; a child whose test that leaves open, and what is drawn from, gets it again in 64 bits. (Half of the 64-bit operations that a sum of weights for every
+// node would be; an SM does 64 of these a cycle.)
 //
-// A request belongs to a cluster of CTAs, each with a part of the vocabulary, a warp of it 32 vectors wide and so on to its end; only the rows on the path are read. A level is a pass over the
-// node's logits (largest and sum, each thread relative to its own largest), an exchange over the cluster's shared memory, and the children's tests, whose tokens, numbers and values were
-// fetched meanwhile. What decides comes from rank 0's loads and from the exchanged sums alone, so that the CTAs of a cluster always take the same way.
+// A request belongs to a cluster of CTAs, each with a part of the vocabulary, a warp of it to a warp; only the rows on the path are read. A level is a pass over the node's logits (largest and sum), an
+// exchange over the cluster's shared memory, and the children's tests, whose tokens, numbers and values were fetched meanwhile. What decides comes from rank 0's loads and from the exchanged sums
+// alone, so that the CTAs of a cluster always take the same way.
 #include <cuda.h>
 
 #include <algorithm>
@@ -26,30 +28,30 @@ namespace pv {
 
 using pipe::s32;
 
-constexpr uint32_t WARPS = 16, THREADS = 32 * WARPS, MOST_CTAS = 8;  // of a cluster
-constexpr int UNROLL = 4;                                             // vectors a thread has in flight
+constexpr uint32_t WARPS = 16, THREADS = 32 * WARPS, MOST_CTAS = 16;  // of a cluster
+constexpr uint32_t BATCH = 16, FAST = 32;                             // tokens that a thread has in flight in a pass of 64 and of 32 bits
 
-// Shared memory: what the exchanges bring (two sets: a CTA writes a set again only when all have read it, which they say with the exchange between), the request, its
-// nodes, and a bit for each token of the part that is out of the distribution.
-struct Exchange {
-    double sum[2][MOST_CTAS];
-    float top[2][MOST_CTAS];
-    uint32_t at[2][MOST_CTAS];
-};
+// How far a sum of weights in 32 bits is off, relative: z - top, log2(e), that over T and the product are rounded, 4 2^-24 of the exponent x of e^x, whose mean over the weights is at most ln 2^22 = 15.3 (their
+// entropy); a weight is the product of powers of 2, 2^-22 and a product's 2^-24 each, to the thread's largest (as that grows, at most 64 times: PART_MOST), the warp's, the CTA's and the
+// cluster's; at most 90 additions, 2^-24 each. In all 3e-5, of which 2^-14 is twice as much.
+constexpr double SURE = 0x1p-14;
+constexpr uint32_t PART_MOST = 64 * 32 * 16;  // a warp's places
+
+// What the warps of the cluster tell each other comes in two sets: a warp writes a set again only when all have read it, which they say with the exchange between.
 struct Shared {
-    Exchange ex;
-    double warp_sum[WARPS];
-    float warp_top[WARPS];
-    uint32_t warp_at[WARPS];
-    uint32_t n;
+    uint64_t quick[2][MOST_CTAS * WARPS];  // a warp's largest logit and its sum in 32 bits; at temperature 0 the largest logit (as `ordered`) and the complement of its place
+    double sum[2][MOST_CTAS * WARPS];      // a warp's sum in 64 bits
+    double root[16];                       // 2^(j / 16)
+    uint32_t n;                            // of the request
     float temperature;
 };
-struct Node {      // what rank 0 tells of a child
+struct Node {  // a drafted token
     int32_t token;
-    float accept, logit, draft;
+    float accept, logit, draft;  // (the latter two when the walk is at its parent)
 };
 
-// value, inverse, node and parent of each of `most` tokens, and a bit for each token of the vocabulary's part
+// value, taken, node and parent of each of `most` tokens, and a bit for each token of the vocabulary's part
+constexpr int SMEM_MOST = 160 * 1024;
 constexpr size_t shared_bytes(uint32_t most, uint32_t part) { return sizeof(Shared) + most * (2 * sizeof(double) + sizeof(Node) + 4) + (size_t)WARPS * part / 8; }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -67,6 +69,7 @@ __device__ __forceinline__ uint32_t of_rank(const void *p, uint32_t rank) {
 }
 __device__ __forceinline__ void put(uint32_t at, uint32_t x) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); }
 __device__ __forceinline__ void put(uint32_t at, float x) { put(at, __float_as_uint(x)); }
+__device__ __forceinline__ void put(uint32_t at, uint64_t x) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(x) : "memory"); }
 __device__ __forceinline__ void put(uint32_t at, double x) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(x) : "memory"); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -80,12 +83,52 @@ __device__ __forceinline__ void better(float &top, uint32_t &at, float t, uint32
     top = max_nan(top, t);
 }
 
-// e^((z - top) / T): 0 for -inf, whatever T is
-__device__ __forceinline__ double weight(float z, float top, double inv_t) { return z == -INFINITY ? 0.0 : exp(((double)z - (double)top) * inv_t); }
+// Weights e^((z - top) / T), relative error 2e-13: with c = 16 log2(e) / T and n the whole number nearest to (z - top) c, 2^(n / 16) from a table of 16 (of which any lanes may read any without a bank
+// conflict) and the exponent, times the series of 2^(f / 16), |f| <= 1/2, to the fifth power: twelve operations of 64 bits. A weight below e^-700 is 0, as that of -inf is, whatever T is.
+struct Weight {
+    const double *root;
+    double top, c = 0.0;
+    float low;
+    __device__ __forceinline__ Weight(const double *table, float t) : root(table), top((double)t), low(t) {}
+    __device__ __forceinline__ void set(float temperature) {
+        c = 23.083120654223414 / (double)temperature;
+        low = fmaxf((float)top - 700.0f * temperature, -3.4028235e38f);
+    }
+    __device__ __forceinline__ double operator()(float z) const {
+        const double d = (double)z - top, magic = 6755399441055744.0;  // 1.5 2^52
+        const double k = fma(d, c, magic), f = fma(d, c, magic - k);
+        const int n = __double2loint(k);
+        // (ln 2 / 16)^i / i!
+        double p = fma(f, 1.271587195055813e-09, 1.467610032291943e-07);
+        p = fma(f, p, 1.3550807779497455e-05);
+        p = fma(f, p, 0.0009383847928089871);
+        p = fma(f, p, 0.04332169878499658);
+        p = fma(f, p, 1.0);
+        p *= root[n & 15];
+        p = __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
+        return z < low ? 0.0 : p;
+    }
+};
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// max(x, 0) by the sign bit
+__device__ __forceinline__ double positive(double x) {
+    const int keep = ~(__double2hiint(x) >> 31);
+    return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
+}
+// Whole numbers in the order of the floats, NaN on top
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return x != x ? ~0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-// E elements of a row from `i` (a multiple of E) on; `none` behind the vocabulary
-template <int SRC, int E, bool VEC> __device__ __forceinline__ void load_row(float (&x)[E], const void *row, uint32_t i, uint32_t vocab, float none) {
-    if (VEC && i + E <= vocab) {
+// E elements of a row whose tokens are the places [from, from + vocab) behind `row`, which is aligned to 16 bytes, from place `i` (a multiple of E) on; `none` outside
+template <int SRC, int E> __device__ __forceinline__ void load_row(float *x, const void *row, uint32_t i, uint32_t from, uint32_t end, float none) {
+    if (i >= from && i + E <= end) {
         if constexpr (SRC == ACT_F32) {
 #pragma unroll
             for (int e = 0; e < E; e += 4) {
@@ -102,224 +145,336 @@ template <int SRC, int E, bool VEC> __device__ __forceinline__ void load_row(flo
         return;
     }
 #pragma unroll
-    for (int e = 0; e < E; e++) x[e] = i + e < vocab ? load_act(row, i + e, SRC) : none;
+    for (int e = 0; e < E; e++) x[e] = i + e >= from && i + e < end ? load_act(row, i + e, SRC) : none;
+}
+// A row of f32 that is not aligned as the other one is
+template <int E> __device__ __forceinline__ void load_apart(float *x, const float *row, uint32_t i, uint32_t from, uint32_t end) {
+#pragma unroll
+    for (int e = 0; e < E; e++) x[e] = i + e >= from && i + e < end ? row[i + e - from] : 0.0f;
 }
 
-template <int SRC, bool VEC> __global__ void __launch_bounds__(THREADS, 2) paged_verify_kernel(const PagedVerifyArgs a, uint32_t ctas, uint32_t part) {
-    constexpr int E = SRC == ACT_F32 ? 4 : 8;
+template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_kernel(const PagedVerifyArgs a, uint32_t ctas, uint32_t part) {
+    constexpr int E = SRC == ACT_F32 ? 4 : 8, U = BATCH / E, V = FAST / E;
+    constexpr uint32_t EB = act_elem_bytes(SRC);
     extern __shared__ __align__(16) uint8_t smem[];
     Shared &sh = *(Shared *)smem;
     const uint32_t most = a.s.max_new;
-    double *const value = (double *)(smem + sizeof(Shared));              // a child's P(x), kept up with what is taken from P
-    double *const inverse = value + most;                                 // 1 / sum of what the draft left, a rejection each
-    Node *const node = (Node *)(inverse + most);
-    int32_t *const parent = (int32_t *)(node + most);
-    uint32_t *const gone = (uint32_t *)(parent + most);                   // bits of the part's tokens
+    Node *const node = (Node *)(smem + sizeof(Shared));
+    double *const value = (double *)(node + most);                        // what is left of a child's weight
+    double *const taken = value + most;                                   // sums in front of the rejections: each takes the draft's share of its one from every weight
+    int32_t *const parent = (int32_t *)(taken + most);
+    uint32_t *const gone = (uint32_t *)(parent + most);                   // bits of the CTA's places
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank();
-    const uint32_t first = (rank * WARPS + warp) * part, last = min(first + part, a.vocab);  // the warp's tokens
-    const uint32_t part0 = rank * WARPS * part, part_words = WARPS * part / 32;
+    const uint32_t me = rank * WARPS + warp, warps = ctas * WARPS;        // of the cluster's warps
+    const uint32_t first = me * part, part0 = rank * WARPS * part;        // the warp's places, the CTA's
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (tid < 16) sh.root[tid] = exp2((double)tid / 16.0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     uint32_t set = 0;
     const bool fits = *a.stamped == a.stamp;
     if (!fits && blockIdx.x == 0 && tid == 0 && a.status) atomicOr(a.status, (int)PAGED_STATUS_PLAN);
 
-    // ---- what the CTAs exchange
-    auto warp_sum = [&](double s) {
+    auto warp_sum = [&](auto s) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         return s;
     };
-    // The sum over the cluster of the threads' sums, in the ranks' order; warp_sum[] keeps the warps'
-    auto exchange_sum = [&](double s, double *before_rank = nullptr) -> double {
-        s = warp_sum(s);
-        if (lane == 0) sh.warp_sum[warp] = s;
-        __syncthreads();
-        if (warp == 0 && lane < ctas) {
-            double t = 0.0;
-            for (uint32_t w = 0; w < WARPS; w++) t += sh.warp_sum[w];
-            put(of_rank(&sh.ex.sum[set][rank], lane), t);
+    // Where running sums over the lanes' parts, `front` in front of them, pass `goal`: the part (32: none has a weight) and the sum in front of it. Where none does, by a rounding, it is the
+    // last part with a weight.
+    auto place_of = [&](double own, double front, double goal, double &before) -> uint32_t {
+        double inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
         }
-        cluster_sync();
-        double all = 0.0;
-        for (uint32_t c = 0; c < ctas; c++) {
-            if (before_rank) before_rank[c] = all;
-            all += sh.ex.sum[set][c];
-        }
-        set ^= 1;
-        return all;
+        const uint32_t some = __ballot_sync(0xffffffffu, own > 0.0), past = __ballot_sync(0xffffffffu, own > 0.0 && front + inc > goal);
+        if (!some) return 32;
+        const uint32_t at = past ? __ffs(past) - 1 : 31 - __clz(some);
+        before = __shfl_sync(0xffffffffu, front + (inc - own), at);
+        return at;
     };
 
-    cluster_sync();  // (all of them are there: their memory may be written)
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all of them are there: their memory may be written
+    __syncthreads();
     const uint32_t clusters = gridDim.x / ctas;
     for (uint32_t r = blockIdx.x / ctas; r < a.s.requests; r += clusters) {
         const uint4 rec = ((const uint4 *)a.request)[r];
-        const uint32_t q0 = rec.x;
-        if (rank == 0) {
-            const uint32_t n = fits ? min(rec.y - rec.x, most) : 0;
-            const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-            for (uint32_t t = tid; t < n; t += THREADS) {
-                const int32_t p = a.parents ? a.parents[q0 + t] : (int32_t)t - 1;
-                for (uint32_t c = 0; c < ctas; c++) put(of_rank(parent + t, c), (uint32_t)p);
-            }
-            if (tid < ctas) put(of_rank(&sh.n, tid), n), put(of_rank(&sh.temperature, tid), temperature);
-        }
-        cluster_sync();
-        const uint32_t n = sh.n;
-        const float temperature = sh.temperature;
-        const bool cold = !(temperature > 0.0f);
-        const double inv_t = cold ? 0.0 : 1.0 / (double)temperature;
-        uint32_t v = 0, length = n ? 1 : 0;
+        // (what decides is rank 0's; where the others' own differ, since the caller writes them meanwhile, only numbers do)
+        const float own_temperature = a.temperature ? a.temperature[r] : 1.0f;
+        const uint32_t q0 = rec.x, own_n = fits ? min(rec.y - rec.x, most) : 0;
+        uint32_t n = own_n;
+        bool cold = !(own_temperature > 0.0f);
+        float temperature = own_temperature;
+        uint32_t v = 0, length = 0;
         int32_t answer = -1;
-        if (n && rank == 0 && tid == 0) a.path[(size_t)r * most] = 0;
-        while (n) {
-            // ---- rank 0 fetches what the children's tests need
-            const char *const row = (const char *)a.logits + (q0 + v) * a.logits_row * act_elem_bytes(SRC);
+        for (;;) {  // a level
+            const char *const start = (const char *)a.logits + (q0 + v) * a.logits_row * EB;
+            const uint32_t from = (uint32_t)((uintptr_t)start & 15) / EB, end = from + a.vocab, last = own_n ? min(first + part, end) : 0u;
+            const char *const row = start - from * EB;
             const float *const draft = a.draft ? a.draft + (q0 + v) * a.draft_row : nullptr;
-            if (rank == 0) {
-                for (uint32_t t = v + 1 + tid; t < n; t += THREADS) {
-                    if (parent[t] != (int32_t)v) continue;
-                    Node x{a.tokens[q0 + t], a.accept[q0 + t], 0.0f, 0.0f};
-                    if ((uint32_t)x.token < a.vocab) {
-                        x.logit = load_act(row, (uint32_t)x.token, SRC);
-                        if (draft) x.draft = draft[x.token];
-                    } else {
-                        if (a.status) atomicOr(a.status, (int)PAGED_STATUS_INDEX);
-                        x.token = -1;  // (never accepted)
-                    }
-                    for (uint32_t c = 0; c < ctas; c++) {
-                        const uint32_t to = of_rank(node + t, c);
-                        put(to, (uint32_t)x.token), put(to + 4, x.accept), put(to + 8, x.logit), put(to + 12, x.draft);
-                    }
-                }
-            }
-            // ---- the largest logit and the sum of the weights
-            float top = -INFINITY;
-            uint32_t at = ~0u;
-            double sum = 0.0;
-            for (uint32_t i0 = first + lane * E; i0 < last; i0 += 32 * E * UNROLL) {
-                float x[UNROLL][E];
+            const bool same = ((uintptr_t)(draft - from) & 15) == 0;
+            // ---- the largest logit, and the sum of the weights in 32 bits, relative to each thread's largest
+            float x[V][E];
+            auto fetch = [&](uint32_t c0) {
 #pragma unroll
-                for (int u = 0; u < UNROLL; u++) {
-                    const uint32_t i = i0 + 32 * E * u;
-                    if (i < last) load_row<SRC, E, VEC>(x[u], row, i, a.vocab, -INFINITY);
+                for (int u = 0; u < V; u++) {
+                    const uint32_t i = c0 + lane * E + 32 * E * u;
+                    if (i < last) load_row<SRC, E>(x[u], row, i, from, end, -INFINITY);
                     else
 #pragma unroll
                         for (int e = 0; e < E; e++) x[u][e] = -INFINITY;
                 }
-                const float was = top;
-#pragma unroll
-                for (int u = 0; u < UNROLL; u++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) better(top, at, x[u][e], i0 + 32 * E * u + e);
-                if (cold || top == -INFINITY) continue;
-                if (top != was) sum *= weight(was, top, inv_t);
-#pragma unroll
-                for (int u = 0; u < UNROLL; u++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) sum += weight(x[u][e], top, inv_t);
+            };
+            fetch(first);
+            // (meanwhile rank 0 fetches what the tests of the children need, a thread for a token)
+            if (rank == 0 && length == 0) {
+                for (uint32_t t = tid; t < n; t += THREADS) {
+                    const int32_t p = a.parents ? a.parents[q0 + t] : (int32_t)t - 1, token = a.tokens[q0 + t];
+                    const float accept = a.accept[q0 + t];
+                    parent[t] = p, node[t].token = token, node[t].accept = accept;
+                    for (uint32_t c = 1; c < ctas; c++) {
+                        put(of_rank(parent + t, c), (uint32_t)p);
+                        put(of_rank(node + t, c), (uint64_t)(uint32_t)token | (uint64_t)__float_as_uint(accept) << 32);
+                    }
+                }
+                if (tid < ctas) put(of_rank(&sh.n, tid), n), put(of_rank(&sh.temperature, tid), own_temperature);
             }
-            const float mine = top;
+            float child_logit = 0.0f, child_draft = 0.0f;
+            auto is_child = [&](uint32_t t) { return t > v && t < n && parent[t] == (int32_t)v; };
+            auto fetch_child = [&](uint32_t t) {
+                if (!is_child(t)) return;
+                const uint32_t token = (uint32_t)node[t].token;
+                if (token >= a.vocab) {
+                    if (a.status) atomicOr(a.status, (int)PAGED_STATUS_INDEX);
+                    return;
+                }
+                child_logit = load_act(start, token, SRC);
+                if (draft) child_draft = draft[token];
+            };
+            auto tell_child = [&](uint32_t t) {
+                if (!is_child(t)) return;
+                for (uint32_t c = 0; c < ctas; c++) put(of_rank(&node[t].logit, c), (uint64_t)__float_as_uint(child_logit) | (uint64_t)__float_as_uint(child_draft) << 32);
+            };
+            if (rank == 0) {
+                for (uint32_t t = tid + THREADS; t < n; t += THREADS) fetch_child(t), tell_child(t);
+                fetch_child(tid);
+            }
+            const float scale = fminf(1.44269504f / temperature, 3e38f);
+            float top = -INFINITY, sum = 0.0f;
+            uint32_t at = ~0u;
+            for (uint32_t c0 = first; c0 < last;) {
+                if (cold) {
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float t = __shfl_xor_sync(0xffffffffu, top, o);
-                better(top, at, t, __shfl_xor_sync(0xffffffffu, at, o));
+                    for (int u = 0; u < V; u++)
+                        if (c0 + 32 * E * u < last)
+#pragma unroll
+                            for (int e = 0; e < E; e++) better(top, at, x[u][e], c0 + lane * E + 32 * E * u + e);
+                } else {
+                    float largest[4] = {top, top, top, top};
+#pragma unroll
+                    for (int u = 0; u < V; u++)
+                        if (c0 + 32 * E * u < last)
+#pragma unroll
+                            for (int e = 0; e < E; e++) largest[e & 3] = max_nan(largest[e & 3], x[u][e]);
+                    const float was = top;
+                    top = max_nan(max_nan(largest[0], largest[1]), max_nan(largest[2], largest[3]));
+                    if (top != -INFINITY) {
+                        if (was != -INFINITY) sum *= exp2_fast((was - top) * scale);
+                        float s[4] = {};
+#pragma unroll
+                        for (int u = 0; u < V; u++)
+                            if (c0 + 32 * E * u < last)
+#pragma unroll
+                                for (int e = 0; e < E; e++) s[e & 3] += x[u][e] == -INFINITY ? 0.0f : exp2_fast((x[u][e] - top) * scale);
+                        sum += (s[0] + s[1]) + (s[2] + s[3]);
+                    }
+                }
+                c0 += 32 * FAST;
+                if (c0 < last) fetch(c0);
             }
-            sum = warp_sum(sum * weight(mine, top, inv_t));
-            if (lane == 0) sh.warp_top[warp] = top, sh.warp_at[warp] = at, sh.warp_sum[warp] = sum;
-            __syncthreads();
-            if (warp == 0 && lane < ctas) {
-                top = -INFINITY, at = ~0u;
-                for (uint32_t w = 0; w < WARPS; w++) better(top, at, sh.warp_top[w], sh.warp_at[w]);
-                sum = 0.0;
-                for (uint32_t w = 0; w < WARPS; w++) sum += sh.warp_sum[w] * weight(sh.warp_top[w], top, inv_t);
-                put(of_rank(&sh.ex.sum[set][rank], lane), sum);
-                put(of_rank(&sh.ex.top[set][rank], lane), top);
-                put(of_rank(&sh.ex.at[set][rank], lane), at);
+            {
+                const float mine = top;
+                uint64_t told;
+                top = unordered(__reduce_max_sync(0xffffffffu, ordered(top)));
+                if (cold) {
+                    at = __reduce_min_sync(0xffffffffu, mine == top ? at : ~0u);
+                    told = (uint64_t)ordered(top) << 32 | (uint32_t)~at;
+                } else {
+                    sum = warp_sum(mine == -INFINITY ? 0.0f : sum * exp2_fast((mine - top) * scale));
+                    told = (uint64_t)__float_as_uint(sum) << 32 | __float_as_uint(top);
+                }
+                if (lane < ctas) put(of_rank(&sh.quick[set][me], lane), told);
             }
+            if (rank == 0) tell_child(tid);
             cluster_sync();
-            top = -INFINITY, at = ~0u;
-            for (uint32_t c = 0; c < ctas; c++) better(top, at, sh.ex.top[set][c], sh.ex.at[set][c]);
-            double total = 0.0;
-            for (uint32_t c = 0; c < ctas; c++) total += sh.ex.sum[set][c] * weight(sh.ex.top[set][c], top, inv_t);
+            if (length == 0) {
+                n = sh.n;
+                temperature = sh.temperature;
+                cold = !(temperature > 0.0f);
+                if (n == 0) break;
+                if (rank == 0 && tid == 0) a.path[(size_t)r * most] = 0;
+                length = 1;
+            }
+            uint32_t best = 0;  // the token of the largest logit
+            if (cold) {
+                uint32_t hi = 0, lo = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < MOST_CTAS * WARPS / 32; k++) {
+                    const uint64_t q = lane + 32 * k < warps ? sh.quick[set][lane + 32 * k] : 0;
+                    if ((uint32_t)(q >> 32) > hi || ((uint32_t)(q >> 32) == hi && (uint32_t)q > lo)) hi = (uint32_t)(q >> 32), lo = (uint32_t)q;
+                }
+                const uint32_t most_hi = __reduce_max_sync(0xffffffffu, hi);
+                best = ~__reduce_max_sync(0xffffffffu, hi == most_hi ? lo : 0u) - from;
+                top = unordered(most_hi);
+            } else {
+                float mine = -INFINITY, tops[MOST_CTAS * WARPS / 32], parts_of[MOST_CTAS * WARPS / 32];
+#pragma unroll
+                for (uint32_t k = 0; k < MOST_CTAS * WARPS / 32; k++) {
+                    const uint64_t q = lane + 32 * k < warps ? sh.quick[set][lane + 32 * k] : 0x00000000ff800000ull;
+                    tops[k] = __uint_as_float((uint32_t)q), parts_of[k] = __uint_as_float((uint32_t)(q >> 32));
+                    mine = max_nan(mine, tops[k]);
+                }
+                top = unordered(__reduce_max_sync(0xffffffffu, ordered(mine)));
+                sum = 0.0f;
+#pragma unroll
+                for (uint32_t k = 0; k < MOST_CTAS * WARPS / 32; k++) sum = fmaf(parts_of[k], tops[k] == -INFINITY ? 0.0f : exp2_fast((tops[k] - top) * scale), sum);
+                sum = warp_sum(sum);
+            }
             set ^= 1;
             if (!(top < INFINITY) || top == -INFINITY) {  // NaN, +inf, or nothing at all
                 if (rank == 0 && tid == 0 && a.status) atomicOr(a.status, (int)PAGED_STATUS_LOGITS);
                 break;
             }
             // ---- the children
-            const double inv_total = 1.0 / total;
-            for (uint32_t t = v + 1 + tid; t < n; t += THREADS)
-                if (parent[t] == (int32_t)v) {
-                    const Node x = node[t];
-                    value[t] = x.token < 0 ? 0.0 : cold ? ((uint32_t)x.token == at ? 1.0 : 0.0) : weight(x.logit, top, inv_t) * (draft ? inv_total : 1.0);
-                }
-            if (!draft && !cold)
-                for (uint32_t i = tid; i < part_words; i += THREADS) gone[i] = 0;
-            __syncthreads();
-            uint32_t next = 0, stages = 0;  // the accepted child (0: none), rejections that took something
-            double rest = total;            // without a draft: what the distribution's weights add up to
-            // what is left of a token with weight w and draft probability d
-            auto left = [&](double w, double d) {
-                w *= inv_total;
-                for (uint32_t k = 0; k < stages; k++) w = fmax(w - d, 0.0) * inverse[k];
-                return w;
-            };
-            // f(token, weight left) over the warp's tokens, in their order within a thread
-            auto over = [&](auto &&f) {
-                for (uint32_t i = first + lane * E; i < last; i += 32 * E) {
-                    float x[E], d[E];
-                    load_row<SRC, E, VEC>(x, row, i, a.vocab, -INFINITY);
-                    if (draft) load_row<ACT_F32, E, VEC>(d, draft, i, a.vocab, 0.0f);
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        double w = weight(x[e], top, inv_t);
-                        if (draft) w = left(w, (double)d[e]);
-                        else if (gone[(i + e - part0) >> 5] >> ((i + e) & 31) & 1) w = 0.0;
-                        f(w, draft ? (double)d[e] : 0.0);
-                    }
-                }
-            };
-            for (uint32_t t = v + 1; t < n && !next; t++) {
-                if (parent[t] != (int32_t)v) continue;
-                const Node x = node[t];
-                if (x.token < 0) continue;
+            uint32_t next = 0, stages = 0;       // the accepted child (0: none), rejections that took something
+            bool exact = false, parts = false;   // in 64 bits from here on; the last exchange's sums are those of what is left
+            double rest = (double)sum;           // what the distribution's weights add up to,
+            double full = rest, unsure = SURE;   // and did before tokens left it; how far off that may be
+            Weight weight(sh.root, top);
+            uint32_t t = v + 1;
+            for (;;) {
+                while (t < n && (parent[t] != (int32_t)v || (uint32_t)node[t].token >= a.vocab)) t++;
                 if (cold) {
-                    if ((uint32_t)x.token == at) next = t;
-                } else if (draft) {
-                    if ((double)x.accept * (double)x.draft < value[t]) {
+                    if (t == n) break;
+                    if ((uint32_t)node[t].token == best) {
                         next = t;
-                    } else {
-                        double s = 0.0;
-                        over([&](double w, double d) { s += fmax(w - d, 0.0); });
-                        s = exchange_sum(s);
-                        if (s > 0.0) {  // (else nothing is left, and the distribution stays)
-                            const double inv = 1.0 / s;
-                            for (uint32_t j = t + 1 + tid; j < n; j += THREADS)
-                                if (parent[j] == (int32_t)v) value[j] = fmax(value[j] - (double)node[j].draft, 0.0) * inv;
-                            if (tid == 0) inverse[stages] = inv;
-                            stages++;
-                            __syncthreads();
-                        }
+                        break;
                     }
-                } else {
-                    if ((double)x.accept * rest < value[t]) {
-                        next = t;
-                    } else if (value[t] > 0.0) {
-                        __syncthreads();  // (value[] has been read)
-                        for (uint32_t j = t + tid; j < n; j += THREADS)
-                            if (parent[j] == (int32_t)v && node[j].token == x.token) value[j] = 0.0;
-                        const uint32_t bit = (uint32_t)x.token - part0;
-                        if (tid == 0 && (uint32_t)x.token >= part0 && bit < WARPS * part) gone[bit >> 5] |= 1u << (bit & 31);
-                        __syncthreads();
-                        rest -= weight(x.logit, top, inv_t);
-                        if (!(rest > total * 0x1p-10)) {  // what is left was lost in the difference: add it up
-                            double s = 0.0;
-                            over([&](double w, double) { s += w; });
-                            rest = exchange_sum(s);
-                        }
-                    }
+                    t++;
+                    continue;
                 }
+                if (!exact) {
+                    if (t < n) {  // most children's tests need no more than 32 bits
+                        const Node y = node[t];
+                        const float line = (draft ? y.accept * y.draft : y.accept) * sum, mine = y.logit == -INFINITY ? 0.0f : exp2_fast((y.logit - top) * scale);
+                        if (mine - line > fmaxf(mine * (float)SURE, 1e-30f)) {
+                            next = t;
+                            break;
+                        }
+                    }
+                    exact = true;
+                    weight.set(temperature);
+                    for (uint32_t k = v + 1 + tid; k < n; k += THREADS)
+                        if (parent[k] == (int32_t)v) value[k] = weight(node[k].logit);
+                    if (!draft)
+                        for (uint32_t i = tid; i < WARPS * part / 32; i += THREADS) gone[i] = 0;
+                    __syncthreads();
+                }
+                // the child's test; what is to be added up next: nothing (the next child), what is left, or what the draft leaves of that
+                bool minus = false, again = false;
+                if (t < n) {
+                    const Node y = node[t];
+                    const double u = draft ? (double)y.accept * (double)y.draft : (double)y.accept, line = u * rest, mine = value[t];
+                    again = unsure != 0.0 && !(fabs(line - mine) > fabs(u) * full * SURE);
+                    if (!again) {
+                        if (line < mine) {
+                            next = t;
+                            break;
+                        }
+                        if (draft) {
+                            again = unsure != 0.0;  // (what it leaves depends on the sum)
+                            minus = !again;
+                        } else {
+                            t++;
+                            if (!(mine > 0.0)) continue;
+                            __syncthreads();  // (value[] has been read)
+                            for (uint32_t k = t - 1 + tid; k < n; k += THREADS)
+                                if (parent[k] == (int32_t)v && node[k].token == y.token) value[k] = 0.0;
+                            const uint32_t bit = (uint32_t)y.token + from - part0;
+                            if (tid == 0 && bit < WARPS * part) gone[bit >> 5] |= 1u << (bit & 31);
+                            __syncthreads();
+                            rest -= weight(y.logit);
+                            if (rest > full * 0x1p-10) continue;
+                            again = true;  // what is left was lost in the difference
+                        }
+                    }
+                } else if (parts) {
+                    break;
+                }
+                double s2[2] = {};
+#pragma unroll 1
+                for (uint32_t i0 = first + lane * E; i0 < last; i0 += 32 * BATCH) {
+                    float z[U][E], d[U][E];
+                    double w[BATCH];
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const uint32_t i = i0 + 32 * E * u;
+#pragma unroll
+                        for (int e = 0; e < E; e++) z[u][e] = -INFINITY, d[u][e] = 0.0f;
+                        if (i >= last) continue;
+                        load_row<SRC, E>(z[u], row, i, from, end, -INFINITY);
+                        if (draft && (stages || minus)) {
+                            if (same) load_row<ACT_F32, E>(d[u], draft - from, i, from, end, 0.0f);
+                            else load_apart<E>(d[u], draft, i, from, end);
+                        }
+                    }
+                    if (!draft)
+#pragma unroll
+                        for (int u = 0; u < U; u++) {
+                            const uint32_t i = i0 + 32 * E * u, bits = i < last ? gone[(i - part0) >> 5] >> (i & 31) : 0u;
+                            if (bits & ((1u << E) - 1))
+#pragma unroll
+                                for (int e = 0; e < E; e++) z[u][e] = bits >> e & 1 ? -INFINITY : z[u][e];
+                        }
+#pragma unroll
+                    for (int e = 0; e < (int)BATCH; e++) w[e] = weight(z[e / E][e % E]);
+                    for (uint32_t k = 0; k < stages; k++) {
+                        const double share = -taken[k];
+#pragma unroll
+                        for (int e = 0; e < (int)BATCH; e++) w[e] = positive(fma((double)d[e / E][e % E], share, w[e]));
+                    }
+                    if (minus) {
+#pragma unroll
+                        for (int e = 0; e < (int)BATCH; e++) w[e] = positive(fma((double)d[e / E][e % E], -rest, w[e]));
+                    }
+#pragma unroll
+                    for (int e = 0; e < (int)BATCH; e++) s2[e & 1] += w[e];
+                }
+                const double own = warp_sum(s2[0] + s2[1]);
+                if (lane < ctas) put(of_rank(&sh.sum[set][me], lane), own);
+                cluster_sync();
+                double left2[2] = {};
+#pragma unroll
+                for (uint32_t k = 0; k < MOST_CTAS * WARPS / 32; k++) left2[k & 1] += lane + 32 * k < warps ? sh.sum[set][lane + 32 * k] : 0.0;
+                const double left = warp_sum(left2[0] + left2[1]);
+                set ^= 1;
+                if (minus) {
+                    t++;
+                    parts = left > 0.0;
+                    if (!parts) continue;  // (nothing is left, and the distribution stays)
+                    for (uint32_t k = t + tid; k < n; k += THREADS)
+                        if (parent[k] == (int32_t)v) value[k] = positive(fma((double)node[k].draft, -rest, value[k]));
+                    if (tid == 0) taken[stages] = rest;
+                    stages++;
+                    rest = left;
+                    __syncthreads();
+                    continue;
+                }
+                rest = full = left;
+                unsure = 0.0;
+                if (!again) break;
             }
             if (next) {
                 if (rank == 0 && tid == 0) a.path[(size_t)r * most + length] = (int32_t)next;
@@ -329,72 +484,77 @@ template <int SRC, bool VEC> __global__ void __launch_bounds__(THREADS, 2) paged
             }
             // ---- no child: the token behind the path
             if (cold) {
-                answer = (int32_t)at;
+                answer = (int32_t)best;
                 break;
             }
-            double s = 0.0, before[MOST_CTAS];
-            over([&](double w, double) { s += w; });
-            const double all = exchange_sum(s, before);
-            const double goal = (double)a.pick[r] * all;
-            uint32_t who = ctas;
-            for (uint32_t c = 0; c < ctas; c++) {
-                const double own = sh.ex.sum[set ^ 1][c];
-                if (own > 0.0 && (who == ctas || !(before[who] + sh.ex.sum[set ^ 1][who] > goal))) who = c;
-            }
-            if (who == rank) {
-                double front = before[rank];
-                uint32_t w = WARPS;
-                double w_front = front;
-                for (uint32_t i = 0; i < WARPS; i++) {
-                    const double own = sh.warp_sum[i];
-                    if (own > 0.0 && (w == WARPS || !(w_front + sh.warp_sum[w] > goal))) w = i, w_front = front;
-                    front += own;
+            // the warp whose tokens the number falls among, from the warps' sums (a lane has some behind each other); its lanes' tokens, then
+            const double goal = (double)a.pick[r] * rest;
+            const double *const sums = sh.sum[set ^ 1];
+            const uint32_t each = (warps + 31) / 32;
+            double before = 0.0, mine = 0.0;
+            for (uint32_t k = 0; k < each; k++) mine += lane * each + k < warps ? sums[lane * each + k] : 0.0;
+            uint32_t who = place_of(mine, 0.0, goal, before);
+            answer = who < 32 ? -2 : -1;  // (-2: written by that warp)
+            if (who < 32) {
+                const uint32_t begin = who * each;
+                double run = before;
+                who = begin;
+                for (uint32_t k = begin; k < min(begin + each, warps); k++) {
+                    if (sums[k] > 0.0) who = k, before = run;
+                    run += sums[k];
+                    if (sums[k] > 0.0 && run > goal) break;
                 }
-                if (w == warp) {
-                    double run = w_front;
-                    uint32_t found = ~0u, some = ~0u;  // the first past the goal, the last with a weight
-                    for (uint32_t i0 = first; i0 < last && found == ~0u; i0 += 32 * E) {
-                        const uint32_t i = i0 + lane * E;
-                        float x[E], d[E];
-                        double wt[E], mine = 0.0;
+                if (who == me) {
+                    uint32_t token = 0;
+                    bool found = false;
+#pragma unroll 1
+                    for (uint32_t c0 = first; c0 < last && !found; c0 += 32 * BATCH) {  // a lane has BATCH tokens behind each other
+                        const uint32_t i0 = c0 + lane * BATCH;
+                        float z[U][E], d[U][E];
+                        double wt[BATCH], own = 0.0;
 #pragma unroll
-                        for (int e = 0; e < E; e++) x[e] = -INFINITY, d[e] = 0.0f;
-                        if (i < last) {
-                            load_row<SRC, E, VEC>(x, row, i, a.vocab, -INFINITY);
-                            if (draft) load_row<ACT_F32, E, VEC>(d, draft, i, a.vocab, 0.0f);
-                        }
+                        for (int u = 0; u < U; u++) {
+                            const uint32_t i = i0 + E * u;
 #pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            wt[e] = weight(x[e], top, inv_t);
-                            if (draft) wt[e] = left(wt[e], (double)d[e]);
-                            else if (i < last && gone[(i + e - part0) >> 5] >> ((i + e) & 31) & 1) wt[e] = 0.0;
-                            mine += wt[e];
-                        }
-                        double inc = mine;
+                            for (int e = 0; e < E; e++) z[u][e] = -INFINITY, d[u][e] = 0.0f;
+                            if (i >= last) continue;
+                            load_row<SRC, E>(z[u], row, i, from, end, -INFINITY);
+                            if (!draft) {
+                                const uint32_t bits = gone[(i - part0) >> 5] >> (i & 31);
 #pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const double y = __shfl_up_sync(0xffffffffu, inc, o);
-                            if (lane >= o) inc += y;
-                        }
-                        double c = run + (inc - mine);
-                        uint32_t hit = ~0u, pos = ~0u;
-#pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            c += wt[e];
-                            if (wt[e] > 0.0) {
-                                pos = i + e;
-                                if (hit == ~0u && c > goal) hit = i + e;
+                                for (int e = 0; e < E; e++) z[u][e] = bits >> e & 1 ? -INFINITY : z[u][e];
+                            } else if (stages) {
+                                if (same) load_row<ACT_F32, E>(d[u], draft - from, i, from, end, 0.0f);
+                                else load_apart<E>(d[u], draft, i, from, end);
                             }
                         }
-                        found = __reduce_min_sync(0xffffffffu, hit);
-                        const uint32_t any = __ballot_sync(0xffffffffu, pos != ~0u);
-                        if (any) some = __shfl_sync(0xffffffffu, pos, 31 - __clz(any));
-                        run += __shfl_sync(0xffffffffu, inc, 31);
+#pragma unroll
+                        for (int e = 0; e < (int)BATCH; e++) wt[e] = weight(z[e / E][e % E]);
+                        for (uint32_t k = 0; k < stages; k++) {
+                            const double share = -taken[k];
+#pragma unroll
+                            for (int e = 0; e < (int)BATCH; e++) wt[e] = positive(fma((double)d[e / E][e % E], share, wt[e]));
+                        }
+#pragma unroll
+                        for (int e = 0; e < (int)BATCH; e++) own += wt[e];
+                        const uint32_t l = place_of(own, before, goal, before);
+                        if (l == 32) continue;
+                        // (the lane's first token past the goal, else its last one with a weight)
+                        double past_sum = before;
+                        uint32_t at_last = 0;
+                        bool past = false;
+#pragma unroll
+                        for (int e = 0; e < (int)BATCH; e++) {
+                            past_sum += wt[e];
+                            if (wt[e] > 0.0 && !past) at_last = i0 + e, past = past_sum > goal;
+                        }
+                        token = __shfl_sync(0xffffffffu, at_last, l);
+                        before = __shfl_sync(0xffffffffu, past_sum, l);
+                        found = __shfl_sync(0xffffffffu, (int)past, l);
                     }
-                    if (lane == 0) a.next[r] = (int32_t)(found != ~0u ? found : some);
+                    if (lane == 0) a.next[r] = (int32_t)(token - from);
                 }
             }
-            answer = who < ctas ? -2 : -1;  // (written by that CTA)
             break;
         }
         if (rank == 0) {
@@ -410,23 +570,30 @@ template <int SRC, bool VEC> __global__ void __launch_bounds__(THREADS, 2) paged
 
 }  // namespace pv
 
-template <int SRC, bool VEC> static cudaError_t verify_launch(const PagedVerifyArgs &a, uint32_t ctas, int sm_count, bool pdl, cudaStream_t stream) {
-    auto *kernel = pv::paged_verify_kernel<SRC, VEC>;
-    constexpr uint32_t E = SRC == ACT_F32 ? 4 : 8, unit = 32 * E;
-    const uint32_t warps = ctas * pv::WARPS, part = ((a.vocab + warps - 1) / warps + unit - 1) / unit * unit;
-    const size_t smem = pv::shared_bytes(a.s.max_new, part);
+// A warp's places with so many CTAs a request, whole vectors of all its lanes
+static uint32_t verify_part(const PagedVerifyArgs &a, uint32_t ctas) {
+    const uint32_t E = 16 / act_elem_bytes(a.type), unit = 32 * E, warps = ctas * pv::WARPS, places = a.vocab + E - 1;  // (a row may begin inside a vector)
+    return ((places + warps - 1) / warps + unit - 1) / unit * unit;
+}
+
+template <int SRC> static cudaError_t verify_launch(const PagedVerifyArgs &a, uint32_t ctas, int sm_count, bool pdl, cudaStream_t stream) {
+    auto *kernel = pv::paged_verify_kernel<SRC>;
     static std::once_flag once[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    std::call_once(once[dev & 63], [&] { e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pv::shared_bytes(PAGED_TREE_MOST, PAGED_VERIFY_VOCAB / pv::WARPS / pv::MOST_CTAS)); });
+    std::call_once(once[dev & 63], [&] {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pv::SMEM_MOST);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    });
     if (e != cudaSuccess) return e;
+    const uint32_t part = verify_part(a, ctas);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    const uint32_t clusters = std::min<uint32_t>(a.s.requests, std::max<uint32_t>(1, 2 * (uint32_t)sm_count / ctas));
+    const uint32_t clusters = std::min<uint32_t>(a.s.requests, std::max<uint32_t>(1, (uint32_t)sm_count / ctas));
     cfg.gridDim = dim3(clusters * ctas);
     cfg.blockDim = dim3(pv::THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = pv::shared_bytes(a.s.max_new, part);
     cfg.stream = stream;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ctas;
@@ -439,14 +606,14 @@ template <int SRC, bool VEC> static cudaError_t verify_launch(const PagedVerifyA
 }
 
 cudaError_t launch_paged_verify(const PagedVerifyArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
-    const uint32_t eb = act_elem_bytes(a.type);
-    const bool vec = (uintptr_t)a.logits % 16 == 0 && a.logits_row * eb % 16 == 0 && (!a.draft || ((uintptr_t)a.draft % 16 == 0 && a.draft_row % 4 == 0));
-    const uint32_t ctas = pv::MOST_CTAS;
-    auto run = [&](auto src) {
-        constexpr int S = decltype(src)::value;
-        return vec ? verify_launch<S, true>(a, ctas, sm_count, pdl, stream) : verify_launch<S, false>(a, ctas, sm_count, pdl, stream);
-    };
-    return a.type == ACT_F32 ? run(std::integral_constant<int, ACT_F32>()) : a.type == ACT_F16 ? run(std::integral_constant<int, ACT_F16>()) : run(std::integral_constant<int, ACT_BF16>());
+    // As many CTAs a request as leave a warp 500 tokens, and no more than two for each SM in all: one chain over 128256 tokens with 4, 8, 16 CTAs 41.0, 28.5, 25.0 us; 16 trees over 32000 with 2, 4, 8 26.0, 21.9,
+    // 27.8; 64 trees over 128256 with 2, 4, 8 114, 110, 157
+    uint32_t ctas = pv::MOST_CTAS;
+    while (ctas > 1 && ((uint64_t)a.s.requests * ctas > 2 * (uint64_t)sm_count || a.vocab < 500 * pv::WARPS * ctas)) ctas /= 2;
+    while (ctas < pv::MOST_CTAS && verify_part(a, ctas) > pv::PART_MOST) ctas *= 2;
+    return a.type == ACT_F32   ? verify_launch<ACT_F32>(a, ctas, sm_count, pdl, stream)
+           : a.type == ACT_F16 ? verify_launch<ACT_F16>(a, ctas, sm_count, pdl, stream)
+                               : verify_launch<ACT_BF16>(a, ctas, sm_count, pdl, stream);
 }
 
 }  // namespace lb
