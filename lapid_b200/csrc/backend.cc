@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "paged.cuh"
 
 namespace {
 
@@ -2546,14 +2547,19 @@ static void paged_attention_impl(lapid_b200_device *dev, const lapid_b200_paged 
     a.lse = lse ? (float *)lse->ptr : nullptr;
     a.tree = tree ? (const uint32_t *)tree->ptr : nullptr;
     a.status = dev->status_dev;
-    // requests of many rows first: their CTAs run longest
-    if (lb::paged_has_large(a.s)) {
-        a.behind = true;
-        cuda_check(lb::launch_paged_attn_large(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
+    auto launched = [&](cudaError_t e) {
+        cuda_check(e, "paged_attention launch");
         dev->launches++;
+    };
+    // requests of many rows first: their CTAs run longest
+    const bool large = lb::paged_has_large(a.s);
+    if (large) launched(lb::launch_paged_attn_large(a, paged_sms(dev), dev->pdl, dev->stream));
+    if (large && a.s.tree) {  // (all requests are there)
+        if (lb::paged_joins_apart(a.s)) launched(lb::launch_paged_attn_join(a, paged_sms(dev), dev->pdl, dev->stream));
+        return;
     }
-    cuda_check(lb::launch_paged_attn_small(a, paged_sms(dev), dev->pdl, dev->stream), "paged_attention launch");
-    dev->launches++;
+    a.behind = large;
+    launched(lb::launch_paged_attn_small(a, paged_sms(dev), dev->pdl, dev->stream));
 }
 
 lapid_b200_status lapid_b200_paged_attention(lapid_b200_device *dev, const lapid_b200_paged *desc, lapid_b200_buffer *plan,

@@ -469,6 +469,7 @@ uint32_t paged_attn_small_ctas(int sm_count);
 uint32_t paged_attn_large_ctas(int sm_count);
 cudaError_t launch_paged_attn_small(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream);
 cudaError_t launch_paged_attn_large(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream);
+cudaError_t launch_paged_attn_join(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream);  // of a tree, behind it: tiles cut into many pieces
 
 // ---- paged_draft.cu, paged_verify.cu: drafted tokens over the paged cache
 constexpr uint32_t PAGED_TREE_MOST = 1024;  // new tokens of a request whose tokens are a tree, or are verified

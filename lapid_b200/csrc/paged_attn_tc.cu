@@ -75,7 +75,7 @@ template <int DP> struct Cfg {
     static constexpr int STAGE = HALVES * HALF;
     static constexpr int Q_BYTES = 2 * HALVES * Q_HALF;
     static constexpr int STAGES = (224 * 1024 - Q_BYTES) / (2 * STAGE);  // of keys, and as many of values
-    static constexpr int SMEM = Q_BYTES + 2 * STAGES * STAGE + 512 + 1024;
+    static constexpr int SMEM = Q_BYTES + 2 * STAGES * STAGE + 512 + 1024 + 2 * TILE * 4;
     // tensor memory: O of tile t at DP t, S at T_COL + T_STEP t, P behind it
     static constexpr int T_COL = 2 * DP, T_STEP = (512 - T_COL) / 2;
     static_assert(KEYS + KEYS / 2 <= T_STEP && KEYS % 16 == 0, "tensor memory");
@@ -410,6 +410,124 @@ template <int DP, bool BF16> __device__ __forceinline__ void join_pieces(const P
     }
 }
 
+// Drafted tokens are few rows over many keys: their tiles are cut into many pieces. From JOIN_APART of them on the CTAs only leave theirs in the plan, and the kernel below adds them up on all SMs: a tile of 256 rows
+// over 32768 keys is 18 pieces of 133 KB, which one CTA takes 40 us for (64 tokens over 32768 keys, 8 key heads: XX us, with the last CTA of a tile at it 75.7).
+constexpr uint32_t JOIN_APART = 4, JOIN_COLS = 8, JOIN_THREADS = 256;
+static_assert(JOIN_THREADS >= PAGED_MAX_SMS, "a thread for each end of a span");
+
+// Each CTA finds the cut tiles, a thread for the end of each span, and how many (32 rows, JOIN_COLS columns) they have; its warps take every so many of these.
+template <int DP, bool BF16> __global__ void __launch_bounds__(JOIN_THREADS, 1) paged_attn_join_kernel(PagedAttnArgs p) {
+    constexpr uint32_t KEYS = Cfg<DP>::KEYS, PF = ROWS * (DP + 2), PER = DP / JOIN_COLS;  // column groups of a row
+    constexpr int B = 8;  // pieces in flight
+    __shared__ uint32_t ends[JOIN_THREADS], sums[JOIN_THREADS / 32];
+    struct Found {
+        uint32_t first, last, q0, n, head, tile;
+    };
+    __shared__ Found found[JOIN_THREADS];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const PagedShape &s = p.s;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t *const starts = p.plan + p.l.start_large;
+    const uint32_t ctas = starts[0] == p.stamp ? starts[2] : 0u;
+    uint32_t mine = 0;
+    if (tid + 1 < ctas) {
+        const PagedStart at = paged_load_start(starts + (tid + 1) * (sizeof(PagedStart) / 4));
+        const uint32_t i0 = at.u0 - at.place;  // where the tile begins that goes on behind the span of CTA `tid`: is it its first?
+        if (at.place && i0 >= paged_span(at.units, ctas, tid)) {
+            const uint32_t token0 = 2 * at.tile * s.tt, tokens = min(2 * s.tt, at.n - token0);
+            const PagedTile tile = paged_tile_of(s, at.n, at.kv, token0, token0 + tokens - 1, KEYS);
+            const uint32_t first = paged_holder(at.units, ctas, i0 + PAGED_LARGE_EXTRA), last = paged_holder(at.units, ctas, i0 + PAGED_LARGE_EXTRA + tile.steps - 1);
+            if (last - first + 1 >= JOIN_APART) {
+                const uint32_t a = min(tokens, s.tt) * s.g, b = (tokens > s.tt ? tokens - s.tt : 0u) * s.g;
+                mine = ((a + 31) / 32 + (b + 31) / 32) * PER;
+                found[tid] = Found{first, last, at.q0, at.n, at.head, at.tile};
+            }
+        }
+    }
+    uint32_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+    }
+    if (lane == 31) sums[warp] = inc;
+    __syncthreads();
+    for (uint32_t w = 0; w < warp; w++) inc += sums[w];
+    ends[tid] = inc;
+    __syncthreads();
+    const uint32_t total = ends[JOIN_THREADS - 1];
+    const float *const parts = (const float *)((const uint8_t *)p.plan + p.l.part_large);
+    for (uint32_t item = blockIdx.x * (JOIN_THREADS / 32) + warp; item < total; item += gridDim.x * (JOIN_THREADS / 32)) {
+        uint32_t lo = 0, hi = JOIN_THREADS - 1;  // the first end above the item
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (ends[mid] > item) hi = mid;
+            else lo = mid + 1;
+        }
+        const Found at = found[lo];
+        const uint32_t first = at.first, last = at.last, local_item = item - (lo ? ends[lo - 1] : 0u), tile0 = 2 * at.tile * s.tt;
+        uint32_t group = local_item / PER;
+        const uint32_t col = (local_item - group * PER) * JOIN_COLS, groups0 = (min(s.tt, at.n - tile0) * s.g + 31) / 32, t = group >= groups0 ? 1 : 0;
+        group -= t * groups0;
+        const uint32_t token0 = tile0 + t * s.tt, rows = min(s.tt, at.n - token0) * s.g, r = 32 * group + lane, row = t * TILE + r;
+        if (r < rows && col < s.d) {
+            float mm = -INFINITY, ll = 0.0f, v[JOIN_COLS];
+#pragma unroll
+            for (int e = 0; e < (int)JOIN_COLS; e++) v[e] = 0.0f;
+#pragma unroll 1
+            for (uint32_t i = first; i <= last; i += B) {
+                float m[B], l[B];
+                float4 y[B][JOIN_COLS / 4];
+#pragma unroll
+                for (uint32_t k = 0; k < B; k++) {
+                    const float *src = parts + (size_t)(2 * min(i + k, last) + (i + k == first ? 1 : 0)) * PF;  // (the last one again where there are no more, with the weight 0)
+                    m[k] = __ldcg(src + DP * ROWS + row);
+                    l[k] = __ldcg(src + (DP + 1) * ROWS + row);
+#pragma unroll
+                    for (uint32_t e = 0; e < JOIN_COLS / 4; e++) y[k][e] = __ldcg((const float4 *)src + (col / 4 + e) * ROWS + row);
+                }
+#pragma unroll
+                for (uint32_t k = 1; k < B; k++)
+                    if (i + k > last) m[k] = -INFINITY;
+                float top = mm;
+#pragma unroll
+                for (uint32_t k = 0; k < B; k++) top = fmaxf(top, m[k]);
+                const float base = top == -INFINITY ? 0.0f : top, keep = exp2_fast(mm - base);
+                mm = top;
+                ll *= keep;
+#pragma unroll
+                for (int e = 0; e < (int)JOIN_COLS; e++) v[e] *= keep;
+#pragma unroll
+                for (uint32_t k = 0; k < B; k++) {
+                    const float f = exp2_fast(m[k] - base);
+                    ll = fmaf(l[k], f, ll);
+#pragma unroll
+                    for (uint32_t e = 0; e < JOIN_COLS / 4; e++) {
+                        v[4 * e] = fmaf(y[k][e].x, f, v[4 * e]);
+                        v[4 * e + 1] = fmaf(y[k][e].y, f, v[4 * e + 1]);
+                        v[4 * e + 2] = fmaf(y[k][e].z, f, v[4 * e + 2]);
+                        v[4 * e + 3] = fmaf(y[k][e].w, f, v[4 * e + 3]);
+                    }
+                }
+            }
+            const float il = ll == 0.0f ? 0.0f : 1.0f / ll;
+            const uint32_t local = r / s.g, qh = at.head * s.g + (r - local * s.g);
+            const uint64_t token = at.q0 + token0 + local;
+            unsigned short *const to = (unsigned short *)p.out + p.ov.off + token * p.ov.token + (uint64_t)qh * p.ov.head + col;
+            const uint4 z = make_uint4(pack<BF16>(v[0] * il, v[1] * il), pack<BF16>(v[2] * il, v[3] * il), pack<BF16>(v[4] * il, v[5] * il), pack<BF16>(v[6] * il, v[7] * il));
+            if (((uintptr_t)to & 15) == 0) {
+                *(uint4 *)to = z;
+            } else {
+                const uint32_t w[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) to[2 * e] = (unsigned short)w[e], to[2 * e + 1] = (unsigned short)(w[e] >> 16);
+            }
+            if (p.lse && col == 0) p.lse[token * s.hq + qh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+        }
+    }
+}
+
 // TREE: the new tokens are a request's drafted ones, and of those a token sees its ancestors and itself
 template <int DP, bool BF16, bool TREE>
 __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q, PagedAttnArgs p, bool q_boxes) {
@@ -423,6 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
     uint64_t *q_full = v_empty + C::STAGES, *q_empty = q_full + 2, *s_full = q_empty + 2, *ready = s_full + 2, *o_full = ready + 4, *drained = o_full + 2;
     uint32_t *tmem_slot = (uint32_t *)(drained + 2);
     volatile uint32_t *is_last = tmem_slot + 1;
+    float *const meet = (float *)(tmem_slot + 4);  // of a tree: m and l of the second stream's rows
     const PagedShape &s = p.s;
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -501,6 +620,66 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             while (work && healthy) {
                 Walk next = w;
                 const bool follows = next_piece<C::KEYS>(p, next);
+                const bool split = TREE && !w.two;  // both streams have the tile, t the steps t, t + 2, ..
+                if constexpr (TREE) {
+                    auto skip = [&](uint64_t *full, uint64_t *empty, uint32_t &st, uint32_t &ph) -> bool {  // a step of the other stream's
+                        if (!warp_wait(full + st, ph)) return false;
+                        if (lane == 0) mbar_arrive(empty + st);
+                        if (++st == C::STAGES) st = 0, ph ^= 1;
+                        return true;
+                    };
+                    auto skip_k = [&]() { return skip(k_full, k_empty, ks, kph); };
+                    auto skip_v = [&]() { return skip(v_full, v_empty, vs, vph); };
+                    if (split) {
+                        const uint32_t own = (w.steps + 1 - t) / 2, low = tile_low(p, w);
+                        if (!(healthy = warp_wait(q_full + t, piece & 1))) break;
+                        piece++;
+                        if (own == 0) {
+                            if (!(healthy = skip_k() && skip_v())) break;
+                            if (lane == 0) mbar_arrive(q_empty + t);
+                            w = next, work = follows;
+                            continue;
+                        }
+                        auto product = [&](uint32_t i) -> bool {  // the weights of its step i times the values
+                            if ((i || t) && !skip_v()) return false;
+                            if (!warp_wait(v_full + vs, vph)) return false;
+                            const uint32_t key0 = (w.t.first + w.step + 2 * i + t) * C::KEYS;
+                            if (key0 < low || key0 + C::KEYS > w.t.hi) {
+                                for (uint32_t e = lane; e < C::KEYS * (DP / 8); e += 32) {
+                                    const uint32_t key = e / (DP / 8), ch = e % (DP / 8);
+                                    if (key0 + key < low || key0 + key >= w.t.hi)
+                                        *(uint4 *)(v_ring + vs * C::STAGE + (ch / 8) * C::HALF + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                                }
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                                __syncwarp();
+                            }
+                            return true;
+                        };
+                        if (!(healthy = (t == 0 || skip_k()) && warp_wait(k_full + ks, kph))) break;
+                        fence_after();
+                        scores(own == 1);
+                        for (uint32_t i = 0; i <= own; i++) {  // event i, as below
+                            const bool more = i + 1 < own;
+                            if (!(healthy = (!more || (skip_k() && warp_wait(k_full + ks, kph))) && (!i || product(i - 1)) && warp_wait(ready + 2 * (events & 1) + t, (events >> 1) & 1))) break;
+                            events++;
+                            fence_after();
+                            if (more) scores(i + 2 == own);
+                            if (i && elect_one()) {
+                                const uint64_t vd = desc_t(s32(v_ring) + vs * C::STAGE, C::HALF);
+#pragma unroll
+                                for (int e = 0; e < C::KEYS / 16; e++) mma_ts(o_col, p_col + 8 * e, vd + e * (2048 >> 4), idesc_o, (i > 1 || e) ? 1u : 0u);
+                                commit(o_full + t);
+                                commit(v_empty + vs);
+                            }
+                            __syncwarp();
+                            if (i && ++vs == C::STAGES) vs = 0, vph ^= 1;
+                        }
+                        if (!healthy) break;
+                        if (((w.steps - 1) & 1) != t && !(healthy = skip_k() && skip_v())) break;  // (the last step is the other's)
+                        w = next, work = follows;
+                        continue;
+                    }
+                }
                 if (t == 1 && !w.two) {  // the other tile's alone
                     for (uint32_t j = 0; j < w.steps && healthy; j++) {
                         if (!(healthy = warp_wait(k_full + ks, kph) && warp_wait(v_full + vs, vph))) break;
@@ -511,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                     w = next, work = follows;
                     continue;
                 }
-                const bool next_mine = follows && (t == 0 || next.two);
+                const bool next_mine = follows && (TREE ? next.two : t == 0 || next.two);  // (of a tree: a tile that both streams have begins when it is come to)
                 const uint32_t low = tile_low(p, w);
                 if (!begun) {
                     if (!(healthy = warp_wait(k_full + ks, kph) && warp_wait(q_full + t, piece & 1))) break;
@@ -599,10 +778,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             const uint32_t tile_rows = s.tt * s.g;
             const bool vec = ((uintptr_t)p.q & 15) == 0 && ((p.qv.off | p.qv.head | p.qv.token) & 7) == 0;
             auto load_q = [&]() {
-                for (int t = 0; t < (w.two ? 2 : 1); t++) {
+                for (int t = 0; t < (TREE || w.two ? 2 : 1); t++) {
                     if (piece[t] && !(healthy = warp_wait(q_empty + t, (piece[t] - 1) & 1))) return;
                     piece[t]++;
-                    const uint32_t token0 = (2 * w.tile + t) * s.tt;
+                    const uint32_t token0 = (2 * w.tile + (w.two ? t : 0)) * s.tt;
                     uint8_t *const dst0 = smem + t * C::HALVES * Q_HALF;
                     if (q_boxes) {  // (tokens behind the request's are some other's, or zeros: such rows go nowhere)
                         if (elect_one()) {
@@ -677,14 +856,21 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
         uint32_t k = 0, events = 0;  // steps so far, and times that it was ready
         const uint32_t local = row / s.g, member = row - local * s.g;
         for (; work; work = next_piece<C::KEYS>(p, w)) {
-            if (t == 1 && !w.two) continue;
-            const uint32_t token = (2 * w.tile + t) * s.tt + local, qh = w.head * s.g + member;
+            if (!TREE && t == 1 && !w.two) continue;
+            // Of a tree: a tile of up to 128 rows is both streams', each with every other step, since one alone is a chain that leaves memory waiting (16 requests of eight tokens over up to 8192 keys 76.7 us). What the
+            // second one has is added up at the end: its O lies in the same lanes of tensor memory.
+            const bool split = TREE && !w.two;
+            const uint32_t own = split ? (w.steps + 1 - t) / 2 : w.steps, step0 = w.t.first + w.step + (split ? t : 0u), stride = split ? 2 : 1;
+            const uint32_t token = (2 * w.tile + (split ? 0u : t)) * s.tt + local, qh = w.head * s.g + member;
             const bool real = local < s.tt && token < w.n;
             // (rows that are none see everything: their results go nowhere, and they ask for no mask)
             // (of a tree: hi and lo are those of the cached keys)
             const uint32_t cached = w.kv - w.n;
             const uint32_t *const tree = TREE ? p.tree + (size_t)(w.q0 + (real ? token : 0u)) * (1 + s.tree) : nullptr;
             const uint32_t hi = !real ? ~0u : TREE ? cached : paged_hi(s, w.n, w.kv, token), lo = !real ? 0u : TREE ? paged_tree_lo(s, cached, *tree) : paged_lo(s, hi);
+            // A warp without a row only says that it is ready: the special-function unit and the schedulers are the others'. (16 requests of eight tokens, 32 rows each, XX us, with it 71.) Its weights are whatever
+            // lies in tensor memory: they reach its own rows of O alone, which go nowhere.
+            const bool idle = TREE && !__any_sync(0xffffffffu, real);
             float m = -INFINITY, base = 0.0f;  // the maximum that the weights refer to
             uint64_t l0 = 0, l1 = 0;           // two pairs of sums
             const uint64_t c2 = pack2(c, c);
@@ -700,13 +886,24 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 if (lane == 0) mbar_arrive(ready + 2 * (events & 1) + t);
                 events++;
             };
-            if (healthy && (healthy = wait_scores(k))) {
-                load_scores(x, s_col);
-                loaded(x);
+            if (healthy && own && (healthy = wait_scores(k))) {
+                if (!idle) {
+                    load_scores(x, s_col);
+                    loaded(x);
+                }
                 say_ready();
             }
-            for (uint32_t j = 0; j < w.steps && healthy; j++) {
-                const uint32_t key0 = (w.t.first + w.step + j) * C::KEYS;
+            for (uint32_t j = 0; j < own && healthy; j++) {
+                if constexpr (TREE) {
+                    if (idle) {
+                        if (k > 0 && !(healthy = warp_wait(o_full + t, (k - 1) & 1))) break;
+                        k++;
+                        if (j + 1 < own && !(healthy = wait_scores(k))) break;
+                        say_ready();
+                        continue;
+                    }
+                }
+                const uint32_t key0 = (step0 + stride * j) * C::KEYS;
                 if (__any_sync(0xffffffffu, (real && key0 + C::KEYS > hi) || key0 < lo)) {
                     // a bit for each column that the row sees
                     const uint32_t from = lo > key0 ? min(lo - key0, (uint32_t)C::KEYS) : 0u, to = hi > key0 ? min(hi - key0, (uint32_t)C::KEYS) : 0u;
@@ -761,7 +958,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 if (!sound) l0 = pack2(NAN, NAN);
                 store_weights(p_col, wt);
                 k++;
-                const bool more = j + 1 < w.steps;
+                const bool more = j + 1 < own;
                 if (more && !(healthy = wait_scores(k))) break;
                 if (more) load_scores(x, s_col);
                 st_wait();
@@ -781,7 +978,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             const uint32_t first = whole ? b : paged_holder(units, ctas, first_unit), last = whole ? b : paged_holder(units, ctas, first_unit + w.t.steps - 1);
             uint32_t *const count = p.plan + p.l.count_large + 2 * first + t;
             uint32_t others = 0;
-            if (b == first && !whole && ((last == first + 2 && (w.n - 2 * w.tile * s.tt) * s.g > 64) || (last == first + 1 && w.t.steps - w.steps + 2 * PAGED_LARGE_EXTRA <= u1 - u0))) {
+            if ((!split || t == 0) && b == first && !whole && ((last == first + 2 && (w.n - 2 * w.tile * s.tt) * s.g > 64) || (last == first + 1 && w.t.steps - w.steps + 2 * PAGED_LARGE_EXTRA <= u1 - u0))) {
                 if (row == 0) {
                     uint32_t there;
                     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(count) : "memory");
@@ -793,8 +990,27 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 others = is_last[t];
                 tile_sync();
             }
-            if (healthy) healthy = warp_wait(o_full + t, (k - 1) & 1);
+            if (healthy && own) healthy = warp_wait(o_full + t, (k - 1) & 1);
             fence_after();
+            float second = 0.0f, first_part = 1.0f;  // what the second stream's O and the first's count
+            if constexpr (TREE) {
+                if (split) {
+                    if (t == 1) meet[row] = m, meet[TILE + row] = l;
+                    fence_before();
+                    asm volatile("bar.sync 3, 256;" ::: "memory");
+                    if (t == 1) {
+                        asm volatile("bar.sync 4, 256;" ::: "memory");  // its O has been read
+                        continue;
+                    }
+                    fence_after();
+                    if (w.steps > 1) {
+                        const float m1 = meet[row], mm = fmaxf(m, m1), mb = mm == -INFINITY ? 0.0f : mm;
+                        first_part = exp2_fast(m - mb), second = exp2_fast(m1 - mb);
+                        m = mm;
+                        l = fmaf(meet[TILE + row], second, l * first_part);
+                    }
+                }
+            }
             unsigned short *orow = (unsigned short *)p.out + p.ov.off + (uint64_t)(w.q0 + token) * p.ov.token + (uint64_t)qh * p.ov.head;
             auto store_lse = [&](float mm, float ll) {
                 if (p.lse && real) p.lse[(size_t)(w.q0 + token) * s.hq + qh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
@@ -820,13 +1036,21 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
 #pragma unroll
                 for (int i = 0; i < 4; i++) rows4[i] = (unsigned short *)__shfl_sync(0xffffffffu, real ? (unsigned long long)orow : 0ull, (lane & 28) + i);
 #pragma unroll 1
-            for (int i = 0; i < DP / 32; i++) {
+            for (int i = 0; i < (idle ? 0 : DP / 32); i++) {
                 uint32_t o[32];
                 tmem_ld32(o, o_col + 32 * i);
                 loaded(o);
                 float v[32];
 #pragma unroll
-                for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * keep;
+                for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * (TREE ? first_part * keep : keep);
+                if constexpr (TREE) {
+                    if (split && w.steps > 1) {
+                        tmem_ld32(o, o_col + DP + 32 * i);
+                        loaded(o);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = fmaf(__uint_as_float(o[e]), second * keep, v[e]);
+                    }
+                }
 #pragma unroll 1
                 for (uint32_t k = 0; k < others; k++) {
                     const float4 *src = (const float4 *)(theirs + (size_t)k * 2 * PF) + 8 * i * ROWS + prow;
@@ -853,11 +1077,17 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 }
             }
             fence_before();
+            if constexpr (TREE) {
+                if (split) asm volatile("bar.sync 4, 256;" ::: "memory");
+            }
             if (here) {
                 store_lse(m, l);
                 continue;
             }
             if (real) mine[DP * ROWS + prow] = m, mine[(DP + 1) * ROWS + prow] = l;
+            if constexpr (TREE) {
+                if (last - first + 1 >= JOIN_APART && paged_joins_apart(s)) continue;  // (paged_attn_join_kernel)
+            }
             tile_sync();
             if (row == 0) {
                 uint32_t before;
@@ -904,6 +1134,20 @@ template <int DP, bool BF16, bool TREE> static cudaError_t large_launch(const Pa
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, mk, mv, mq, a, boxes);
+}
+
+cudaError_t launch_paged_attn_join(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)sm_count);
+    cfg.blockDim = dim3(pt::JOIN_THREADS);
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    if (a.s.d > 64) return a.s.bf16 ? cudaLaunchKernelEx(&cfg, pt::paged_attn_join_kernel<128, true>, a) : cudaLaunchKernelEx(&cfg, pt::paged_attn_join_kernel<128, false>, a);
+    return a.s.bf16 ? cudaLaunchKernelEx(&cfg, pt::paged_attn_join_kernel<64, true>, a) : cudaLaunchKernelEx(&cfg, pt::paged_attn_join_kernel<64, false>, a);
 }
 
 cudaError_t launch_paged_attn_large(const PagedAttnArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
