@@ -46,7 +46,7 @@ PagedPlanLayout paged_plan_layout(const PagedShape &s) {
     return l;
 }
 
-bool paged_has_large(const PagedShape &s) { return (uint64_t)s.max_new * s.g > PAGED_SMALL_LIMIT && s.tt > 0; }
+bool paged_has_large(const PagedShape &s) { return !paged_is_small(s, s.max_new); }
 
 uint32_t paged_stamp(const PagedShape &s) {
     uint32_t h = 2166136261u;  // (Fowler, Noll and Vo's hash over the words a plan depends on)

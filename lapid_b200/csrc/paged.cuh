@@ -59,10 +59,10 @@ __host__ __device__ inline PagedTile paged_tile(const PagedShape &s, uint32_t n,
 }
 __host__ __device__ inline uint32_t paged_tiles(const PagedShape &s, uint32_t n, uint32_t rows) { return (n * s.g + rows - 1) / rows; }
 // Requests of few rows go to one kernel, the others to the other. Of a tree's step all go to one: trees are of a size, and a launch that finds nothing to do takes 2 us.
-__host__ __device__ inline bool paged_is_small(const PagedShape &s, uint32_t n) { return (s.tree ? s.max_new : n) * s.g <= PAGED_SMALL_LIMIT || s.tt == 0; }
-// A tree's tiles of more than 64 rows that are cut into many pieces are added up by a kernel of its own (paged_attn_tc.cu); of fewer rows the last CTA of a tile is quicker than a launch (32 rows over 4096
-// keys 16.4 and 19.5 us)
-__host__ __device__ inline bool paged_joins_apart(const PagedShape &s) { return s.tree && s.max_new * s.g > 64; }
+__host__ __device__ inline bool paged_is_small(const PagedShape &s, uint32_t n) { return (s.tree ? s.max_new * s.g <= PAGED_SMALL_LIMIT_TREE : n * s.g <= PAGED_SMALL_LIMIT) || s.tt == 0; }
+// A tree's tiles of more than 32 rows that are cut into many pieces are added up by a kernel of its own (paged_attn_tc.cu); of fewer rows the last CTA of a tile is quicker than a launch (32 rows over 4096
+// keys 15.4 and 16.8 us, 64 rows 20.2 and 16.4)
+__host__ __device__ inline bool paged_joins_apart(const PagedShape &s) { return s.tree && s.max_new * s.g > 32; }
 __host__ __device__ inline uint32_t paged_large_rows(const PagedShape &s) { return 2 * s.tt * s.g; }
 
 // What a CTA of an attention launch begins with (one 64-byte line of the plan, so that one load brings it all); u0 == u1: it has nothing to do

@@ -75,7 +75,7 @@ template <int DP> struct Cfg {
     static constexpr int STAGE = HALVES * HALF;
     static constexpr int Q_BYTES = 2 * HALVES * Q_HALF;
     static constexpr int STAGES = (224 * 1024 - Q_BYTES) / (2 * STAGE);  // of keys, and as many of values
-    static constexpr int SMEM = Q_BYTES + 2 * STAGES * STAGE + 512 + 1024 + 2 * TILE * 4;
+    static constexpr int SMEM = Q_BYTES + 2 * STAGES * STAGE + 512 + 1024 + 2 * TILE * 4 + 16;
     // tensor memory: O of tile t at DP t, S at T_COL + T_STEP t, P behind it
     static constexpr int T_COL = 2 * DP, T_STEP = (512 - T_COL) / 2;
     static_assert(KEYS + KEYS / 2 <= T_STEP && KEYS % 16 == 0, "tensor memory");
@@ -410,15 +410,85 @@ template <int DP, bool BF16> __device__ __forceinline__ void join_pieces(const P
     }
 }
 
+// The same for a tile that both streams have: its eight warps share the groups of 32 rows and of 16 columns.
+template <int DP, bool BF16> __device__ __forceinline__ void join_pieces_both(const PagedAttnArgs &p, const Cut &c, uint32_t warp, bool vec) {
+    constexpr uint32_t PF = ROWS * (DP + 2), COLS = 16;
+    constexpr int B = 6;  // pieces in flight
+    const PagedShape &s = p.s;
+    const float *const parts = (const float *)((const uint8_t *)p.plan + p.l.part_large);
+    const uint32_t lane = threadIdx.x & 31, token0 = 2 * c.tile * s.tt, rows = min(s.tt, c.n - token0) * s.g, groups = (rows + 31) / 32;
+#pragma unroll 1
+    for (uint32_t item = warp; item < groups * (DP / COLS); item += 8) {
+        const uint32_t ch = item / groups, r = 32 * (item - ch * groups) + lane;
+        if (r >= rows || COLS * ch >= s.d) continue;
+        float mm = -INFINITY, ll = 0.0f, v[COLS];
+#pragma unroll
+        for (int e = 0; e < (int)COLS; e++) v[e] = 0.0f;
+#pragma unroll 1
+        for (uint32_t i0 = c.first; i0 <= c.last; i0 += B) {
+            float m[B], l[B];
+            float4 y[B][COLS / 4];
+#pragma unroll
+            for (uint32_t k = 0; k < B; k++) {
+                const float *src = parts + (size_t)(2 * min(i0 + k, c.last) + (i0 + k == c.first ? 1 : 0)) * PF;  // (the last one again where there are no more, with the weight 0)
+                m[k] = __ldcg(src + DP * ROWS + r);
+                l[k] = __ldcg(src + (DP + 1) * ROWS + r);
+#pragma unroll
+                for (uint32_t e = 0; e < COLS / 4; e++) y[k][e] = __ldcg((const float4 *)src + (COLS / 4 * ch + e) * ROWS + r);
+            }
+#pragma unroll
+            for (uint32_t k = 1; k < B; k++)
+                if (i0 + k > c.last) m[k] = -INFINITY;
+            float top = mm;
+#pragma unroll
+            for (uint32_t k = 0; k < B; k++) top = fmaxf(top, m[k]);
+            const float base = top == -INFINITY ? 0.0f : top, keep = exp2_fast(mm - base);
+            mm = top;
+            ll *= keep;
+#pragma unroll
+            for (int e = 0; e < (int)COLS; e++) v[e] *= keep;
+#pragma unroll
+            for (uint32_t k = 0; k < B; k++) {
+                const float f = i0 + k > c.last ? 0.0f : exp2_fast(m[k] - base);
+                ll = fmaf(l[k], f, ll);
+#pragma unroll
+                for (uint32_t e = 0; e < COLS / 4; e++) {
+                    v[4 * e] = fmaf(y[k][e].x, f, v[4 * e]);
+                    v[4 * e + 1] = fmaf(y[k][e].y, f, v[4 * e + 1]);
+                    v[4 * e + 2] = fmaf(y[k][e].z, f, v[4 * e + 2]);
+                    v[4 * e + 3] = fmaf(y[k][e].w, f, v[4 * e + 3]);
+                }
+            }
+        }
+        const float il = ll == 0.0f ? 0.0f : 1.0f / ll;
+        const uint32_t local = r / s.g, qh = c.head * s.g + (r - local * s.g);
+        const uint64_t at = c.q0 + token0 + local;
+        unsigned short *const row = (unsigned short *)p.out + p.ov.off + at * p.ov.token + (uint64_t)qh * p.ov.head;
+#pragma unroll
+        for (uint32_t e = 0; e < COLS; e += 8) {
+            if (COLS * ch + e >= s.d) break;
+            const uint32_t z[4] = {pack<BF16>(v[e] * il, v[e + 1] * il), pack<BF16>(v[e + 2] * il, v[e + 3] * il), pack<BF16>(v[e + 4] * il, v[e + 5] * il), pack<BF16>(v[e + 6] * il, v[e + 7] * il)};
+            unsigned short *const to = row + COLS * ch + e;
+            if (vec) {
+                *(uint4 *)to = make_uint4(z[0], z[1], z[2], z[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) to[2 * i] = (unsigned short)z[i], to[2 * i + 1] = (unsigned short)(z[i] >> 16);
+            }
+        }
+        if (p.lse && ch == 0) p.lse[at * s.hq + qh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+    }
+}
+
 // Drafted tokens are few rows over many keys: their tiles are cut into many pieces. From JOIN_APART of them on the CTAs only leave theirs in the plan, and the kernel below adds them up on all SMs: a tile of 256 rows
-// over 32768 keys is 18 pieces of 133 KB, which one CTA takes 40 us for (64 tokens over 32768 keys, 8 key heads: XX us, with the last CTA of a tile at it 75.7).
+// over 32768 keys is 18 pieces of 133 KB, which one CTA takes 40 us for (64 tokens over 32768 keys, 8 key heads: 50.8 us, with the last CTA of a tile at it 75.7).
 constexpr uint32_t JOIN_APART = 4, JOIN_COLS = 8, JOIN_THREADS = 256;
 static_assert(JOIN_THREADS >= PAGED_MAX_SMS, "a thread for each end of a span");
 
 // Each CTA finds the cut tiles, a thread for the end of each span, and how many (32 rows, JOIN_COLS columns) they have; its warps take every so many of these.
 template <int DP, bool BF16> __global__ void __launch_bounds__(JOIN_THREADS, 1) paged_attn_join_kernel(PagedAttnArgs p) {
     constexpr uint32_t KEYS = Cfg<DP>::KEYS, PF = ROWS * (DP + 2), PER = DP / JOIN_COLS;  // column groups of a row
-    constexpr int B = 8;  // pieces in flight
+    constexpr int B = 10;  // pieces in flight
     __shared__ uint32_t ends[JOIN_THREADS], sums[JOIN_THREADS / 32];
     struct Found {
         uint32_t first, last, q0, n, head, tile;
@@ -854,10 +924,12 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
         constexpr uint32_t PF = ROWS * (DP + 2);
         auto tile_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory"); };
         uint32_t k = 0, events = 0;  // steps so far, and times that it was ready
+        uint32_t splits = 0;         // tiles that both streams had; whether they add up the pieces of one (a word is written again only behind the barrier of the tile between)
+        volatile uint32_t *const joins = (volatile uint32_t *)(meet + 2 * TILE);
         const uint32_t local = row / s.g, member = row - local * s.g;
         for (; work; work = next_piece<C::KEYS>(p, w)) {
             if (!TREE && t == 1 && !w.two) continue;
-            // Of a tree: a tile of up to 128 rows is both streams', each with every other step, since one alone is a chain that leaves memory waiting (16 requests of eight tokens over up to 8192 keys 76.7 us). What the
+            // Of a tree: a tile of up to 128 rows is both streams', each with every other step, since one alone is a chain that leaves memory waiting (the same requests 74.2 us so, 72.0 with both streams' warps adding up pieces). What the
             // second one has is added up at the end: its O lies in the same lanes of tensor memory.
             const bool split = TREE && !w.two;
             const uint32_t own = split ? (w.steps + 1 - t) / 2 : w.steps, step0 = w.t.first + w.step + (split ? t : 0u), stride = split ? 2 : 1;
@@ -868,7 +940,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             const uint32_t cached = w.kv - w.n;
             const uint32_t *const tree = TREE ? p.tree + (size_t)(w.q0 + (real ? token : 0u)) * (1 + s.tree) : nullptr;
             const uint32_t hi = !real ? ~0u : TREE ? cached : paged_hi(s, w.n, w.kv, token), lo = !real ? 0u : TREE ? paged_tree_lo(s, cached, *tree) : paged_lo(s, hi);
-            // A warp without a row only says that it is ready: the special-function unit and the schedulers are the others'. (16 requests of eight tokens, 32 rows each, XX us, with it 71.) Its weights are whatever
+            // A warp without a row only says that it is ready: the special-function unit and the schedulers are the others'. (16 requests of eight tokens, 32 rows each, over up to 8192 keys 76.7 us, with it 80.3.) Its weights are whatever
             // lies in tensor memory: they reach its own rows of O alone, which go nowhere.
             const bool idle = TREE && !__any_sync(0xffffffffu, real);
             float m = -INFINITY, base = 0.0f;  // the maximum that the weights refer to
@@ -999,7 +1071,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                     fence_before();
                     asm volatile("bar.sync 3, 256;" ::: "memory");
                     if (t == 1) {
-                        asm volatile("bar.sync 4, 256;" ::: "memory");  // its O has been read
+                        asm volatile("bar.sync 4, 256;" ::: "memory");  // its O has been read, and it is known who adds up the pieces
+                        if (joins[splits & 1]) join_pieces_both<DP, BF16>(p, Cut{first, last, w.q0, w.n, w.head, w.tile}, warp, vec);
+                        splits++;
+                        tile_sync();
                         continue;
                     }
                     fence_after();
@@ -1077,16 +1152,25 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 }
             }
             fence_before();
-            if constexpr (TREE) {
-                if (split) asm volatile("bar.sync 4, 256;" ::: "memory");
-            }
+            // the second stream goes on, to add up pieces or to its next tile
+            auto release = [&](bool join) {
+                if constexpr (TREE) {
+                    if (row == 0) joins[splits & 1] = join;
+                    asm volatile("bar.sync 4, 256;" ::: "memory");
+                    splits++;
+                }
+            };
             if (here) {
+                if (split) release(false);
                 store_lse(m, l);
                 continue;
             }
             if (real) mine[DP * ROWS + prow] = m, mine[(DP + 1) * ROWS + prow] = l;
             if constexpr (TREE) {
-                if (last - first + 1 >= JOIN_APART && paged_joins_apart(s)) continue;  // (paged_attn_join_kernel)
+                if (last - first + 1 >= JOIN_APART && paged_joins_apart(s)) {  // (paged_attn_join_kernel)
+                    if (split) release(false);
+                    continue;
+                }
             }
             tile_sync();
             if (row == 0) {
@@ -1097,6 +1181,15 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 is_last[t] = end;
             }
             tile_sync();
+            if constexpr (TREE) {
+                if (split) {
+                    const bool join = is_last[0];
+                    release(join);
+                    if (join) join_pieces_both<DP, BF16>(p, Cut{first, last, w.q0, w.n, w.head, w.tile}, warp, vec);
+                    tile_sync();
+                    continue;
+                }
+            }
             if (is_last[t]) join_pieces<DP, BF16>(p, Cut{first, last, w.q0, w.n, w.head, w.tile}, t, vec, wide);
             tile_sync();  // (without it the compiler merges this end with the others' and spills 330 bytes in the steps: 640 instead of 580 us for 512 rows over 32768 keys)
         }

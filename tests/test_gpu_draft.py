@@ -103,13 +103,13 @@ def test_shapes(be, n, shape):
 
 
 @pytest.mark.parametrize("dtype", [lp.DType.BF16, lp.DType.F16])
-@pytest.mark.parametrize("sizes", [[1, 3, 4], [40, 64, 7]])
+@pytest.mark.parametrize("sizes", [[1, 1, 1], [1, 3, 4], [40, 64, 7]])
 def test_a_chain_is_the_causal_mask(be, sizes, dtype):
-    """Both against the definition (in `run`); of few rows, where a tree's keys are added up in the same order, bit for bit."""
+    """Both against the definition (in `run`); of single tokens, where a tree's keys are added up in the same order, bit for bit."""
     cached = [70, 0, 131]
     a = R.Step(be, sizes, cached, dtype=dtype, hq=8, hkv=2, d=128, seed=4).run()
     b = D.TreeStep(be, [chain(n) for n in sizes], cached, dtype=dtype, hq=8, hkv=2, d=128, seed=4).run()
-    if max(sizes) * 4 <= 16:
+    if max(sizes) == 1:
         assert np.array_equal(a.b["out"].download(), b.b["out"].download()) and np.array_equal(a.b["lse"].download(), b.b["lse"].download())
     assert np.array_equal(a.b["positions"].download(), b.b["positions"].download())
 
