@@ -2688,6 +2688,7 @@ lapid_b200_status lapid_b200_paged_commit(lapid_b200_device *dev, const lapid_b2
         if (!a.s.tree && a.s.mask != lb::PAGED_CAUSAL) fail("invalid_launch", "paged_commit: the description's mask must be TREE or CAUSAL");
         if (a.s.tree && !path) fail("invalid_argument", "paged_commit: path is NULL (the accepted tokens of a tree do not lie behind each other)");
         if (n_free >= (1ull << 31)) fail("too_large", "paged_commit: n_free must be below 2^31");
+        if (path && a.s.max_new > lb::PAGED_TREE_MOST) fail("unsupported", "paged_commit: at most 1024 new tokens a request with a path, max_new is " + std::to_string(a.s.max_new));
         if (n_caches > 1u << 16) fail("too_large", "paged_commit: at most 65536 caches");
         if (n_caches && !caches) fail("invalid_argument", "paged_commit: caches is NULL");
         const uint64_t R = a.s.requests, cache = (uint64_t)a.s.pages * a.s.hkv * a.s.page * a.s.d * 2;
@@ -2724,7 +2725,7 @@ lapid_b200_status lapid_b200_paged_commit(lapid_b200_device *dev, const lapid_b2
             a.pages = done == 0;
             a.caches = path ? (uint32_t)std::min<uint64_t>(n_caches - done, lb::PAGED_COMMIT_CACHES) : 0u;
             for (uint32_t i = 0; i < a.caches; i++) a.cache[i] = caches[done + i]->ptr;
-            cuda_check(lb::launch_paged_commit(a, dev->pdl, dev->stream), "paged_commit launch");
+            cuda_check(lb::launch_paged_commit(a, dev->sm_count, dev->pdl, dev->stream), "paged_commit launch");
             dev->launches++;
             done += a.caches;
         } while (path && done < n_caches);

@@ -498,7 +498,7 @@ struct PagedCommitArgs {
     bool pages;  // the lengths and the list of free pages too (the first launch of a call)
     void *cache[PAGED_COMMIT_CACHES];
 };
-cudaError_t launch_paged_commit(const PagedCommitArgs &a, bool pdl, cudaStream_t stream);
+cudaError_t launch_paged_commit(const PagedCommitArgs &a, int sm_count, bool pdl, cudaStream_t stream);
 struct PagedVerifyArgs {
     PagedShape s;
     const uint32_t *request, *stamped;

@@ -147,66 +147,75 @@ __device__ void commit_pages(const PagedCommitArgs &a) {
     if (threadIdx.x == 0) *a.used = (int32_t)all_kept;
 }
 
-// blockIdx.x: a cache, and behind them (where the launch has pages) one CTA for the lengths and pages; blockIdx.y walks the requests
-__global__ void __launch_bounds__(COMMIT_THREADS) paged_commit_kernel(const __grid_constant__ PagedCommitArgs a) {
+// A CTA has one request and some of the caches: where its tokens lie and where they go is found once, in shared memory, and what is asked for first (record, accepted, path) does not wait for each other.
+// blockIdx.x: a group of caches, and behind them (where the launch has pages) one CTA for the lengths and pages; blockIdx.y walks the requests
+__global__ void __launch_bounds__(COMMIT_THREADS) paged_commit_kernel(const __grid_constant__ PagedCommitArgs a, uint32_t each) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr uint32_t NONE = ~0u, B = 4;  // tokens whose bytes are in flight
+    __shared__ uint32_t from[PAGED_TREE_MOST], to[PAGED_TREE_MOST];  // rows of a cache, of the first head
     const PagedShape &s = a.s;
+    const uint32_t groups = (a.caches + each - 1) / each;
     if (!plan_fits(a.stamped, a.stamp, a.status)) return;
-    if (blockIdx.x == a.caches) {
+    if (blockIdx.x == groups) {
         if (blockIdx.y == 0) commit_pages(a);
         return;
     }
-    if (!a.path) return;
-    constexpr uint32_t B = 4;  // tokens whose bytes are in flight
-    const uint32_t shift = 31 - __clz(s.page), chunks = s.d / 8;
-    uint4 *const cache = (uint4 *)a.cache[blockIdx.x];
+    const uint32_t shift = 31 - __clz(s.page), chunks = s.d / 8, columns = s.hkv * chunks;
     for (uint32_t r = blockIdx.y; r < s.requests; r += gridDim.y) {
+        const int32_t *const path = a.path + (size_t)r * s.max_new, *const table = a.table + (size_t)r * s.max_blocks;
+        const int32_t mine = threadIdx.x < s.max_new ? path[threadIdx.x] : -1, before = threadIdx.x && threadIdx.x < s.max_new ? path[threadIdx.x - 1] : -1;
         const uint4 x = ((const uint4 *)a.request)[r];
         const uint32_t n = x.y - x.x, cached = x.z - n;
-        const int32_t *const path = a.path + (size_t)r * s.max_new, *const table = a.table + (size_t)r * s.max_blocks;
         bool bad = false;
         const uint32_t k = accepted_of(a, r, n, bad);
-        for (uint32_t i = threadIdx.x; i < k; i += COMMIT_THREADS) bad |= !path_sound(path, i, n);
+        if (threadIdx.x < k) bad |= mine < 0 || (uint32_t)mine >= n || (threadIdx.x && before >= mine);
+        for (uint32_t i = threadIdx.x + COMMIT_THREADS; i < k; i += COMMIT_THREADS) bad |= !path_sound(path, i, n);
+        auto row_of = [&](uint32_t token) -> uint32_t {
+            const uint32_t pos = cached + token, block = pos >> shift;
+            const int32_t page = block < s.max_blocks ? table[block] : -1;
+            if (page >= 0 && (uint32_t)page < s.pages) return (uint32_t)page * s.hkv * s.page + (pos & (s.page - 1));
+            if (a.status) atomicOr(a.status, (int)PAGED_STATUS_INDEX);
+            return NONE;
+        };
         if (__syncthreads_or(bad)) continue;  // (the pages' CTA tells of it)
-        for (uint32_t c = threadIdx.x; c < s.hkv * chunks; c += COMMIT_THREADS) {
-            const uint32_t head = c / chunks, part = c - head * chunks;
-            auto at = [&](uint32_t token) -> uint4 * {
-                const uint32_t pos = cached + token, block = pos >> shift;
-                const int32_t page = block < s.max_blocks ? table[block] : -1;
-                if (page < 0 || (uint32_t)page >= s.pages) {
-                    if (a.status) atomicOr(a.status, (int)PAGED_STATUS_INDEX);
-                    return nullptr;
-                }
-                return cache + (((size_t)page * s.hkv + head) * s.page + (pos & (s.page - 1))) * chunks + part;
-            };
+        for (uint32_t i = threadIdx.x; i < k; i += COMMIT_THREADS) {
+            const uint32_t src = (uint32_t)(i == threadIdx.x ? mine : path[i]);
+            uint32_t f = NONE, t = NONE;
+            if (src != i) f = row_of(src), t = row_of(i);
+            from[i] = f, to[i] = f == NONE ? NONE : t;
+        }
+        __syncthreads();
+        // a thread has 16 bytes of a head, and takes the tokens in their order
+        const uint32_t first = blockIdx.x * each, count = min(each, a.caches - first);
+        for (uint32_t c = threadIdx.x; c < columns * count; c += COMMIT_THREADS) {
+            const uint32_t cache = c / columns, col = c - cache * columns, head = col / chunks;
+            uint4 *const base = (uint4 *)a.cache[first + cache] + (size_t)head * s.page * chunks + (col - head * chunks);
             for (uint32_t i0 = 0; i0 < k; i0 += B) {
                 uint4 v[B];
-                uint4 *to[B];
+                uint32_t at[B];
 #pragma unroll
                 for (uint32_t i = 0; i < B; i++) {
-                    to[i] = nullptr;
-                    if (i0 + i >= k) continue;
-                    const uint32_t src = (uint32_t)path[i0 + i];
-                    if (src == i0 + i) continue;
-                    const uint4 *from = at(src);
-                    to[i] = from ? at(i0 + i) : nullptr;
-                    if (to[i]) v[i] = *from;
+                    at[i] = i0 + i < k ? to[i0 + i] : NONE;
+                    if (at[i] != NONE) v[i] = base[(size_t)from[i0 + i] * chunks];
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < B; i++)
-                    if (to[i]) *to[i] = v[i];
+                    if (at[i] != NONE) base[(size_t)at[i] * chunks] = v[i];
             }
         }
+        __syncthreads();  // (the rows are read)
     }
 }
 
-cudaError_t launch_paged_commit(const PagedCommitArgs &a, bool pdl, cudaStream_t stream) {
-    const uint32_t x = a.caches + (a.pages ? 1 : 0);
+cudaError_t launch_paged_commit(const PagedCommitArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
+    // caches for each CTA: one, or as many as leave some eight CTAs an SM
+    const uint64_t all = (uint64_t)a.caches * a.s.requests, most = 8 * (uint64_t)sm_count;
+    const uint32_t each = (uint32_t)(all > most ? (all + most - 1) / most : 1), groups = (a.caches + each - 1) / each;
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[1];
-    draft_config(cfg, attr, dim3(x, a.s.requests < 65535 ? (a.s.requests ? a.s.requests : 1) : 65535), COMMIT_THREADS, pdl, stream);
-    return cudaLaunchKernelEx(&cfg, paged_commit_kernel, a);
+    draft_config(cfg, attr, dim3(groups + (a.pages ? 1 : 0), a.s.requests < 65535 ? (a.s.requests ? a.s.requests : 1) : 65535), COMMIT_THREADS, pdl, stream);
+    return cudaLaunchKernelEx(&cfg, paged_commit_kernel, a, each);
 }
 
 }  // namespace lb

@@ -577,6 +577,7 @@ def test_calls_that_are_refused(be):
     refused("invalid_launch", com, full)
     refused("invalid_launch", com, cross)
     refused("invalid_argument", com, path=None)
+    refused("unsupported", com, replace(causal, max_new=1025, tokens=1))
     refused("out_of_bounds", com, layers=((b["k"], i(8)),))
     refused("buffer_aliasing", com, layers=((b["k"], b["k"]),))
     refused("buffer_aliasing", com, layers=((b["k"], b["v"]), (b["v"], be.alloc(1 << 20))))
