@@ -35,7 +35,7 @@ constexpr uint32_t BATCH = 16, FAST = 32;                             // tokens 
 // entropy); a weight is the product of powers of 2, 2^-22 and a product's 2^-24 each, to the thread's largest (as that grows, at most 64 times: PART_MOST), the warp's, the CTA's and the
 // cluster's; at most 90 additions, 2^-24 each. In all 3e-5, of which 2^-14 is twice as much.
 constexpr double SURE = 0x1p-14;
-constexpr uint32_t PART_MOST = 64 * 32 * 16;  // a warp's places
+constexpr uint32_t PART_MOST = 64 * 32 * 16;  // a warp's places: 32 rounds of FAST a thread
 
 // What the warps of the cluster tell each other comes in two sets: a warp writes a set again only when all have read it, which they say with the exchange between.
 struct Shared {
@@ -199,6 +199,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all of them are there: their memory may be written
     __syncthreads();
     const uint32_t clusters = gridDim.x / ctas;
+#pragma unroll 1
     for (uint32_t r = blockIdx.x / ctas; r < a.s.requests; r += clusters) {
         const uint4 rec = ((const uint4 *)a.request)[r];
         // (what decides is rank 0's; where the others' own differ, since the caller writes them meanwhile, only numbers do)
@@ -230,10 +231,12 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
             fetch(first);
             // (meanwhile rank 0 fetches what the tests of the children need, a thread for a token)
             if (rank == 0 && length == 0) {
+#pragma unroll 1
                 for (uint32_t t = tid; t < n; t += THREADS) {
                     const int32_t p = a.parents ? a.parents[q0 + t] : (int32_t)t - 1, token = a.tokens[q0 + t];
                     const float accept = a.accept[q0 + t];
                     parent[t] = p, node[t].token = token, node[t].accept = accept;
+#pragma unroll 1
                     for (uint32_t c = 1; c < ctas; c++) {
                         put(of_rank(parent + t, c), (uint32_t)p);
                         put(of_rank(node + t, c), (uint64_t)(uint32_t)token | (uint64_t)__float_as_uint(accept) << 32);
@@ -253,17 +256,24 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                 child_logit = load_act(start, token, SRC);
                 if (draft) child_draft = draft[token];
             };
-            auto tell_child = [&](uint32_t t) {
-                if (!is_child(t)) return;
-                for (uint32_t c = 0; c < ctas; c++) put(of_rank(&node[t].logit, c), (uint64_t)__float_as_uint(child_logit) | (uint64_t)__float_as_uint(child_draft) << 32);
+            auto tell_child = [&](uint32_t t) {  // (a lane for a CTA)
+                uint32_t children = __ballot_sync(0xffffffffu, is_child(t));
+                while (children) {
+                    const uint32_t who = __ffs(children) - 1;
+                    children &= children - 1;
+                    const float x = __shfl_sync(0xffffffffu, child_logit, who), y = __shfl_sync(0xffffffffu, child_draft, who);
+                    if (lane < ctas) put(of_rank(&node[t - lane + who].logit, lane), (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32);
+                }
             };
             if (rank == 0) {
-                for (uint32_t t = tid + THREADS; t < n; t += THREADS) fetch_child(t), tell_child(t);
+#pragma unroll 1
+                for (uint32_t t0 = THREADS; t0 < n; t0 += THREADS) fetch_child(t0 + tid), tell_child(t0 + tid);
                 fetch_child(tid);
             }
             const float scale = fminf(1.44269504f / temperature, 3e38f);
             float top = -INFINITY, sum = 0.0f;
             uint32_t at = ~0u;
+#pragma unroll 1
             for (uint32_t c0 = first; c0 < last;) {
                 if (cold) {
 #pragma unroll
@@ -376,9 +386,11 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                     }
                     exact = true;
                     weight.set(temperature);
+#pragma unroll 1
                     for (uint32_t k = v + 1 + tid; k < n; k += THREADS)
                         if (parent[k] == (int32_t)v) value[k] = weight(node[k].logit);
                     if (!draft)
+#pragma unroll 1
                         for (uint32_t i = tid; i < WARPS * part / 32; i += THREADS) gone[i] = 0;
                     __syncthreads();
                 }
@@ -400,6 +412,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                             t++;
                             if (!(mine > 0.0)) continue;
                             __syncthreads();  // (value[] has been read)
+#pragma unroll 1
                             for (uint32_t k = t - 1 + tid; k < n; k += THREADS)
                                 if (parent[k] == (int32_t)v && node[k].token == y.token) value[k] = 0.0;
                             const uint32_t bit = (uint32_t)y.token + from - part0;
@@ -440,6 +453,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                         }
 #pragma unroll
                     for (int e = 0; e < (int)BATCH; e++) w[e] = weight(z[e / E][e % E]);
+#pragma unroll 1
                     for (uint32_t k = 0; k < stages; k++) {
                         const double share = -taken[k];
 #pragma unroll
@@ -464,6 +478,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                     t++;
                     parts = left > 0.0;
                     if (!parts) continue;  // (nothing is left, and the distribution stays)
+#pragma unroll 1
                     for (uint32_t k = t + tid; k < n; k += THREADS)
                         if (parent[k] == (int32_t)v) value[k] = positive(fma((double)node[k].draft, -rest, value[k]));
                     if (tid == 0) taken[stages] = rest;
@@ -492,6 +507,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
             const double *const sums = sh.sum[set ^ 1];
             const uint32_t each = (warps + 31) / 32;
             double before = 0.0, mine = 0.0;
+#pragma unroll 1
             for (uint32_t k = 0; k < each; k++) mine += lane * each + k < warps ? sums[lane * each + k] : 0.0;
             uint32_t who = place_of(mine, 0.0, goal, before);
             answer = who < 32 ? -2 : -1;  // (-2: written by that warp)
@@ -499,6 +515,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                 const uint32_t begin = who * each;
                 double run = before;
                 who = begin;
+#pragma unroll 1
                 for (uint32_t k = begin; k < min(begin + each, warps); k++) {
                     if (sums[k] > 0.0) who = k, before = run;
                     run += sums[k];
@@ -530,6 +547,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                         }
 #pragma unroll
                         for (int e = 0; e < (int)BATCH; e++) wt[e] = weight(z[e / E][e % E]);
+#pragma unroll 1
                         for (uint32_t k = 0; k < stages; k++) {
                             const double share = -taken[k];
 #pragma unroll
@@ -562,6 +580,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                 a.accepted[r] = (int32_t)length;
                 if (answer != -2) a.next[r] = answer;
             }
+#pragma unroll 1
             for (uint32_t i = length + tid; i < most; i += THREADS) a.path[(size_t)r * most + i] = -1;
         }
         cluster_sync();  // the request's nodes have been read by all

@@ -226,6 +226,18 @@ def test_verify_many_requests_and_wide_trees(be, drawn):
 
 
 @pytest.mark.parametrize("drawn", [False, True])
+def test_verify_full_servers(be, drawn):
+    """More requests than there are SMs, so that a CTA or two have a row and go over it many times."""
+    rng = np.random.default_rng(15)
+    Walks(be, [D.random_parents(rng, 3, 2) for _ in range(200)], 20011, dtype=lp.DType.F32 if drawn else lp.DType.BF16, drawn=drawn, seed=16, spread=3.0).run().check()
+
+
+@pytest.mark.parametrize("vocab,dtype,drawn", [(300007, lp.DType.F32, True), (1 << 20, lp.DType.F16, False), (1 << 22, lp.DType.BF16, False)])
+def test_verify_large_vocabularies(be, vocab, dtype, drawn):
+    Walks(be, [[-1, 0]], vocab, dtype=dtype, drawn=drawn, seed=17).run().check()
+
+
+@pytest.mark.parametrize("drawn", [False, True])
 @pytest.mark.parametrize("row", [1000, 1001, 1003, 1004])
 def test_rows_of_any_distance(be, row, drawn):
     rng = np.random.default_rng(row)
