@@ -16,7 +16,6 @@
 #include <cstdlib>
 #include <cstring>
 #include <algorithm>
-#include <functional>
 #include <map>
 #include <mutex>
 #include <new>
@@ -1653,20 +1652,24 @@ bool paged_overlap(const lapid_b200_buffer *a, const lapid_b200_buffer *b) {
     const char *x = (const char *)a->ptr, *y = (const char *)b->ptr;
     return x < y + b->bytes && y < x + a->bytes;
 }
-// No output shares memory with an input or with another output (any may be NULL). In the order of their addresses: a commit has the caches of all layers.
-void paged_apart(const std::string &call, const std::vector<const lapid_b200_buffer *> &ins, const std::vector<const lapid_b200_buffer *> &outs) {
-    std::vector<std::pair<const lapid_b200_buffer *, bool>> all;
-    for (const lapid_b200_buffer *b : ins)
-        if (b && b->bytes) all.push_back({b, false});
-    for (const lapid_b200_buffer *b : outs)
-        if (b && b->bytes) all.push_back({b, true});
-    std::sort(all.begin(), all.end(), [](const auto &x, const auto &y) { return std::less<const void *>()(x.first->ptr, y.first->ptr); });
-    const char *in_end = nullptr, *out_end = nullptr;  // of those that begin no later
-    for (const auto &[b, out] : all) {
-        const char *begin = (const char *)b->ptr, *end = begin + b->bytes;
-        if (out && begin < out_end) fail("buffer_aliasing", call + ": two outputs alias");
-        if (begin < (out ? in_end : out_end)) fail("buffer_aliasing", call + ": an output aliases an input");
-        (out ? out_end : in_end) = std::max(out ? out_end : in_end, end);
+// No output shares memory with an input or with another output (any may be NULL): in the order of their addresses, since a commit has the caches of all layers.
+void paged_apart(const char *call, std::initializer_list<const lapid_b200_buffer *> ins, std::initializer_list<const lapid_b200_buffer *> outs, lapid_b200_buffer *const *more = nullptr,
+                 uint64_t n_more = 0) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> all;  // begin and end of the outputs
+    all.reserve(outs.size() + n_more);
+    auto add = [&](const lapid_b200_buffer *b) {
+        if (b && b->bytes) all.push_back({(uintptr_t)b->ptr, (uintptr_t)b->ptr + b->bytes});
+    };
+    for (uint64_t i = 0; i < n_more; i++) add(more[i]);
+    for (const lapid_b200_buffer *b : outs) add(b);
+    std::sort(all.begin(), all.end());
+    for (size_t i = 1; i < all.size(); i++)
+        if (all[i].first < all[i - 1].second) fail("buffer_aliasing", std::string(call) + ": two outputs alias");
+    for (const lapid_b200_buffer *b : ins) {
+        if (!b || !b->bytes) continue;
+        const uintptr_t begin = (uintptr_t)b->ptr, end = begin + b->bytes;
+        const auto at = std::lower_bound(all.begin(), all.end(), std::make_pair(end, (uintptr_t)0));  // the first output that begins behind the input
+        if (at != all.begin() && std::prev(at)->second > begin) fail("buffer_aliasing", std::string(call) + ": an output aliases an input");
     }
 }
 int paged_sms(const lapid_b200_device *dev) { return dev->sm_count < (int)lb::PAGED_MAX_SMS ? dev->sm_count : (int)lb::PAGED_MAX_SMS; }
@@ -2700,12 +2703,8 @@ lapid_b200_status lapid_b200_paged_commit(lapid_b200_device *dev, const lapid_b2
         if (free_pages || n_free) paged_buffer(dev, free_pages, "paged_commit: free_pages", n_free * 4);
         paged_buffer(dev, kv_lens, "paged_commit: kv_lens", R * 4);
         paged_buffer(dev, used, "paged_commit: used", 4);
-        std::vector<const lapid_b200_buffer *> outs = {free_pages, kv_lens, used};
-        for (uint64_t i = 0; i < n_caches; i++) {
-            paged_buffer(dev, caches[i], "paged_commit: a cache", cache);
-            outs.push_back(caches[i]);
-        }
-        paged_apart("paged_commit", {plan, block_table, path, accepted}, outs);
+        for (uint64_t i = 0; i < n_caches; i++) paged_buffer(dev, caches[i], "paged_commit: a cache", cache);
+        paged_apart("paged_commit", {plan, block_table, path, accepted}, {free_pages, kv_lens, used}, caches, n_caches);
         if (R == 0) n_caches = 0;
         std::lock_guard<std::mutex> lock(dev->mu);
         dev->make_current();
