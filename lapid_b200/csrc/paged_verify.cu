@@ -64,6 +64,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t of_rank(const void *p, uint32_t rank) {
@@ -96,7 +97,7 @@ struct Weight {
     __device__ __forceinline__ Weight(const double *table, float t) : root(table), top((double)t), low(t) {}
     __device__ __forceinline__ void set(float temperature) {
         c = 23.083120654223414 / (double)temperature;
-        low = fmaxf((float)top - 700.0f * temperature, -3.4028235e38f);
+        low = fmaxf(__double2float_ru(top - 700.0 * (double)temperature), -3.4028235e38f);  // (rounded up: below e^-708 the exponent has no place)
     }
     __device__ __forceinline__ double operator()(float z) const {
         const double d = (double)z - top, magic = 6755399441055744.0;  // 1.5 2^52

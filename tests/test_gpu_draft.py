@@ -258,6 +258,19 @@ def test_temperatures(be, temperature, drawn):
     w.run().check()
 
 
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("scale,temperature", [(1e5, 1e-4), (1e5, 2e-5), (-3e4, 5e-5), (1e30, 1.0), (65504.0, 0.3)])
+def test_large_logits_at_low_temperatures(be, scale, temperature, drawn):
+    """Neighbouring numbers are many times T apart: a weight whose exponent is past what 64 bits hold is 0."""
+    rng = np.random.default_rng(3)
+    w = Walks(be, [D.random_parents(rng, 5, 2) for _ in range(6)], 333, drawn=drawn, seed=19, temperature=temperature)
+    step = np.spacing(np.float32(abs(scale))).astype(np.float64)
+    w.bits[:] = (scale - step * rng.integers(0, 15, w.bits.shape)).astype(np.float32)
+    w.logits = w.bits.astype(np.float64)
+    w.pick[:] = 0.3 + 0.1 * np.arange(6)
+    w.run().check()
+
+
 def test_a_chain_without_parents(be):
     for drawn in (False, True):
         Walks(be, [chain(n) for n in (1, 4, 0, 9)], 777, drawn=drawn, seed=3, near=0.2, chain=True).run().check()
