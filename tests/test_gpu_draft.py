@@ -74,6 +74,10 @@ CASES = {
     "many_256": dict(sizes=[64, 100, 130], cached=[17, 0, 161], hq=8, hkv=2, d=128, page=64),
     "many_odd": dict(sizes=[33, 50], cached=[3, 64], hq=3, hkv=1, d=80),
     "alone": dict(sizes=[70, 300], cached=[1, 1], hq=1, hkv=1, d=96, page=128),
+    # a tile of one token and of two, more words of ancestors than one
+    "group_100": dict(sizes=[3, 1, 5], cached=[200, 0, 33], hq=100, hkv=1, d=24),
+    "group_50": dict(sizes=[1, 2, 7], cached=[700, 1, 40], hq=100, hkv=2, d=64, page=64),
+    "words": dict(sizes=[600, 33], cached=[70, 1500], hq=1, hkv=1, d=32),
     # few and many beside each other, a request without tokens
     "mixed": dict(sizes=[1, 40, 0, 3, 90], cached=[300, 150, 20, 0, 2], hq=4, hkv=1, d=128),
 }
