@@ -14,8 +14,7 @@
 // alone, so that the CTAs of a cluster always take the same way.
 //
 // What bounds it is the chain of a level, some 7000 cycles (the row and the children's values 1350, weights 1340, sums 620, telling and the barrier 900, reading them 1280, the test 890, going on 450), and at the end 64-bit weights, 25 to 30
-// instructions each. One chain of eight over 128256 tokens 25 us, of which 11 are three levels and 8 the two sums behind a rejection; 16 trees over 32000 21.6; 64 trees over 128256 109, at 42 % of the issue rate; 32 greedy ones over 50257
-// 21.
+// instructions each. One chain of eight over 128256 tokens 24.3 us, of which 11 are three levels and 8 the two sums behind a rejection; 16 trees over 32000 21.3; 64 trees over 128256 94 to 97; 32 greedy ones over 50257 21.
 #include <cuda.h>
 
 #include <algorithm>
@@ -33,13 +32,12 @@ namespace pv {
 using pipe::s32;
 
 constexpr uint32_t WARPS = 16, THREADS = 32 * WARPS, MOST_CTAS = 16;  // of a cluster
-constexpr uint32_t BATCH = 16, FAST = 32;                             // tokens that a thread has in flight in a pass of 64 and of 32 bits
 
 // How far a sum of weights in 32 bits is off, relative: z - top, log2(e), that over T and the product are rounded, 4 2^-24 of the exponent x of e^x, whose mean over the weights is at most ln 2^22 = 15.3 (their
-// entropy); a weight is the product of powers of 2, 2^-22 and a product's 2^-24 each, to the thread's largest (as that grows, at most 32 times: PART_MOST), the warp's, the CTA's and the
+// entropy); a weight is the product of powers of 2, 2^-22 and a product's 2^-24 each, to the thread's largest (as that grows, at most 64 times: PART_MOST), the warp's, the CTA's and the
 // cluster's; at most 90 additions, 2^-24 each. In all 3e-5, of which 2^-14 is twice as much.
 constexpr double SURE = 0x1p-14;
-constexpr uint32_t PART_MOST = 64 * 32 * 16;  // a warp's places: 32 rounds of FAST a thread
+constexpr uint32_t PART_MOST = 64 * 32 * 16;  // a warp's places
 
 // What the warps of the cluster tell each other comes in two sets: a warp writes a set again only when all have read it, which they say with the exchange between.
 struct Shared {
@@ -110,7 +108,7 @@ struct Weight {
         p = fma(f, p, 0.04332169878499658);
         p = fma(f, p, 1.0);
         p *= root[n & 15];
-        p = __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
+        p = __hiloint2double(__double2hiint(p) + (n & ~15) * 65536, __double2loint(p));
         return z < low ? 0.0 : p;
     }
 };
@@ -158,7 +156,9 @@ template <int E> __device__ __forceinline__ void load_apart(float *x, const floa
     for (int e = 0; e < E; e++) x[e] = i + e >= from && i + e < end ? row[i + e - from] : 0.0f;
 }
 
-template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_kernel(const PagedVerifyArgs a, uint32_t ctas, uint32_t part) {
+// CTAS_SM: 1, or where there are more CTAs than SMs 2, so that one request's weights are formed while another one's CTAs wait for each other (64 trees over 128256 tokens 106.9 and 93.9 us, one chain 24.3 and 25.6)
+template <int SRC, int CTAS_SM> __global__ void __launch_bounds__(THREADS, CTAS_SM) paged_verify_kernel(const PagedVerifyArgs a, uint32_t ctas, uint32_t part) {
+    constexpr uint32_t BATCH = 16 / CTAS_SM, FAST = 32 / CTAS_SM;  // tokens that a thread has in flight in a pass of 64 and of 32 bits
     constexpr int E = SRC == ACT_F32 ? 4 : 8, U = BATCH / E, V = FAST / E;
     constexpr uint32_t EB = act_elem_bytes(SRC);
     extern __shared__ __align__(16) uint8_t smem[];
@@ -275,7 +275,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                 for (uint32_t t0 = THREADS; t0 < n; t0 += THREADS) fetch_child(t0 + tid), tell_child(t0 + tid);
                 fetch_child(tid);
             }
-            const float scale = fminf(1.44269504f / temperature, 3e38f);
+            const float scale = fminf(fmaxf(1.44269504f / temperature, 1e-45f), 3e38f);  // (not 0, not infinite: -inf times it is -inf, 0 times it 0)
             float top = -INFINITY, sum = 0.0f;
             uint32_t at = ~0u;
 #pragma unroll 1
@@ -296,13 +296,13 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                     const float was = top;
                     top = max_nan(max_nan(largest[0], largest[1]), max_nan(largest[2], largest[3]));
                     if (top != -INFINITY) {
-                        if (was != -INFINITY) sum *= exp2_fast((was - top) * scale);
+                        sum *= exp2_fast((was - top) * scale);
                         float s[4] = {};
 #pragma unroll
                         for (int u = 0; u < V; u++)
                             if (c0 + 32 * E * u < last)
 #pragma unroll
-                                for (int e = 0; e < E; e++) s[e & 3] += x[u][e] == -INFINITY ? 0.0f : exp2_fast((x[u][e] - top) * scale);
+                                for (int e = 0; e < E; e++) s[e & 3] += exp2_fast((x[u][e] - top) * scale);
                         sum += (s[0] + s[1]) + (s[2] + s[3]);
                     }
                 }
@@ -354,7 +354,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                 top = unordered(__reduce_max_sync(0xffffffffu, ordered(mine)));
                 sum = 0.0f;
 #pragma unroll
-                for (uint32_t k = 0; k < MOST_CTAS * WARPS / 32; k++) sum = fmaf(parts_of[k], tops[k] == -INFINITY ? 0.0f : exp2_fast((tops[k] - top) * scale), sum);
+                for (uint32_t k = 0; k < MOST_CTAS * WARPS / 32; k++) sum = fmaf(parts_of[k], exp2_fast((tops[k] - top) * scale), sum);
                 sum = warp_sum(sum);
             }
             set ^= 1;
@@ -383,7 +383,7 @@ template <int SRC> __global__ void __launch_bounds__(THREADS, 1) paged_verify_ke
                 if (!exact) {
                     if (t < n) {  // most children's tests need no more than 32 bits
                         const Node y = node[t];
-                        const float line = (draft ? y.accept * y.draft : y.accept) * sum, mine = y.logit == -INFINITY ? 0.0f : exp2_fast((y.logit - top) * scale);
+                        const float line = (draft ? y.accept * y.draft : y.accept) * sum, mine = exp2_fast((y.logit - top) * scale);
                         if (mine - line > fmaxf(mine * (float)SURE, 1e-30f)) {
                             next = t;
                             break;
@@ -600,8 +600,8 @@ static uint32_t verify_part(const PagedVerifyArgs &a, uint32_t ctas) {
     return ((places + warps - 1) / warps + unit - 1) / unit * unit;
 }
 
-template <int SRC> static cudaError_t verify_launch(const PagedVerifyArgs &a, uint32_t ctas, int sm_count, bool pdl, cudaStream_t stream) {
-    auto *kernel = pv::paged_verify_kernel<SRC>;
+template <int SRC, int CTAS_SM> static cudaError_t verify_launch(const PagedVerifyArgs &a, uint32_t ctas, int sm_count, bool pdl, cudaStream_t stream) {
+    auto *kernel = pv::paged_verify_kernel<SRC, CTAS_SM>;
     static std::once_flag once[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -614,7 +614,7 @@ template <int SRC> static cudaError_t verify_launch(const PagedVerifyArgs &a, ui
     const uint32_t part = verify_part(a, ctas);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    const uint32_t clusters = std::min<uint32_t>(a.s.requests, std::max<uint32_t>(1, (uint32_t)sm_count / ctas));
+    const uint32_t clusters = std::min<uint32_t>(a.s.requests, std::max<uint32_t>(1, CTAS_SM * (uint32_t)sm_count / ctas));
     cfg.gridDim = dim3(clusters * ctas);
     cfg.blockDim = dim3(pv::THREADS);
     cfg.dynamicSmemBytes = pv::shared_bytes(a.s.max_new, part);
@@ -630,14 +630,17 @@ template <int SRC> static cudaError_t verify_launch(const PagedVerifyArgs &a, ui
 }
 
 cudaError_t launch_paged_verify(const PagedVerifyArgs &a, int sm_count, bool pdl, cudaStream_t stream) {
-    // As many CTAs a request as leave a warp 500 tokens, and no more than two for each SM in all: one chain over 128256 tokens with 4, 8, 16 CTAs 41.0, 28.5, 25.0 us; 16 trees over 32000 with 2, 4, 8 26.0, 21.9,
-    // 27.8; 64 trees over 128256 with 2, 4, 8 114, 110, 157
+    // As many CTAs a request as leave a warp 500 tokens, and no more than two for each SM in all, of 16 one: one chain over 128256 tokens with 4, 8, 16 CTAs 41.0, 28.5, 24.3 us; 16 trees over 32000 with 2, 4, 8 26.0,
+    // 21.3, 27.8; over 128256 16 trees with 8 and 16 44.0 and 50.7, 24 and 32 trees with 4, 8, 16 66, 61, 68 and 67, 63, 83, 64 trees with 2, 4, 8 114, 97, 107
     uint32_t ctas = pv::MOST_CTAS;
-    while (ctas > 1 && ((uint64_t)a.s.requests * ctas > 2 * (uint64_t)sm_count || a.vocab < 500 * pv::WARPS * ctas)) ctas /= 2;
+    while (ctas > 1 && ((uint64_t)a.s.requests * ctas > (ctas > 8 ? 1 : 2) * (uint64_t)sm_count || a.vocab < 500 * pv::WARPS * ctas)) ctas /= 2;
     while (ctas < pv::MOST_CTAS && verify_part(a, ctas) > pv::PART_MOST) ctas *= 2;
-    return a.type == ACT_F32   ? verify_launch<ACT_F32>(a, ctas, sm_count, pdl, stream)
-           : a.type == ACT_F16 ? verify_launch<ACT_F16>(a, ctas, sm_count, pdl, stream)
-                               : verify_launch<ACT_BF16>(a, ctas, sm_count, pdl, stream);
+    const bool many = (uint64_t)a.s.requests * ctas > (uint64_t)sm_count;
+    auto run = [&](auto src) {
+        constexpr int S = decltype(src)::value;
+        return many ? verify_launch<S, 2>(a, ctas, sm_count, pdl, stream) : verify_launch<S, 1>(a, ctas, sm_count, pdl, stream);
+    };
+    return a.type == ACT_F32 ? run(std::integral_constant<int, ACT_F32>()) : a.type == ACT_F16 ? run(std::integral_constant<int, ACT_F16>()) : run(std::integral_constant<int, ACT_BF16>());
 }
 
 }  // namespace lb
