@@ -1117,14 +1117,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                 loaded(o);
                 float v[32];
 #pragma unroll
-                for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * (TREE ? first_part * keep : keep);
-                if constexpr (TREE) {
+                for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * (TREE ? first_part : keep);
+                if constexpr (TREE) {  // (the streams first, then the pieces: the same roundings whoever adds these up)
                     if (split && w.steps > 1) {
                         tmem_ld32(o, o_col + DP + 32 * i);
                         loaded(o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = fmaf(__uint_as_float(o[e]), second * keep, v[e]);
+                        for (int e = 0; e < 32; e++) v[e] = fmaf(__uint_as_float(o[e]), second, v[e]);
                     }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] *= keep;
                 }
 #pragma unroll 1
                 for (uint32_t k = 0; k < others; k++) {

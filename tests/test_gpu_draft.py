@@ -99,6 +99,22 @@ def test_long_caches_are_cut_and_joined(be, n, hq, hkv):
     D.TreeStep(be, [D.random_parents(rng, n, 3)], [7000], hq=hq, hkv=hkv, d=128, page=64, seed=n).run()
 
 
+@pytest.mark.parametrize("sizes,cached,g", [([8] * 40, 400, 4), ([8] * 16, 3000, 4), ([40] * 9, 500, 4), ([64], 6000, 4), ([3, 90], 1000, 2)])
+def test_the_same_bits_call_after_call(be, sizes, cached, g):
+    """Whoever adds up the pieces of a cut tile, and whenever they come."""
+    rng = np.random.default_rng(7)
+    s = D.TreeStep(be, [D.random_parents(rng, n, 3) for n in sizes], [cached + 17 * i for i in range(len(sizes))], hq=2 * g, hkv=2, d=128, seed=3).upload()
+    s.make_plan()
+    s.attend()
+    be.synchronize()
+    first = s.b["out"].download(), s.b["lse"].download()
+    for _ in range(6):
+        for _ in range(25):
+            s.attend()
+        be.synchronize()
+        assert np.array_equal(s.b["out"].download(), first[0]) and np.array_equal(s.b["lse"].download(), first[1])
+
+
 @pytest.mark.parametrize("shape", ["star", "chain", "roots"])
 @pytest.mark.parametrize("n", [4, 40])
 def test_shapes(be, n, shape):
