@@ -937,9 +937,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
             const bool real = local < s.tt && token < w.n;
             // (rows that are none see everything: their results go nowhere, and they ask for no mask)
             // (of a tree: hi and lo are those of the cached keys)
-            const uint32_t cached = w.kv - w.n;
-            const uint32_t *const tree = TREE ? p.tree + (size_t)(w.q0 + (real ? token : 0u)) * (1 + s.tree) : nullptr;
-            const uint32_t hi = !real ? ~0u : TREE ? cached : paged_hi(s, w.n, w.kv, token), lo = !real ? 0u : TREE ? paged_tree_lo(s, cached, *tree) : paged_lo(s, hi);
+            auto tree_row = [&]() { return p.tree + (size_t)(w.q0 + token) * (1 + s.tree); };
+            const uint32_t hi = !real ? ~0u : TREE ? w.kv - w.n : paged_hi(s, w.n, w.kv, token), lo = !real ? 0u : TREE ? paged_tree_lo(s, w.kv - w.n, *tree_row()) : paged_lo(s, hi);
             // A warp without a row only says that it is ready: the special-function unit and the schedulers are the others'. (16 requests of eight tokens, 32 rows each, over up to 8192 keys 76.7 us, with it 80.3.) Its weights are whatever
             // lies in tensor memory: they reach its own rows of O alone, which go nowhere.
             const bool idle = TREE && !__any_sync(0xffffffffu, real);
@@ -984,7 +983,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_large_kernel(const __gr
                         const uint32_t below = to > g ? (to - g >= 32 ? ~0u : (1u << (to - g)) - 1) : 0u, out = from > g ? (from - g >= 32 ? ~0u : (1u << (from - g)) - 1) : 0u;
                         uint32_t bits = below & ~out;
                         if constexpr (TREE) {
-                            if (real) bits |= paged_tree_bits(tree, s.tree, (int32_t)(key0 + g - cached));
+                            if (real) bits |= paged_tree_bits(tree_row(), s.tree, (int32_t)(key0 + g - hi));
                         }
 #pragma unroll
                         for (uint32_t i = 0; i < 32 && g + i < (uint32_t)C::KEYS; i++)
