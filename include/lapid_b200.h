@@ -496,8 +496,8 @@ LAPID_B200_API lapid_b200_status lapid_b200_paged_tree_attention(lapid_b200_devi
  *   without (NULL: candidates that were chosen):                                                                      when accept[c] < P(x);         else P(x) <- 0, scaled to sum 1
  * (where nothing would be left, P stays). The walk goes on at the accepted child. Where none is, next is the first token t with P(0) + .. + P(t) > pick. accept f32 [tokens], pick f32 [requests]: random
  * numbers in [0, 1). Out: path i32 [requests, max_new], the walk's nodes (the first is 0), -1 behind them; accepted i32 [requests], how many; next i32 [requests], the token behind the last. A
- * drafted token outside the vocabulary is reported and not accepted; where a row has NaN, +inf or nothing but -inf the walk ends there and next is -1. Of a request without new tokens accepted is 0 and next -1. Weights, sums and
- * comparisons are 64 bits wide. parents as in paged_tree; NULL with the mask CAUSAL: every token's parent is the one in front of it. At most 1024 new tokens a request. */
+ * drafted token outside the vocabulary is reported and not accepted; where a row has NaN, +inf or nothing but -inf the walk ends there and next is -1. Of a request without new tokens accepted is 0 and next -1. What decides is 64 bits wide
+ * (a sum of 32 bits only where its error cannot matter). parents as in paged_tree; NULL with the mask CAUSAL: every token's parent is the one in front of it. At most 1024 new tokens a request. */
 LAPID_B200_API lapid_b200_status lapid_b200_paged_verify(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan, int32_t logits_dtype,
                                                          uint64_t vocab, const lapid_b200_buffer *logits, uint64_t logits_row, const lapid_b200_buffer *draft,
                                                          uint64_t draft_row, const lapid_b200_buffer *tokens, const lapid_b200_buffer *parents,

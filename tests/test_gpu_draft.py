@@ -701,6 +701,36 @@ def test_calls_on_another_stream_and_in_a_graph(be):
     mine.close()
 
 
+@pytest.mark.parametrize("n,cached", [(8, 2000), (64, 3000), (1, 900)])
+def test_attention_in_a_graph(be, n, cached):
+    """Tree and attention captured once and replayed on other trees: what calls give."""
+    import torch
+    stream = torch.cuda.Stream()
+    mine = lp.Backend(0)
+    mine.set_stream(stream.cuda_stream)
+    rng = np.random.default_rng(n)
+    s = D.TreeStep(mine, [D.random_parents(rng, n, 3)], [cached], hq=8, hkv=2, d=128, page=64).upload()
+    b = s.b
+    s.make_plan()
+    s.attend()
+    mine.synchronize()
+    calls = [mine.packed_paged_tree(s.spec, b["plan"], b["parents"], b["positions"], b["tree"]),
+             mine.packed_paged_tree_attention(s.spec, b["plan"], b["tree"], b["q"], b["k"], b["v"], b["table"], b["out"], lse=b["lse"])]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for call in calls:
+            call()
+    for _ in range(3):
+        s.parents = [D.random_parents(rng, n, 4, 0.1)]
+        b["parents"].write(0, np.array(s.parents[0], np.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        mine.synchronize()
+        s.check()
+    del graph
+    mine.close()
+
+
 def test_two_calls_at_once(be):
     """Two handles' verifications on two streams side by side."""
     import torch
