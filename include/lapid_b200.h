@@ -506,7 +506,8 @@ LAPID_B200_API lapid_b200_status lapid_b200_paged_verify(lapid_b200_device *dev,
 /* Keeps of every request the accepted[r] (0 to its new length) tokens path[r][0 ..) (rising; as verify writes them): in each of the n_caches caches (keys and values of all layers, in any order) what lies at
  * cached + path[r][i] moves to cached + i. At most 1024 new tokens a request with a path; path NULL, with the mask CAUSAL: the first ones, which lie there already. Out: kv_lens (cached + accepted: the next step's cached_lens) and used, in the place of what paged_plan
  * wrote there, and free_pages: of the pages that the step took (the first ones of the list) the kept ones first, then the others, so that the caller drops `used` of them from the front as behind any step. A request
- * whose accepted length or path is out of range is reported and keeps nothing. Not to be run twice on one step: what it moves has moved. */
+ * whose accepted length or path is out of range is reported and keeps nothing. Where the step's pages ran out (the plan reports it) no request keeps anything: kv_lens are the cached lengths, used is 0
+ * and free_pages stays, so that the step can be run again when there are more. Not to be run twice on one step: what it moves has moved. */
 LAPID_B200_API lapid_b200_status lapid_b200_paged_commit(lapid_b200_device *dev, const lapid_b200_paged *desc, const lapid_b200_buffer *plan,
                                                          lapid_b200_buffer *const *caches, uint64_t n_caches, const lapid_b200_buffer *block_table,
                                                          const lapid_b200_buffer *path, const lapid_b200_buffer *accepted, lapid_b200_buffer *free_pages,

@@ -91,21 +91,28 @@ __device__ __forceinline__ bool path_sound(const int32_t *path, uint32_t i, uint
     return p >= 0 && (uint32_t)p < n && (i == 0 || path[i - 1] < p);
 }
 
-// Lengths, and the step's pages in the list: by one CTA, a thread a request
+// Lengths, and the step's pages in the list: by one CTA, a thread a request. Where a page that the step needs is missing the list stays as it is and no request keeps anything.
 __device__ void commit_pages(const PagedCommitArgs &a) {
     constexpr uint32_t WARPS = COMMIT_THREADS / 32;
     __shared__ uint32_t sums[2][WARPS];
     const PagedShape &s = a.s;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, shift = 31 - __clz(s.page);
     uint32_t all_kept = 0;  // over all requests
+    bool missing = false;
     for (int pass = 0; pass < 2; pass++) {
         uint32_t kept = 0, back = 0;  // in front of this chunk
         for (uint32_t r0 = 0; r0 < s.requests; r0 += COMMIT_THREADS) {
             const uint32_t r = r0 + threadIdx.x;
-            uint32_t have = 0, keep = 0, need = 0, end = 0;
+            uint32_t have = 0, keep = 0, need = 0, end = 0, at_first = 0;
+            bool lacks = false;
             if (r < s.requests) {
                 const uint4 x = ((const uint4 *)a.request)[r];
                 const uint32_t n = x.y - x.x, cached = x.z - n;
+                at_first = cached;
+                have = (cached + s.page - 1) >> shift, need = (x.z + s.page - 1) >> shift;
+                const int32_t *const table = a.table + (size_t)r * s.max_blocks;
+                auto page_of = [&](uint32_t b) -> uint32_t { return b >= need ? 0u : b < s.max_blocks ? (uint32_t)table[b] : ~0u; };
+                const uint32_t page0 = page_of(have), page1 = page_of(have + 1);  // (asked for before the path is)
                 bool bad = false;
                 uint32_t k = accepted_of(a, r, n, bad);
                 if (a.path)
@@ -113,7 +120,9 @@ __device__ void commit_pages(const PagedCommitArgs &a) {
                 if (bad) k = 0;
                 if (bad && a.status) atomicOr(a.status, (int)PAGED_STATUS_INDEX);
                 end = cached + k;
-                have = (cached + s.page - 1) >> shift, keep = (end + s.page - 1) >> shift, need = (x.z + s.page - 1) >> shift;
+                keep = (end + s.page - 1) >> shift;
+                lacks = page0 >= s.pages || page1 >= s.pages;
+                for (uint32_t b = have + 2; b < need; b++) lacks |= page_of(b) >= s.pages;
             }
             uint32_t ki = keep - have, bi = need - keep;
 #pragma unroll
@@ -123,7 +132,7 @@ __device__ void commit_pages(const PagedCommitArgs &a) {
             }
             __syncthreads();
             if (lane == 31) sums[0][warp] = ki, sums[1][warp] = bi;
-            __syncthreads();
+            missing |= __syncthreads_or(lacks) != 0;
             uint32_t k_all = 0, b_all = 0, k_front = 0, b_front = 0;
 #pragma unroll
             for (uint32_t w = 0; w < WARPS; w++) {
@@ -133,10 +142,10 @@ __device__ void commit_pages(const PagedCommitArgs &a) {
             if (s.requests <= COMMIT_THREADS) all_kept = k_all;
             if (r < s.requests && (pass || s.requests <= COMMIT_THREADS)) {
                 uint32_t to_kept = kept + k_front + ki - (keep - have), to_back = all_kept + back + b_front + bi - (need - keep);
-                a.kv_lens[r] = (int32_t)end;
-                for (uint32_t b = have; b < need; b++) {
+                a.kv_lens[r] = (int32_t)(missing ? at_first : end);
+                for (uint32_t b = have; b < need && !missing; b++) {
                     const uint32_t to = b < keep ? to_kept++ : to_back++;
-                    if (to < a.n_free) a.free_pages[to] = b < s.max_blocks ? a.table[(size_t)r * s.max_blocks + b] : -1;
+                    if (to < a.n_free) a.free_pages[to] = a.table[(size_t)r * s.max_blocks + b];
                 }
             }
             kept += k_all, back += b_all;
@@ -144,7 +153,7 @@ __device__ void commit_pages(const PagedCommitArgs &a) {
         all_kept = kept;
         if (s.requests <= COMMIT_THREADS) break;
     }
-    if (threadIdx.x == 0) *a.used = (int32_t)all_kept;
+    if (threadIdx.x == 0) *a.used = missing ? 0 : (int32_t)all_kept;
 }
 
 // A CTA has one request and some of the caches: where its tokens lie and where they go is found once, in shared memory, and what is asked for first (record, accepted, path) does not wait for each other.

@@ -524,6 +524,34 @@ def test_commit_of_chains_and_without_caches(be):
     k.check()
 
 
+@pytest.mark.parametrize("ends", ["list", "entries"])
+@pytest.mark.parametrize("requests", [5, 128, 300])
+def test_a_step_whose_pages_ran_out_keeps_nothing(be, requests, ends):
+    """Plan and commit may lie in one graph: where the pages ran out, lengths and list stay, so that the step can be run again."""
+    rng = np.random.default_rng(requests)
+    new, cached = rng.integers(1, 40, requests).tolist(), rng.integers(0, 50, requests).tolist()
+    path = paths(rng, new)
+    k = Kept(be, new, cached, [len(p) for p in path], path, hkv=1, d=16, caches=2)
+    taken = int(k.b["used"].download().view(np.int32)[0])
+    lens, z = [be.upload(np.array(x, np.int32)) for x in (new, cached)], [be.upload(np.zeros(sum(new) + 1, np.int32)) for _ in range(2)]
+    plan = lambda free, n: be.paged_plan(k.spec, *lens, k.b["table"], *z, k.b["kv"], k.b["used"], k.b["plan"], free_pages=free, n_free=n)
+    few = k.free[:taken - 2] if ends == "list" else np.concatenate([k.free[:taken - 2], np.full(9, -1, np.int32)])
+    short = be.upload(few)
+    plan(short, len(few))
+    be.paged_commit(k.spec, k.b["plan"], k.layers(), k.b["table"], k.b["path"], k.b["accepted"], k.b["kv"], k.b["used"], free_pages=short, n_free=len(few))
+    with pytest.raises(lp.LapidError) as e:
+        be.synchronize()
+    assert e.value.code == "out_of_memory"
+    assert k.b["kv"].download().view(np.int32)[:requests].tolist() == cached
+    assert int(k.b["used"].download().view(np.int32)[0]) == 0
+    assert np.array_equal(short.download().view(np.int32)[:len(few)], few)
+    k.before = [c.download().view(np.int16)[: x.size].reshape(x.shape).copy() for c, x in zip(k.caches, k.before)]  # (what lies behind the cached tokens may have moved)
+    plan(k.b["free"], len(k.free))
+    k.commit()
+    be.synchronize()
+    k.check()
+
+
 @pytest.mark.parametrize("accepted,path", [([3, 2], [[0, 2, 2], [0, 1]]), ([3, 2], [[0, 3, 2], [0, 1]]), ([2, 2], [[0, 5], [0, 1]]), ([2, 2], [[-1, 1], [0, 1]]), ([6, 2], [[0, 1, 2, 3, 4], [0, 1]]),
                                            ([-1, 2], [[], [0, 1]]), ([1 << 30, 2], [[], [0, 1]])])
 def test_a_path_that_is_none_keeps_nothing(be, accepted, path):
