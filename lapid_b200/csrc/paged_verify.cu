@@ -122,9 +122,9 @@ __device__ __forceinline__ double positive(double x) {
     const int keep = ~(__double2hiint(x) >> 31);
     return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
 }
-// Whole numbers in the order of the floats, NaN on top
+// Whole numbers in the order of the floats, the same one for both zeros (-0.0 + 0.0 is 0.0), NaN on top
 __device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);
     return x != x ? ~0u : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }

@@ -278,6 +278,30 @@ def test_temperatures(be, temperature, drawn):
     w.run().check()
 
 
+@pytest.mark.parametrize("dtype", [lp.DType.F32, lp.DType.BF16, lp.DType.F16])
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("requests,vocab", [(1, 300), (1, 4099), (200, 4099), (1, 32000), (40, 32000), (1, 70001)])
+def test_the_first_of_two_zeros_whatever_their_signs(be, requests, vocab, drawn, dtype):
+    """At temperature 0 the largest logit is a zero: -0.0 and 0.0 are equal, and the first one is taken, in whichever warps or CTAs of the request they lie."""
+    w = Walks(be, [[-1, 0, 0, 1] for _ in range(requests)], vocab, dtype=dtype, drawn=drawn, seed=vocab, temperature=0.0)
+    w.logits[:] = w.logits - 20.0 - np.abs(w.logits)
+    at = np.array([3, vocab // 5, vocab // 2, vocab - 2])
+    signs = np.array([[-1, 1, -1, 1], [1, -1, 1, -1], [-1, -1, -1, 1], [-1, 1, 1, 1]])
+    for t in range(w.tokens):
+        first = t // 4 % 4
+        w.logits[t, at[first:]] = np.copysign(0.0, signs[t % 4][first:])
+    if dtype == lp.DType.F32:
+        w.bits = w.logits.astype(np.float32)
+    else:
+        w.logits, w.bits = R.to_half(w.logits, dtype)
+    w.logits = w.logits + 0.0  # (the definition's: one zero)
+    w.tokens_of[:] = at[np.arange(w.tokens) % 4]
+    for r in range(requests):  # children of the first node: the second of the zeros, then the first
+        first = r % 4
+        w.tokens_of[4 * r + 1], w.tokens_of[4 * r + 2] = at[min(first + 1, 3)], at[first]
+    w.run().check()
+
+
 @pytest.mark.parametrize("drawn", [False, True])
 @pytest.mark.parametrize("scale,temperature", [(1e5, 1e-4), (1e5, 2e-5), (-3e4, 5e-5), (1e30, 1.0), (65504.0, 0.3)])
 def test_large_logits_at_low_temperatures(be, scale, temperature, drawn):
