@@ -5,9 +5,10 @@
 // left, max(P - D, 0) / sum of it; without D (candidates that were chosen, not drawn) when u_c < P(x), else x leaves P. An accepted child is the next v; when none is,
 // the token behind the path is the first t with P(0) + .. + P(t) > w. Whatever the drafts are, the tokens are then distributed as the model's own.
 //
-// Decisions are comparisons, so what decides is 64 bits wide: a result differs from the definition's only where u or w is within 1e-12 of a border. A node's sum is formed in 32 bits first,
-// which is off by less than SURE of it; a child whose test that leaves open, and what is drawn from, gets it again in 64 bits. (Half of the 64-bit operations that a sum of weights for every
-// node would be; an SM does 64 of these a cycle.)
+// Decisions are comparisons, so what decides is 64 bits wide. With u = 2^-53 a sum of weights is off by at most 7e-14 of itself (a weight e^-x by (x + 8) u, x at most 15.3 in their mean; at most 530 additions), so a
+// result differs from the definition's only where a number drawn is within 2e-13 of a border; within 1e-10 behind rejected candidates, whose weights are taken off a sum while 2^-10 of it is left; and behind rejected
+// drafts within 3e-13 over the part of all probability that max(P - D, 0) left (a draft that is the model but for its rounding to 32 bits leaves some 1e-8). (These are bounds.) A node's sum is formed in 32 bits first, which is off by less than SURE of it; a child whose test that leaves open, and what is drawn from, gets it again in 64 bits. (Half of the 64-bit
+// operations that a sum of weights for every node would be; an SM does 64 of these a cycle.)
 //
 // A request belongs to a cluster of CTAs, each with a part of the vocabulary, a warp of it to a warp; only the rows on the path are read. A level is a pass over the node's logits (largest and sum), an
 // exchange over the cluster's shared memory, and the children's tests, whose tokens, numbers and values were fetched meanwhile. What decides comes from rank 0's loads and from the exchanged sums
@@ -86,8 +87,9 @@ __device__ __forceinline__ void better(float &top, uint32_t &at, float t, uint32
     top = max_nan(top, t);
 }
 
-// Weights e^((z - top) / T), relative error 2e-13: with c = 16 log2(e) / T and n the whole number nearest to (z - top) c, 2^(n / 16) from a table of 16 (of which any lanes may read any without a bank
-// conflict) and the exponent, times the series of 2^(f / 16), |f| <= 1/2, to the fifth power: twelve operations of 64 bits. A weight below e^-700 is 0, as that of -inf is, whatever T is.
+// Weights e^((z - top) / T): with c = 16 log2(e) / T and n the whole number nearest to (z - top) c, 2^(n / 16) from a table of 16 (of which any lanes may read any without a bank
+// conflict) and the exponent, times the series of 2^(f / 16), |f| <= 1/2, to the sixth power, which leaves 4.4e-16: thirteen operations of 64 bits. (To the fifth it would leave 1.5e-13, which is seen where a draft that
+// is nearly the model leaves 1e-8 of all probability.) A weight below e^-700 is 0, as that of -inf is, whatever T is.
 struct Weight {
     const double *root;
     double top, c = 0.0;
@@ -102,7 +104,8 @@ struct Weight {
         const double k = fma(d, c, magic), f = fma(d, c, magic - k);
         const int n = __double2loint(k);
         // (ln 2 / 16)^i / i!
-        double p = fma(f, 1.271587195055813e-09, 1.467610032291943e-07);
+        double p = fma(f, 9.181219573844438e-12, 1.271587195055813e-09);
+        p = fma(f, p, 1.467610032291943e-07);
         p = fma(f, p, 1.3550807779497455e-05);
         p = fma(f, p, 0.0009383847928089871);
         p = fma(f, p, 0.04332169878499658);

@@ -379,6 +379,45 @@ def test_a_draft_that_is_the_model(be):
     assert accepted.min() == 6 and (nxt >= 0).all()
 
 
+def test_borders_of_what_a_rejected_draft_leaves(be):
+    """The draft is the model but for the rounding to 32 bits: a hundred millionth of the probability is left, and an error of a weight counts a hundred million times as much. The numbers drawn are the f32 ones next to
+    the borders between the tokens of what is left, outside of what arithmetic of 64 bits allows. With u = 2^-53 and m the mean of x: a weight e^-x is off by x u (log2(e) / T is rounded once where T is 1) and 8 u (the
+    series 4 u, its last sum, the table and the product 1 u each, what is before them less than one); their sum by (m + 8) u, and 10 u for at most ten additions; the differences, relative to all probability, by the
+    sum of the two; a border is a quotient of two sums of these, so twice that over what is left, and 40 u for the additions."""
+    u, vocab, each = 2.0 ** -53, 40, []
+    rng = np.random.default_rng(31)
+    while len(each) < 1000:
+        # the largest logit apart, half of the probability; the others half a step of the table of 16 below one another's places
+        z = (-(rng.integers(70, 110, vocab) + 0.49) * math.log(2) / 16).astype(np.float32)
+        x, top = (int(i) for i in rng.choice(vocab, 2, replace=False))
+        z[top] = 0.0
+        low = z.astype(np.longdouble)
+        p = np.exp(low)
+        p /= p.sum()
+        d = p.astype(np.float64).astype(np.float32)
+        d[x] = d[x] * np.float32(1 + 2.0 ** -21)  # (the drafted token: rejected by any number near 1)
+        left = np.maximum(p - d.astype(np.longdouble), 0)
+        all_left = left.sum()
+        border = np.cumsum(left) / all_left
+        m = float(-(p * low).sum())
+        slack = (2 * (2 * (m + 8) + 10) * u) / float(all_left) + 40 * u
+        for b in border[left > 0][:-1]:
+            for side in (-1, 1):
+                pick = np.float32(b + side * slack)
+                while side * (np.longdouble(pick) - b) < slack:
+                    pick = np.nextafter(pick, np.float32(side))
+                if 0 < pick < 1 and np.abs(border - np.longdouble(pick)).min() >= slack:
+                    each.append((z, d, x, pick, int(np.nonzero(border > np.longdouble(pick))[0][0])))
+    w = Walks(be, [[-1, 0] for _ in each], vocab, drawn=True, seed=1)
+    want = []
+    for r, (z, d, x, pick, token) in enumerate(each):
+        w.bits[2 * r], w.draft[2 * r], w.tokens_of[2 * r + 1], w.pick[r] = z, d, x, pick
+        want.append(token)
+    w.accept[:] = np.float32(1 - 2.0 ** -24)
+    path, accepted, nxt = w.run().got()
+    assert np.all(accepted == 1) and np.array_equal(nxt, want)
+
+
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), "none"])
 def test_rows_that_are_no_distribution(be, value):
     w = Walks(be, [chain(4), chain(3), [-1, 0, 0]], 600, seed=2)
