@@ -587,6 +587,24 @@ def test_commit_of_chains_and_without_caches(be):
     k.check()
 
 
+def test_commit_of_more_requests_than_a_grid_is_high(be):
+    rng = np.random.default_rng(70)
+    new, cached = rng.integers(0, 4, 70000).tolist(), rng.integers(0, 13, 70000).tolist()
+    path = paths(rng, new)
+    k = Kept(be, new, cached, [len(p) for p in path], path, hkv=1, d=16, caches=2)
+    k.commit()
+    be.synchronize()
+    k.check()
+
+
+def test_commit_of_long_chains(be):
+    """Without a path there is no largest number of new tokens."""
+    k = Kept(be, [2000, 1500, 0], [30, 0, 5], [1999, 3, 0], None, mask=Mask.CAUSAL)
+    k.commit()
+    be.synchronize()
+    k.check()
+
+
 @pytest.mark.parametrize("ends", ["list", "entries"])
 @pytest.mark.parametrize("requests", [5, 128, 300])
 def test_a_step_whose_pages_ran_out_keeps_nothing(be, requests, ends):
