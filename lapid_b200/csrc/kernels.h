@@ -396,7 +396,8 @@ constexpr uint32_t PAGED_SMALL_ROWS = 16, PAGED_SMALL_KEYS = 64;       // tile a
 // and of 32 47.8 and 63.3 us at 16 requests over 2048 to 4096 keys, 19.1 and 21.0 at one over 8192, 56.0 and 76.1 at 64 over 512 to 1024; at d = 64 22.7 and 25.5.
 constexpr uint32_t PAGED_SMALL_LIMIT = 16;
 // Of a tree, whose tiles of up to 128 rows the other kernel takes in two streams: 16 rows over 256, 4096, 16384 and 32768 keys there 10.3, 16.5, 26.7 and 37.4 us, here 13.3, 18.6, 31.1 and 41.1, of 16 requests over
-// 1024 and 8192 20.6 and 61.7, here 20.4 and 62.1; 8 rows over 256, 4096 and 32768 10.3, 16.3 and 37.2, here 12.0, 16.5 and 38.3, of 16 requests 20.4 and 60.9, here 18.3 and 60.0.
+// 1024 and 8192 20.6 and 61.7, here 20.4 and 62.1; 8 rows over 256, 4096 and 32768 10.3, 16.3 and 37.2, here 12.0, 16.5 and 38.3, of 16 requests 20.4 and 60.9, here 18.3 and 60.0. (A limit for one request:
+// where there are many, up to 16 rows the kernel for few is as quick or up to a tenth quicker, which the rule does not look at. All with groups of four heads of 128.)
 constexpr uint32_t PAGED_SMALL_LIMIT_TREE = 4;
 constexpr uint32_t PAGED_LARGE_ROWS = 256;                             // tile (at most) of the tensor-memory kernel
 // Steps that beginning and ending one of its tiles takes as long as. (With 2 in place of 3: 100 and 200 tokens 13.9 and 16.9 instead of 9.2 and 10.7 us, 2048 44.7 instead of 45.3,
@@ -420,7 +421,7 @@ struct PagedShape {
     float scale;
 };
 // Places in a plan buffer (32-bit words; `past`, at the same place whatever the description: 1 from when the kernel for many rows has waited for what is in front of it until
-// both are over; `request`: the row of q where its tokens begin, the one where they end, its keys, 0; the partial results behind them at byte offsets)
+// both are over, of a tree until the next plan, since no kernel for few rows is behind it; `request`: the row of q where its tokens begin, the one where they end, its keys, 0; the partial results behind them at byte offsets)
 struct PagedPlanLayout {
     uint32_t past, request, units_small, units_large, start_small, start_large, count_small, count_large;
     size_t part_small, part_large, bytes;  // part_*: [CTA][2] results of cut tiles: rows x (d padded + 2) f32

@@ -481,7 +481,7 @@ template <int DP, bool BF16> __device__ __forceinline__ void join_pieces_both(co
 }
 
 // Drafted tokens are few rows over many keys: their tiles are cut into many pieces. From JOIN_APART of them on the CTAs only leave theirs in the plan, and the kernel below adds them up on all SMs: a tile of 256 rows
-// over 32768 keys is 18 pieces of 133 KB, which one CTA takes 40 us for (64 tokens over 32768 keys, 8 key heads: 50.8 us, with the last CTA of a tile at it 75.7).
+// over 32768 keys is 18 pieces of 133 KB, which one CTA takes 40 us for (64 tokens over 32768 keys, 8 key heads: 51 to 53 us, with the last CTA of a tile at it 75.7).
 constexpr uint32_t JOIN_APART = 4, JOIN_COLS = 8, JOIN_THREADS = 256;
 static_assert(JOIN_THREADS >= PAGED_MAX_SMS, "a thread for each end of a span");
 

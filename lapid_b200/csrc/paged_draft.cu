@@ -2,10 +2,10 @@
 //
 // tree    depth(t) = depth(parent) + 1, 0 without one; position = cached + depth; bit i of t: i is t or an ancestor of it (with a window: depth(t) - depth(i) < window).
 //         A parent comes in front of its children, so a thread walks from its token to the root, setting bits on the way: a word is complete when the walk leaves it for
-//         one further in front. Bound by latency: the record, the parents, a walk of as many shared loads as the token has ancestors: 8 trees of 16 tokens 3.4 us, 512 of up to 64 5.1.
+//         one further in front. Bound by latency: the record, the parents, a walk of as many shared loads as the token has ancestors: 8 trees of 16 tokens 3.3 to 3.5 us, 512 of up to 64 5.1 to 5.3.
 // commit  keys and values at cached + path[i] go to cached + i, in every layer. Since path[i] >= i and the path rises, a thread that owns 16 bytes of a head and takes the path's
 //         tokens in their order never overwrites what it has still to read. Pages that only rejected tokens lie in go back: the step's pages are the first ones of the
-//         list, and are written there again, the kept ones first (requests in order), so that the caller drops the kept ones alone. Bound by latency, then by HBM: one request of 16 tokens in 32 layers 5.3 us, 32 of up to 24 10 to 12.6 us for 46 MB.
+//         list, and are written there again, the kept ones first (requests in order), so that the caller drops the kept ones alone. Bound by latency, then by HBM: one request of 16 tokens in 32 layers 4.9 to 5.3 us, 32 of up to 24 10 to 12.6 us for 46 MB.
 #include "common.cuh"
 #include "paged.cuh"
 

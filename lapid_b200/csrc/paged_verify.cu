@@ -6,16 +6,18 @@
 // the token behind the path is the first t with P(0) + .. + P(t) > w. Whatever the drafts are, the tokens are then distributed as the model's own.
 //
 // Decisions are comparisons, so what decides is 64 bits wide. With u = 2^-53 a sum of weights is off by at most 7e-14 of itself (a weight e^-x by (x + 8) u, x at most 15.3 in their mean; at most 530 additions), so a
-// result differs from the definition's only where a number drawn is within 2e-13 of a border; within 1e-10 behind rejected candidates, whose weights are taken off a sum while 2^-10 of it is left; and behind rejected
-// drafts within 3e-13 over the part of all probability that max(P - D, 0) left (a draft that is the model but for its rounding to 32 bits leaves some 1e-8). (These are bounds.) A node's sum is formed in 32 bits first, which is off by less than SURE of it; a child whose test that leaves open, and what is drawn from, gets it again in 64 bits. (Half of the 64-bit
-// operations that a sum of weights for every node would be; an SM does 64 of these a cycle.)
+// result differs from the definition's only where a number drawn is next to a border: within 2e-13 of it; within 1e-10 behind rejected candidates, whose weights are taken off a sum while 2^-10 of it is left; behind
+// rejected drafts within 3e-13 over the part of all probability that max(P - D, 0) left (a draft that is the model but for its rounding to 32 bits leaves some 1e-8).
+// A node's sum is formed in 32 bits first, which is off by less than SURE of it; a child whose test that leaves open, and what is drawn from, gets it again in 64 bits. (Half of the 64-bit operations that a sum of
+// weights for every node would be; an SM does 64 of these a cycle.)
 //
 // A request belongs to a cluster of CTAs, each with a part of the vocabulary, a warp of it to a warp; only the rows on the path are read. A level is a pass over the node's logits (largest and sum), an
 // exchange over the cluster's shared memory, and the children's tests, whose tokens, numbers and values were fetched meanwhile. What decides comes from rank 0's loads and from the exchanged sums
 // alone, so that the CTAs of a cluster always take the same way.
 //
 // What bounds it is the chain of a level, some 7000 cycles (the row and the children's values 1350, weights 1340, sums 620, telling and the barrier 900, reading them 1280, the test 890, going on 450), and at the end 64-bit weights, 25 to 30
-// instructions each. One chain of eight over 128256 tokens 24.3 us, of which 11 are three levels and 8 the two sums behind a rejection; 16 trees over 32000 21.3; 64 trees over 128256 94 to 97; 32 greedy ones over 50257 21.
+// instructions each. By the paths drawn one chain of eight over 128256 tokens takes 24 to 30 us, of which 11 are three levels and 8 the two sums behind a rejection; 16 trees over 32000 20 to 22; 64 trees over 128256 92 to
+// 98; 32 greedy ones over 50257 22 to 23. (The figures beside the choices below were taken with a weight's series one power shorter, which is 1.5 % less.)
 #include <cuda.h>
 
 #include <algorithm>
@@ -36,7 +38,8 @@ constexpr uint32_t WARPS = 16, THREADS = 32 * WARPS, MOST_CTAS = 16;  // of a cl
 
 // How far a sum of weights in 32 bits is off, relative: z - top, log2(e), that over T and the product are rounded, 4 2^-24 of the exponent x of e^x, whose mean over the weights is at most ln 2^22 = 15.3 (their
 // entropy); a weight is the product of powers of 2, 2^-22 and a product's 2^-24 each, to the thread's largest (as that grows, at most 64 times: PART_MOST), the warp's, the CTA's and the
-// cluster's; at most 90 additions, 2^-24 each. In all 3e-5, of which 2^-14 is twice as much.
+// cluster's; at most 90 additions, 2^-24 each. In all 3e-5, of which 2^-14 is twice as much. A child's own weight in 32 bits, where its test is decided by it, is 1e-30 or more, so x at most 69.1 and it is off by
+// 1.7e-5: both together stay below 2^-14 too.
 constexpr double SURE = 0x1p-14;
 constexpr uint32_t PART_MOST = 64 * 32 * 16;  // a warp's places
 
